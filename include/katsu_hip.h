@@ -273,6 +273,48 @@ int katsu_hip_gradcam_f32_dev(const float *act, const float *grad, size_t n, siz
 int katsu_hip_resize_bilinear_f32_dev(const float *src, size_t n, size_t ih, size_t iw,
                                       size_t oh, size_t ow, float *dst, void *stream);
 
+/* ---- Language-model operators ---------------------------------------------
+ * What a block of a language model computes between its matrix products.  No
+ * counterpart in the reference's code.  All take device pointers and a stream,
+ * in float32 or bfloat16; sums, softmax statistics and norms are float32 or
+ * wider.  Results do not depend on the order of atomics: the same call gives
+ * the same bits. */
+typedef enum katsu_dtype { KATSU_F32 = 0, KATSU_BF16 = 1 } katsu_dtype;
+
+/* Attention over packed sequences.  q and out hold tokens_q tokens of `heads`
+ * heads, k and v tokens_k tokens of kv_heads (which divides heads; query head
+ * h reads key head h / (heads/kv_heads)), all of head_dim channels (1..128).
+ * Strides are in elements, [0] between tokens and [1] between heads; channels
+ * are adjacent.  Sequence s has queries cu_q[s] .. cu_q[s+1] and keys cu_k[s]
+ * .. cu_k[s+1], or with k_lens the first k_lens[s] of those (slots of a cache);
+ * cu_q and cu_k are device arrays of seqs + 1 int32 that start at 0 and do not
+ * fall, both NULL for one sequence of all tokens; values outside the tensors
+ * are taken as their ends.
+ *   S = scale q.k over the visible keys, P = softmax(S), out = P v,
+ *   lse[head][token] = log sum exp S       (natural logarithm)
+ * With causal set query i of Lq sees key j of Lk if j <= i + Lk - Lq: the last
+ * query sees every key.  A query that sees none gives out 0 and lse -inf.
+ * What masked places hold changes nothing, Inf and NaN included.
+ * scale must be positive and finite. */
+typedef struct katsu_attention {
+    int32_t dtype;  /* katsu_dtype of q, k, v, out */
+    int32_t causal;
+    uint64_t heads, kv_heads, head_dim;
+    uint64_t seqs, tokens_q, tokens_k;
+    int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2];
+    float scale;
+} katsu_attention;
+
+/* The forward pass; lse may be NULL.  `workspace` of
+ * katsu_hip_attention_fwd_workspace bytes (device memory, 256-byte aligned)
+ * holds the parts of a key axis split over workgroups; NULL uses a
+ * library-owned buffer, allocated on first need and kept. */
+int katsu_hip_attention_fwd_workspace(const katsu_attention *d, size_t *bytes);
+int katsu_hip_attention_fwd_dev(const katsu_attention *d, const void *q, const void *k,
+                                const void *v, const int32_t *cu_q, const int32_t *cu_k,
+                                const int32_t *k_lens, void *out, float *lse, void *workspace,
+                                size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,8 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libkatsu_hip.so")
 
+F32, BF16 = 0, 1  # katsu_dtype
+
 OK, E_INVALID, E_NODEVICE, E_OOM, E_LAUNCH, E_SCRATCH = 0, 1, 2, 3, 4, 5
 
 # Every symbol include/katsu_hip.h declares.
@@ -29,6 +31,7 @@ EXPORTS = (
     "katsu_hip_fill_f32_dev", "katsu_hip_add_scalar_f32_dev", "katsu_hip_sum_f32_dev",
     "katsu_hip_mean_rows_f32_dev", "katsu_hip_broadcast_rows_f32_dev",
     "katsu_hip_gradcam_f32_dev", "katsu_hip_resize_bilinear_f32_dev",
+    "katsu_hip_attention_fwd_workspace", "katsu_hip_attention_fwd_dev",
 )
 
 
@@ -43,6 +46,16 @@ class ConvGeom(ctypes.Structure):
     """katsu_conv_geom: the fields of the reference's Geometry (conv2d.rs:168-180)."""
     _fields_ = [(f, ctypes.c_uint64) for f in
                 ("n", "c", "h", "w", "k", "r", "s", "stride", "pad", "oh", "ow")]
+
+
+class Attention(ctypes.Structure):
+    """katsu_attention: the shapes and strides of an attention call."""
+    _fields_ = ([(f, ctypes.c_int32) for f in ("dtype", "causal")] +
+                [(f, ctypes.c_uint64) for f in ("heads", "kv_heads", "head_dim", "seqs",
+                                                "tokens_q", "tokens_k")] +
+                [(f, ctypes.c_int64 * 2) for f in ("q_stride", "k_stride", "v_stride",
+                                                   "out_stride")] +
+                [("scale", ctypes.c_float)])
 
 
 _lib = None
@@ -96,6 +109,9 @@ def lib():
         L.katsu_hip_broadcast_rows_f32_dev.argtypes = [vp, sz, sz, fp, vp, fp, vp]
         L.katsu_hip_gradcam_f32_dev.argtypes = [vp, vp, sz, sz, sz, vp, vp]
         L.katsu_hip_resize_bilinear_f32_dev.argtypes = [vp, sz, sz, sz, sz, sz, vp, vp]
+        ap = ctypes.POINTER(Attention)
+        L.katsu_hip_attention_fwd_workspace.argtypes = [ap, ctypes.POINTER(sz)]
+        L.katsu_hip_attention_fwd_dev.argtypes = [ap, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
         for name in EXPORTS:
             if name not in ("katsu_hip_version", "katsu_hip_strerror", "katsu_hip_shutdown",
                             "katsu_hip_noalloc_scratch_bytes",

@@ -1,0 +1,377 @@
+// attention.hpp -- attention over packed sequences, in float32 and bfloat16:
+// what the forward and the two backward kernels share.
+//
+// Sequence s has queries cu_q[s] .. cu_q[s+1] and keys cu_k[s] .. + Lk.  Query i
+// sees key j if j < Lk and, with causal set, j <= i + Lk - Lq (the last query
+// sees the last key).  H query heads share Hkv key heads, G = H/Hkv neighbours
+// each.
+//
+// The matrix instruction computes D[32 x 32] += A[32 x k] B[k x 32]; lane l holds
+// column l % 32 of D, rows 8*(v/4) + 4*(l/32) + v%4 in its 16 registers v, and a
+// 16-byte piece of row (column) l % 32 of A (B), that of the k's of its half l/32.
+// Scores are computed with the keys along the rows, S^T = K Q^T: a lane then
+// holds 16 keys' scores of one query, so a row's maximum and sum stay in the lane
+// and its partner in the other half.  The keys a register holds and the k's that
+// a half of the next product's B operand takes are matched by choosing that
+// product's A rows accordingly, so the probabilities go from one matrix
+// instruction to the next without leaving the registers.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "split3.hpp"
+
+namespace katsu {
+
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+
+// By value: __builtin_bit_cast of a vector's element takes element 0 with this compiler.
+__device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
+__device__ __forceinline__ uint32_t as_bits(float x) { return __builtin_bit_cast(uint32_t, x); }
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+
+// One operand: elements between tokens and between heads; channels are adjacent.
+struct AttnTensor {
+    const void *p;
+    int64_t token, head;
+};
+struct AttnArgs {
+    AttnTensor q, k, v, out, dout, dq, dk, dv;
+    float *lse, *delta;               // [H][Tq]
+    const int32_t *cu_q, *cu_k, *k_lens;
+    int64_t Tq, Tk;
+    int B, H, Hkv, G, D, causal;
+    float scale, scale2;              // of the scores; times log2(e)
+    int slots, splits;                // tiles of all sequences; parts of the key axis
+    float *part, *part_ml;            // the parts' sums [split][token][head][DP]; maxima and totals
+};
+
+// ---- the sequence a tile belongs to -----------------------------------------
+// Tiles of `unit` rows, `mult` rows a token, are numbered so that sequence s
+// begins at cu[s]*mult/unit + s: it has at most that many tiles until the next
+// one begins, so a launch can be sized, and a tile placed, without the lengths
+// being known on the host.
+
+__device__ __forceinline__ int64_t cu_at(const int32_t *cu, int i, int64_t total) {
+    const int64_t c = cu[i];
+    return c < 0 ? 0 : c < total ? c : total;  // whatever the array holds, accesses stay inside
+}
+__device__ __forceinline__ int first_slot(const int32_t *cu, int i, int64_t total, int mult,
+                                          int unit) {
+    return cu ? (int)(cu_at(cu, i, total) * mult / unit) + i : 0;
+}
+
+struct AttnSeq {
+    int s, q0, lq, k0, lk;
+};
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// The last sequence whose first slot is not beyond `slot`; 64 candidates a step.
+__device__ __forceinline__ AttnSeq find_seq(const AttnArgs &a, const int32_t *cu, int64_t total,
+                                            int mult, int unit, int slot, int lane) {
+    int lo = 0, n = a.B;
+    if (cu) {
+        while (n > 1) {
+            const int step = (n + 63) >> 6, i = lane * step;
+            const bool ok = i < n && first_slot(cu, lo + i, total, mult, unit) <= slot;
+            const int at = max(__popcll(__ballot(ok)) - 1, 0) * step;
+            lo += at;
+            n = min(step, n - at);
+        }
+    }
+    AttnSeq r;
+    lo = uni(lo);
+    r.s = lo;
+    const int64_t qa = a.cu_q ? cu_at(a.cu_q, lo, a.Tq) : 0;
+    const int64_t qb = a.cu_q ? cu_at(a.cu_q, lo + 1, a.Tq) : a.Tq;
+    const int64_t ka = a.cu_k ? cu_at(a.cu_k, lo, a.Tk) : 0;
+    const int64_t kb = a.cu_k ? cu_at(a.cu_k, lo + 1, a.Tk) : a.Tk;
+    int64_t lk = kb > ka ? kb - ka : 0;
+    if (a.k_lens) {
+        const int64_t c = a.k_lens[lo];
+        lk = c < 0 ? 0 : c < lk ? c : lk;
+    }
+    r.q0 = uni((int)qa);
+    r.lq = uni((int)(qb > qa ? qb - qa : 0));
+    r.k0 = uni((int)ka);
+    r.lk = uni((int)lk);
+    return r;
+}
+
+// ---- tiles in LDS -------------------------------------------------------------
+// A tile's rows are RB bytes of 16-byte chunks (DP channels, those past D zero).
+// Row r's chunk c lies at place c ^ swz(r): the 32 rows that a fragment reads at
+// one chunk, and the 4 rows by 64 bytes that a transposing read takes, then
+// spread over all banks (measured in a loop: 240 and 200 bytes a cycle and CU,
+// the transposing read 63 with c ^ (r & 15)).
+template <typename T, int DP>
+struct Rows {
+    static constexpr int RB = DP * (int)sizeof(T), CH = RB / 16, E = 16 / (int)sizeof(T);
+    __device__ static __forceinline__ int swz(int r) {
+        return CH == 8 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+    }
+    __device__ static __forceinline__ int at(int r, int c) { return r * RB + ((c ^ swz(r)) << 4); }
+};
+
+typedef __attribute__((address_space(3))) void attn_lds_void;
+constexpr int kAttnOOB = (int)0x80000000;  // beyond any tile: such a load returns zero
+
+// Copies a tile of ROWS rows to LDS, spread over NW waves, of which this is
+// wave w.  DMA: by loads that go to LDS directly, 16 bytes a lane, not waited
+// for here; rows and chunks that do not exist are out of the buffer's range and
+// arrive as zeros.  Else (rows that are not a multiple of 16 bytes, or not
+// aligned so) element by element.
+template <typename T, int DP, int ROWS, int NW, bool DMA>
+struct TileCopy {
+    using R = Rows<T, DP>;
+    static constexpr int N = ROWS * R::RB / 1024 / NW;
+    static_assert(N >= 1, "tile too small for the waves");
+    int off[DMA ? N : 1];
+    int64_t stride;  // bytes between rows
+    int row_bytes, D, lane, w;
+
+    __device__ __forceinline__ void init(int wave, int ln, int64_t token_stride, int d) {
+        stride = token_stride * (int64_t)sizeof(T);
+        D = d;
+        row_bytes = d * (int)sizeof(T);
+        lane = ln;
+        w = wave;
+        if constexpr (DMA) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int b = (w * N + i) * 1024 + lane * 16;
+                const int r = b / R::RB, c = (b % R::RB / 16) ^ R::swz(r);
+                off[i] = c * 16 < row_bytes ? r * (int)stride + c * 16 : kAttnOOB;
+            }
+        }
+    }
+    // The tile whose first row is at base; `valid` rows exist (any number).
+    __device__ __forceinline__ void load(const char *base, int valid, char *lds) const {
+        valid = min(valid, ROWS);
+        if constexpr (DMA) {
+            const int bytes = valid > 0 ? (valid - 1) * (int)stride + row_bytes : 0;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<char *>(base), (short)0, bytes, 0x00020000);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    rs, (attn_lds_void *)(lds + (w * N + i) * 1024), 16, off[i], 0, 0, 0);
+        } else {
+            for (int c = w * 64 + lane; c < ROWS * R::CH; c += NW * 64) {
+                const int r = c / R::CH, ch = c % R::CH;
+                T e[R::E];
+#pragma unroll
+                for (int i = 0; i < R::E; ++i) {
+                    const int d = ch * R::E + i;
+                    e[i] = r < valid && d < D
+                               ? reinterpret_cast<const T *>(base + r * stride)[d]
+                               : (T)0.f;
+                }
+                uintx4 u;
+                __builtin_memcpy(&u, e, 16);
+                *reinterpret_cast<uintx4 *>(lds + R::at(r, ch)) = u;
+            }
+        }
+    }
+};
+__device__ __forceinline__ void attn_wait_dma() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// ---- fragments and products ---------------------------------------------------
+
+// A fragment: 16 bytes a lane, k's [E*h, E*h + E) of the 2E that it covers.
+template <typename T>
+__device__ __forceinline__ floatx16 attn_mma(uintx4 a, uintx4 b, floatx16 c) {
+    if constexpr (sizeof(T) == 2) {
+        return mfma32(a, b, c);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            c = __builtin_amdgcn_mfma_f32_32x32x2f32(as_float(a[e]), as_float(b[e]), c, 0, 0, 0);
+        return c;
+    }
+}
+// Rows r0 + l%32 of a tile at step's chunks: the operand of a product over channels.
+template <typename T, int DP>
+__device__ __forceinline__ uintx4 row_frag(const char *lds, int r0, int step, int l31, int h) {
+    return *reinterpret_cast<const uintx4 *>(lds + r0 * Rows<T, DP>::RB +
+                                             Rows<T, DP>::at(l31, 2 * step + h));
+}
+// Channel 32*db + l%32 of a tile's rows: the operand of a product over rows, for
+// the rows whose values registers E*f .. E*f + E - 1 of a 32 x 32 result hold.
+template <typename T, int DP>
+__device__ __forceinline__ uintx4 col_frag(const char *lds, int r0, int f, int db, int lane) {
+    using R = Rows<T, DP>;
+    const int h = lane >> 5;
+    uintx4 u;
+    if constexpr (sizeof(T) == 2) {
+        // In each 16 lanes, lanes 4e .. 4e+3 read 16 channels of row e; lane i
+        // receives channel i of the four rows.
+        const int c = db * 4 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int r = 8 * p + 4 * h + ((lane & 15) >> 2);
+            const int b = (r0 + 16 * f) * R::RB + R::at(r, c) + (lane & 1) * 8;
+            const uintx2 t = __builtin_bit_cast(
+                uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) shortx4 *)(lds + b)));
+            u[2 * p] = t[0];
+            u[2 * p + 1] = t[1];
+        }
+    } else {
+        const int d = db * 32 + (lane & 31);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            u[e] = *reinterpret_cast<const uint32_t *>(lds + r0 * R::RB +
+                                                       R::at(8 * f + 4 * h + e, d >> 2) + (d & 3) * 4);
+    }
+    return u;
+}
+// Registers E*f .. of a result as the operand of a product over its rows.  In
+// bfloat16 they are rounded here: 2^-9 of each probability, no more than its
+// row's rounding of the output; the row's total is summed before.
+template <typename T>
+__device__ __forceinline__ uintx4 reg_frag(const floatx16 &x, int f) {
+    uintx4 u;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            u[i] = __builtin_bit_cast(
+                uint32_t, __builtin_convertvector(floatx2{x[8 * f + 2 * i], x[8 * f + 2 * i + 1]},
+                                                  bf16x2));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = as_bits(x[4 * f + i]);
+    }
+    return u;
+}
+// The row of a result that register v of half h holds.
+__device__ __forceinline__ int reg_row(int v, int h) { return 8 * (v >> 2) + 4 * h + (v & 3); }
+
+// x of the lower half's lane and of the upper one's, in both.
+__device__ __forceinline__ void halves(float x, float &lo, float &hi) {
+    const uint32_t u = as_bits(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    lo = as_float(r[0]);
+    hi = as_float(r[1]);
+}
+__device__ __forceinline__ float half_max(float x) {
+    float a, b;
+    halves(x, a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float half_sum(float x) {
+    float a, b;
+    halves(x, a, b);
+    return a + b;
+}
+
+// Row r's fragments of a [token][head][D] operand, straight from memory: NS of
+// them, zero where the row or the channels do not exist.
+template <typename T, int DP, bool VEC>
+__device__ __forceinline__ void load_row(const AttnTensor &t, int64_t token, int head, bool valid,
+                                         int D, int h, uintx4 *f) {
+    using R = Rows<T, DP>;
+    const T *p = reinterpret_cast<const T *>(t.p) + token * t.token + head * t.head;
+#pragma unroll
+    for (int s = 0; s < R::CH / 2; ++s) {
+        const int d = (2 * s + h) * R::E;
+        uintx4 u = {0, 0, 0, 0};
+        if constexpr (VEC) {
+            if (valid && d < D) u = *reinterpret_cast<const uintx4 *>(p + d);
+        } else {
+            T e[R::E];
+#pragma unroll
+            for (int i = 0; i < R::E; ++i) e[i] = valid && d + i < D ? p[d + i] : (T)0.f;
+            __builtin_memcpy(&u, e, 16);
+        }
+        f[s] = u;
+    }
+}
+// Channels 32*db + 8g + 4h .. + 3 (registers 4g .. 4g+3 of x) of a row, times `by`.
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_row(T *p, const floatx16 &x, float by, int db, int h, int D) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int d = db * 32 + 8 * g + 4 * h;
+        T e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = (T)(x[4 * g + i] * by);
+        if constexpr (VEC) {
+            if (d < D) __builtin_memcpy(__builtin_assume_aligned(p + d, 4 * sizeof(T)), e, sizeof e);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (d + i < D) p[d + i] = e[i];
+        }
+    }
+}
+
+// ---- non-finite values in masked places -----------------------------------------
+// A masked key's probability is zero, but a matrix product still multiplies it by
+// what the masked row holds, and 0 * Inf is NaN.  In the tiles that the mask cuts,
+// the kernels look for such values first; where there are any, their products run
+// on the tile with those values cleared, and what the unmasked ones among them
+// contribute is added apart.
+
+template <typename T>
+__device__ __forceinline__ bool nonfinite_bits(uint32_t x) {
+    return (x & (sizeof(T) == 2 ? 0x7f80u : 0x7f800000u)) ==
+           (sizeof(T) == 2 ? 0x7f80u : 0x7f800000u);
+}
+// Whether rows [r0, r0 + ROWS) of a tile hold one; the same answer in every lane.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ bool tile_nonfinite(const char *lds, int lane) {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    us2 m2 = {0, 0};
+    uint32_t m1 = 0;
+#pragma unroll 4
+    for (int i = 0; i < ROWS * DP * (int)sizeof(T) / 1024; ++i) {
+        const uintx4 u = *reinterpret_cast<const uintx4 *>(lds + i * 1024 + lane * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (sizeof(T) == 2)
+                m2 = __builtin_elementwise_max(m2, __builtin_bit_cast(us2, u[e] & 0x7f807f80u));
+            else
+                m1 = max(m1, u[e] & 0x7f800000u);
+        }
+    }
+    const bool bad = sizeof(T) == 2 ? (m2[0] == 0x7f80 || m2[1] == 0x7f80) : m1 == 0x7f800000u;
+    return __ballot(bad) != 0;
+}
+template <typename T>
+__device__ __forceinline__ uintx4 clear_nonfinite(uintx4 u) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t lo = nonfinite_bits<T>(u[e]) ? 0 : u[e] & 0xffffu;
+            const uint32_t hi = nonfinite_bits<T>(u[e] >> 16) ? 0 : u[e] & 0xffff0000u;
+            u[e] = lo | hi;
+        } else {
+            u[e] = nonfinite_bits<T>(u[e]) ? 0 : u[e];
+        }
+    }
+    return u;
+}
+// Adds to acc (channels 32*db + reg_row, this lane's column) the non-finite values of the
+// tile's rows [lo, hi).  A probability is above zero, so it changes neither an infinity's
+// sign nor a NaN.
+template <typename T, int DP>
+__device__ __forceinline__ void add_nonfinite(const char *lds, int lo, int hi, int db, int h,
+                                              floatx16 &acc) {
+    using R = Rows<T, DP>;
+    for (int r = lo; r < hi; ++r) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            const int d = db * 32 + reg_row(v, h);
+            const T x = *reinterpret_cast<const T *>(lds + R::at(r, d / R::E) +
+                                                     d % R::E * (int)sizeof(T));
+            const float y = (float)x;
+            acc[v] += y - y == 0.f ? 0.f : y;
+        }
+    }
+}
+
+}  // namespace katsu

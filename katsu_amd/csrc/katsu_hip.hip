@@ -24,6 +24,7 @@
 #include "elementwise.hpp"
 #include "gemm.hpp"
 #include "hostcopy.hpp"
+#include "lm.hpp"
 #include "pointwise.hpp"
 #include "smallc.hpp"
 #include "split.hpp"
@@ -89,15 +90,15 @@ int map_hip(hipError_t e) {
 
 // Library-owned scratch of the device entry points: the dW split partials
 // (when the caller passes no workspace), the GEMM's split-K partials, the
-// sum's chunk partials and Grad-CAM's channel weights, one buffer per
-// purpose.  The buffers are shared by every stream, so a call may run under
+// sum's chunk partials, Grad-CAM's channel weights and the language-model
+// operators' partials, one buffer per purpose.  The buffers are shared by every stream, so a call may run under
 // HIP graph capture on another stream than the eager call that sized them
 // (no allocation is then needed); calls that overlap in time on two streams
 // race on them.  A buffer that must grow is replaced, and the old block is
 // kept until katsu_hip_shutdown, because a graph captured earlier still
 // addresses it.  Its own mutex: the host-pointer entry points hold State::mu
 // while their device calls take scratch.
-enum class ScratchKind : int { Dw = 0, Gemm = 1, Sum = 2, Cam = 3, Count = 4 };
+enum class ScratchKind : int { Dw = 0, Gemm = 1, Sum = 2, Cam = 3, Lm = 4, Count = 5 };
 
 struct ScratchPool {
     std::mutex mu;
@@ -161,6 +162,14 @@ int ws_take(const WsSource &src, size_t need, hipStream_t st, float **out) {
     }
     if (!src.lib) return KATSU_E_INVALID;
     return scratch_get(ScratchKind::Dw, st, need, out);
+}
+
+// The caller's workspace if it passes one (checked), else the library's.
+int lm_scratch(void *ws, size_t bytes, size_t need, hipStream_t st, void **out) {
+    *out = ws;
+    if (need == 0) return KATSU_OK;
+    if (ws) return bytes < need ? KATSU_E_INVALID : KATSU_OK;
+    return scratch_get(ScratchKind::Lm, st, need, (float **)out);
 }
 
 int init_locked(State &s) {
@@ -3232,6 +3241,27 @@ int katsu_hip_resize_bilinear_f32_dev(const float *src, size_t n, size_t ih, siz
     resize_bilinear<<<ew_blocks(total), 256, 0, (hipStream_t)stream>>>(
         src, (int64_t)n, (int)ih, (int)iw, (int)oh, (int)ow, dst);
     return launch_status();
+}
+
+int katsu_hip_attention_fwd_workspace(const katsu_attention *d, size_t *bytes) {
+    if (!d || !bytes || !attention_ok(*d)) return KATSU_E_INVALID;
+    *bytes = attention_fwd_bytes(*d);
+    return KATSU_OK;
+}
+
+int katsu_hip_attention_fwd_dev(const katsu_attention *d, const void *q, const void *k,
+                                const void *v, const int32_t *cu_q, const int32_t *cu_k,
+                                const int32_t *k_lens, void *out, float *lse, void *workspace,
+                                size_t workspace_bytes, void *stream) {
+    if (!d || !attention_ok(*d)) return KATSU_E_INVALID;
+    if (d->seqs == 0 || d->tokens_q == 0) return KATSU_OK;
+    if (!q || !out || (d->tokens_k > 0 && (!k || !v))) return KATSU_E_INVALID;
+    if ((!cu_q || !cu_k) && (d->seqs != 1 || cu_q || cu_k)) return KATSU_E_INVALID;
+    hipStream_t st = (hipStream_t)stream;
+    void *ws = nullptr;
+    const int rc = lm_scratch(workspace, workspace_bytes, attention_fwd_bytes(*d), st, &ws);
+    if (rc) return rc;
+    return attention_fwd(*d, q, k, v, cu_q, cu_k, k_lens, out, lse, ws, st);
 }
 
 }  // extern "C"

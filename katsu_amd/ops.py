@@ -9,7 +9,7 @@ import ctypes
 
 import torch
 
-from ._abi import check, geometry, lib
+from ._abi import BF16, F32, Attention, check, geometry, lib
 
 
 # A small call's time is its host side (a pass of four 48 x 56 products and
@@ -238,3 +238,81 @@ def resize_bilinear(maps, size):
     check(lib().katsu_hip_resize_bilinear_f32_dev(_p(maps), n, h, w, oh, ow, _p(out),
                                                    _stream()), "resize_bilinear")
     return out
+
+
+# ---- language-model operators (float32 or bfloat16 device tensors) ----
+
+_DTYPE = {torch.float32: F32, torch.bfloat16: BF16}
+
+
+def _dev_lm(first, *ts):
+    """float32 or bfloat16 device tensors, all of the first one's type and device."""
+    if not first.is_cuda or first.dtype not in _DTYPE:
+        raise ValueError("float32 or bfloat16 device tensors expected")
+    for t in ts:
+        if t is not None and (t.dtype is not first.dtype or t.device != first.device):
+            raise ValueError("all operands must have one type and device")
+
+
+def _heads(t, what):
+    """A [tokens, heads, channels] tensor's strides; its channels must be adjacent."""
+    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+        raise ValueError(f"{what} must be [tokens, heads, channels] with adjacent channels")
+    return t.stride(0), t.stride(1)
+
+
+def _int32(t, n, dev, what):
+    if t is not None and not (t.dtype is torch.int32 and t.device == dev and t.dim() == 1
+                              and t.is_contiguous() and t.numel() == n):
+        raise ValueError(f"{what} must be {n} contiguous int32 values on the operands' device")
+
+
+def _attention(q, k, v, out, cu_q, cu_k, k_lens, causal, scale):
+    _dev_lm(q, k, v, out)
+    strides = [_heads(t, w) for t, w in ((q, "q"), (k, "k"), (v, "v"), (out, "out"))]
+    tq, heads, dim = q.shape
+    if k.shape != v.shape or k.shape[2] != dim or out.shape != q.shape:
+        raise ValueError("k and v must have one shape, q's channels, and out q's shape")
+    if k.shape[1] == 0 or heads % k.shape[1]:
+        raise ValueError("query heads must be a multiple of key heads")
+    if (cu_q is None) != (cu_k is None):
+        raise ValueError("cu_q and cu_k go together")
+    seqs = 1 if cu_q is None else cu_q.numel() - 1
+    if seqs < 0:
+        raise ValueError("cu_q holds the sequences' starts and the end")
+    _int32(cu_q, seqs + 1, q.device, "cu_q")
+    _int32(cu_k, seqs + 1, q.device, "cu_k")
+    _int32(k_lens, seqs, q.device, "k_lens")
+    return Attention(_DTYPE[q.dtype], bool(causal), heads, k.shape[1], dim, seqs, tq, k.shape[0],
+                     *strides, dim ** -0.5 if scale is None else scale)
+
+
+def attention_workspace_bytes(q, k, v, cu_q=None, cu_k=None, k_lens=None, causal=True, scale=None):
+    """Scratch that an attention call of these operands needs."""
+    d = _attention(q, k, v, q, cu_q, cu_k, k_lens, causal, scale)
+    nbytes = ctypes.c_size_t(0)
+    check(lib().katsu_hip_attention_fwd_workspace(ctypes.byref(d), ctypes.byref(nbytes)),
+          "attention_workspace")
+    return nbytes.value
+
+
+def _workspace(t):
+    return (0, 0) if t is None else (t.data_ptr(), t.numel() * t.element_size())
+
+
+def attention(q, k, v, cu_q=None, cu_k=None, k_lens=None, causal=True, scale=None, out=None,
+              workspace=None):
+    """(out, lse) of softmax(scale q k^T) v over packed sequences: q [Tq, H, D], k and v
+    [Tk, Hkv, D], channels adjacent, any token and head strides; cu_q and cu_k the int32 starts
+    of the sequences' queries and keys and the end (None: one sequence); k_lens how many of each
+    sequence's keys are in use (a cache's slots).  causal: the last query sees every key, each
+    earlier one a key less.  A query that sees no key gives 0 and lse -inf.  scale: 1/sqrt(D)
+    if None.  lse [H, Tq], float32, is what attention_backward takes.  `workspace`: an optional
+    device tensor of attention_workspace_bytes(); without it the library's own buffer is used."""
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out is None else out
+    d = _attention(q, k, v, out, cu_q, cu_k, k_lens, causal, scale)
+    lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32)
+    check(lib().katsu_hip_attention_fwd_dev(ctypes.byref(d), _p(q), _p(k), _p(v), _p(cu_q),
+                                            _p(cu_k), _p(k_lens), _p(out), _p(lse),
+                                            *_workspace(workspace), _stream()), "attention")
+    return out, lse
