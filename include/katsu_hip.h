@@ -287,9 +287,10 @@ typedef enum katsu_dtype { KATSU_F32 = 0, KATSU_BF16 = 1 } katsu_dtype;
  * Strides are in elements, [0] between tokens and [1] between heads; channels
  * are adjacent.  Sequence s has queries cu_q[s] .. cu_q[s+1] and keys cu_k[s]
  * .. cu_k[s+1], or with k_lens the first k_lens[s] of those (slots of a cache);
- * cu_q and cu_k are device arrays of seqs + 1 int32 that start at 0 and do not
- * fall, both NULL for one sequence of all tokens; values outside the tensors
- * are taken as their ends.
+ * cu_q and cu_k are device arrays of seqs + 1 int32 from 0 to the number of
+ * tokens that do not fall, both NULL for one sequence of all tokens; values
+ * outside the tensors are taken as their ends; what outputs hold for tokens
+ * that no sequence holds is undefined.
  *   S = scale q.k over the visible keys, P = softmax(S), out = P v,
  *   lse[head][token] = log sum exp S       (natural logarithm)
  * With causal set query i of Lq sees key j of Lk if j <= i + Lk - Lq: the last
@@ -314,6 +315,23 @@ int katsu_hip_attention_fwd_dev(const katsu_attention *d, const void *q, const v
                                 const void *v, const int32_t *cu_q, const int32_t *cu_k,
                                 const int32_t *k_lens, void *out, float *lse, void *workspace,
                                 size_t workspace_bytes, void *stream);
+
+/* The backward pass, from dout, the gradient of out, and the forward call's
+ * operands, out and lse (same cu_q and cu_k; no k_lens):
+ *   P = exp(S - lse),  dS = P (dout v^T - dout.out),
+ *   dq = scale dS k,  dk = scale dS^T q and dv = P^T dout summed over the
+ * query heads of a key head.  Outputs are overwritten.  A query that sees no
+ * key gives no gradient, a key that no query sees gets zeros.
+ * Workspace as above, of katsu_hip_attention_bwd_workspace bytes. */
+typedef struct katsu_attention_grads {
+    int64_t dout_stride[2], dq_stride[2], dk_stride[2], dv_stride[2];
+} katsu_attention_grads;
+int katsu_hip_attention_bwd_workspace(const katsu_attention *d, size_t *bytes);
+int katsu_hip_attention_bwd_dev(const katsu_attention *d, const katsu_attention_grads *g,
+                                const void *dout, const void *q, const void *k, const void *v,
+                                const void *out, const float *lse, const int32_t *cu_q,
+                                const int32_t *cu_k, void *dq, void *dk, void *dv,
+                                void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

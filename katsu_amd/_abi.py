@@ -32,6 +32,7 @@ EXPORTS = (
     "katsu_hip_mean_rows_f32_dev", "katsu_hip_broadcast_rows_f32_dev",
     "katsu_hip_gradcam_f32_dev", "katsu_hip_resize_bilinear_f32_dev",
     "katsu_hip_attention_fwd_workspace", "katsu_hip_attention_fwd_dev",
+    "katsu_hip_attention_bwd_workspace", "katsu_hip_attention_bwd_dev",
 )
 
 
@@ -56,6 +57,12 @@ class Attention(ctypes.Structure):
                 [(f, ctypes.c_int64 * 2) for f in ("q_stride", "k_stride", "v_stride",
                                                    "out_stride")] +
                 [("scale", ctypes.c_float)])
+
+
+class AttentionGrads(ctypes.Structure):
+    """katsu_attention_grads: the strides of a backward call's gradients."""
+    _fields_ = [(f, ctypes.c_int64 * 2) for f in ("dout_stride", "dq_stride", "dk_stride",
+                                                  "dv_stride")]
 
 
 _lib = None
@@ -112,6 +119,9 @@ def lib():
         ap = ctypes.POINTER(Attention)
         L.katsu_hip_attention_fwd_workspace.argtypes = [ap, ctypes.POINTER(sz)]
         L.katsu_hip_attention_fwd_dev.argtypes = [ap, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        L.katsu_hip_attention_bwd_workspace.argtypes = [ap, ctypes.POINTER(sz)]
+        L.katsu_hip_attention_bwd_dev.argtypes = [ap, ctypes.POINTER(AttentionGrads), vp, vp, vp,
+                                                  vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
         for name in EXPORTS:
             if name not in ("katsu_hip_version", "katsu_hip_strerror", "katsu_hip_shutdown",
                             "katsu_hip_noalloc_scratch_bytes",

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "attention_bwd.hpp"
 #include "attention_fwd.hpp"
 #include "lm.hpp"
 
@@ -28,6 +29,10 @@ int lds_optin(size_t bytes) {
     static const hipError_t e = hipFuncSetAttribute(
         (const void *)Kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     return status_of(e);
+}
+
+bool strides_ok(const int64_t (&s)[2]) {
+    return s[0] >= 0 && s[1] >= 0 && s[0] <= kI32Max && s[1] <= (int64_t)1 << 40;
 }
 
 int elem(const katsu_attention &d) { return d.dtype == KATSU_F32 ? 4 : 2; }
@@ -115,7 +120,62 @@ int launch_fwd(const AttnArgs &a, int dp, bool vec, bool few, hipStream_t st) {
     return vec ? launch_fwd<T, 128, true>(a, few, st) : launch_fwd<T, 128, false>(a, few, st);
 }
 
+// The backward call's shape.  Blocks of one query head each, and their sums joined
+// afterwards, unless the key heads alone give the card enough to do.
+struct BwdPlan {
+    int dq_slots, dkv_slots;
+    bool each;
+};
+BwdPlan bwd_plan(const katsu_attention &d) {
+    BwdPlan p;
+    const int64_t group = (int64_t)(d.heads / d.kv_heads), B = (int64_t)d.seqs;
+    p.dq_slots = (int)((int64_t)d.tokens_q * group / 128 + B);
+    p.dkv_slots = (int)((int64_t)d.tokens_k / 128 + B);
+    p.each = group > 1 && (int64_t)p.dkv_slots * (int64_t)d.kv_heads < 4 * kCUs;
+    return p;
+}
+size_t stat_floats(const katsu_attention &d) {
+    return (2 * d.tokens_q * d.heads + 63) / 64 * 64;
+}
+
+template <auto Kern>
+int launch(int64_t blocks, int lds, const AttnArgs &a, hipStream_t st) {
+    const int rc = lds_optin<Kern>(lds);
+    if (rc != KATSU_OK || blocks == 0) return rc;
+    Kern<<<dim3((unsigned)blocks), dim3(256), lds, st>>>(a);
+    return status_of(hipGetLastError());
+}
+template <typename T, int DP, bool VEC>
+int launch_bwd(AttnArgs a, const BwdPlan &p, hipStream_t st) {
+    // float32 rows of 128 channels: tiles of half the rows, one wave a SIMD for dk and dv.
+    constexpr bool wide = DP * sizeof(T) == 512;
+    constexpr int BN = wide ? 32 : 64, QT = wide ? 32 : 64;
+    a.slots = p.dq_slots;
+    const int64_t dq_blocks = a.Tq > 0 ? (int64_t)p.dq_slots * a.Hkv : 0;
+    int rc = launch<attention_dq_kernel<T, DP, BN, VEC, 2>>(dq_blocks, AttnDq<T, DP, BN, VEC>::kLds,
+                                                            a, st);
+    if (rc != KATSU_OK || a.Tk == 0) return rc;
+    a.slots = p.dkv_slots;
+    rc = launch<attention_dkv_kernel<T, DP, QT, VEC, wide ? 1 : 2>>(
+        (int64_t)p.dkv_slots * (p.each ? a.H : a.Hkv), AttnDkv<T, DP, QT, VEC>::kLds, a, st);
+    if (rc != KATSU_OK || !p.each) return rc;
+    const int64_t blocks = cdiv(a.Tk * a.Hkv * (DP / 4), 256);
+    attention_group_kernel<T, VEC><<<dim3((unsigned)blocks, 2), 256, 0, st>>>(a, DP);
+    return status_of(hipGetLastError());
+}
+template <typename T>
+int launch_bwd(const AttnArgs &a, const BwdPlan &p, int dp, bool vec, hipStream_t st) {
+    if (dp == 64)
+        return vec ? launch_bwd<T, 64, true>(a, p, st) : launch_bwd<T, 64, false>(a, p, st);
+    return vec ? launch_bwd<T, 128, true>(a, p, st) : launch_bwd<T, 128, false>(a, p, st);
+}
+
 }  // namespace
+
+bool attention_grads_ok(const katsu_attention_grads &g) {
+    return strides_ok(g.dout_stride) && strides_ok(g.dq_stride) && strides_ok(g.dk_stride) &&
+           strides_ok(g.dv_stride);
+}
 
 bool attention_ok(const katsu_attention &d) {
     if (d.dtype != KATSU_F32 && d.dtype != KATSU_BF16) return false;
@@ -126,12 +186,14 @@ bool attention_ok(const katsu_attention &d) {
     if (d.tokens_q > (uint64_t)kI32Max || d.tokens_k > (uint64_t)kI32Max ||
         d.seqs > (uint64_t)kI32Max)
         return false;
-    for (const int64_t *s : {d.q_stride, d.k_stride, d.v_stride, d.out_stride})
-        if (s[0] < 0 || s[1] < 0 || s[0] > kI32Max || s[1] > (kI32Max << 20)) return false;
+    if (!strides_ok(d.q_stride) || !strides_ok(d.k_stride) || !strides_ok(d.v_stride) ||
+        !strides_ok(d.out_stride))
+        return false;
     // Tiles and blocks are counted in 32 bits.
-    const uint64_t rows = d.tokens_q * (d.heads / d.kv_heads);
+    const uint64_t group = d.heads / d.kv_heads;
+    const uint64_t rows = std::max(d.tokens_q * group, d.tokens_k * group);
     return (rows / 32 + d.seqs) * d.kv_heads < (uint64_t)kI32Max / 4 &&
-           d.tokens_q * d.heads < ((uint64_t)1 << 40);
+           std::max(d.tokens_q, d.tokens_k) * d.heads < (uint64_t)kI32Max * 4;
 }
 
 size_t attention_fwd_bytes(const katsu_attention &d) {
@@ -165,6 +227,40 @@ int attention_fwd(const katsu_attention &d, const void *q, const void *k, const 
     else
         attention_join_kernel<__bf16><<<blocks, 256, 0, st>>>(a, dp);
     return status_of(hipGetLastError());
+}
+
+size_t attention_bwd_bytes(const katsu_attention &d) {
+    if (d.seqs == 0) return 0;
+    const size_t part = bwd_plan(d).each ? 2 * d.heads * d.tokens_k * (size_t)dp_of(d) : 0;
+    return (stat_floats(d) + part) * sizeof(float);
+}
+
+int attention_bwd(const katsu_attention &d, const katsu_attention_grads &g, const void *dout,
+                  const void *q, const void *k, const void *v, const void *out, const float *lse,
+                  const int32_t *cu_q, const int32_t *cu_k, void *dq, void *dk, void *dv, void *ws,
+                  hipStream_t st) {
+    const BwdPlan p = bwd_plan(d);
+    AttnArgs a = base_args(d, cu_q, cu_k, nullptr);
+    bool vec = true;
+    auto take = [&](AttnTensor &t, const void *ptr, const int64_t (&stride)[2]) {
+        t = tensor(ptr, stride);
+        vec = vec && vec_ok(d, ptr, stride);
+    };
+    take(a.q, q, d.q_stride);
+    take(a.k, k, d.k_stride);
+    take(a.v, v, d.v_stride);
+    take(a.out, out, d.out_stride);
+    take(a.dout, dout, g.dout_stride);
+    take(a.dq, dq, g.dq_stride);
+    take(a.dk, dk, g.dk_stride);
+    take(a.dv, dv, g.dv_stride);
+    a.lse = const_cast<float *>(lse);
+    a.lse2 = (float *)ws;
+    a.delta = a.lse2 + d.tokens_q * d.heads;
+    if (p.each) a.part = a.lse2 + stat_floats(d);
+    const int dp = dp_of(d);
+    return d.dtype == KATSU_F32 ? launch_bwd<float>(a, p, dp, vec, st)
+                                : launch_bwd<__bf16>(a, p, dp, vec, st);
 }
 
 }  // namespace katsu

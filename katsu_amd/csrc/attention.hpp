@@ -40,7 +40,8 @@ struct AttnTensor {
 };
 struct AttnArgs {
     AttnTensor q, k, v, out, dout, dq, dk, dv;
-    float *lse, *delta;               // [H][Tq]
+    float *lse;                       // [H][Tq]
+    float *lse2, *delta;              // backward, [H][Tq]: lse times log2(e), do.o
     const int32_t *cu_q, *cu_k, *k_lens;
     int64_t Tq, Tk;
     int B, H, Hkv, G, D, causal;
@@ -356,9 +357,9 @@ __device__ __forceinline__ uintx4 clear_nonfinite(uintx4 u) {
     return u;
 }
 // Adds to acc (channels 32*db + reg_row, this lane's column) the non-finite values of the
-// tile's rows [lo, hi).  A probability is above zero, so it changes neither an infinity's
-// sign nor a NaN.
-template <typename T, int DP>
+// tile's rows [lo, hi), each times a factor: a probability, which is above zero and changes
+// neither an infinity's sign nor a NaN, or (NANS) one that is zero or NaN itself.
+template <typename T, int DP, bool NANS>
 __device__ __forceinline__ void add_nonfinite(const char *lds, int lo, int hi, int db, int h,
                                               floatx16 &acc) {
     using R = Rows<T, DP>;
@@ -369,7 +370,7 @@ __device__ __forceinline__ void add_nonfinite(const char *lds, int lo, int hi, i
             const T x = *reinterpret_cast<const T *>(lds + R::at(r, d / R::E) +
                                                      d % R::E * (int)sizeof(T));
             const float y = (float)x;
-            acc[v] += y - y == 0.f ? 0.f : y;
+            acc[v] += y - y == 0.f ? 0.f : NANS ? y - y : y;
         }
     }
 }

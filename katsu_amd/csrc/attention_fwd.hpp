@@ -92,7 +92,7 @@ struct AttnFwd {
                 }
             const int seen = min(max(jmax + 1 - key0, 0), BN);
 #pragma unroll
-            for (int d = 0; d < ND; ++d) add_nonfinite<T, DP>(vl, 0, seen, d, h, o[d]);
+            for (int d = 0; d < ND; ++d) add_nonfinite<T, DP, false>(vl, 0, seen, d, h, o[d]);
         } else {
 #pragma unroll
             for (int b = 0; b < NB; ++b)

@@ -3264,4 +3264,27 @@ int katsu_hip_attention_fwd_dev(const katsu_attention *d, const void *q, const v
     return attention_fwd(*d, q, k, v, cu_q, cu_k, k_lens, out, lse, ws, st);
 }
 
+int katsu_hip_attention_bwd_workspace(const katsu_attention *d, size_t *bytes) {
+    if (!d || !bytes || !attention_ok(*d)) return KATSU_E_INVALID;
+    *bytes = attention_bwd_bytes(*d);
+    return KATSU_OK;
+}
+
+int katsu_hip_attention_bwd_dev(const katsu_attention *d, const katsu_attention_grads *g,
+                                const void *dout, const void *q, const void *k, const void *v,
+                                const void *out, const float *lse, const int32_t *cu_q,
+                                const int32_t *cu_k, void *dq, void *dk, void *dv,
+                                void *workspace, size_t workspace_bytes, void *stream) {
+    if (!d || !g || !attention_ok(*d) || !attention_grads_ok(*g)) return KATSU_E_INVALID;
+    if (d->seqs == 0 || (d->tokens_q == 0 && d->tokens_k == 0)) return KATSU_OK;
+    if (d->tokens_q > 0 && (!dout || !q || !out || !lse || !dq)) return KATSU_E_INVALID;
+    if (d->tokens_k > 0 && (!k || !v || !dk || !dv)) return KATSU_E_INVALID;
+    if ((!cu_q || !cu_k) && (d->seqs != 1 || cu_q || cu_k)) return KATSU_E_INVALID;
+    hipStream_t st = (hipStream_t)stream;
+    void *ws = nullptr;
+    const int rc = lm_scratch(workspace, workspace_bytes, attention_bwd_bytes(*d), st, &ws);
+    if (rc) return rc;
+    return attention_bwd(*d, *g, dout, q, k, v, out, lse, cu_q, cu_k, dq, dk, dv, ws, st);
+}
+
 }  // extern "C"

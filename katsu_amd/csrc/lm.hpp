@@ -18,4 +18,12 @@ int attention_fwd(const katsu_attention &d, const void *q, const void *k, const 
                   const int32_t *cu_q, const int32_t *cu_k, const int32_t *k_lens, void *out,
                   float *lse, void *ws, hipStream_t st);
 
+
+bool attention_grads_ok(const katsu_attention_grads &g);
+size_t attention_bwd_bytes(const katsu_attention &d);
+int attention_bwd(const katsu_attention &d, const katsu_attention_grads &g, const void *dout,
+                  const void *q, const void *k, const void *v, const void *out, const float *lse,
+                  const int32_t *cu_q, const int32_t *cu_k, void *dq, void *dk, void *dv, void *ws,
+                  hipStream_t st);
+
 }  // namespace katsu

@@ -9,7 +9,7 @@ import ctypes
 
 import torch
 
-from ._abi import BF16, F32, Attention, check, geometry, lib
+from ._abi import BF16, F32, Attention, AttentionGrads, check, geometry, lib
 
 
 # A small call's time is its host side (a pass of four 48 x 56 products and
@@ -287,12 +287,13 @@ def _attention(q, k, v, out, cu_q, cu_k, k_lens, causal, scale):
                      *strides, dim ** -0.5 if scale is None else scale)
 
 
-def attention_workspace_bytes(q, k, v, cu_q=None, cu_k=None, k_lens=None, causal=True, scale=None):
-    """Scratch that an attention call of these operands needs."""
-    d = _attention(q, k, v, q, cu_q, cu_k, k_lens, causal, scale)
+def attention_workspace_bytes(q, k, v, cu_q=None, cu_k=None, backward=False):
+    """Scratch that attention (or attention_backward) needs for these operands."""
+    d = _attention(q, k, v, q, cu_q, cu_k, None, True, None)
     nbytes = ctypes.c_size_t(0)
-    check(lib().katsu_hip_attention_fwd_workspace(ctypes.byref(d), ctypes.byref(nbytes)),
-          "attention_workspace")
+    fn = (lib().katsu_hip_attention_bwd_workspace if backward
+          else lib().katsu_hip_attention_fwd_workspace)
+    check(fn(ctypes.byref(d), ctypes.byref(nbytes)), "attention_workspace")
     return nbytes.value
 
 
@@ -316,3 +317,27 @@ def attention(q, k, v, cu_q=None, cu_k=None, k_lens=None, causal=True, scale=Non
                                             _p(cu_k), _p(k_lens), _p(out), _p(lse),
                                             *_workspace(workspace), _stream()), "attention")
     return out, lse
+
+
+def attention_backward(dout, q, k, v, out, lse, cu_q=None, cu_k=None, causal=True, scale=None,
+                       dq=None, dk=None, dv=None, workspace=None):
+    """(dq, dk, dv) of attention's out with gradient dout, from the forward call's operands and
+    its out and lse.  Any token and head strides; `workspace` of
+    attention_workspace_bytes(..., backward=True)."""
+    d = _attention(q, k, v, out, cu_q, cu_k, None, causal, scale)
+    dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if dq is None else dq
+    dk = torch.empty(k.shape, device=q.device, dtype=q.dtype) if dk is None else dk
+    dv = torch.empty(v.shape, device=q.device, dtype=q.dtype) if dv is None else dv
+    _dev_lm(q, dout, dq, dk, dv)
+    if dout.shape != q.shape or dq.shape != q.shape or dk.shape != k.shape or dv.shape != k.shape:
+        raise ValueError("gradients must have their operands' shapes")
+    if (lse.dtype is not torch.float32 or lse.device != q.device or not lse.is_contiguous()
+            or lse.shape != (q.shape[1], q.shape[0])):
+        raise ValueError("lse must be what attention returned")
+    g = AttentionGrads(*(_heads(t, w) for t, w in ((dout, "dout"), (dq, "dq"), (dk, "dk"),
+                                                   (dv, "dv"))))
+    check(lib().katsu_hip_attention_bwd_dev(ctypes.byref(d), ctypes.byref(g), _p(dout), _p(q),
+                                            _p(k), _p(v), _p(out), _p(lse), _p(cu_q), _p(cu_k),
+                                            _p(dq), _p(dk), _p(dv), *_workspace(workspace),
+                                            _stream()), "attention_backward")
+    return dq, dk, dv
