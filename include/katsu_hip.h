@@ -333,6 +333,72 @@ int katsu_hip_attention_bwd_dev(const katsu_attention *d, const katsu_attention_
                                 const int32_t *cu_k, void *dq, void *dk, void *dv,
                                 void *workspace, size_t workspace_bytes, void *stream);
 
+/* Rotary positions.  Of each head's head_dim channels the first rotary_dim (R,
+ * even) turn in pairs, (a, b) -> (a cos - b sin, a sin + b cos): pair i is
+ * channels i and i + R/2, or 2i and 2i + 1 with interleaved set; the rest is
+ * copied.  Token t turns by row positions[t] of table ([length][R] float32:
+ * R/2 cosines, then R/2 sines; rows outside it are taken as its ends), or by
+ * row t if positions is NULL.  inverse turns back: the gradient of a turn.
+ * q and k ([tokens][heads][head_dim], strides in elements as above) go in one
+ * launch; k may be NULL with k_heads 0.  Outputs may be the inputs. */
+typedef struct katsu_rotary {
+    int32_t dtype, interleaved, inverse;
+    uint64_t tokens, heads, k_heads, head_dim, rotary_dim, length;
+    int64_t q_stride[2], k_stride[2], q_out_stride[2], k_out_stride[2];
+} katsu_rotary;
+int katsu_hip_rotary_dev(const katsu_rotary *d, const void *q, const void *k, const float *table,
+                         const int32_t *positions, void *q_out, void *k_out, void *stream);
+
+/* Fills such a table: position p's pair i turns by p f_i, computed in float64,
+ * f_i = base^(-2i/R).  factor >= 1 scales for a context longer than the model
+ * was trained on, length = factor times that: f_i / factor, or with
+ * by_wavelength f_i kept where it turns 32 times or more within the original
+ * length, divided where it turns once or less, mixed linearly between, and
+ * cosines and sines times 0.1 ln(factor) + 1 (the scheme published as YaRN). */
+int katsu_hip_rotary_table_f32_dev(float *table, size_t length, size_t rotary_dim, double base,
+                                   double factor, int by_wavelength, void *stream);
+
+/* Between two blocks of a model, rows x cols, cols <= 16384, all tensors of
+ * one type and contiguous:
+ *   n = o / sqrt(mean(o^2) + eps) * w_post     (n = o if w_post is NULL)
+ *   y = x + alpha * gate * n
+ *   h = y / sqrt(mean(y^2) + eps) * w_pre      (no h if w_pre is NULL)
+ * with a gate of cols values, of rows x cols, or none (gate_rows).  h is of y
+ * before its rounding.  stats [2][rows] (or NULL) receives 1/sqrt(..) of o
+ * and y, 0 for a norm that is not taken: what the backward call reads.
+ * y may be x, h may be o. */
+typedef enum katsu_gate { KATSU_GATE_NONE = 0, KATSU_GATE_CHANNEL = 1,
+                          KATSU_GATE_ELEMENT = 2 } katsu_gate;
+typedef struct katsu_block_norm {
+    int32_t dtype, gate_rows;  /* katsu_dtype, katsu_gate */
+    uint64_t rows, cols;
+    float alpha, eps;          /* eps: of the forward call only */
+} katsu_block_norm;
+int katsu_hip_block_norm_dev(const katsu_block_norm *d, const void *x, const void *o,
+                             const void *gate, const void *w_post, const void *w_pre, void *y,
+                             void *h, float *stats, void *stream);
+
+/* Its gradient: from dy (gradient that reaches y otherwise) and dh, with the
+ * forward call's y, o and stats: dx (all of y's gradient), d_o, dgate (shaped
+ * as gate), dw_post and dw_pre; outputs are overwritten.  Sums over rows are
+ * in float32, in a fixed order, through a workspace as above. */
+int katsu_hip_block_norm_bwd_workspace(const katsu_block_norm *d, size_t *bytes);
+int katsu_hip_block_norm_bwd_dev(const katsu_block_norm *d, const void *dy, const void *dh,
+                                 const void *y, const void *o, const float *stats,
+                                 const void *gate, const void *w_post, const void *w_pre,
+                                 void *dx, void *d_o, void *dgate, void *dw_post, void *dw_pre,
+                                 void *workspace, size_t workspace_bytes, void *stream);
+
+/* norm[0] = sqrt(sum over the n tensors of all squares), squares summed in
+ * float64; out = in * min(1, max_norm / (norm + 1e-6)), tensor by tensor (out
+ * may be in).  dtypes, in, out and counts are host arrays; the tensors are
+ * contiguous device memory of katsu_dtype dtypes[i].  A norm that is NaN
+ * makes all outputs NaN, an infinite one zero (NaN where in is infinite).
+ * max_norm must not be negative.  Partial sums are in library scratch. */
+int katsu_hip_clip_grad_norm_dev(const int32_t *dtypes, const void *const *in, void *const *out,
+                                 const size_t *counts, size_t n, float max_norm, float *norm,
+                                 void *stream);
+
 #ifdef __cplusplus
 }
 #endif

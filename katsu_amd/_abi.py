@@ -33,6 +33,9 @@ EXPORTS = (
     "katsu_hip_gradcam_f32_dev", "katsu_hip_resize_bilinear_f32_dev",
     "katsu_hip_attention_fwd_workspace", "katsu_hip_attention_fwd_dev",
     "katsu_hip_attention_bwd_workspace", "katsu_hip_attention_bwd_dev",
+    "katsu_hip_rotary_dev", "katsu_hip_rotary_table_f32_dev",
+    "katsu_hip_block_norm_dev", "katsu_hip_block_norm_bwd_workspace",
+    "katsu_hip_block_norm_bwd_dev", "katsu_hip_clip_grad_norm_dev",
 )
 
 
@@ -63,6 +66,22 @@ class AttentionGrads(ctypes.Structure):
     """katsu_attention_grads: the strides of a backward call's gradients."""
     _fields_ = [(f, ctypes.c_int64 * 2) for f in ("dout_stride", "dq_stride", "dk_stride",
                                                   "dv_stride")]
+
+
+class Rotary(ctypes.Structure):
+    """katsu_rotary: the shapes and strides of a rotary call."""
+    _fields_ = ([(f, ctypes.c_int32) for f in ("dtype", "interleaved", "inverse")] +
+                [(f, ctypes.c_uint64) for f in ("tokens", "heads", "k_heads", "head_dim",
+                                                "rotary_dim", "length")] +
+                [(f, ctypes.c_int64 * 2) for f in ("q_stride", "k_stride", "q_out_stride",
+                                                   "k_out_stride")])
+
+
+class BlockNorm(ctypes.Structure):
+    """katsu_block_norm: the shape and scalars of a block norm call."""
+    _fields_ = ([(f, ctypes.c_int32) for f in ("dtype", "gate_rows")] +
+                [(f, ctypes.c_uint64) for f in ("rows", "cols")] +
+                [(f, ctypes.c_float) for f in ("alpha", "eps")])
 
 
 _lib = None
@@ -122,6 +141,14 @@ def lib():
         L.katsu_hip_attention_bwd_workspace.argtypes = [ap, ctypes.POINTER(sz)]
         L.katsu_hip_attention_bwd_dev.argtypes = [ap, ctypes.POINTER(AttentionGrads), vp, vp, vp,
                                                   vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        db = ctypes.c_double
+        L.katsu_hip_rotary_dev.argtypes = [ctypes.POINTER(Rotary), vp, vp, vp, vp, vp, vp, vp]
+        L.katsu_hip_rotary_table_f32_dev.argtypes = [vp, sz, sz, db, db, i, vp]
+        bp = ctypes.POINTER(BlockNorm)
+        L.katsu_hip_block_norm_dev.argtypes = [bp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+        L.katsu_hip_block_norm_bwd_workspace.argtypes = [bp, ctypes.POINTER(sz)]
+        L.katsu_hip_block_norm_bwd_dev.argtypes = [bp] + [vp] * 14 + [sz, vp]
+        L.katsu_hip_clip_grad_norm_dev.argtypes = [vp, vp, vp, vp, sz, fp, vp, vp]
         for name in EXPORTS:
             if name not in ("katsu_hip_version", "katsu_hip_strerror", "katsu_hip_shutdown",
                             "katsu_hip_noalloc_scratch_bytes",

@@ -30,7 +30,8 @@ HIP_FLAGS = [
     "-ffp-contract=fast-honor-pragmas", "-Wall", "-Wno-unused-function",
 ]
 
-SOURCES = [os.path.join(CSRC, f) for f in ("katsu_hip.hip", "split.hip", "attention.hip")]
+SOURCES = [os.path.join(CSRC, f) for f in ("katsu_hip.hip", "split.hip", "attention.hip",
+                                             "lmblock.hip")]
 FRONTEND_SRC = os.path.join(HERE, "cpp", "katsu.cpp")
 FRONTEND_LIB = os.path.join(LIB_DIR, "libkatsu.so")
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wextra"]

@@ -1,0 +1,102 @@
+// gradclip.hpp -- the global norm of many gradient tensors, and clipping by it:
+//   norm = sqrt(sum of all squares),  out = g min(1, max_norm / (norm + 1e-6))
+//
+// Two launches for up to kClipTensors tensors, whose addresses travel as kernel
+// arguments: the first sums squares into one float64 part a block, the second has every
+// block add the parts in the same order and scale its share.  Squares are summed in
+// float64: they cannot overflow, and HBM is the bound either way (one fused
+// multiply-add for 2 or 4 bytes read).
+#pragma once
+
+#include "lmvec.hpp"
+
+namespace katsu {
+
+constexpr int kClipTensors = 96;
+constexpr int kClipBlocks = 1024, kClipChunk = 16384;  // blocks at most; values a step
+
+struct ClipTable {
+    const void *in[kClipTensors];
+    void *out[kClipTensors];
+    int64_t count[kClipTensors];
+    uint32_t first[kClipTensors + 1];  // chunks before each tensor
+    uint8_t half[kClipTensors];        // bfloat16
+    int n;
+};
+
+// Calls f(tensor, first value, values) for this block's chunks.
+template <class F>
+__device__ __forceinline__ void each_chunk(const ClipTable &t, F f) {
+    const uint32_t total = t.first[t.n];
+    int k = 0;
+    for (uint32_t c = blockIdx.x; c < total; c += gridDim.x) {
+        while (t.first[k + 1] <= c) ++k;
+        const int64_t at = (int64_t)(c - t.first[k]) * kClipChunk;
+        const int64_t left = t.count[k] - at;
+        f(k, at, left < kClipChunk ? (int)left : kClipChunk);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ double squares(const T *p, int n) {
+    constexpr int E = Piece<T>::E;
+    double s = 0.;
+#pragma unroll 4
+    for (int i = threadIdx.x * E; i < n; i += 256 * E) {
+        float x[E];
+        load_piece(p, i, n, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s = __builtin_fma((double)x[e], (double)x[e], s);
+    }
+    return s;
+}
+template <typename T>
+__device__ __forceinline__ void scale_chunk(const T *p, T *q, int n, float by) {
+    constexpr int E = Piece<T>::E;
+#pragma unroll 4
+    for (int i = threadIdx.x * E; i < n; i += 256 * E) {
+        float x[E];
+        load_piece(p, i, n, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] *= by;
+        store_piece(q, i, n, x);
+    }
+}
+__device__ __forceinline__ double block_sum_f64(double v, double *part) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return ((part[0] + part[1]) + part[2]) + part[3];
+}
+
+__global__ void __launch_bounds__(256) clip_squares_kernel(const ClipTable t, double *parts) {
+    __shared__ double part[4];
+    double s = 0.;
+    each_chunk(t, [&](int k, int64_t at, int n) {
+        s += t.half[k] ? squares((const __bf16 *)t.in[k] + at, n)
+                       : squares((const float *)t.in[k] + at, n);
+    });
+    s = block_sum_f64(s, part);
+    if (threadIdx.x == 0) parts[blockIdx.x] = s;
+}
+
+__global__ void __launch_bounds__(256) clip_scale_kernel(const ClipTable t, const double *parts,
+                                                         int nparts, float max_norm, float *norm) {
+    __shared__ double part[4];
+    double s = 0.;
+    for (int i = threadIdx.x; i < nparts; i += 256) s += parts[i];
+    s = sqrt(block_sum_f64(s, part));
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)s;
+    const double q = (double)max_norm / (s + 1e-6);
+    const float by = q >= 1. ? 1.f : (float)q;  // a norm that is NaN gives NaN
+    each_chunk(t, [&](int k, int64_t at, int n) {
+        if (by == 1.f && t.in[k] == t.out[k]) return;  // in place, nothing to do
+        if (t.half[k])
+            scale_chunk((const __bf16 *)t.in[k] + at, (__bf16 *)t.out[k] + at, n, by);
+        else
+            scale_chunk((const float *)t.in[k] + at, (float *)t.out[k] + at, n, by);
+    });
+}
+
+}  // namespace katsu

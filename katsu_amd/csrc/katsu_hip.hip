@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 #include <map>
@@ -3285,6 +3286,79 @@ int katsu_hip_attention_bwd_dev(const katsu_attention *d, const katsu_attention_
     const int rc = lm_scratch(workspace, workspace_bytes, attention_bwd_bytes(*d), st, &ws);
     if (rc) return rc;
     return attention_bwd(*d, *g, dout, q, k, v, out, lse, cu_q, cu_k, dq, dk, dv, ws, st);
+}
+
+int katsu_hip_rotary_dev(const katsu_rotary *d, const void *q, const void *k, const float *table,
+                         const int32_t *positions, void *q_out, void *k_out, void *stream) {
+    if (!d || !rotary_ok(*d)) return KATSU_E_INVALID;
+    if (d->tokens == 0 || d->heads + d->k_heads == 0) return KATSU_OK;
+    if (!table || (d->heads && (!q || !q_out)) || (d->k_heads && (!k || !k_out)))
+        return KATSU_E_INVALID;
+    return rotary(*d, q, k, table, positions, q_out, k_out, (hipStream_t)stream);
+}
+
+int katsu_hip_rotary_table_f32_dev(float *table, size_t length, size_t rotary_dim, double base,
+                                   double factor, int by_wavelength, void *stream) {
+    if (rotary_dim == 0 || rotary_dim % 2 != 0 || rotary_dim > 65536 ||
+        length > (size_t)kI32Max || !(base > 0.) || !std::isfinite(base) || !(factor >= 1.) ||
+        !std::isfinite(factor))
+        return KATSU_E_INVALID;
+    if (length == 0) return KATSU_OK;
+    if (!table) return KATSU_E_INVALID;
+    return rotary_table(table, (int64_t)length, (int)rotary_dim, base, factor, by_wavelength,
+                        (hipStream_t)stream);
+}
+
+int katsu_hip_block_norm_dev(const katsu_block_norm *d, const void *x, const void *o,
+                             const void *gate, const void *w_post, const void *w_pre, void *y,
+                             void *h, float *stats, void *stream) {
+    if (!d || !block_norm_ok(*d)) return KATSU_E_INVALID;
+    if (d->rows == 0) return KATSU_OK;
+    if (!x || !o || !y || (d->gate_rows && !gate) || (w_pre && !h)) return KATSU_E_INVALID;
+    return block_norm(*d, x, o, gate, w_post, w_pre, y, h, stats, (hipStream_t)stream);
+}
+
+int katsu_hip_block_norm_bwd_workspace(const katsu_block_norm *d, size_t *bytes) {
+    if (!d || !bytes || !block_norm_ok(*d)) return KATSU_E_INVALID;
+    *bytes = block_norm_bwd_bytes(*d);
+    return KATSU_OK;
+}
+
+int katsu_hip_block_norm_bwd_dev(const katsu_block_norm *d, const void *dy, const void *dh,
+                                 const void *y, const void *o, const float *stats,
+                                 const void *gate, const void *w_post, const void *w_pre,
+                                 void *dx, void *d_o, void *dgate, void *dw_post, void *dw_pre,
+                                 void *workspace, size_t workspace_bytes, void *stream) {
+    if (!d || !block_norm_ok(*d)) return KATSU_E_INVALID;
+    if ((d->gate_rows == KATSU_GATE_CHANNEL && !dgate) || (w_post && !dw_post) ||
+        (w_pre && !dw_pre))
+        return KATSU_E_INVALID;
+    if (d->rows > 0 && (!dy || !o || !stats || !dx || !d_o || (d->gate_rows && (!gate || !dgate)) ||
+                        (w_pre && (!dh || !y))))
+        return KATSU_E_INVALID;
+    hipStream_t st = (hipStream_t)stream;
+    void *ws = nullptr;
+    const int rc = lm_scratch(workspace, workspace_bytes, block_norm_bwd_bytes(*d), st, &ws);
+    if (rc) return rc;
+    return block_norm_bwd(*d, dy, dh, y, o, stats, gate, w_post, w_pre, dx, d_o, dgate, dw_post,
+                          dw_pre, ws, st);
+}
+
+int katsu_hip_clip_grad_norm_dev(const int32_t *dtypes, const void *const *in, void *const *out,
+                                 const size_t *counts, size_t n, float max_norm, float *norm,
+                                 void *stream) {
+    if (!norm || !(max_norm >= 0.f) || (n > 0 && (!dtypes || !in || !out || !counts)))
+        return KATSU_E_INVALID;
+    for (size_t i = 0; i < n; ++i) {
+        if (dtypes[i] != KATSU_F32 && dtypes[i] != KATSU_BF16) return KATSU_E_INVALID;
+        if (counts[i] > ((size_t)1 << 38) || (counts[i] > 0 && (!in[i] || !out[i])))
+            return KATSU_E_INVALID;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    void *ws = nullptr;
+    const int rc = lm_scratch(nullptr, 0, clip_bytes(n), st, &ws);
+    if (rc) return rc;
+    return clip_grad_norm(dtypes, in, out, counts, n, max_norm, norm, ws, st);
 }
 
 }  // extern "C"

@@ -9,7 +9,8 @@ import ctypes
 
 import torch
 
-from ._abi import BF16, F32, Attention, AttentionGrads, check, geometry, lib
+from ._abi import (BF16, F32, Attention, AttentionGrads, BlockNorm, Rotary, check, geometry,
+                   lib)
 
 
 # A small call's time is its host side (a pass of four 48 x 56 products and
@@ -341,3 +342,135 @@ def attention_backward(dout, q, k, v, out, lse, cu_q=None, cu_k=None, causal=Tru
                                             _p(dq), _p(dk), _p(dv), *_workspace(workspace),
                                             _stream()), "attention_backward")
     return dq, dk, dv
+
+
+def rotary_table(length, dim, base=10000.0, factor=1.0, by_wavelength=True, device="cuda"):
+    """[length, dim] float32: the cosines and sines of `length` positions' angles for `dim`
+    turning channels, computed in float64.  factor > 1: for a context of `length` tokens, factor
+    times what the model was trained on: all frequencies divided by it, or (by_wavelength) only
+    those that turn seldom within the original length."""
+    t = torch.empty((length, dim), device=device, dtype=torch.float32)
+    with torch.cuda.device(t.device):
+        check(lib().katsu_hip_rotary_table_f32_dev(_p(t), length, dim, base, factor,
+                                                   int(by_wavelength and factor != 1.0),
+                                                   _stream()), "rotary_table")
+    return t
+
+
+def rotary(q, k, table, positions=None, interleaved=False, inverse=False, out_q=None, out_k=None):
+    """(q', k'): the first table.shape[1] channels of each head of q and k [tokens, heads,
+    channels] (k may be None) turned by their tokens' positions, rows of `table` (int32; None:
+    0, 1, ..).  Pairs are channels i and i + R/2, or neighbours with interleaved.  inverse turns
+    back: the gradient of a turn.  The outputs may be the inputs."""
+    out_q = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out_q is None else out_q
+    if k is not None and out_k is None:
+        out_k = torch.empty(k.shape, device=q.device, dtype=q.dtype)
+    _dev_lm(q, k, out_q, out_k)
+    tokens, heads, dim = q.shape if q.dim() == 3 else (0, 0, 0)
+    strides = [(0, 0) if t is None else _heads(t, w)
+               for t, w in ((q, "q"), (k, "k"), (out_q, "out_q"), (out_k, "out_k"))]
+    if out_q.shape != q.shape or (k is not None and (
+            out_k.shape != k.shape or k.shape[0] != tokens or k.shape[2] != dim)):
+        raise ValueError("q and k must have the same tokens and channels, outputs their shapes")
+    if (table.dim() != 2 or table.dtype is not torch.float32 or table.device != q.device
+            or not table.is_contiguous()):
+        raise ValueError("table must be contiguous float32 [length, channels that turn]")
+    _int32(positions, tokens, q.device, "positions")
+    d = Rotary(_DTYPE[q.dtype], bool(interleaved), bool(inverse), tokens, heads,
+               0 if k is None else k.shape[1], dim, table.shape[1], table.shape[0], *strides)
+    check(lib().katsu_hip_rotary_dev(ctypes.byref(d), _p(q), _p(k), _p(table), _p(positions),
+                                     _p(out_q), _p(out_k), _stream()), "rotary")
+    return out_q, out_k
+
+
+def _block_norm(rows, gate, w_post, w_pre, alpha, eps):
+    """Checks the operands of a block norm against its first [rows, cols] one."""
+    first = rows[0]
+    _dev_lm(*rows, gate, w_post, w_pre)
+    if first.dim() != 2:
+        raise ValueError("operands must be [rows, cols]")
+    cols = first.shape[1]
+    for t in rows:
+        if t is not None and (t.shape != first.shape or not t.is_contiguous()):
+            raise ValueError("operands must be contiguous and of one shape")
+    for t in (w_post, w_pre):
+        if t is not None and (t.shape != (cols,) or not t.is_contiguous()):
+            raise ValueError("weights must be contiguous [cols]")
+    if gate is not None and (gate.shape not in (first.shape, (cols,)) or not gate.is_contiguous()):
+        raise ValueError("gate must be contiguous, [cols] or [rows, cols]")
+    return BlockNorm(_DTYPE[first.dtype], 0 if gate is None else gate.dim(), *first.shape,
+                     alpha, eps)
+
+
+def block_norm(x, o, gate=None, w_post=None, w_pre=None, alpha=1.0, eps=1e-6, out_y=None,
+               out_h=None):
+    """(y, h, stats) between two blocks: o, a block's output, is divided by its rows' root mean
+    square and multiplied by w_post (if given), by the gate ([cols] or [rows, cols], if given)
+    and alpha, and added to the residual x: y.  h is y divided by its root mean square, times
+    w_pre (None without w_pre): the next block's input.  stats [2, rows] float32 is for
+    block_norm_backward.  out_y may be x, out_h may be o."""
+    d = _block_norm((x, o, out_y, out_h), gate, w_post, w_pre, alpha, eps)
+    y = torch.empty_like(x) if out_y is None else out_y
+    h = None if w_pre is None else torch.empty_like(x) if out_h is None else out_h
+    stats = torch.empty((2, x.shape[0]), device=x.device, dtype=torch.float32)
+    check(lib().katsu_hip_block_norm_dev(ctypes.byref(d), _p(x), _p(o), _p(gate), _p(w_post),
+                                         _p(w_pre), _p(y), _p(h), _p(stats), _stream()),
+          "block_norm")
+    return y, h, stats
+
+
+def block_norm_backward(dy, dh, y, o, stats, gate=None, w_post=None, w_pre=None, alpha=1.0,
+                        workspace=None):
+    """(dx, do, dgate, dw_post, dw_pre) from dy, the gradient that reaches y otherwise, and dh,
+    with block_norm's y and stats; None for operands that were not given (dh and y may then be
+    None without w_pre)."""
+    if w_pre is not None and (dh is None or y is None):
+        raise ValueError("dh and y are needed with w_pre")
+    d = _block_norm((dy, dh, y, o), gate, w_post, w_pre, alpha, 0.0)
+    if (stats.dtype is not torch.float32 or stats.device != dy.device
+            or stats.shape != (2, dy.shape[0]) or not stats.is_contiguous()):
+        raise ValueError("stats must be what block_norm returned")
+    dx, do = torch.empty_like(dy), torch.empty_like(dy)
+    dgate, dw_post, dw_pre = (None if t is None else torch.empty_like(t)
+                              for t in (gate, w_post, w_pre))
+    check(lib().katsu_hip_block_norm_bwd_dev(
+        ctypes.byref(d), _p(dy), _p(dh), _p(y), _p(o), _p(stats), _p(gate), _p(w_post), _p(w_pre),
+        _p(dx), _p(do), _p(dgate), _p(dw_post), _p(dw_pre), *_workspace(workspace), _stream()),
+        "block_norm_backward")
+    return dx, do, dgate, dw_post, dw_pre
+
+
+def block_norm_workspace_bytes(dy):
+    """Scratch that block_norm_backward needs for gradients of this shape."""
+    d = _block_norm((dy,), None, None, None, 1.0, 0.0)
+    nbytes = ctypes.c_size_t(0)
+    check(lib().katsu_hip_block_norm_bwd_workspace(ctypes.byref(d), ctypes.byref(nbytes)),
+          "block_norm_workspace")
+    return nbytes.value
+
+
+def clip_grad_norm(grads, max_norm, out=None):
+    """The root of the sum of all squares of `grads` (a list of contiguous device tensors of
+    either type), as a float32 device tensor [1]; each gradient times
+    min(1, max_norm / (norm + 1e-6)) is written to `out` (in place if None)."""
+    out = grads if out is None else out
+    n = len(grads)
+    if n == 0:
+        raise ValueError("no gradients")
+    dev = grads[0].device
+    if len(out) != n:
+        raise ValueError("one output for each gradient")
+    for g, o in zip(grads, out):
+        if (g.dtype not in _DTYPE or g.device != dev or not g.is_cuda or not g.is_contiguous()
+                or (o is not g and (o.dtype is not g.dtype or o.device != dev
+                                    or o.shape != g.shape or not o.is_contiguous()))):
+            raise ValueError("gradients and outputs must be contiguous float32 or bfloat16 "
+                             "tensors on one device, each output of its gradient's shape and type")
+    norm = torch.empty(1, device=dev, dtype=torch.float32)
+    ptrs, counts = ctypes.c_void_p * n, ctypes.c_size_t * n
+    check(lib().katsu_hip_clip_grad_norm_dev(
+        (ctypes.c_int32 * n)(*[_DTYPE[g.dtype] for g in grads]),
+        ptrs(*[g.data_ptr() for g in grads]), ptrs(*[o.data_ptr() for o in out]),
+        counts(*[g.numel() for g in grads]), n, max_norm, norm.data_ptr(), _stream()),
+        "clip_grad_norm")
+    return norm
