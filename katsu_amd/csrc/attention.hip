@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "attention_bwd.hpp"
 #include "attention_fwd.hpp"
@@ -69,7 +70,8 @@ AttnTensor tensor(const void *p, const int64_t (&stride)[2]) {
     return {p, stride[0], stride[1]};
 }
 
-int dp_of(const katsu_attention &d) { return d.head_dim <= 64 ? 64 : 128; }
+// Channels of a row in LDS and in the parts.
+int width_of(const katsu_attention &d) { return d.head_dim <= 64 ? 64 : 128; }
 
 // The forward call's shape: tiles of 32 rows whose waves share the keys, or of 128.
 struct FwdPlan {
@@ -91,37 +93,58 @@ FwdPlan fwd_plan(const katsu_attention &d) {
 }
 size_t part_floats(const katsu_attention &d, const FwdPlan &p) {
     if (p.splits <= 1) return 0;
-    return (size_t)p.splits * d.tokens_q * d.heads * (size_t)(dp_of(d) + 2);
+    return (size_t)p.splits * d.tokens_q * d.heads * (size_t)(width_of(d) + 2);
 }
 
-template <typename T, int DP, int WM, int WK, int BN, bool VEC, int OCC>
-int launch_fwd(const AttnArgs &a, hipStream_t st) {
-    using K = AttnFwd<T, DP, WM, WK, BN, VEC>;
-    constexpr auto kern = attention_fwd_kernel<T, DP, WM, WK, BN, VEC, OCC>;
-    static_assert(K::kLds <= 160 * 1024, "LDS");
-    const int rc = lds_optin<kern>(K::kLds);
-    if (rc != KATSU_OK) return rc;
-    const int64_t blocks = (int64_t)a.slots * a.Hkv * a.splits;
-    kern<<<dim3((unsigned)blocks), dim3(K::THREADS), K::kLds, st>>>(a);
+// Calls f with the operand type, the blocks of 32 channels and whether rows are whole
+// 16-byte chunks, as constants (rows that are not take the next of 64 or 128 channels).
+template <class F>
+int by_shape(const katsu_attention &d, bool vec, F f) {
+    const int nd = (int)cdiv((int64_t)d.head_dim, 32);
+    auto with = [&](auto t) {
+        auto with_nd = [&](auto n) {
+            constexpr int ND = decltype(n)::value;
+            if constexpr (ND % 2 == 0)
+                if (!vec) return f(t, n, std::false_type());
+            return f(t, n, std::true_type());
+        };
+        const int m = vec ? nd : (nd + 1) / 2 * 2;
+        if (m == 1) return with_nd(std::integral_constant<int, 1>());
+        if (m == 2) return with_nd(std::integral_constant<int, 2>());
+        if (m == 3) return with_nd(std::integral_constant<int, 3>());
+        return with_nd(std::integral_constant<int, 4>());
+    };
+    return d.dtype == KATSU_F32 ? with(float()) : with(__bf16());
+}
+
+template <auto Kern>
+int launch(int64_t blocks, int threads, int lds, const AttnArgs &a, hipStream_t st) {
+    const int rc = lds_optin<Kern>(lds);
+    if (rc != KATSU_OK || blocks == 0) return rc;
+    Kern<<<dim3((unsigned)blocks), dim3(threads), lds, st>>>(a);
     return status_of(hipGetLastError());
 }
-template <typename T, int DP, bool VEC>
+
+template <typename T, int ND, int WM, int WK, int BN, bool VEC, int OCC>
+int launch_fwd(const AttnArgs &a, hipStream_t st) {
+    using K = AttnFwd<T, ND, WM, WK, BN, VEC>;
+    static_assert(K::kLds <= 160 * 1024, "LDS");
+    return launch<attention_fwd_kernel<T, ND, WM, WK, BN, VEC, OCC>>(
+        (int64_t)a.slots * a.Hkv * a.splits, K::THREADS, K::kLds, a, st);
+}
+template <typename T, int ND, bool VEC>
 int launch_fwd(const AttnArgs &a, bool few, hipStream_t st) {
     // float32 rows of 128 channels: half the keys a tile, so that two blocks share a CU;
     // with few rows two waves instead of four.
-    constexpr bool wide = DP * sizeof(T) == 512;
-    if (few) return launch_fwd<T, DP, 1, wide ? 2 : 4, 32, VEC, 1>(a, st);
-    return launch_fwd<T, DP, 4, 1, wide ? 32 : 64, VEC, 2>(a, st);
-}
-template <typename T>
-int launch_fwd(const AttnArgs &a, int dp, bool vec, bool few, hipStream_t st) {
-    if (dp == 64)
-        return vec ? launch_fwd<T, 64, true>(a, few, st) : launch_fwd<T, 64, false>(a, few, st);
-    return vec ? launch_fwd<T, 128, true>(a, few, st) : launch_fwd<T, 128, false>(a, few, st);
+    constexpr bool wide = Rows<T, ND>::RB == 512;
+    if (few) return launch_fwd<T, ND, 1, wide ? 2 : 4, 32, VEC, 1>(a, st);
+    return launch_fwd<T, ND, 4, 1, wide ? 32 : 64, VEC, 2>(a, st);
 }
 
 // The backward call's shape.  Blocks of one query head each, and their sums joined
-// afterwards, unless the key heads alone give the card enough to do.
+// afterwards, unless the key heads alone give the card enough to do; in float32 always,
+// as a sum over all of a group's rows in one accumulator loses too much (8 heads of 1900
+// rows: dk 1.1e-6 off, 5.8e-7 with a head at a time).
 struct BwdPlan {
     int dq_slots, dkv_slots;
     bool each;
@@ -131,43 +154,32 @@ BwdPlan bwd_plan(const katsu_attention &d) {
     const int64_t group = (int64_t)(d.heads / d.kv_heads), B = (int64_t)d.seqs;
     p.dq_slots = (int)((int64_t)d.tokens_q * group / 128 + B);
     p.dkv_slots = (int)((int64_t)d.tokens_k / 128 + B);
-    p.each = group > 1 && (int64_t)p.dkv_slots * (int64_t)d.kv_heads < 4 * kCUs;
+    p.each = group > 1 && (d.dtype == KATSU_F32 ||
+                           (int64_t)p.dkv_slots * (int64_t)d.kv_heads < 4 * kCUs);
     return p;
 }
 size_t stat_floats(const katsu_attention &d) {
     return (2 * d.tokens_q * d.heads + 63) / 64 * 64;
 }
 
-template <auto Kern>
-int launch(int64_t blocks, int lds, const AttnArgs &a, hipStream_t st) {
-    const int rc = lds_optin<Kern>(lds);
-    if (rc != KATSU_OK || blocks == 0) return rc;
-    Kern<<<dim3((unsigned)blocks), dim3(256), lds, st>>>(a);
-    return status_of(hipGetLastError());
-}
-template <typename T, int DP, bool VEC>
+template <typename T, int ND, bool VEC>
 int launch_bwd(AttnArgs a, const BwdPlan &p, hipStream_t st) {
-    // float32 rows of 128 channels: tiles of half the rows, one wave a SIMD for dk and dv.
-    constexpr bool wide = DP * sizeof(T) == 512;
-    constexpr int BN = wide ? 32 : 64, QT = wide ? 32 : 64;
+    // Rows of 512 bytes: tiles of half the rows, one wave a SIMD for dk and dv.
+    constexpr int RB = Rows<T, ND>::RB;
+    constexpr int BN = RB == 512 ? 32 : 64, QT = ND > 2 ? 32 : 64;
+    using Dq = AttnDq<T, ND, BN, VEC>;
+    using Dkv = AttnDkv<T, ND, QT, VEC>;
     a.slots = p.dq_slots;
-    const int64_t dq_blocks = a.Tq > 0 ? (int64_t)p.dq_slots * a.Hkv : 0;
-    int rc = launch<attention_dq_kernel<T, DP, BN, VEC, 2>>(dq_blocks, AttnDq<T, DP, BN, VEC>::kLds,
-                                                            a, st);
+    int rc = launch<attention_dq_kernel<T, ND, BN, VEC, 2>>(
+        a.Tq > 0 ? (int64_t)p.dq_slots * a.Hkv : 0, Dq::THREADS, Dq::kLds, a, st);
     if (rc != KATSU_OK || a.Tk == 0) return rc;
     a.slots = p.dkv_slots;
-    rc = launch<attention_dkv_kernel<T, DP, QT, VEC, wide ? 1 : 2>>(
-        (int64_t)p.dkv_slots * (p.each ? a.H : a.Hkv), AttnDkv<T, DP, QT, VEC>::kLds, a, st);
+    rc = launch<attention_dkv_kernel<T, ND, QT, VEC, RB == 512 ? 1 : 2>>(
+        (int64_t)p.dkv_slots * (p.each ? a.H : a.Hkv), Dkv::THREADS, Dkv::kLds, a, st);
     if (rc != KATSU_OK || !p.each) return rc;
-    const int64_t blocks = cdiv(a.Tk * a.Hkv * (DP / 4), 256);
-    attention_group_kernel<T, VEC><<<dim3((unsigned)blocks, 2), 256, 0, st>>>(a, DP);
+    const int64_t blocks = cdiv(a.Tk * a.Hkv * (Dkv::W / 4), 256);
+    attention_group_kernel<T, VEC><<<dim3((unsigned)blocks, 2), 256, 0, st>>>(a, Dkv::W);
     return status_of(hipGetLastError());
-}
-template <typename T>
-int launch_bwd(const AttnArgs &a, const BwdPlan &p, int dp, bool vec, hipStream_t st) {
-    if (dp == 64)
-        return vec ? launch_bwd<T, 64, true>(a, p, st) : launch_bwd<T, 64, false>(a, p, st);
-    return vec ? launch_bwd<T, 128, true>(a, p, st) : launch_bwd<T, 128, false>(a, p, st);
 }
 
 }  // namespace
@@ -213,25 +225,26 @@ int attention_fwd(const katsu_attention &d, const void *q, const void *k, const 
     a.lse = lse;
     a.slots = p.slots;
     a.splits = p.splits;
-    const int dp = dp_of(d);
+    const int width = width_of(d);
     a.part = (float *)ws;
-    a.part_ml = a.part + (size_t)a.splits * d.tokens_q * d.heads * dp;
+    a.part_ml = a.part + (size_t)a.splits * d.tokens_q * d.heads * width;
     const bool vec = vec_ok(d, q, d.q_stride) && vec_ok(d, k, d.k_stride) &&
                      vec_ok(d, v, d.v_stride) && vec_ok(d, out, d.out_stride);
-    const int rc = d.dtype == KATSU_F32 ? launch_fwd<float>(a, dp, vec, p.few, st)
-                                        : launch_fwd<__bf16>(a, dp, vec, p.few, st);
+    const int rc = by_shape(d, vec, [&](auto t, auto nd, auto v) {
+        return launch_fwd<decltype(t), decltype(nd)::value, decltype(v)::value>(a, p.few, st);
+    });
     if (rc != KATSU_OK || a.splits == 1) return rc;
     const unsigned blocks = (unsigned)cdiv(a.Tq * a.H, 4);
     if (d.dtype == KATSU_F32)
-        attention_join_kernel<float><<<blocks, 256, 0, st>>>(a, dp);
+        attention_join_kernel<float><<<blocks, 256, 0, st>>>(a, width);
     else
-        attention_join_kernel<__bf16><<<blocks, 256, 0, st>>>(a, dp);
+        attention_join_kernel<__bf16><<<blocks, 256, 0, st>>>(a, width);
     return status_of(hipGetLastError());
 }
 
 size_t attention_bwd_bytes(const katsu_attention &d) {
     if (d.seqs == 0) return 0;
-    const size_t part = bwd_plan(d).each ? 2 * d.heads * d.tokens_k * (size_t)dp_of(d) : 0;
+    const size_t part = bwd_plan(d).each ? 2 * d.heads * d.tokens_k * (size_t)width_of(d) : 0;
     return (stat_floats(d) + part) * sizeof(float);
 }
 
@@ -255,12 +268,11 @@ int attention_bwd(const katsu_attention &d, const katsu_attention_grads &g, cons
     take(a.dk, dk, g.dk_stride);
     take(a.dv, dv, g.dv_stride);
     a.lse = const_cast<float *>(lse);
-    a.lse2 = (float *)ws;
-    a.delta = a.lse2 + d.tokens_q * d.heads;
-    if (p.each) a.part = a.lse2 + stat_floats(d);
-    const int dp = dp_of(d);
-    return d.dtype == KATSU_F32 ? launch_bwd<float>(a, p, dp, vec, st)
-                                : launch_bwd<__bf16>(a, p, dp, vec, st);
+    a.start = (float *)ws;
+    if (p.each) a.part = a.start + stat_floats(d);
+    return by_shape(d, vec, [&](auto t, auto nd, auto v) {
+        return launch_bwd<decltype(t), decltype(nd)::value, decltype(v)::value>(a, p, st);
+    });
 }
 
 }  // namespace katsu

@@ -41,13 +41,13 @@ struct AttnTensor {
 struct AttnArgs {
     AttnTensor q, k, v, out, dout, dq, dk, dv;
     float *lse;                       // [H][Tq]
-    float *lse2, *delta;              // backward, [H][Tq]: lse times log2(e), do.o
+    float *start;                     // backward, [2][H][Tq]: -lse / scale, -do.o
     const int32_t *cu_q, *cu_k, *k_lens;
     int64_t Tq, Tk;
     int B, H, Hkv, G, D, causal;
     float scale, scale2;              // of the scores; times log2(e)
     int slots, splits;                // tiles of all sequences; parts of the key axis
-    float *part, *part_ml;            // the parts' sums [split][token][head][DP]; maxima and totals
+    float *part, *part_ml;            // the parts' sums [split][token][head][W]; maxima and totals
 };
 
 // ---- the sequence a tile belongs to -----------------------------------------
@@ -103,19 +103,32 @@ __device__ __forceinline__ AttnSeq find_seq(const AttnArgs &a, const int32_t *cu
 }
 
 // ---- tiles in LDS -------------------------------------------------------------
-// A tile's rows are RB bytes of 16-byte chunks (DP channels, those past D zero).
-// Row r's chunk c lies at place c ^ swz(r): the 32 rows that a fragment reads at
-// one chunk, and the 4 rows by 64 bytes that a transposing read takes, then
-// spread over all banks (measured in a loop: 240 and 200 bytes a cycle and CU,
-// the transposing read 63 with c ^ (r & 15)).
-template <typename T, int DP>
+// ND blocks of 32 channels are computed with; a tile's rows are RB bytes, of 64 or 128
+// channels, those that the operand does not have zero, in 16-byte chunks.  Row r's chunk c
+// lies at place c ^ swz(r): the 32 rows that a fragment reads at one chunk, and the 4 rows
+// by 64 bytes that a transposing read takes, then spread over all banks (measured in a
+// loop: 240 and 200 bytes a cycle and CU, the transposing read 63 with c ^ (r & 15)).
+template <typename T, int ND>
 struct Rows {
-    static constexpr int RB = DP * (int)sizeof(T), CH = RB / 16, E = 16 / (int)sizeof(T);
+    static constexpr int W = ND <= 2 ? 64 : 128;                  // channels of a row in LDS
+    static constexpr int E = 16 / (int)sizeof(T), RB = W * (int)sizeof(T), CH = RB / 16;
+    static constexpr int NS = ND * 32 / (2 * E);                  // fragments of a row
+    static constexpr int NF = 16 / E;                             // of a 32 x 32 result
     __device__ static __forceinline__ int swz(int r) {
         return CH == 8 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
     }
     __device__ static __forceinline__ int at(int r, int c) { return r * RB + ((c ^ swz(r)) << 4); }
 };
+
+typedef __attribute__((address_space(3))) char *lds_char;
+typedef uint32_t lds_at;  // a byte address in LDS
+__device__ __forceinline__ lds_at lds_addr(const char *p) {
+    return (lds_at)(uintptr_t)(lds_char)const_cast<char *>(p);
+}
+template <typename V>
+__device__ __forceinline__ V lds_read(lds_at a) {
+    return *(const __attribute__((address_space(3))) V *)(uintptr_t)a;
+}
 
 typedef __attribute__((address_space(3))) void attn_lds_void;
 constexpr int kAttnOOB = (int)0x80000000;  // beyond any tile: such a load returns zero
@@ -125,9 +138,9 @@ constexpr int kAttnOOB = (int)0x80000000;  // beyond any tile: such a load retur
 // for here; rows and chunks that do not exist are out of the buffer's range and
 // arrive as zeros.  Else (rows that are not a multiple of 16 bytes, or not
 // aligned so) element by element.
-template <typename T, int DP, int ROWS, int NW, bool DMA>
+template <typename T, int ND, int ROWS, int NW, bool DMA>
 struct TileCopy {
-    using R = Rows<T, DP>;
+    using R = Rows<T, ND>;
     static constexpr int N = ROWS * R::RB / 1024 / NW;
     static_assert(N >= 1, "tile too small for the waves");
     int off[DMA ? N : 1];
@@ -194,39 +207,53 @@ __device__ __forceinline__ floatx16 attn_mma(uintx4 a, uintx4 b, floatx16 c) {
         return c;
     }
 }
+// Places in a tile are a lane's own part, which the tile's address is added to, changed by
+// constants: an exclusive or of bits below a row's size, and an offset.  The tile's address
+// changes from step to step, so the compiler cannot keep one register for each place.
+//
 // Rows r0 + l%32 of a tile at step's chunks: the operand of a product over channels.
-template <typename T, int DP>
-__device__ __forceinline__ uintx4 row_frag(const char *lds, int r0, int step, int l31, int h) {
-    return *reinterpret_cast<const uintx4 *>(lds + r0 * Rows<T, DP>::RB +
-                                             Rows<T, DP>::at(l31, 2 * step + h));
+template <typename T, int ND>
+__device__ __forceinline__ lds_at row_lane(int lane) {
+    return Rows<T, ND>::at(lane & 31, lane >> 5);
 }
-// Channel 32*db + l%32 of a tile's rows: the operand of a product over rows, for
-// the rows whose values registers E*f .. E*f + E - 1 of a 32 x 32 result hold.
-template <typename T, int DP>
-__device__ __forceinline__ uintx4 col_frag(const char *lds, int r0, int f, int db, int lane) {
-    using R = Rows<T, DP>;
+template <typename T, int ND>
+__device__ __forceinline__ uintx4 row_frag(lds_at row, int r0, int step) {
+    return lds_read<uintx4>((row ^ (step << 5)) + r0 * Rows<T, ND>::RB);
+}
+// Channel 32*db + l%32 of a tile's rows r0 ..: the operand of a product over rows, for the
+// rows whose values registers E*f .. E*f + E - 1 of a 32 x 32 result hold.
+//
+// bfloat16: in each 16 lanes, lanes 4e .. 4e+3 read 16 channels of row e, and lane i
+// receives channel i of the four rows; the two reads are rows 16f + 8p + 4h + 0..3.
+// float32: rows 8f + 4h + e, one read each.
+template <typename T, int ND>
+__device__ __forceinline__ lds_at col_lane(int lane) {
+    using R = Rows<T, ND>;
     const int h = lane >> 5;
+    if (sizeof(T) == 2)
+        return R::at(4 * h + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) +
+               (lane & 1) * 8;
+    return R::at(4 * h, (lane & 31) >> 2) + (lane & 3) * 4;
+}
+template <typename T, int ND>
+__device__ __forceinline__ uintx4 col_frag(lds_at col, int r0, int f, int db) {
+    using R = Rows<T, ND>;
     uintx4 u;
     if constexpr (sizeof(T) == 2) {
-        // In each 16 lanes, lanes 4e .. 4e+3 read 16 channels of row e; lane i
-        // receives channel i of the four rows.
-        const int c = db * 4 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-            const int r = 8 * p + 4 * h + ((lane & 15) >> 2);
-            const int b = (r0 + 16 * f) * R::RB + R::at(r, c) + (lane & 1) * 8;
+            const lds_at a = (col ^ (((db << 2) ^ (2 * p)) << 4)) + (r0 + 16 * f + 8 * p) * R::RB;
             const uintx2 t = __builtin_bit_cast(
                 uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) shortx4 *)(lds + b)));
+                            (__attribute__((address_space(3))) shortx4 *)(uintptr_t)a));
             u[2 * p] = t[0];
             u[2 * p + 1] = t[1];
         }
     } else {
-        const int d = db * 32 + (lane & 31);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            u[e] = *reinterpret_cast<const uint32_t *>(lds + r0 * R::RB +
-                                                       R::at(8 * f + 4 * h + e, d >> 2) + (d & 3) * 4);
+            u[e] = lds_read<uint32_t>((col ^ (((db << 3) ^ (e << 2) ^ (2 * (f & 1))) << 4)) +
+                                      (r0 + 8 * f + e) * R::RB);
     }
     return u;
 }
@@ -251,6 +278,74 @@ __device__ __forceinline__ uintx4 reg_frag(const floatx16 &x, int f) {
 // The row of a result that register v of half h holds.
 __device__ __forceinline__ int reg_row(int v, int h) { return 8 * (v >> 2) + 4 * h + (v & 3); }
 
+// The LDS reads of a product are kept one step ahead of its matrix instructions, and no
+// further: the compiler would put all of them in front, and has no registers for them.  The
+// fence keeps reads and matrix instructions in their steps; vector instructions may cross it.
+__device__ __forceinline__ void step_fence() { __builtin_amdgcn_sched_barrier(0x277); }
+
+template <int ND>
+struct ColFrags {
+    uintx4 x[ND];
+};
+template <typename T, int ND>
+__device__ __forceinline__ ColFrags<ND> col_frags(lds_at col, int r0, int f) {
+    ColFrags<ND> c;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) c.x[d] = col_frag<T, ND>(col, r0, f, d);
+    return c;
+}
+// acc[d] += (channels 32*d .. of the tile's rows r0 .. r0 + 31)^T x; `c` is the first step's
+// operand, read already.  `ahead` reads what follows the product during its last step.
+template <typename T, int ND, class F>
+__device__ __forceinline__ void col_product(floatx16 (&acc)[ND], lds_at col, int r0,
+                                            ColFrags<ND> c, const floatx16 &x, F ahead) {
+    constexpr int NF = Rows<T, ND>::NF;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        ColFrags<ND> n;
+        if (f + 1 < NF)
+            n = col_frags<T, ND>(col, r0, f + 1);
+        else
+            ahead();
+        const uintx4 p = reg_frag<T>(x, f);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] = attn_mma<T>(c.x[d], p, acc[d]);
+        step_fence();
+        if (f + 1 < NF) c = n;
+    }
+}
+// acc += (rows r0 .. of the tile at row) . b(step), over the channels, two fragments a step.
+template <typename T, int ND, class B, class F>
+__device__ __forceinline__ void row_product(floatx16 &acc, lds_at row, int r0, B b, F ahead) {
+    constexpr int NS = Rows<T, ND>::NS;
+    uintx4 c[2], n[2], y[2], z[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (i < NS) {
+            c[i] = row_frag<T, ND>(row, r0, i);
+            y[i] = b(i);
+        }
+#pragma unroll
+    for (int st = 0; st < NS; st += 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (st + 2 + i < NS) {
+                n[i] = row_frag<T, ND>(row, r0, st + 2 + i);
+                z[i] = b(st + 2 + i);
+            }
+        if (st + 2 >= NS) ahead();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (st + i < NS) acc = attn_mma<T>(c[i], y[i], acc);
+        step_fence();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            c[i] = n[i];
+            y[i] = z[i];
+        }
+    }
+}
+
 // x of the lower half's lane and of the upper one's, in both.
 __device__ __forceinline__ void halves(float x, float &lo, float &hi) {
     const uint32_t u = as_bits(x);
@@ -271,13 +366,13 @@ __device__ __forceinline__ float half_sum(float x) {
 
 // Row r's fragments of a [token][head][D] operand, straight from memory: NS of
 // them, zero where the row or the channels do not exist.
-template <typename T, int DP, bool VEC>
+template <typename T, int ND, bool VEC>
 __device__ __forceinline__ void load_row(const AttnTensor &t, int64_t token, int head, bool valid,
                                          int D, int h, uintx4 *f) {
-    using R = Rows<T, DP>;
+    using R = Rows<T, ND>;
     const T *p = reinterpret_cast<const T *>(t.p) + token * t.token + head * t.head;
 #pragma unroll
-    for (int s = 0; s < R::CH / 2; ++s) {
+    for (int s = 0; s < R::NS; ++s) {
         const int d = (2 * s + h) * R::E;
         uintx4 u = {0, 0, 0, 0};
         if constexpr (VEC) {
@@ -311,68 +406,57 @@ __device__ __forceinline__ void store_row(T *p, const floatx16 &x, float by, int
 }
 
 // ---- non-finite values in masked places -----------------------------------------
-// A masked key's probability is zero, but a matrix product still multiplies it by
-// what the masked row holds, and 0 * Inf is NaN.  In the tiles that the mask cuts,
-// the kernels look for such values first; where there are any, their products run
-// on the tile with those values cleared, and what the unmasked ones among them
-// contribute is added apart.
+// A masked key's probability is zero, but a matrix product still multiplies it by what the
+// masked row holds, and 0 * Inf is NaN.  In the tiles that the mask cuts a wave looks for
+// such values; if there are any, it computes its rows again at the end, over the keys that
+// they see and no others, in the plain way (`careful`: a lane a row and half of the
+// channels).
 
-template <typename T>
-__device__ __forceinline__ bool nonfinite_bits(uint32_t x) {
-    return (x & (sizeof(T) == 2 ? 0x7f80u : 0x7f800000u)) ==
-           (sizeof(T) == 2 ? 0x7f80u : 0x7f800000u);
-}
-// Whether rows [r0, r0 + ROWS) of a tile hold one; the same answer in every lane.
-template <typename T, int DP, int ROWS>
-__device__ __forceinline__ bool tile_nonfinite(const char *lds, int lane) {
+// Whether rows [r0, r0 + ROWS) of the tile at `a` hold one; the same answer in every lane.
+template <typename T, int ND, int ROWS>
+__device__ __forceinline__ bool tile_nonfinite(lds_at a, int lane) {
     typedef unsigned short us2 __attribute__((ext_vector_type(2)));
     us2 m2 = {0, 0};
     uint32_t m1 = 0;
 #pragma unroll 4
-    for (int i = 0; i < ROWS * DP * (int)sizeof(T) / 1024; ++i) {
-        const uintx4 u = *reinterpret_cast<const uintx4 *>(lds + i * 1024 + lane * 16);
+    for (int i = 0; i < ROWS * Rows<T, ND>::RB / 1024; ++i) {
+        const uintx4 u = lds_read<uintx4>(a + i * 1024 + lane * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
+            const uint32_t x = u[e];
             if constexpr (sizeof(T) == 2)
-                m2 = __builtin_elementwise_max(m2, __builtin_bit_cast(us2, u[e] & 0x7f807f80u));
+                m2 = __builtin_elementwise_max(m2, __builtin_bit_cast(us2, x & 0x7f807f80u));
             else
-                m1 = max(m1, u[e] & 0x7f800000u);
+                m1 = max(m1, x & 0x7f800000u);
         }
     }
     const bool bad = sizeof(T) == 2 ? (m2[0] == 0x7f80 || m2[1] == 0x7f80) : m1 == 0x7f800000u;
     return __ballot(bad) != 0;
 }
+// Channels c0 .. of a row: the first n of them exist.
 template <typename T>
-__device__ __forceinline__ uintx4 clear_nonfinite(uintx4 u) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if constexpr (sizeof(T) == 2) {
-            const uint32_t lo = nonfinite_bits<T>(u[e]) ? 0 : u[e] & 0xffffu;
-            const uint32_t hi = nonfinite_bits<T>(u[e] >> 16) ? 0 : u[e] & 0xffff0000u;
-            u[e] = lo | hi;
-        } else {
-            u[e] = nonfinite_bits<T>(u[e]) ? 0 : u[e];
-        }
-    }
-    return u;
+__device__ __forceinline__ T *plain_at(const AttnTensor &t, int64_t token, int head, int c0) {
+    return (T *)const_cast<void *>(t.p) + token * t.token + head * t.head + c0;
 }
-// Adds to acc (channels 32*db + reg_row, this lane's column) the non-finite values of the
-// tile's rows [lo, hi), each times a factor: a probability, which is above zero and changes
-// neither an infinity's sign nor a NaN, or (NANS) one that is zero or NaN itself.
-template <typename T, int DP, bool NANS>
-__device__ __forceinline__ void add_nonfinite(const char *lds, int lo, int hi, int db, int h,
-                                              floatx16 &acc) {
-    using R = Rows<T, DP>;
-    for (int r = lo; r < hi; ++r) {
+// x . y over n channels of this lane and its partner's.
+template <typename T>
+__device__ __forceinline__ float plain_dot(const T *x, const T *y, int n) {
+    float s = 0.f;
+    for (int i = 0; i < n; ++i) s += (float)x[i] * (float)y[i];
+    return half_sum(s);
+}
+// acc += by x, acc's N channels in registers.
+template <typename T, int N>
+__device__ __forceinline__ void plain_add(float (&acc)[N], float by, const T *x, int n) {
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            const int d = db * 32 + reg_row(v, h);
-            const T x = *reinterpret_cast<const T *>(lds + R::at(r, d / R::E) +
-                                                     d % R::E * (int)sizeof(T));
-            const float y = (float)x;
-            acc[v] += y - y == 0.f ? 0.f : NANS ? y - y : y;
-        }
-    }
+    for (int i = 0; i < N; ++i)
+        if (i < n) acc[i] += by * (float)x[i];
+}
+template <typename T, int N>
+__device__ __forceinline__ void plain_store(T *p, const float (&acc)[N], float by, int n) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (i < n) p[i] = (T)(acc[i] * by);
 }
 
 }  // namespace katsu

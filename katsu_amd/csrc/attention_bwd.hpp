@@ -13,54 +13,45 @@
 
 namespace katsu {
 
-// ---- dq, delta and lse2 --------------------------------------------------------
+// ---- dq, and where the sums of dk and dv start --------------------------------------------------------
 // As the forward pass: a wave owns 32 rows (a row's scores in one lane and its partner),
 // the block's waves share the key tiles.
-template <typename T, int DP, int BN, bool VEC>
+template <typename T, int ND, int BN, bool VEC>
 struct AttnDq {
-    using R = Rows<T, DP>;
+    using R = Rows<T, ND>;
     static constexpr int BM = 128, THREADS = 256;
-    static constexpr int NS = R::CH / 2, ND = DP / 32, NB = BN / 32, NF = 16 / R::E;
+    static constexpr int NS = R::NS, NB = BN / 32;
     static constexpr int kTile = BN * R::RB, kLds = 4 * kTile;
-    using Copy = TileCopy<T, DP, BN, 4, VEC>;
+    using Copy = TileCopy<T, ND, BN, 4, VEC>;
 
-    template <bool MASK>
-    __device__ static __forceinline__ void tile(const char *kl, const char *vl,
-                                                const uintx4 (&qf)[NS], const uintx4 (&gf)[NS],
-                                                floatx16 (&dq)[ND], float lse2, float delta,
-                                                float scale2, int key0, int jmax, int lane) {
-        const int l31 = lane & 31, h = lane >> 5;
-        const bool bad = MASK && tile_nonfinite<T, DP, BN>(kl, lane);
+    // P and dP of 32 keys.
+    __device__ static __forceinline__ void probs(lds_at row, const uintx4 (&qf)[NS],
+                                                 const uintx4 (&gf)[NS], floatx16 &p, floatx16 &g,
+                                                 float lse2, float scale2, int b) {
+        floatx16 s = {};
+        g = floatx16{};
+        row_product<T, ND>(s, row, 32 * b, [&](int st) { return qf[st]; }, [] {});
+        row_product<T, ND>(g, row + kTile, 32 * b, [&](int st) { return gf[st]; }, [] {});
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+            p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], scale2, -lse2));
+    }
+    __device__ static __forceinline__ void tile(lds_at row, lds_at col, const uintx4 (&qf)[NS],
+                                                const uintx4 (&gf)[NS], floatx16 (&dq)[ND],
+                                                float lse2, float delta, float scale2, bool mask,
+                                                int jmax, int h) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            floatx16 s = {}, g = {};
+            floatx16 p, g;
+            probs(row, qf, gf, p, g, lse2, scale2, b);
 #pragma unroll
-            for (int st = 0; st < NS; ++st)
-                s = attn_mma<T>(row_frag<T, DP>(kl, 32 * b, st, l31, h), qf[st], s);
+            for (int v = 0; v < 16; ++v) g[v] = p[v] * (g[v] - delta);
+            if (mask) {
 #pragma unroll
-            for (int st = 0; st < NS; ++st)
-                g = attn_mma<T>(row_frag<T, DP>(vl, 32 * b, st, l31, h), gf[st], g);
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], scale2, -lse2));
-                g[v] = p * (g[v] - delta);
-                if (MASK && key0 + 32 * b + reg_row(v, h) > jmax) g[v] = 0.f;
+                for (int v = 0; v < 16; ++v)
+                    if (32 * b + reg_row(v, h) > jmax) g[v] = 0.f;
             }
-#pragma unroll
-            for (int f = 0; f < NF; ++f) {
-                const uintx4 p = reg_frag<T>(g, f);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    uintx4 k = col_frag<T, DP>(kl, 32 * b, f, d, lane);
-                    if (MASK && bad) k = clear_nonfinite<T>(k);
-                    dq[d] = attn_mma<T>(k, p, dq[d]);
-                }
-            }
-        }
-        if (MASK && bad) {
-            const int seen = min(max(jmax + 1 - key0, 0), BN);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) add_nonfinite<T, DP, true>(kl, 0, seen, d, h, dq[d]);
+            col_product<T, ND>(dq, col, 32 * b, col_frags<T, ND>(col, 32 * b, 0), g, [] {});
         }
     }
 
@@ -78,17 +69,13 @@ struct AttnDq {
         const bool valid = r < rows;
         const int tok = (int)(r / a.G), head = kvh * a.G + (int)(r % a.G);
         const int shift = sq.lk - sq.lq;
-        const int jmax = !valid ? -1 : a.causal ? min(tok + shift, sq.lk - 1) : sq.lk - 1;
-        const int wtop = (int)(min(row0 + wave * 32 + 31, rows - 1) / a.G);
-        const int wend = row0 + wave * 32 >= rows ? 0
-                         : a.causal ? min(max(wtop + shift + 1, 0), sq.lk) : sq.lk;
-        const int wall = row0 + wave * 32 + 31 >= rows ? 0
-                         : a.causal
-                             ? min(max((int)((row0 + wave * 32) / a.G) + shift + 1, 0), sq.lk)
-                             : sq.lk;
-        const int btop = (int)(min(row0 + BM - 1, rows - 1) / a.G);
-        const int end = a.causal ? min(max(btop + shift + 1, 0), sq.lk) : sq.lk;
-        const int tiles = (end + BN - 1) / BN;
+        auto sees = [&](int64_t row) {  // how many keys
+            return !a.causal ? sq.lk : min(max((int)(row / a.G) + shift + 1, 0), sq.lk);
+        };
+        const int seen = sees(min(r, rows - 1)), jmax = seen - 1;
+        const int wend = sees(min(row0 + wave * 32 + 31, rows - 1));
+        const int wall = sees(row0 + wave * 32);
+        const int tiles = (sees(min(row0 + BM - 1, rows - 1)) + BN - 1) / BN;
 
         Copy ck, cv;
         ck.init(wave, lane, a.k.token, a.D);
@@ -105,8 +92,8 @@ struct AttnDq {
 
         const int64_t token = sq.q0 + tok, at = head * a.Tq + token;
         uintx4 qf[NS], gf[NS];
-        load_row<T, DP, VEC>(a.out, token, head, valid, a.D, h, qf);
-        load_row<T, DP, VEC>(a.dout, token, head, valid, a.D, h, gf);
+        load_row<T, ND, VEC>(a.out, token, head, valid, a.D, h, qf);
+        load_row<T, ND, VEC>(a.dout, token, head, valid, a.D, h, gf);
         float delta = 0.f;
 #pragma unroll
         for (int s = 0; s < NS; ++s)
@@ -122,103 +109,125 @@ struct AttnDq {
             }
         delta = half_sum(delta);
         const float lse2 = valid ? a.lse[at] * kLog2e : 0.f;
-        if (valid && h == 0) {
-            a.lse2[at] = lse2;
-            a.delta[at] = delta;
-        }
-        load_row<T, DP, VEC>(a.q, token, head, valid, a.D, h, qf);
+        load_row<T, ND, VEC>(a.q, token, head, valid, a.D, h, qf);
 
         floatx16 dq[ND] = {};
+        bool bad = false;
+        const lds_at row = row_lane<T, ND>(lane), col = col_lane<T, ND>(lane);
+        const lds_at base = lds_addr(lds);
         for (int t = 0, buf = 0; t < tiles; ++t, buf ^= 1) {
             attn_wait_dma();
             __syncthreads();  // the tile is there, the other buffer read
             if (t + 1 < tiles) fetch(t + 1, buf ^ 1);
-            const char *kl = lds + buf * (2 * kTile), *vl = kl + kTile;
-            if (t * BN + BN <= wall)
-                tile<false>(kl, vl, qf, gf, dq, lse2, delta, a.scale2, t * BN, jmax, lane);
-            else if (t * BN < wend)
-                tile<true>(kl, vl, qf, gf, dq, lse2, delta, a.scale2, t * BN, jmax, lane);
+            const lds_at b = base + buf * (2 * kTile);
+            if (sizeof(T) == 2 && wend <= BN && t == 0) {
+                // Rows whose keys are one tile: dP is near delta there, and out's rounding to
+                // bfloat16 as large as what dS is to be; delta is sum P dP as well.
+                delta = 0.f;
+#pragma unroll 1
+                for (int q = 0; q < NB; ++q) {
+                    floatx16 p, g;
+                    probs(b + row, qf, gf, p, g, lse2, a.scale2, q);
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (32 * q + reg_row(v, h) <= jmax) delta += p[v] * g[v];
+                }
+                delta = half_sum(delta);
+            }
+            if (t * BN < wend) {
+                const bool mask = t * BN + BN > wall;
+                if (mask) bad |= tile_nonfinite<T, ND, BN>(b, lane);
+                tile(b + row, b + col, qf, gf, dq, lse2, delta, a.scale2, mask, jmax - t * BN, h);
+            }
+        }
+        if (valid && h == 0) {
+            a.start[at] = -lse2 / a.scale2;
+            a.start[a.H * a.Tq + at] = -delta;
+        }
+        if (bad) {
+            constexpr int N = ND * 16;
+            const int c0 = h * N, n = min(max(a.D - c0, 0), N);
+            const T *q = plain_at<T>(a.q, valid ? token : 0, head, c0);
+            const T *g = plain_at<T>(a.dout, valid ? token : 0, head, c0);
+            float acc[N] = {};
+            for (int j = 0; j < seen; ++j) {
+                const T *k = plain_at<T>(a.k, sq.k0 + j, kvh, c0);
+                const float s = plain_dot(q, k, n);
+                const float dp = plain_dot(g, plain_at<T>(a.v, sq.k0 + j, kvh, c0), n);
+                plain_add(acc,
+                          __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.scale2, -lse2)) * (dp - delta),
+                          k, n);
+            }
+            if (valid) plain_store(plain_at<T>(a.dq, token, head, c0), acc, a.scale, n);
+            return;
         }
         if (!valid) return;
-        T *p = (T *)const_cast<void *>(a.dq.p) + token * a.dq.token + head * a.dq.head;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) store_row<T, VEC>(p, dq[d], a.scale, d, h, a.D);
+        for (int d = 0; d < ND; ++d)
+            store_row<T, VEC>(plain_at<T>(a.dq, token, head, 0), dq[d], a.scale, d, h, a.D);
     }
 };
 
 // ---- dk and dv -------------------------------------------------------------------
-// A wave owns 32 keys: their k and v rows in registers as B operands, the sums of dk and
+// A wave owns 32 keys: their k rows in registers as B operands, their v rows there or
+// (VLDS: bfloat16 rows of 128, whose sums need the registers) in LDS, the sums of dk and
 // dv transposed (a lane holds its key's channels).  The block's four waves share tiles of
 // QT queries, q and do, of the group's heads in turn, or of one head: then the heads' sums
 // go to `part` in float32 and attention_group_kernel adds them in the heads' order.
-template <typename T, int DP, int QT, bool VEC>
+template <typename T, int ND, int QT, bool VEC>
 struct AttnDkv {
-    using R = Rows<T, DP>;
+    using R = Rows<T, ND>;
     static constexpr int BK = 128, THREADS = 256;
-    static constexpr int NS = R::CH / 2, ND = DP / 32, NQ = QT / 32, NF = 16 / R::E;
-    static constexpr int kTile = QT * R::RB, kStage = 2 * kTile + 512, kLds = 2 * kStage;
-    using Copy = TileCopy<T, DP, QT, 4, VEC>;
-    static_assert(QT <= 64, "a wave copies the rows' lse2 and delta");
+    static constexpr int NS = R::NS, NQ = QT / 32, W = R::W;
+    static constexpr bool VLDS = sizeof(T) == 2 && ND > 2;
+    static constexpr int kTile = QT * R::RB, kStage = 2 * kTile + 512;
+    static constexpr int kKeys = VLDS ? BK * R::RB : 0, kLds = kKeys + 2 * kStage;
+    using Copy = TileCopy<T, ND, QT, 4, VEC>;
+    static_assert(QT <= 64, "a wave copies the rows' starts");
 
-    // 32 queries (rows r0.. of the tile, query i0 + r0 first) against the wave's keys.
-    template <bool MASK>
-    __device__ static __forceinline__ void block(const char *ql, const char *gl,
-                                                 const float *stats, const uintx4 (&kf)[NS],
-                                                 const uintx4 (&vf)[NS], floatx16 (&dk)[ND],
-                                                 floatx16 (&dv)[ND], float scale2, int r0,
-                                                 int ifirst, int lane) {
-        const int l31 = lane & 31, h = lane >> 5;
-        floatx16 s = {}, g = {};
+    // 32 queries (rows r0 .. of the tile) against the wave's keys.  row, col: this lane's
+    // places in q's tile, followed by do's; vrow: in the block's v rows; stats: -lse / scale and
+    // -delta.
+    __device__ static __forceinline__ void block(lds_at row, lds_at col, lds_at stats, lds_at vrow,
+                                                 const uintx4 (&kf)[NS], const uintx4 *vf,
+                                                 floatx16 (&dk)[ND], floatx16 (&dv)[ND],
+                                                 float scale2, int r0, bool mask, int ifirst,
+                                                 int h) {
+        floatx16 s, g;
 #pragma unroll
-        for (int st = 0; st < NS; ++st)
-            s = attn_mma<T>(row_frag<T, DP>(ql, r0, st, l31, h), kf[st], s);
-#pragma unroll
-        for (int st = 0; st < NS; ++st)
-            g = attn_mma<T>(row_frag<T, DP>(gl, r0, st, l31, h), vf[st], g);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const floatx4 lse2 = *reinterpret_cast<const floatx4 *>(stats + r0 + 8 * q + 4 * h);
-            const floatx4 delta =
-                *reinterpret_cast<const floatx4 *>(stats + 64 + r0 + 8 * q + 4 * h);
+        for (int q = 0; q < 4; ++q) {  // sums that start from -lse / scale and -delta
+            const floatx4 x = lds_read<floatx4>(stats + (r0 + 8 * q + 4 * h) * 4);
+            const floatx4 y = lds_read<floatx4>(stats + 256 + (r0 + 8 * q + 4 * h) * 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int v = 4 * q + e;
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], scale2, -lse2[e]));
-                s[v] = p;
-                g[v] = p * (g[v] - delta[e]);
-                if (MASK && r0 + reg_row(v, h) < ifirst) s[v] = g[v] = 0.f;
+                s[4 * q + e] = x[e];
+                g[4 * q + e] = y[e];
             }
         }
-        const bool badg = MASK && tile_nonfinite<T, DP, 32>(gl + r0 * R::RB, lane);
-        const bool badq = MASK && tile_nonfinite<T, DP, 32>(ql + r0 * R::RB, lane);
+        ColFrags<ND> c;
+        row_product<T, ND>(s, row, r0, [&](int st) { return kf[st]; }, [] {});
+        row_product<T, ND>(
+            g, row + kTile, r0,
+            [&](int st) {
+                if constexpr (VLDS)
+                    return row_frag<T, ND>(vrow, 0, st);
+                else
+                    return vf[st];
+            },
+            [&] { c = col_frags<T, ND>(col + kTile, r0, 0); });
 #pragma unroll
-        for (int f = 0; f < NF; ++f) {
-            const uintx4 p = reg_frag<T>(s, f);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                uintx4 x = col_frag<T, DP>(gl, r0, f, d, lane);
-                if (MASK && badg) x = clear_nonfinite<T>(x);
-                dv[d] = attn_mma<T>(x, p, dv[d]);
-            }
+        for (int v = 0; v < 16; ++v) {
+            s[v] = __builtin_amdgcn_exp2f(s[v] * scale2);
+            g[v] *= s[v];
         }
+        if (mask) {
 #pragma unroll
-        for (int f = 0; f < NF; ++f) {
-            const uintx4 p = reg_frag<T>(g, f);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                uintx4 x = col_frag<T, DP>(ql, r0, f, d, lane);
-                if (MASK && badq) x = clear_nonfinite<T>(x);
-                dk[d] = attn_mma<T>(x, p, dk[d]);
-            }
+            for (int v = 0; v < 16; ++v)
+                if (r0 + reg_row(v, h) < ifirst) s[v] = g[v] = 0.f;
         }
-        if (MASK && (badg || badq)) {
-            const int lo = r0 + min(max(ifirst - r0, 0), 32);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                if (badg) add_nonfinite<T, DP, false>(gl, lo, r0 + 32, d, h, dv[d]);
-                if (badq) add_nonfinite<T, DP, true>(ql, lo, r0 + 32, d, h, dk[d]);
-            }
-        }
+        col_product<T, ND>(dv, col + kTile, r0, c, s,
+                           [&] { c = col_frags<T, ND>(col, r0, 0); });
+        col_product<T, ND>(dk, col, r0, c, g, [] {});
     }
 
     __device__ static void run(const AttnArgs &a, char *lds) {
@@ -249,11 +258,10 @@ struct AttnDkv {
         const char *qp = (const char *)a.q.p + (sq.q0 * a.q.token + head0 * a.q.head) * sizeof(T);
         const char *gp =
             (const char *)a.dout.p + (sq.q0 * a.dout.token + head0 * a.dout.head) * sizeof(T);
-        // Tile n of the heads' tiles: head n / tiles, rows (t0 + n % tiles) * QT ..; the four
-        // waves copy it, the first also the rows' lse2 and delta, as zeros past the end: such
-        // rows have P = 1 and q, do, delta = 0, and add nothing.
+        // The rows' starts of the sums are copied too, by the first wave, as zeros past the
+        // end: such rows have P = 1, and q, do and dS = 0, and add nothing.
         auto fetch = [&](int g, int t, int buf) {
-            char *d = lds + buf * kStage;
+            char *d = lds + kKeys + buf * kStage;
             const int64_t i = (int64_t)(t0 + t) * QT;
             const int left = sq.lq - (int)i;
             cq.load(qp + i * cq.stride + g * a.q.head * (int64_t)sizeof(T), left, d);
@@ -264,7 +272,7 @@ struct AttnDkv {
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
                     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                        (w ? a.delta : a.lse2) + at, (short)0, bytes, 0x00020000);
+                        a.start + w * (a.H * a.Tq) + at, (short)0, bytes, 0x00020000);
                     __builtin_amdgcn_raw_ptr_buffer_load_lds(
                         rs, (attn_lds_void *)(d + 2 * kTile + w * 256), 4, lane * 4, 0, 0, 0);
                 }
@@ -274,10 +282,22 @@ struct AttnDkv {
         if (total > 0) fetch(0, 0, 0);
 
         const int64_t token = sq.k0 + key;
-        uintx4 kf[NS], vf[NS];
-        load_row<T, DP, VEC>(a.k, token, kvh, valid, a.D, h, kf);
-        load_row<T, DP, VEC>(a.v, token, kvh, valid, a.D, h, vf);
+        uintx4 kf[NS], vf[VLDS ? 1 : NS];
+        load_row<T, ND, VEC>(a.k, token, kvh, valid, a.D, h, kf);
+        if constexpr (VLDS) {
+            TileCopy<T, ND, 32, 1, VEC> cv;  // each wave its own rows
+            cv.init(0, lane, a.v.token, a.D);
+            cv.load((const char *)a.v.p +
+                        ((int64_t)(sq.k0 + wkey) * a.v.token + kvh * a.v.head) * sizeof(T),
+                    sq.lk - wkey, lds + wave * 32 * R::RB);
+        } else {
+            load_row<T, ND, VEC>(a.v, token, kvh, valid, a.D, h, vf);
+        }
         floatx16 dk[ND] = {}, dv[ND] = {};
+        bool bad = false;
+        const lds_at row = row_lane<T, ND>(lane), col = col_lane<T, ND>(lane);
+        const lds_at base = lds_addr(lds) + kKeys;
+        lds_at vrow = row + lds_addr(lds) + wave * 32 * R::RB;
         int g = 0, t = 0;
         for (int n = 0, buf = 0; n < total; ++n, buf ^= 1) {
             attn_wait_dma();
@@ -288,61 +308,84 @@ struct AttnDkv {
                 ++g;
             }
             if (n + 1 < total) fetch(g, t, buf ^ 1);
-            const char *ql = lds + buf * kStage, *gl = ql + kTile;
-            const float *stats = reinterpret_cast<const float *>(gl + kTile);
+            const lds_at b = base + buf * kStage, stats = b + 2 * kTile;
+            asm("" : "+v"(vrow));  // no register for each of its places
 #pragma unroll
             for (int q = 0; q < NQ; ++q) {
-                if (i0 + 32 * q >= wall)
-                    block<false>(ql, gl, stats, kf, vf, dk, dv, a.scale2, 32 * q, 0, lane);
-                else if (i0 + 32 * q + 31 >= wfirst)
-                    block<true>(ql, gl, stats, kf, vf, dk, dv, a.scale2, 32 * q, ifirst - i0,
-                                lane);
+                if (i0 + 32 * q + 31 < wfirst) continue;
+                const bool mask = i0 + 32 * q < wall;
+                if (mask)
+                    bad |= tile_nonfinite<T, ND, 32>(b + 32 * q * R::RB, lane) ||
+                           tile_nonfinite<T, ND, 32>(b + kTile + 32 * q * R::RB, lane);
+                block(b + row, b + col, stats, vrow, kf, vf, dk, dv, a.scale2, 32 * q, mask,
+                      ifirst - i0, h);
             }
         }
-        if (!valid) return;
-        if (each) {
-            float *pk = a.part + (hd * a.Tk + token) * DP, *pv = pk + a.H * a.Tk * DP;
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                store_row<float, true>(pk, dk[d], a.scale, d, h, DP);
-                store_row<float, true>(pv, dv[d], 1.f, d, h, DP);
+        float *pk = a.part + (hd * a.Tk + token) * W, *pv = pk + a.H * a.Tk * W;
+        if (bad) {
+            constexpr int N = ND * 16;
+            const int c0 = h * N, n = min(max(a.D - c0, 0), N);
+            const T *k = plain_at<T>(a.k, valid ? token : 0, kvh, c0);
+            const T *v = plain_at<T>(a.v, valid ? token : 0, kvh, c0);
+            float ak[N] = {}, av[N] = {};
+            for (int gg = 0; gg < heads; ++gg)
+                for (int i = max(ifirst, 0); i < sq.lq; ++i) {
+                    const int64_t at = (head0 + gg) * a.Tq + sq.q0 + i;
+                    const T *q = plain_at<T>(a.q, sq.q0 + i, head0 + gg, c0);
+                    const T *d = plain_at<T>(a.dout, sq.q0 + i, head0 + gg, c0);
+                    const float s = plain_dot(q, k, n), dp = plain_dot(d, v, n);
+                    const float p = __builtin_amdgcn_exp2f((s + a.start[at]) * a.scale2);
+                    plain_add(av, p, d, n);
+                    plain_add(ak, p * (dp + a.start[a.H * a.Tq + at]), q, n);
+                }
+            if (!valid) return;
+            if (each) {
+                plain_store(pk + c0, ak, a.scale, n);
+                plain_store(pv + c0, av, 1.f, n);
+            } else {
+                plain_store(plain_at<T>(a.dk, token, kvh, c0), ak, a.scale, n);
+                plain_store(plain_at<T>(a.dv, token, kvh, c0), av, 1.f, n);
             }
             return;
         }
-        T *pk = (T *)const_cast<void *>(a.dk.p) + token * a.dk.token + kvh * a.dk.head;
-        T *pv = (T *)const_cast<void *>(a.dv.p) + token * a.dv.token + kvh * a.dv.head;
+        if (!valid) return;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            store_row<T, VEC>(pk, dk[d], a.scale, d, h, a.D);
-            store_row<T, VEC>(pv, dv[d], 1.f, d, h, a.D);
+            if (each) {
+                store_row<float, true>(pk, dk[d], a.scale, d, h, W);
+                store_row<float, true>(pv, dv[d], 1.f, d, h, W);
+            } else {
+                store_row<T, VEC>(plain_at<T>(a.dk, token, kvh, 0), dk[d], a.scale, d, h, a.D);
+                store_row<T, VEC>(plain_at<T>(a.dv, token, kvh, 0), dv[d], 1.f, d, h, a.D);
+            }
         }
     }
 };
 
-template <typename T, int DP, int BN, bool VEC, int OCC>
+template <typename T, int ND, int BN, bool VEC, int OCC>
 __global__ void __launch_bounds__(256, OCC) attention_dq_kernel(const AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    AttnDq<T, DP, BN, VEC>::run(a, lds);
+    AttnDq<T, ND, BN, VEC>::run(a, lds);
 }
-template <typename T, int DP, int QT, bool VEC, int OCC>
+template <typename T, int ND, int QT, bool VEC, int OCC>
 __global__ void __launch_bounds__(256, OCC) attention_dkv_kernel(const AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    AttnDkv<T, DP, QT, VEC>::run(a, lds);
+    AttnDkv<T, ND, QT, VEC>::run(a, lds);
 }
 
 // dk and dv of a key head: the sums of its group's heads, in their order.  A thread: four
 // channels of one token and key head, of dk (blockIdx.y 0) or dv.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) attention_group_kernel(const AttnArgs a, int DP) {
-    const int per = DP / 4;
+__global__ void __launch_bounds__(256) attention_group_kernel(const AttnArgs a, int W) {
+    const int per = W / 4;
     const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int d = (int)(n % per) * 4, kvh = (int)(n / per % a.Hkv);
     const int64_t token = n / per / a.Hkv;
     if (token >= a.Tk || d >= a.D) return;
     const AttnTensor &t = blockIdx.y ? a.dv : a.dk;
-    const float *p = a.part + ((blockIdx.y ? a.H : 0) + kvh * a.G) * a.Tk * DP + token * DP + d;
+    const float *p = a.part + ((blockIdx.y ? a.H : 0) + kvh * a.G) * a.Tk * W + token * W + d;
     floatx4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int g = 0; g < a.G; ++g) x += *reinterpret_cast<const floatx4 *>(p + g * a.Tk * DP);
+    for (int g = 0; g < a.G; ++g) x += *reinterpret_cast<const floatx4 *>(p + g * a.Tk * W);
     T *o = (T *)const_cast<void *>(t.p) + token * t.token + kvh * t.head + d;
     T e[4];
 #pragma unroll

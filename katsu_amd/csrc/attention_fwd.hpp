@@ -16,45 +16,44 @@
 
 namespace katsu {
 
-// 2^3: until a row's maximum has grown by more, its sums stay on the old one.
-// Any reference gives the same quotient; 2^8 times 2^-24 sums lose nothing.
+// Until a row's maximum has grown by 2^8, its sums stay on the old one: any reference
+// gives the same quotient, and sums 2^8 larger lose nothing in float32.
 constexpr float kAttnSlack = 8.f;
 
-template <typename T, int DP, int WM, int WK, int BN, bool VEC>
+template <typename T, int ND, int WM, int WK, int BN, bool VEC>
 struct AttnFwd {
-    using R = Rows<T, DP>;
+    using R = Rows<T, ND>;
     static constexpr int BM = 32 * WM, NW = WM * WK, THREADS = 64 * NW;
-    static constexpr int NS = R::CH / 2, ND = DP / 32, NB = BN / 32, NF = 16 / R::E;
+    static constexpr int NS = R::NS, NB = BN / 32, W = R::W;
     static constexpr int kTile = BN * R::RB;               // K or V
     static constexpr int kStages = 4 * kTile * WK;         // two of both, per key wave
-    static constexpr int kMerge = WK > 1 ? WK * (ND * 4096 + 256) : 0;
+    static constexpr int kMerge = WK > 1 ? WK * (ND * 4096 + 256) + 16 : 0;
     static constexpr int kLds = kStages > kMerge ? kStages : kMerge;
-    using Copy = TileCopy<T, DP, BN, (WK > 1 ? 1 : WM), VEC>;
+    using Copy = TileCopy<T, ND, BN, (WK > 1 ? 1 : WM), VEC>;
 
-    // One key tile: scores, the running softmax, the values.
-    template <bool MASK>
-    __device__ static __forceinline__ void tile(const char *kl, const char *vl,
-                                                const uintx4 (&qf)[NS], floatx16 (&o)[ND], float &m,
-                                                float &l, float scale2, int key0, int jmax,
-                                                int lane) {
-        const int l31 = lane & 31, h = lane >> 5;
+    // One key tile: scores, the running softmax, the values.  row, col: this lane's places
+    // in the tile of keys and in that of values.
+    __device__ static __forceinline__ void tile(lds_at row, lds_at col, const uintx4 (&qf)[NS],
+                                                floatx16 (&o)[ND], float &m, float &l,
+                                                float scale2, bool mask, int jmax, int h) {
         floatx16 s[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            floatx16 c = {};
+            s[b] = floatx16{};
+            row_product<T, ND>(s[b], row, 32 * b, [&](int st) { return qf[st]; }, [] {});
+        }
+        if (mask) {
 #pragma unroll
-            for (int st = 0; st < NS; ++st)
-                c = attn_mma<T>(row_frag<T, DP>(kl, 32 * b, st, l31, h), qf[st], c);
-            s[b] = c;
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    if (32 * b + reg_row(v, h) > jmax) s[b][v] = -INFINITY;
         }
         float mx = -INFINITY;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                if (MASK && key0 + 32 * b + reg_row(v, h) > jmax) s[b][v] = -INFINITY;
-                mx = fmaxf(mx, s[b][v]);
-            }
+            for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[b][v]);
         mx = half_max(mx) * scale2;
         if (__ballot(mx > m + kAttnSlack)) {  // the first keys: m is -inf
             const float mn = fmaxf(m, mx);
@@ -76,34 +75,69 @@ struct AttnFwd {
                 sum += s[b][v];
             }
         l += sum;
-        bool bad = false;
-        if constexpr (MASK) bad = tile_nonfinite<T, DP, BN>(vl, lane);
-        if (MASK && bad) {
-#pragma unroll 1
-            for (int b = 0; b < NB; ++b)
+        ColFrags<ND> c = col_frags<T, ND>(col, 0, 0);
 #pragma unroll
-                for (int f = 0; f < NF; ++f) {
-                    uintx4 p = reg_frag<T>(s[0], f);
-                    if (NB > 1 && b == 1) p = reg_frag<T>(s[NB - 1], f);
-#pragma unroll
-                    for (int d = 0; d < ND; ++d)
-                        o[d] = attn_mma<T>(
-                            clear_nonfinite<T>(col_frag<T, DP>(vl, 32 * b, f, d, lane)), p, o[d]);
-                }
-            const int seen = min(max(jmax + 1 - key0, 0), BN);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) add_nonfinite<T, DP, false>(vl, 0, seen, d, h, o[d]);
-        } else {
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int f = 0; f < NF; ++f) {
-                    const uintx4 p = reg_frag<T>(s[b], f);
-#pragma unroll
-                    for (int d = 0; d < ND; ++d)
-                        o[d] = attn_mma<T>(col_frag<T, DP>(vl, 32 * b, f, d, lane), p, o[d]);
-                }
+        for (int b = 0; b < NB; ++b)
+            col_product<T, ND>(o, col, 32 * b, c, s[b], [&] {
+                if (b + 1 < NB) c = col_frags<T, ND>(col, 32 * (b + 1), 0);
+            });
+    }
+
+    // A row's result, of keys [j0, j1) of the sequence: parts of a split key axis as they are.
+    struct Row {
+        int64_t token;
+        int head, split;
+        bool valid;
+    };
+    __device__ static __forceinline__ float *part_of(const AttnArgs &a, const Row &r) {
+        return a.part + (r.split * (a.Tq * a.H) + r.token * a.H + r.head) * W;
+    }
+    // The row's maximum and total; a total of -1 says that it saw no key.
+    __device__ static __forceinline__ void finish_row(const AttnArgs &a, const Row &r, float m,
+                                                      float l) {
+        if (a.splits > 1) {
+            float *ml = a.part_ml + (r.split * (a.Tq * a.H) + r.token * a.H + r.head) * 2;
+            ml[0] = m;
+            ml[1] = l;
+        } else if (a.lse) {
+            a.lse[r.head * a.Tq + r.token] =
+                l < 0.f ? -INFINITY : kLn2 * (m + __builtin_amdgcn_logf(l));
         }
+    }
+    __device__ static __forceinline__ void finish(const AttnArgs &a, const Row &r,
+                                                  const floatx16 &x, int db, int h, float m,
+                                                  float l) {
+        if (!r.valid) return;
+        if (db == 0 && h == 0) finish_row(a, r, m, l);
+        if (a.splits > 1)
+            store_row<float, true>(part_of(a, r), x, 1.f, db, h, W);
+        else
+            store_row<T, VEC>(plain_at<T>(a.out, r.token, r.head, 0), x, l < 0.f ? 0.f : 1.f / l,
+                              db, h, a.D);
+    }
+    __device__ static __forceinline__ void careful(const AttnArgs &a, const Row &r, int64_t k0,
+                                                   int kvh, int j0, int j1, int h) {
+        constexpr int N = ND * 16;
+        const int c0 = h * N, n = min(max(a.D - c0, 0), N);
+        const T *q = plain_at<T>(a.q, r.valid ? r.token : 0, r.head, c0);
+        float m = -INFINITY, l = j0 < j1 ? 0.f : -1.f, acc[N] = {};
+        for (int j = j0; j < j1; ++j) {
+            const float s =
+                plain_dot(q, plain_at<T>(a.k, k0 + j, kvh, c0), n) * a.scale2;
+            const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
+            const float by = __builtin_amdgcn_exp2f(m - ref), p = __builtin_amdgcn_exp2f(s - ref);
+            m = mn;
+            l = l * by + p;
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] *= by;
+            plain_add(acc, p, plain_at<T>(a.v, k0 + j, kvh, c0), n);
+        }
+        if (!r.valid) return;
+        if (h == 0) finish_row(a, r, m, l);
+        if (a.splits > 1)
+            plain_store(part_of(a, r) + c0, acc, 1.f, n);
+        else
+            plain_store(plain_at<T>(a.out, r.token, r.head, c0), acc, l < 0.f ? 0.f : 1.f / l, n);
     }
 
     __device__ static void run(const AttnArgs &a, char *lds) {
@@ -121,27 +155,18 @@ struct AttnFwd {
             (int64_t)(slot - uni(first_slot(a.cu_q, sq.s, a.Tq, a.G, BM))) * BM;
         if (row0 >= rows) return;
         const int64_t r = row0 + wm * 32 + l31;
-        const bool valid = r < rows;
-        const int tok = (int)(r / a.G), head = kvh * a.G + (int)(r % a.G);
+        const int tok = (int)(r / a.G);
+        const Row me = {sq.q0 + tok, kvh * a.G + (int)(r % a.G), split, r < rows};
         const int shift = sq.lk - sq.lq;  // query i sees keys up to i + shift
-        const int jmax = !valid ? -1 : a.causal ? min(tok + shift, sq.lk - 1) : sq.lk - 1;
-        // Keys that this wave's rows see at most, and those that all of them see.
-        const int wtop = (int)(min(row0 + wm * 32 + 31, rows - 1) / a.G);
-        const int wend = row0 + wm * 32 >= rows ? 0
-                         : a.causal ? min(max(wtop + shift + 1, 0), sq.lk) : sq.lk;
-        const int wall = row0 + wm * 32 + 31 >= rows ? 0
-                         : a.causal
-                             ? min(max((int)((row0 + wm * 32) / a.G) + shift + 1, 0), sq.lk)
-                             : sq.lk;
-        const int btop = (int)(min(row0 + BM - 1, rows - 1) / a.G);
-        const int end = a.causal ? min(max(btop + shift + 1, 0), sq.lk) : sq.lk;
-        const int tiles = (end + BN - 1) / BN, per = (tiles + a.splits - 1) / a.splits;
-        const int t0 = split * per + wk, t1 = min(tiles, (split + 1) * per);
-
-        uintx4 qf[NS];
-        load_row<T, DP, VEC>(a.q, sq.q0 + tok, head, valid, a.D, h, qf);
-        floatx16 o[ND] = {};
-        float m = -INFINITY, l = 0.f;
+        auto sees = [&](int64_t row) {    // how many keys
+            return !a.causal ? sq.lk : min(max((int)(row / a.G) + shift + 1, 0), sq.lk);
+        };
+        // Rows past the sequence's end are computed with whatever they give, and not stored.
+        const int seen = sees(min(r, rows - 1)), jmax = seen - 1;
+        const int wend = sees(min(row0 + wm * 32 + 31, rows - 1)), wall = sees(row0 + wm * 32);
+        const int tiles = (sees(min(row0 + BM - 1, rows - 1)) + BN - 1) / BN;
+        const int per = (tiles + a.splits - 1) / a.splits;
+        const int f0 = split * per, t0 = f0 + wk, t1 = min(tiles, f0 + per);
 
         Copy ck, cv;
         ck.init(WK > 1 ? 0 : wave, lane, a.k.token, a.D);
@@ -156,48 +181,38 @@ struct AttnFwd {
             cv.load(vp + j * cv.stride, sq.lk - t * BN, d + kTile);
         };
         if (t0 < t1) fetch(t0, 0);
-        int buf = 0;
-        for (int t = t0; t < t1; t += WK, buf ^= 1) {
+        uintx4 qf[NS];
+        load_row<T, ND, VEC>(a.q, me.token, me.head, me.valid, a.D, h, qf);
+        floatx16 o[ND] = {};
+        float m = -INFINITY, l = 0.f;
+        bool bad = false;
+        const lds_at row = row_lane<T, ND>(lane), col = col_lane<T, ND>(lane) + kTile;
+        lds_at at = lds_addr(mine);
+        for (int t = t0, buf = 0; t < t1; t += WK, buf ^= 1) {
             attn_wait_dma();
             if constexpr (WK == 1) __syncthreads();  // the tile is there, the other buffer read
             if (t + WK < t1) fetch(t + WK, buf ^ 1);
-            const char *kl = mine + buf * (2 * kTile), *vl = kl + kTile;
-            if (t * BN + BN <= wall)
-                tile<false>(kl, vl, qf, o, m, l, a.scale2, t * BN, jmax, lane);
-            else if (t * BN < wend)
-                tile<true>(kl, vl, qf, o, m, l, a.scale2, t * BN, jmax, lane);
+            const lds_at b = at + buf * (2 * kTile);
+            if (t * BN < wend) {
+                const bool mask = t * BN + BN > wall;
+                if (mask) bad |= tile_nonfinite<T, ND, BN>(b + kTile, lane);
+                tile(b + row, b + col, qf, o, m, l, a.scale2, mask, jmax - t * BN, h);
+            }
         }
         l = half_sum(l);
-
-        const int64_t token = sq.q0 + tok, grow = token * a.H + head;
-        // Whether this row saw a key here: one that saw none is zero, whatever keys hold.
-        const bool saw = t0 < t1 && t0 * BN <= jmax;
-        auto finish = [&](const floatx16 &x, int db, float M, float L) {
-            if (!valid) return;
-            const bool some = !(L < 0.f);
-            if (a.splits > 1) {
-                float *p = a.part + (split * (a.Tq * a.H) + grow) * DP;
-                store_row<float, true>(p, x, 1.f, db, h, DP);
-                if (db == 0 && h == 0) {
-                    float *ml = a.part_ml + (split * (a.Tq * a.H) + grow) * 2;
-                    ml[0] = M;
-                    ml[1] = L;
-                }
+        if (!(t0 < t1 && t0 * BN < seen)) l = -1.f;  // this row saw no key here
+        const int j0 = f0 * BN, j1 = min(t1 * BN, seen);
+        if constexpr (WK == 1) {
+            if (bad) {
+                careful(a, me, sq.k0, kvh, j0, j1, h);
                 return;
             }
-            T *p = (T *)const_cast<void *>(a.out.p) + token * a.out.token + head * a.out.head;
-            store_row<T, VEC>(p, x, some ? 1.f / L : 0.f, db, h, a.D);
-            if (db == 0 && h == 0 && a.lse)
-                a.lse[head * a.Tq + token] =
-                    some ? kLn2 * (M + __builtin_amdgcn_logf(L)) : -INFINITY;
-        };
-        if (!saw) l = -1.f;  // no total is negative
-        if constexpr (WK == 1) {
 #pragma unroll
-            for (int d = 0; d < ND; ++d) finish(o[d], d, m, l);
+            for (int d = 0; d < ND; ++d) finish(a, me, o[d], d, h, m, l);
         } else {
             float *om = reinterpret_cast<float *>(lds);
             float *ml = om + WK * ND * 1024;
+            int *flag = reinterpret_cast<int *>(ml + WK * 64);
             __syncthreads();
 #pragma unroll
             for (int d = 0; d < ND; ++d)
@@ -207,7 +222,15 @@ struct AttnFwd {
                 ml[wave * 64 + l31] = m;
                 ml[wave * 64 + 32 + l31] = l;
             }
+            if (lane == 0) flag[wave] = bad;
             __syncthreads();
+            int any = 0;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) any |= flag[w];
+            if (uni(any)) {
+                if (wave == 0) careful(a, me, sq.k0, kvh, j0, j1, h);
+                return;
+            }
             float M = -INFINITY, L = -1.f;
 #pragma unroll
             for (int w = 0; w < WK; ++w) M = fmaxf(M, ml[w * 64 + l31]);
@@ -227,21 +250,21 @@ struct AttnFwd {
 #pragma unroll
                     for (int v = 0; v < 16; ++v)
                         if (by[w] != 0.f) x[v] += by[w] * om[((w * ND + d) * 16 + v) * 64 + lane];
-                finish(x, d, M, L);
+                finish(a, me, x, d, h, M, L);
             }
         }
     }
 };
 
-template <typename T, int DP, int WM, int WK, int BN, bool VEC, int OCC>
+template <typename T, int ND, int WM, int WK, int BN, bool VEC, int OCC>
 __global__ void __launch_bounds__(64 * WM * WK, OCC) attention_fwd_kernel(const AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    AttnFwd<T, DP, WM, WK, BN, VEC>::run(a, lds);
+    AttnFwd<T, ND, WM, WK, BN, VEC>::run(a, lds);
 }
 
 // Joins the parts of the key axis: one wave a row, lane l channels l and l + 64.
 template <typename T>
-__global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, int DP) {
+__global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, int W) {
     const int lane = threadIdx.x & 63;
     const int64_t rows = a.Tq * a.H, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= rows) return;
@@ -257,12 +280,12 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, i
         L = (L < 0.f ? 0.f : L) + by * l;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            if (lane + 64 * i < DP) x[i] += by * a.part[(s * rows + row) * DP + lane + 64 * i];
+            if (lane + 64 * i < a.D) x[i] += by * a.part[(s * rows + row) * W + lane + 64 * i];
     }
     const bool some = !(L < 0.f);
     const int64_t token = row / a.H;
     const int head = (int)(row % a.H);
-    T *p = (T *)const_cast<void *>(a.out.p) + token * a.out.token + head * a.out.head;
+    T *p = plain_at<T>(a.out, token, head, 0);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
         if (lane + 64 * i < a.D) p[lane + 64 * i] = (T)(some ? x[i] / L : 0.f);
