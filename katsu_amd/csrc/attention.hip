@@ -73,6 +73,12 @@ AttnTensor tensor(const void *p, const int64_t (&stride)[2]) {
 // Channels of a row in LDS and in the parts.
 int width_of(const katsu_attention &d) { return d.head_dim <= 64 ? 64 : 128; }
 
+// Runs that an axis of `len` is split into: two blocks a CU, a run at least `least` long.
+int runs(int64_t blocks, int64_t len, int64_t least) {
+    return (int)std::max<int64_t>(
+        1, std::min(2 * kCUs / std::max<int64_t>(blocks, 1), cdiv(len, least)));
+}
+
 // The forward call's shape: tiles of 32 rows whose waves share the keys, or of 128.
 struct FwdPlan {
     bool few;
@@ -86,9 +92,10 @@ FwdPlan fwd_plan(const katsu_attention &d) {
     p.bm = p.few ? 32 : 128;
     p.slots = (int)(rows / p.bm + B);
     const int64_t blocks = (int64_t)p.slots * (int64_t)d.kv_heads;
-    const int64_t keys = cdiv((int64_t)d.tokens_k, B);
-    p.splits = (int)std::max<int64_t>(1, std::min(2 * kCUs / std::max<int64_t>(blocks, 1),
-                                                  cdiv(keys, 256)));
+    // A run's keys are worth more than the launch that joins the runs: in float32 two tiles
+    // (3.4 us each), in bfloat16 four.
+    p.splits = runs(blocks, cdiv((int64_t)d.tokens_k, B),
+                    d.dtype == KATSU_F32 ? (d.head_dim > 64 ? 64 : 128) : 256);
     return p;
 }
 size_t part_floats(const katsu_attention &d, const FwdPlan &p) {
@@ -141,24 +148,30 @@ int launch_fwd(const AttnArgs &a, bool few, hipStream_t st) {
     return launch_fwd<T, ND, 4, 1, wide ? 32 : 64, VEC, 2>(a, st);
 }
 
-// The backward call's shape.  Blocks of one query head each, and their sums joined
-// afterwards, unless the key heads alone give the card enough to do; in float32 always,
-// as a sum over all of a group's rows in one accumulator loses too much (8 heads of 1900
-// rows: dk 1.1e-6 off, 5.8e-7 with a head at a time).
+// The backward call's shape.  dk and dv: blocks of one query head each, unless the key heads
+// alone give the card enough to do; in float32 always, as a sum over all of a group's rows
+// in one accumulator loses too much.  Both kernels: the other axis in runs of at least two
+// tiles where there are few blocks.
 struct BwdPlan {
-    int dq_slots, dkv_slots;
+    int dq_slots, dq_splits, dkv_slots, dkv_splits, parts;
     bool each;
 };
 BwdPlan bwd_plan(const katsu_attention &d) {
     BwdPlan p;
-    const int64_t group = (int64_t)(d.heads / d.kv_heads), B = (int64_t)d.seqs;
+    const int64_t kv = (int64_t)d.kv_heads, group = (int64_t)d.heads / kv, B = (int64_t)d.seqs;
     p.dq_slots = (int)((int64_t)d.tokens_q * group / 128 + B);
     p.dkv_slots = (int)((int64_t)d.tokens_k / 128 + B);
-    p.each = group > 1 && (d.dtype == KATSU_F32 ||
-                           (int64_t)p.dkv_slots * (int64_t)d.kv_heads < 4 * kCUs);
+    p.each = group > 1 && (d.dtype == KATSU_F32 || p.dkv_slots * kv < 4 * kCUs);
+    // Keys of a run of dq, queries of one of dk and dv: two tiles.
+    const bool wide = d.head_dim > 64;
+    p.dq_splits = runs(p.dq_slots * kv, cdiv((int64_t)d.tokens_k, B),
+                       d.dtype == KATSU_F32 && wide ? 64 : 128);
+    p.dkv_splits = runs(p.dkv_slots * kv * (p.each ? group : 1),
+                        cdiv((int64_t)d.tokens_q, B) * (p.each ? 1 : group), wide ? 64 : 128);
+    p.parts = (p.each ? (int)group : 1) * p.dkv_splits;
     return p;
 }
-size_t stat_floats(const katsu_attention &d) {
+size_t start_floats(const katsu_attention &d) {
     return (2 * d.tokens_q * d.heads + 63) / 64 * 64;
 }
 
@@ -170,16 +183,50 @@ int launch_bwd(AttnArgs a, const BwdPlan &p, hipStream_t st) {
     using Dq = AttnDq<T, ND, BN, VEC>;
     using Dkv = AttnDkv<T, ND, QT, VEC>;
     a.slots = p.dq_slots;
+    a.splits = p.dq_splits;
     int rc = launch<attention_dq_kernel<T, ND, BN, VEC, 2>>(
-        a.Tq > 0 ? (int64_t)p.dq_slots * a.Hkv : 0, Dq::THREADS, Dq::kLds, a, st);
-    if (rc != KATSU_OK || a.Tk == 0) return rc;
+        a.Tq > 0 ? (int64_t)p.dq_slots * a.Hkv * a.splits : 0, Dq::THREADS, Dq::kLds, a, st);
+    if (rc != KATSU_OK) return rc;
+    // Sums of parts: dq's are [run][token][head], dk's and dv's [key head][part][token].
+    AttnSum s{};
+    s.D = a.D;
+    s.W = Dkv::W;
+    auto sum = [&](int outs) {
+        const int64_t blocks = cdiv(s.tokens * s.heads * (s.W / 4), 256);
+        attention_sum_kernel<T, VEC><<<dim3((unsigned)blocks, outs), 256, 0, st>>>(s);
+        return status_of(hipGetLastError());
+    };
+    if (a.splits > 1 && a.Tq > 0) {
+        s.out[0] = a.dq;
+        s.part[0] = a.part;
+        s.tokens = a.Tq;
+        s.heads = a.H;
+        s.parts = a.splits;
+        s.head_step = s.W;
+        s.token_step = (int64_t)a.H * s.W;
+        s.part_step = a.Tq * s.token_step;
+        rc = sum(1);
+        if (rc != KATSU_OK) return rc;
+    }
+    if (a.Tk == 0) return KATSU_OK;
     a.slots = p.dkv_slots;
+    a.splits = p.dkv_splits;
+    a.parts = p.parts;
+    a.each = p.each;
     rc = launch<attention_dkv_kernel<T, ND, QT, VEC, RB == 512 ? 1 : 2>>(
-        (int64_t)p.dkv_slots * (p.each ? a.H : a.Hkv), Dkv::THREADS, Dkv::kLds, a, st);
-    if (rc != KATSU_OK || !p.each) return rc;
-    const int64_t blocks = cdiv(a.Tk * a.Hkv * (Dkv::W / 4), 256);
-    attention_group_kernel<T, VEC><<<dim3((unsigned)blocks, 2), 256, 0, st>>>(a, Dkv::W);
-    return status_of(hipGetLastError());
+        (int64_t)p.dkv_slots * a.Hkv * p.parts, Dkv::THREADS, Dkv::kLds, a, st);
+    if (rc != KATSU_OK || p.parts == 1) return rc;
+    s.out[0] = a.dk;
+    s.out[1] = a.dv;
+    s.tokens = a.Tk;
+    s.heads = a.Hkv;
+    s.parts = p.parts;
+    s.token_step = s.W;
+    s.part_step = a.Tk * s.W;
+    s.head_step = s.parts * s.part_step;
+    s.part[0] = a.part;
+    s.part[1] = a.part + a.Hkv * s.head_step;
+    return sum(2);
 }
 
 }  // namespace
@@ -244,8 +291,11 @@ int attention_fwd(const katsu_attention &d, const void *q, const void *k, const 
 
 size_t attention_bwd_bytes(const katsu_attention &d) {
     if (d.seqs == 0) return 0;
-    const size_t part = bwd_plan(d).each ? 2 * d.heads * d.tokens_k * (size_t)width_of(d) : 0;
-    return (stat_floats(d) + part) * sizeof(float);
+    // The parts of dq and those of dk and dv take turns.
+    const BwdPlan p = bwd_plan(d);
+    const size_t dq = p.dq_splits > 1 ? p.dq_splits * d.tokens_q * d.heads : 0;
+    const size_t dkv = p.parts > 1 ? 2 * (size_t)p.parts * d.kv_heads * d.tokens_k : 0;
+    return (start_floats(d) + std::max(dq, dkv) * width_of(d)) * sizeof(float);
 }
 
 int attention_bwd(const katsu_attention &d, const katsu_attention_grads &g, const void *dout,
@@ -269,7 +319,7 @@ int attention_bwd(const katsu_attention &d, const katsu_attention_grads &g, cons
     take(a.dv, dv, g.dv_stride);
     a.lse = const_cast<float *>(lse);
     a.start = (float *)ws;
-    if (p.each) a.part = a.start + stat_floats(d);
+    a.part = a.start + start_floats(d);
     return by_shape(d, vec, [&](auto t, auto nd, auto v) {
         return launch_bwd<decltype(t), decltype(nd)::value, decltype(v)::value>(a, p, st);
     });

@@ -46,8 +46,9 @@ struct AttnArgs {
     int64_t Tq, Tk;
     int B, H, Hkv, G, D, causal;
     float scale, scale2;              // of the scores; times log2(e)
-    int slots, splits;                // tiles of all sequences; parts of the key axis
-    float *part, *part_ml;            // the parts' sums [split][token][head][W]; maxima and totals
+    int slots, splits;                // tiles of all sequences; runs of the other axis's tiles
+    int parts, each;                  // dk, dv: blocks a key tile and head; one head a block
+    float *part, *part_ml;            // the runs' sums; their rows' maxima and totals
 };
 
 // ---- the sequence a tile belongs to -----------------------------------------

@@ -59,7 +59,8 @@ struct AttnDq {
         const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
         const int l31 = lane & 31, h = lane >> 5;
         const unsigned id = blockIdx.x;
-        const int kvh = id % a.Hkv, slot = a.slots - 1 - (int)(id / a.Hkv);
+        const int kvh = id % a.Hkv, split = id / a.Hkv % a.splits;
+        const int slot = a.slots - 1 - (int)(id / a.Hkv / a.splits);
         const AttnSeq sq = find_seq(a, a.cu_q, a.Tq, a.G, BM, slot, lane);
         const int64_t rows = (int64_t)sq.lq * a.G;
         const int64_t row0 =
@@ -76,6 +77,8 @@ struct AttnDq {
         const int wend = sees(min(row0 + wave * 32 + 31, rows - 1));
         const int wall = sees(row0 + wave * 32);
         const int tiles = (sees(min(row0 + BM - 1, rows - 1)) + BN - 1) / BN;
+        const int per = (tiles + a.splits - 1) / a.splits;
+        const int t0 = split * per, t1 = min(tiles, t0 + per);
 
         Copy ck, cv;
         ck.init(wave, lane, a.k.token, a.D);
@@ -88,7 +91,7 @@ struct AttnDq {
             ck.load(kp + j * ck.stride, sq.lk - t * BN, d);
             cv.load(vp + j * cv.stride, sq.lk - t * BN, d + kTile);
         };
-        if (tiles > 0) fetch(0, 0);
+        if (t0 < t1) fetch(t0, 0);
 
         const int64_t token = sq.q0 + tok, at = head * a.Tq + token;
         uintx4 qf[NS], gf[NS];
@@ -115,10 +118,10 @@ struct AttnDq {
         bool bad = false;
         const lds_at row = row_lane<T, ND>(lane), col = col_lane<T, ND>(lane);
         const lds_at base = lds_addr(lds);
-        for (int t = 0, buf = 0; t < tiles; ++t, buf ^= 1) {
+        for (int t = t0, buf = 0; t < t1; ++t, buf ^= 1) {
             attn_wait_dma();
             __syncthreads();  // the tile is there, the other buffer read
-            if (t + 1 < tiles) fetch(t + 1, buf ^ 1);
+            if (t + 1 < t1) fetch(t + 1, buf ^ 1);
             const lds_at b = base + buf * (2 * kTile);
             if (sizeof(T) == 2 && wend <= BN && t == 0) {
                 // Rows whose keys are one tile: dP is near delta there, and out's rounding to
@@ -140,17 +143,18 @@ struct AttnDq {
                 tile(b + row, b + col, qf, gf, dq, lse2, delta, a.scale2, mask, jmax - t * BN, h);
             }
         }
-        if (valid && h == 0) {
+        if (valid && h == 0 && split == 0) {
             a.start[at] = -lse2 / a.scale2;
             a.start[a.H * a.Tq + at] = -delta;
         }
+        float *part = a.part + ((split * a.Tq + token) * a.H + head) * R::W;
         if (bad) {
             constexpr int N = ND * 16;
             const int c0 = h * N, n = min(max(a.D - c0, 0), N);
             const T *q = plain_at<T>(a.q, valid ? token : 0, head, c0);
             const T *g = plain_at<T>(a.dout, valid ? token : 0, head, c0);
             float acc[N] = {};
-            for (int j = 0; j < seen; ++j) {
+            for (int j = t0 * BN; j < min(t1 * BN, seen); ++j) {
                 const T *k = plain_at<T>(a.k, sq.k0 + j, kvh, c0);
                 const float s = plain_dot(q, k, n);
                 const float dp = plain_dot(g, plain_at<T>(a.v, sq.k0 + j, kvh, c0), n);
@@ -158,13 +162,21 @@ struct AttnDq {
                           __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.scale2, -lse2)) * (dp - delta),
                           k, n);
             }
-            if (valid) plain_store(plain_at<T>(a.dq, token, head, c0), acc, a.scale, n);
+            if (!valid) return;
+            if (a.splits > 1)
+                plain_store(part + c0, acc, a.scale, n);
+            else
+                plain_store(plain_at<T>(a.dq, token, head, c0), acc, a.scale, n);
             return;
         }
         if (!valid) return;
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
-            store_row<T, VEC>(plain_at<T>(a.dq, token, head, 0), dq[d], a.scale, d, h, a.D);
+        for (int d = 0; d < ND; ++d) {
+            if (a.splits > 1)
+                store_row<float, true>(part, dq[d], a.scale, d, h, R::W);
+            else
+                store_row<T, VEC>(plain_at<T>(a.dq, token, head, 0), dq[d], a.scale, d, h, a.D);
+        }
     }
 };
 
@@ -172,8 +184,8 @@ struct AttnDq {
 // A wave owns 32 keys: their k rows in registers as B operands, their v rows there or
 // (VLDS: bfloat16 rows of 128, whose sums need the registers) in LDS, the sums of dk and
 // dv transposed (a lane holds its key's channels).  The block's four waves share tiles of
-// QT queries, q and do, of the group's heads in turn, or of one head: then the heads' sums
-// go to `part` in float32 and attention_group_kernel adds them in the heads' order.
+// QT queries, q and do, of the group's heads in turn, or of one head, or of a run of
+// these: then the sums go to `part` in float32 and attention_sum_kernel adds them in order.
 template <typename T, int ND, int QT, bool VEC>
 struct AttnDkv {
     using R = Rows<T, ND>;
@@ -233,12 +245,14 @@ struct AttnDkv {
     __device__ static void run(const AttnArgs &a, char *lds) {
         const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
         const int l31 = lane & 31, h = lane >> 5;
-        // Heads innermost; with a causal mask the keys that most queries see first.
-        const bool each = a.part != nullptr;  // one head a block
-        const unsigned id = blockIdx.x, hs = each ? a.H : a.Hkv;
-        const int hd = id % hs, slot = (int)(id / hs);
-        const int kvh = each ? hd / a.G : hd;
-        const int head0 = each ? hd : hd * a.G, heads = each ? 1 : a.G;
+        // Heads innermost; with a causal mask the keys that most queries see first.  A key
+        // head's queries are `parts` blocks' work: every head's tiles in `splits` runs, or
+        // (!each) all heads' together.
+        const unsigned id = blockIdx.x;
+        const int kvh = id % a.Hkv, p = id / a.Hkv % a.parts;
+        const int slot = (int)(id / a.Hkv / a.parts);
+        const int split = p % a.splits;
+        const int head0 = kvh * a.G + (a.each ? p / a.splits : 0), heads = a.each ? 1 : a.G;
         const AttnSeq sq = find_seq(a, a.cu_k, a.Tk, 1, BK, slot, lane);
         const int key0 = (slot - uni(first_slot(a.cu_k, sq.s, a.Tk, 1, BK))) * BK;
         if (key0 >= sq.lk) return;
@@ -278,8 +292,10 @@ struct AttnDkv {
                 }
             }
         };
-        const int total = tiles * heads;
-        if (total > 0) fetch(0, 0, 0);
+        const int per = (tiles * heads + a.splits - 1) / a.splits;
+        const int n0 = split * per, n1 = min(tiles * heads, n0 + per);
+        int g = n0 < n1 ? n0 / tiles : 0, t = n0 - g * tiles;
+        if (n0 < n1) fetch(g, t, 0);
 
         const int64_t token = sq.k0 + key;
         uintx4 kf[NS], vf[VLDS ? 1 : NS];
@@ -298,8 +314,7 @@ struct AttnDkv {
         const lds_at row = row_lane<T, ND>(lane), col = col_lane<T, ND>(lane);
         const lds_at base = lds_addr(lds) + kKeys;
         lds_at vrow = row + lds_addr(lds) + wave * 32 * R::RB;
-        int g = 0, t = 0;
-        for (int n = 0, buf = 0; n < total; ++n, buf ^= 1) {
+        for (int n = n0, buf = 0; n < n1; ++n, buf ^= 1) {
             attn_wait_dma();
             __syncthreads();  // the tile is there, the other buffer read
             const int i0 = (t0 + t) * QT;
@@ -307,7 +322,7 @@ struct AttnDkv {
                 t = 0;
                 ++g;
             }
-            if (n + 1 < total) fetch(g, t, buf ^ 1);
+            if (n + 1 < n1) fetch(g, t, buf ^ 1);
             const lds_at b = base + buf * kStage, stats = b + 2 * kTile;
             asm("" : "+v"(vrow));  // no register for each of its places
 #pragma unroll
@@ -321,25 +336,28 @@ struct AttnDkv {
                       ifirst - i0, h);
             }
         }
-        float *pk = a.part + (hd * a.Tk + token) * W, *pv = pk + a.H * a.Tk * W;
+        float *pk = a.part + ((int64_t)(kvh * a.parts + p) * a.Tk + token) * W;
+        float *pv = pk + (int64_t)a.Hkv * a.parts * a.Tk * W;
         if (bad) {
             constexpr int N = ND * 16;
             const int c0 = h * N, n = min(max(a.D - c0, 0), N);
             const T *k = plain_at<T>(a.k, valid ? token : 0, kvh, c0);
             const T *v = plain_at<T>(a.v, valid ? token : 0, kvh, c0);
             float ak[N] = {}, av[N] = {};
-            for (int gg = 0; gg < heads; ++gg)
-                for (int i = max(ifirst, 0); i < sq.lq; ++i) {
-                    const int64_t at = (head0 + gg) * a.Tq + sq.q0 + i;
-                    const T *q = plain_at<T>(a.q, sq.q0 + i, head0 + gg, c0);
-                    const T *d = plain_at<T>(a.dout, sq.q0 + i, head0 + gg, c0);
+            for (int m = n0; m < n1; ++m) {  // the tiles' rows that see the key
+                const int gg = head0 + m / tiles, i0 = (t0 + m % tiles) * QT;
+                for (int i = max(ifirst, i0); i < min(sq.lq, i0 + QT); ++i) {
+                    const int64_t at = gg * a.Tq + sq.q0 + i;
+                    const T *q = plain_at<T>(a.q, sq.q0 + i, gg, c0);
+                    const T *d = plain_at<T>(a.dout, sq.q0 + i, gg, c0);
                     const float s = plain_dot(q, k, n), dp = plain_dot(d, v, n);
-                    const float p = __builtin_amdgcn_exp2f((s + a.start[at]) * a.scale2);
-                    plain_add(av, p, d, n);
-                    plain_add(ak, p * (dp + a.start[a.H * a.Tq + at]), q, n);
+                    const float w = __builtin_amdgcn_exp2f((s + a.start[at]) * a.scale2);
+                    plain_add(av, w, d, n);
+                    plain_add(ak, w * (dp + a.start[a.H * a.Tq + at]), q, n);
                 }
+            }
             if (!valid) return;
-            if (each) {
+            if (a.parts > 1) {
                 plain_store(pk + c0, ak, a.scale, n);
                 plain_store(pv + c0, av, 1.f, n);
             } else {
@@ -351,7 +369,7 @@ struct AttnDkv {
         if (!valid) return;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            if (each) {
+            if (a.parts > 1) {
                 store_row<float, true>(pk, dk[d], a.scale, d, h, W);
                 store_row<float, true>(pv, dv[d], 1.f, d, h, W);
             } else {
@@ -373,20 +391,27 @@ __global__ void __launch_bounds__(256, OCC) attention_dkv_kernel(const AttnArgs 
     AttnDkv<T, ND, QT, VEC>::run(a, lds);
 }
 
-// dk and dv of a key head: the sums of its group's heads, in their order.  A thread: four
-// channels of one token and key head, of dk (blockIdx.y 0) or dv.
+// Gradients from their parts, in order.  A thread: four channels of one token and head of
+// each of the launch's gradients (blockIdx.y: dk and dv, or dq).  Part i of a token's head
+// lies at part + head*head_step + i*part_step + token*token_step.
+struct AttnSum {
+    AttnTensor out[2];
+    const float *part[2];
+    int64_t tokens, head_step, part_step, token_step;
+    int heads, parts, D, W;
+};
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) attention_group_kernel(const AttnArgs a, int W) {
-    const int per = W / 4;
+__global__ void __launch_bounds__(256) attention_sum_kernel(const AttnSum a) {
+    const int per = a.W / 4;
     const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int d = (int)(n % per) * 4, kvh = (int)(n / per % a.Hkv);
-    const int64_t token = n / per / a.Hkv;
-    if (token >= a.Tk || d >= a.D) return;
-    const AttnTensor &t = blockIdx.y ? a.dv : a.dk;
-    const float *p = a.part + ((blockIdx.y ? a.H : 0) + kvh * a.G) * a.Tk * W + token * W + d;
+    const int d = (int)(n % per) * 4, head = (int)(n / per % a.heads);
+    const int64_t token = n / per / a.heads;
+    if (token >= a.tokens || d >= a.D) return;
+    const AttnTensor &t = a.out[blockIdx.y];
+    const float *p = a.part[blockIdx.y] + head * a.head_step + token * a.token_step + d;
     floatx4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int g = 0; g < a.G; ++g) x += *reinterpret_cast<const floatx4 *>(p + g * a.Tk * W);
-    T *o = (T *)const_cast<void *>(t.p) + token * t.token + kvh * t.head + d;
+    for (int i = 0; i < a.parts; ++i) x += *reinterpret_cast<const floatx4 *>(p + i * a.part_step);
+    T *o = plain_at<T>(t, token, head, d);
     T e[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) e[i] = (T)x[i];
