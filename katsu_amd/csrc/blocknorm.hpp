@@ -100,9 +100,9 @@ struct NormBwdArgs {
 };
 
 template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_bwd_kernel(
+__global__ void __launch_bounds__(TPR == 64 ? 256 : TPR) block_norm_bwd_kernel(
     const NormBwdArgs a) {
-    constexpr int E = Piece<T>::E, RPB = TPR < 256 ? 256 / TPR : 1;
+    constexpr int E = Piece<T>::E, RPB = TPR == 64 ? 4 : 1;
     __shared__ float part[2][2][16];
     const int set = blockIdx.x * RPB + (RPB > 1 ? threadIdx.x / TPR : 0);
     const int lane = threadIdx.x % TPR;
@@ -194,21 +194,25 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_bwd_kernel(
     }
 }
 
-// Column sums of the parts, in order within each of a block's 4 waves, then the waves'.
+// Column sums of the parts, in order within each of a block's 16 waves, then the waves'.
 template <typename T>
-__global__ void __launch_bounds__(256) block_norm_sum_kernel(const float *part, int sets,
+__global__ void __launch_bounds__(1024) block_norm_sum_kernel(const float *part, int sets,
                                                              int64_t cols, int sums, T *w_pre,
                                                              T *w_post, T *gate) {
-    __shared__ float s[4][64];
+    __shared__ float s[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, which = blockIdx.y;
     const int64_t c = (int64_t)blockIdx.x * 64 + lane;
     float v = 0.f;
-    if (c < cols)
-        for (int i = wave; i < sets; i += 4) v += part[((int64_t)i * sums + which) * cols + c];
+    if (c < cols) {
+#pragma unroll 8
+        for (int i = wave; i < sets; i += 16) v += part[((int64_t)i * sums + which) * cols + c];
+    }
     s[wave][lane] = v;
     __syncthreads();
     if (wave != 0 || c >= cols) return;
-    v = ((s[0][lane] + s[1][lane]) + s[2][lane]) + s[3][lane];
+    v = s[0][lane];
+#pragma unroll
+    for (int w = 1; w < 16; ++w) v += s[w][lane];
     // Of the three, those that there are follow each other in this order.
     const int n = (w_pre != nullptr) + (w_post != nullptr);
     T *out = which == 0 && w_pre ? w_pre : which < n ? w_post : gate;

@@ -24,13 +24,14 @@ struct ClipTable {
     int n;
 };
 
-// Calls f(tensor, first value, values) for this block's chunks.
-template <class F>
+// Calls f(tensor, first value, values) for this block's chunks; BACK: the last ones first.
+template <bool BACK, class F>
 __device__ __forceinline__ void each_chunk(const ClipTable &t, F f) {
     const uint32_t total = t.first[t.n];
-    int k = 0;
-    for (uint32_t c = blockIdx.x; c < total; c += gridDim.x) {
-        while (t.first[k + 1] <= c) ++k;
+    int k = BACK ? t.n - 1 : 0;
+    for (uint32_t i = blockIdx.x; i < total; i += gridDim.x) {
+        const uint32_t c = BACK ? total - 1 - i : i;
+        while (BACK ? t.first[k] > c : t.first[k + 1] <= c) k += BACK ? -1 : 1;
         const int64_t at = (int64_t)(c - t.first[k]) * kClipChunk;
         const int64_t left = t.count[k] - at;
         f(k, at, left < kClipChunk ? (int)left : kClipChunk);
@@ -73,7 +74,7 @@ __device__ __forceinline__ double block_sum_f64(double v, double *part) {
 __global__ void __launch_bounds__(256) clip_squares_kernel(const ClipTable t, double *parts) {
     __shared__ double part[4];
     double s = 0.;
-    each_chunk(t, [&](int k, int64_t at, int n) {
+    each_chunk<false>(t, [&](int k, int64_t at, int n) {
         s += t.half[k] ? squares((const __bf16 *)t.in[k] + at, n)
                        : squares((const float *)t.in[k] + at, n);
     });
@@ -90,7 +91,8 @@ __global__ void __launch_bounds__(256) clip_scale_kernel(const ClipTable t, cons
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)s;
     const double q = (double)max_norm / (s + 1e-6);
     const float by = q >= 1. ? 1.f : (float)q;  // a norm that is NaN gives NaN
-    each_chunk(t, [&](int k, int64_t at, int n) {
+    // Backwards: what the sums read last is in the 256 MB cache still.
+    each_chunk<true>(t, [&](int k, int64_t at, int n) {
         if (by == 1.f && t.in[k] == t.out[k]) return;  // in place, nothing to do
         if (t.half[k])
             scale_chunk((const __bf16 *)t.in[k] + at, (__bf16 *)t.out[k] + at, n, by);

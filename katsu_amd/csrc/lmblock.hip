@@ -74,24 +74,50 @@ int launch_norm(const NormArgs &a, hipStream_t st) {
     });
 }
 
-// Sets of rows, each one part of the column sums: two blocks of 256 threads a CU.
+// The gradient holds five values and three sums of each of a thread's elements: one piece a
+// thread while a block can have that many.
+int bwd_threads(int64_t pieces) {
+    return pieces <= 64 ? 64 : pieces <= 128 ? 128 : pieces <= 256 ? 256 : pieces <= 512 ? 512 : 1024;
+}
+template <typename T, class F>
+int by_row_size_bwd(int64_t cols, F f) {
+    const int64_t pieces = cdiv(cols, Piece<T>::E);
+    std::integral_constant<int, 1> one;
+    switch (bwd_threads(pieces)) {
+        case 64: return f(std::integral_constant<int, 64>(), one);
+        case 128: return f(std::integral_constant<int, 128>(), one);
+        case 256: return f(std::integral_constant<int, 256>(), one);
+        case 512: return f(std::integral_constant<int, 512>(), one);
+        default: break;
+    }
+    if (pieces <= 1024) return f(std::integral_constant<int, 1024>(), one);
+    if (pieces <= 2048)
+        return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
+    if constexpr (sizeof(T) == 4)
+        return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+    return KATSU_E_INVALID;
+}
+
+// Sets of rows, each one part of the column sums: 16 waves a CU, but no more parts than an
+// eighth of the rows, whose bytes they then stay well below.
 int norm_sets(int dtype, int64_t rows, int64_t cols) {
-    const int64_t pieces = cdiv(cols, dtype == KATSU_F32 ? 4 : 8);
-    return (int)std::min<int64_t>(rows, pieces <= 128 ? 2048 : pieces <= 512 ? 512 : 256);
+    const int threads = bwd_threads(cdiv(cols, dtype == KATSU_F32 ? 4 : 8));
+    const int64_t most = std::min<int64_t>(2048, 256 * 1024 / threads);
+    return (int)std::min(rows, std::min(most, std::max<int64_t>(256, rows / 8)));
 }
 
 template <typename T>
 int launch_norm_bwd(const NormBwdArgs &a, void *dw_pre, void *dw_post, void *dgate,
                     hipStream_t st) {
-    const int rc = a.sets == 0 ? KATSU_OK : by_row_size<T>(a.cols, [&](auto tpr, auto nv) {
+    const int rc = a.sets == 0 ? KATSU_OK : by_row_size_bwd<T>(a.cols, [&](auto tpr, auto nv) {
         constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
-        constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+        constexpr int RPB = TPR == 64 ? 4 : 1;
         block_norm_bwd_kernel<T, TPR, NV>
-            <<<dim3((unsigned)cdiv(a.sets, RPB)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(a);
+            <<<dim3((unsigned)cdiv(a.sets, RPB)), dim3(RPB * TPR), 0, st>>>(a);
         return status_of(hipGetLastError());
     });
     if (rc != KATSU_OK || a.sums == 0) return rc;
-    block_norm_sum_kernel<T><<<dim3((unsigned)cdiv(a.cols, 64), a.sums), 256, 0, st>>>(
+    block_norm_sum_kernel<T><<<dim3((unsigned)cdiv(a.cols, 64), a.sums), 1024, 0, st>>>(
         a.part, a.sets, a.cols, a.sums, (T *)dw_pre, (T *)dw_post,
         a.gate && a.gate_row == 0 ? (T *)dgate : nullptr);
     return status_of(hipGetLastError());
