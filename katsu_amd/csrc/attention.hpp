@@ -38,6 +38,7 @@ struct AttnTensor {
     const void *p;
     int64_t token, head;
 };
+enum AttnOrder { kByPlace, kByWork, kInPairs };
 struct AttnArgs {
     AttnTensor q, k, v, out, dout, dq, dk, dv;
     float *lse;                       // [H][Tq]
@@ -48,6 +49,7 @@ struct AttnArgs {
     float scale, scale2;              // of the scores; times log2(e)
     int slots, splits;                // tiles of all sequences; runs of the other axis's tiles
     int parts, each;                  // dk, dv: blocks a key tile and head; one head a block
+    int order;                        // AttnOrder
     float *part, *part_ml;            // the runs' sums; their rows' maxima and totals
 };
 
@@ -71,9 +73,37 @@ struct AttnSeq {
 };
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// The last sequence whose first slot is not beyond `slot`; 64 candidates a step.
-__device__ __forceinline__ AttnSeq find_seq(const AttnArgs &a, const int32_t *cu, int64_t total,
-                                            int mult, int unit, int slot, int lane) {
+__device__ __forceinline__ AttnSeq seq_at(const AttnArgs &a, int s) {
+    AttnSeq r;
+    r.s = s;
+    const int64_t qa = a.cu_q ? cu_at(a.cu_q, s, a.Tq) : 0;
+    const int64_t qb = a.cu_q ? cu_at(a.cu_q, s + 1, a.Tq) : a.Tq;
+    const int64_t ka = a.cu_k ? cu_at(a.cu_k, s, a.Tk) : 0;
+    const int64_t kb = a.cu_k ? cu_at(a.cu_k, s + 1, a.Tk) : a.Tk;
+    int64_t lk = kb > ka ? kb - ka : 0;
+    if (a.k_lens) {
+        const int64_t c = a.k_lens[s];
+        lk = c < 0 ? 0 : c < lk ? c : lk;
+    }
+    r.q0 = uni((int)qa);
+    r.lq = uni((int)(qb > qa ? qb - qa : 0));
+    r.k0 = uni((int)ka);
+    r.lk = uni((int)lk);
+    return r;
+}
+
+// The sequence and the tile in it that the rank-th of a launch's `slots` places works on:
+// false if none.
+struct AttnTile {
+    AttnSeq seq;
+    int at;
+};
+// By place, from the last: the last sequence whose first slot is not beyond it, 64
+// candidates a step.
+__device__ __forceinline__ bool tile_by_place(const AttnArgs &a, const int32_t *cu, int64_t total,
+                                              int mult, int unit, int rank, int lane,
+                                              AttnTile &t) {
+    const int slot = a.slots - 1 - rank;
     int lo = 0, n = a.B;
     if (cu) {
         while (n > 1) {
@@ -84,23 +114,62 @@ __device__ __forceinline__ AttnSeq find_seq(const AttnArgs &a, const int32_t *cu
             n = min(step, n - at);
         }
     }
-    AttnSeq r;
-    lo = uni(lo);
-    r.s = lo;
-    const int64_t qa = a.cu_q ? cu_at(a.cu_q, lo, a.Tq) : 0;
-    const int64_t qb = a.cu_q ? cu_at(a.cu_q, lo + 1, a.Tq) : a.Tq;
-    const int64_t ka = a.cu_k ? cu_at(a.cu_k, lo, a.Tk) : 0;
-    const int64_t kb = a.cu_k ? cu_at(a.cu_k, lo + 1, a.Tk) : a.Tk;
-    int64_t lk = kb > ka ? kb - ka : 0;
-    if (a.k_lens) {
-        const int64_t c = a.k_lens[lo];
-        lk = c < 0 ? 0 : c < lk ? c : lk;
+    t.seq = seq_at(a, uni(lo));
+    t.at = slot - uni(first_slot(cu, t.seq.s, total, mult, unit));
+    return true;
+}
+// By work, the longest first: with a causal mask tile j of a sequence has j + 1 tiles' work,
+// so the ranks go down the levels j, and at each through the sequences that have a tile
+// there.  Up to 64 sequences (a lane each); 64 levels a step, one a lane.  In order of place
+// a launch ends on its longest tiles (2711, 1024, 1777 and 488 tokens packed: 83 us; 78 so).
+// In pairs: where all blocks are on the card at once, two a CU, the second half goes up the
+// levels, so that a CU's two together have the same work as any other's.
+__device__ __forceinline__ bool tile_by_work(const AttnArgs &a, const int32_t *cu, int64_t total,
+                                             int mult, int unit, int rank, int lane,
+                                             AttnTile &t) {
+    if (a.order == kByPlace || a.B > 64) return tile_by_place(a, cu, total, mult, unit, rank, lane, t);
+    int n = 0;  // this lane's sequence's tiles
+    if (lane < a.B) {
+        const int64_t len = cu ? cu_at(cu, lane + 1, total) - cu_at(cu, lane, total) : total;
+        n = len > 0 ? (int)((len * mult + unit - 1) / unit) : 0;
     }
-    r.q0 = uni((int)qa);
-    r.lq = uni((int)(qb > qa ? qb - qa : 0));
-    r.k0 = uni((int)ka);
-    r.lk = uni((int)lk);
-    return r;
+    int most = n, all = n;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        most = max(most, __shfl_xor(most, off, 64));
+        all += __shfl_xor(all, off, 64);
+    }
+    most = uni(most);
+    all = uni(all);
+    if (rank >= all) return false;
+    const int half = (all + 1) / 2;
+    if (a.order == kInPairs && rank >= half) rank = all - 1 - (rank - half);
+    int before = 0, level = 0;
+    for (int top = most; top > 0; top -= 64) {
+        const int l = top - 1 - lane;
+        int c = 0;
+        for (int s = 0; s < a.B; ++s) c += l >= 0 && __builtin_amdgcn_readlane(n, s) > l;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int up = __shfl_up(c, off, 64);
+            c += lane >= off ? up : 0;
+        }
+        const uint64_t over = __ballot(before + c > rank);
+        if (over) {
+            const int f = __builtin_ctzll(over);
+            level = top - 1 - f;
+            if (f > 0) before += __builtin_amdgcn_readlane(c, f - 1);
+            break;
+        }
+        before += __builtin_amdgcn_readlane(c, 63);
+    }
+    const bool has = n > level;
+    const uint64_t ones = __ballot(has);
+    const int mine = __popcll(ones & (((uint64_t)1 << lane) - 1));
+    const uint64_t which = __ballot(has && mine == rank - before);
+    t.seq = seq_at(a, uni(which ? __builtin_ctzll(which) : 0));
+    t.at = uni(level);
+    return which != 0;
 }
 
 // ---- tiles in LDS -------------------------------------------------------------
@@ -131,8 +200,31 @@ __device__ __forceinline__ V lds_read(lds_at a) {
     return *(const __attribute__((address_space(3))) V *)(uintptr_t)a;
 }
 
-typedef __attribute__((address_space(3))) void attn_lds_void;
 constexpr int kAttnOOB = (int)0x80000000;  // beyond any tile: such a load returns zero
+
+// A buffer of `bytes` from base: what lies past its end reads as zero.
+__device__ __forceinline__ uintx4 attn_buffer(const void *base, int bytes) {
+    const uint64_t p = (uint64_t)(uintptr_t)base;
+    return uintx4{(uint32_t)uni((int)(uint32_t)p), (uint32_t)uni((int)(uint32_t)(p >> 32)) & 0xffffu,
+                  (uint32_t)uni(bytes), 0x00020000u};
+}
+// Loads to LDS directly: lane l's 16 (or 4) bytes go to `to` + 16 l (4 l).  Written out, as
+// the compiler has a transposing LDS read wait for every load of the builtin's that is in
+// flight, also into another tile; nothing waits for these but attn_wait_dma.  They have no
+// output register.  M0 is reserved, and nothing else here uses it; the wait state is what it
+// needs between its write and its use.
+__device__ __forceinline__ void dma_b128(uintx4 rs, int off, lds_at to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :
+                 : "v"(off), "s"(rs), "s"(uni((int)to))
+                 : "memory");
+}
+__device__ __forceinline__ void dma_b32(uintx4 rs, int off, lds_at to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
+                 :
+                 : "v"(off), "s"(rs), "s"(uni((int)to))
+                 : "memory");
+}
 
 // Copies a tile of ROWS rows to LDS, spread over NW waves, of which this is
 // wave w.  DMA: by loads that go to LDS directly, 16 bytes a lane, not waited
@@ -168,12 +260,10 @@ struct TileCopy {
         valid = min(valid, ROWS);
         if constexpr (DMA) {
             const int bytes = valid > 0 ? (valid - 1) * (int)stride + row_bytes : 0;
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<char *>(base), (short)0, bytes, 0x00020000);
+            const uintx4 rs = attn_buffer(base, bytes);
+            const lds_at to = lds_addr(lds) + w * N * 1024;
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    rs, (attn_lds_void *)(lds + (w * N + i) * 1024), 16, off[i], 0, 0, 0);
+            for (int i = 0; i < N; ++i) dma_b128(rs, off[i], to + i * 1024);
         } else {
             for (int c = w * 64 + lane; c < ROWS * R::CH; c += NW * 64) {
                 const int r = c / R::CH, ch = c % R::CH;
@@ -281,8 +371,12 @@ __device__ __forceinline__ int reg_row(int v, int h) { return 8 * (v >> 2) + 4 *
 
 // The LDS reads of a product are kept one step ahead of its matrix instructions, and no
 // further: the compiler would put all of them in front, and has no registers for them.  The
-// fence keeps reads and matrix instructions in their steps; vector instructions may cross it.
-__device__ __forceinline__ void step_fence() { __builtin_amdgcn_sched_barrier(0x277); }
+// fence keeps reads (HARD: and matrix instructions) in their steps; vector instructions may
+// cross it.
+template <bool HARD>
+__device__ __forceinline__ void step_fence() {
+    __builtin_amdgcn_sched_barrier(HARD ? 0x676 : 0x277);
+}
 
 template <int ND>
 struct ColFrags {
@@ -297,7 +391,7 @@ __device__ __forceinline__ ColFrags<ND> col_frags(lds_at col, int r0, int f) {
 }
 // acc[d] += (channels 32*d .. of the tile's rows r0 .. r0 + 31)^T x; `c` is the first step's
 // operand, read already.  `ahead` reads what follows the product during its last step.
-template <typename T, int ND, class F>
+template <typename T, int ND, bool HARD, class F>
 __device__ __forceinline__ void col_product(floatx16 (&acc)[ND], lds_at col, int r0,
                                             ColFrags<ND> c, const floatx16 &x, F ahead) {
     constexpr int NF = Rows<T, ND>::NF;
@@ -311,36 +405,39 @@ __device__ __forceinline__ void col_product(floatx16 (&acc)[ND], lds_at col, int
         const uintx4 p = reg_frag<T>(x, f);
 #pragma unroll
         for (int d = 0; d < ND; ++d) acc[d] = attn_mma<T>(c.x[d], p, acc[d]);
-        step_fence();
+        step_fence<HARD>();
         if (f + 1 < NF) c = n;
     }
 }
-// acc += (rows r0 .. of the tile at row) . b(step), over the channels, two fragments a step.
-template <typename T, int ND, class B, class F>
-__device__ __forceinline__ void row_product(floatx16 &acc, lds_at row, int r0, B b, F ahead) {
-    constexpr int NS = Rows<T, ND>::NS;
-    uintx4 c[2], n[2], y[2], z[2];
+// acc[i] += (rows r0 + 32 i .. of the tile at row) . b(step), over the channels, for NB
+// blocks of 32 rows; a step is S fragments.
+template <typename T, int ND, int NB, int S, bool HARD, class B, class F>
+__device__ __forceinline__ void row_product(floatx16 (&acc)[NB], lds_at row, int r0, B b, F ahead) {
+    constexpr int NS = Rows<T, ND>::NS, N = NB * NS;
+    uintx4 c[S], n[S], y[S], z[S];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (i < NS) {
-            c[i] = row_frag<T, ND>(row, r0, i);
-            y[i] = b(i);
+    for (int i = 0; i < S; ++i)
+        if (i < N) {
+            c[i] = row_frag<T, ND>(row, r0 + 32 * (i / NS), i % NS);
+            y[i] = b(i % NS);
         }
+    if (HARD) step_fence<true>();
 #pragma unroll
-    for (int st = 0; st < NS; st += 2) {
+    for (int st = 0; st < N; st += S) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (st + 2 + i < NS) {
-                n[i] = row_frag<T, ND>(row, r0, st + 2 + i);
-                z[i] = b(st + 2 + i);
+        for (int i = 0; i < S; ++i)
+            if (st + S + i < N) {
+                n[i] = row_frag<T, ND>(row, r0 + 32 * ((st + S + i) / NS), (st + S + i) % NS);
+                z[i] = b((st + S + i) % NS);
             }
-        if (st + 2 >= NS) ahead();
+        if (st + S >= N) ahead();
+        if (HARD) step_fence<true>();
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (st + i < NS) acc = attn_mma<T>(c[i], y[i], acc);
-        step_fence();
+        for (int i = 0; i < S; ++i)
+            if (st + i < N) acc[(st + i) / NS] = attn_mma<T>(c[i], y[i], acc[(st + i) / NS]);
+        step_fence<HARD>();
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < S; ++i) {
             c[i] = n[i];
             y[i] = z[i];
         }
@@ -386,6 +483,13 @@ __device__ __forceinline__ void load_row(const AttnTensor &t, int64_t token, int
         }
         f[s] = u;
     }
+}
+// Waits here for loads to registers: where their first use lies in a loop, the compiler has
+// every turn of it wait for all loads in flight.
+template <int N>
+__device__ __forceinline__ void loaded(uintx4 (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
 }
 // Channels 32*db + 8g + 4h .. + 3 (registers 4g .. 4g+3 of x) of a row, times `by`.
 template <typename T, bool VEC>

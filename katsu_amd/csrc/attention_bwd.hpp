@@ -4,6 +4,9 @@
 //   delta_i = do_i . o_i          dP = do v^T          dS = P (dP - delta)
 //   dq = scale dS k               dk = scale dS^T q    dv = P^T do
 //
+// Rows of 128 channels have no registers for hard fences around the row products (4096
+// tokens, 16/4 heads of 128, bfloat16: 508 us with, 485 without; heads of 64: 258 and 263).
+//
 // Two kernels and no atomics: the sums over keys (dq) and over queries (dk, dv) each stay
 // in the registers of the wave that owns the row.  That computes the scores and dP twice,
 // seven products for five, and gives the same bits on every call.
@@ -28,13 +31,13 @@ struct AttnDq {
     __device__ static __forceinline__ void probs(lds_at row, const uintx4 (&qf)[NS],
                                                  const uintx4 (&gf)[NS], floatx16 &p, floatx16 &g,
                                                  float lse2, float scale2, int b) {
-        floatx16 s = {};
-        g = floatx16{};
-        row_product<T, ND>(s, row, 32 * b, [&](int st) { return qf[st]; }, [] {});
-        row_product<T, ND>(g, row + kTile, 32 * b, [&](int st) { return gf[st]; }, [] {});
+        floatx16 s[1] = {}, x[1] = {};
+        row_product<T, ND, 1, 2, R::W == 64>(s, row, 32 * b, [&](int st) { return qf[st]; }, [] {});
+        row_product<T, ND, 1, 2, R::W == 64>(x, row + kTile, 32 * b, [&](int st) { return gf[st]; }, [] {});
+        g = x[0];
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-            p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], scale2, -lse2));
+            p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][v], scale2, -lse2));
     }
     __device__ static __forceinline__ void tile(lds_at row, lds_at col, const uintx4 (&qf)[NS],
                                                 const uintx4 (&gf)[NS], floatx16 (&dq)[ND],
@@ -51,7 +54,7 @@ struct AttnDq {
                 for (int v = 0; v < 16; ++v)
                     if (32 * b + reg_row(v, h) > jmax) g[v] = 0.f;
             }
-            col_product<T, ND>(dq, col, 32 * b, col_frags<T, ND>(col, 32 * b, 0), g, [] {});
+            col_product<T, ND, true>(dq, col, 32 * b, col_frags<T, ND>(col, 32 * b, 0), g, [] {});
         }
     }
 
@@ -60,11 +63,11 @@ struct AttnDq {
         const int l31 = lane & 31, h = lane >> 5;
         const unsigned id = blockIdx.x;
         const int kvh = id % a.Hkv, split = id / a.Hkv % a.splits;
-        const int slot = a.slots - 1 - (int)(id / a.Hkv / a.splits);
-        const AttnSeq sq = find_seq(a, a.cu_q, a.Tq, a.G, BM, slot, lane);
-        const int64_t rows = (int64_t)sq.lq * a.G;
-        const int64_t row0 =
-            (int64_t)(slot - uni(first_slot(a.cu_q, sq.s, a.Tq, a.G, BM))) * BM;
+        AttnTile tl;
+        if (!tile_by_work(a, a.cu_q, a.Tq, a.G, BM, (int)(id / a.Hkv / a.splits), lane, tl))
+            return;
+        const AttnSeq sq = tl.seq;
+        const int64_t rows = (int64_t)sq.lq * a.G, row0 = (int64_t)tl.at * BM;
         if (row0 >= rows) return;
         const int64_t r = row0 + wave * 32 + l31;
         const bool valid = r < rows;
@@ -113,6 +116,9 @@ struct AttnDq {
         delta = half_sum(delta);
         const float lse2 = valid ? a.lse[at] * kLog2e : 0.f;
         load_row<T, ND, VEC>(a.q, token, head, valid, a.D, h, qf);
+        loaded(qf);
+        loaded(gf);
+        asm volatile("" ::"v"(lse2));
 
         floatx16 dq[ND] = {};
         bool bad = false;
@@ -205,7 +211,8 @@ struct AttnDkv {
                                                  floatx16 (&dk)[ND], floatx16 (&dv)[ND],
                                                  float scale2, int r0, bool mask, int ifirst,
                                                  int h) {
-        floatx16 s, g;
+        floatx16 sa[1], ga[1];
+        floatx16 &s = sa[0], &g = ga[0];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {  // sums that start from -lse / scale and -delta
             const floatx4 x = lds_read<floatx4>(stats + (r0 + 8 * q + 4 * h) * 4);
@@ -217,9 +224,9 @@ struct AttnDkv {
             }
         }
         ColFrags<ND> c;
-        row_product<T, ND>(s, row, r0, [&](int st) { return kf[st]; }, [] {});
-        row_product<T, ND>(
-            g, row + kTile, r0,
+        row_product<T, ND, 1, 2, R::W == 64>(sa, row, r0, [&](int st) { return kf[st]; }, [] {});
+        row_product<T, ND, 1, 2, R::W == 64>(
+            ga, row + kTile, r0,
             [&](int st) {
                 if constexpr (VLDS)
                     return row_frag<T, ND>(vrow, 0, st);
@@ -237,25 +244,27 @@ struct AttnDkv {
             for (int v = 0; v < 16; ++v)
                 if (r0 + reg_row(v, h) < ifirst) s[v] = g[v] = 0.f;
         }
-        col_product<T, ND>(dv, col + kTile, r0, c, s,
+        col_product<T, ND, true>(dv, col + kTile, r0, c, s,
                            [&] { c = col_frags<T, ND>(col, r0, 0); });
-        col_product<T, ND>(dk, col, r0, c, g, [] {});
+        col_product<T, ND, true>(dk, col, r0, c, g, [] {});
     }
 
     __device__ static void run(const AttnArgs &a, char *lds) {
         const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
         const int l31 = lane & 31, h = lane >> 5;
-        // Heads innermost; with a causal mask the keys that most queries see first.  A key
-        // head's queries are `parts` blocks' work: every head's tiles in `splits` runs, or
-        // (!each) all heads' together.
+        // A key head's queries are `parts` blocks' work: every head's tiles in `splits` runs,
+        // or (!each) all heads' together.
         const unsigned id = blockIdx.x;
         const int kvh = id % a.Hkv, p = id / a.Hkv % a.parts;
-        const int slot = (int)(id / a.Hkv / a.parts);
         const int split = p % a.splits;
         const int head0 = kvh * a.G + (a.each ? p / a.splits : 0), heads = a.each ? 1 : a.G;
-        const AttnSeq sq = find_seq(a, a.cu_k, a.Tk, 1, BK, slot, lane);
-        const int key0 = (slot - uni(first_slot(a.cu_k, sq.s, a.Tk, 1, BK))) * BK;
-        if (key0 >= sq.lk) return;
+        AttnTile tl;
+        if (!tile_by_work(a, a.cu_k, a.Tk, 1, BK, (int)(id / a.Hkv / a.parts), lane, tl))
+            return;
+        const AttnSeq sq = tl.seq;
+        // The first keys have the most queries: the work of the tiles from the end.
+        const int key0 = ((sq.lk + BK - 1) / BK - 1 - tl.at) * BK;
+        if (key0 < 0) return;
         const int wkey = key0 + wave * 32, key = wkey + l31;
         const bool valid = key < sq.lk;
         const int shift = sq.lk - sq.lq;
@@ -284,12 +293,9 @@ struct AttnDkv {
                 const int64_t at = (head0 + g) * a.Tq + sq.q0 + i;
                 const int bytes = min(left, QT) * 4;
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                        a.start + w * (a.H * a.Tq) + at, (short)0, bytes, 0x00020000);
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                        rs, (attn_lds_void *)(d + 2 * kTile + w * 256), 4, lane * 4, 0, 0, 0);
-                }
+                for (int w = 0; w < 2; ++w)
+                    dma_b32(attn_buffer(a.start + w * (a.H * a.Tq) + at, bytes), lane * 4,
+                            lds_addr(d + 2 * kTile + w * 256));
             }
         };
         const int per = (tiles * heads + a.splits - 1) / a.splits;
@@ -308,7 +314,9 @@ struct AttnDkv {
                     sq.lk - wkey, lds + wave * 32 * R::RB);
         } else {
             load_row<T, ND, VEC>(a.v, token, kvh, valid, a.D, h, vf);
+            loaded(vf);
         }
+        loaded(kf);
         floatx16 dk[ND] = {}, dv[ND] = {};
         bool bad = false;
         const lds_at row = row_lane<T, ND>(lane), col = col_lane<T, ND>(lane);

@@ -36,12 +36,10 @@ struct AttnFwd {
     __device__ static __forceinline__ void tile(lds_at row, lds_at col, const uintx4 (&qf)[NS],
                                                 floatx16 (&o)[ND], float &m, float &l,
                                                 float scale2, bool mask, int jmax, int h) {
-        floatx16 s[NB];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            s[b] = floatx16{};
-            row_product<T, ND>(s[b], row, 32 * b, [&](int st) { return qf[st]; }, [] {});
-        }
+        floatx16 s[NB] = {};
+        ColFrags<ND> c;
+        row_product<T, ND, NB, 4, true>(s, row, 0, [&](int st) { return qf[st]; },
+                                  [&] { c = col_frags<T, ND>(col, 0, 0); });
         if (mask) {
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -75,10 +73,9 @@ struct AttnFwd {
                 sum += s[b][v];
             }
         l += sum;
-        ColFrags<ND> c = col_frags<T, ND>(col, 0, 0);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
-            col_product<T, ND>(o, col, 32 * b, c, s[b], [&] {
+            col_product<T, ND, true>(o, col, 32 * b, c, s[b], [&] {
                 if (b + 1 < NB) c = col_frags<T, ND>(col, 32 * (b + 1), 0);
             });
     }
@@ -145,14 +142,16 @@ struct AttnFwd {
         const int l31 = lane & 31, h = lane >> 5;
         const int wm = WK > 1 ? 0 : wave, wk = WK > 1 ? wave : 0;
         // Key heads innermost (blocks go round-robin over the 8 XCDs, so an XCD's L2
-        // holds few heads' keys); with a causal mask the longest rows first.
+        // holds few heads' keys).
         const unsigned id = blockIdx.x;
         const int kvh = id % a.Hkv, split = id / a.Hkv % a.splits;
-        const int slot = a.slots - 1 - (int)(id / a.Hkv / a.splits);
-        const AttnSeq sq = find_seq(a, a.cu_q, a.Tq, a.G, BM, slot, lane);
-        const int64_t rows = (int64_t)sq.lq * a.G;
-        const int64_t row0 =
-            (int64_t)(slot - uni(first_slot(a.cu_q, sq.s, a.Tq, a.G, BM))) * BM;
+        const int rank = (int)(id / a.Hkv / a.splits);
+        AttnTile tl;
+        if (!(WK > 1 ? tile_by_place(a, a.cu_q, a.Tq, a.G, BM, rank, lane, tl)
+                     : tile_by_work(a, a.cu_q, a.Tq, a.G, BM, rank, lane, tl)))
+            return;
+        const AttnSeq sq = tl.seq;
+        const int64_t rows = (int64_t)sq.lq * a.G, row0 = (int64_t)tl.at * BM;
         if (row0 >= rows) return;
         const int64_t r = row0 + wm * 32 + l31;
         const int tok = (int)(r / a.G);
@@ -183,6 +182,7 @@ struct AttnFwd {
         if (t0 < t1) fetch(t0, 0);
         uintx4 qf[NS];
         load_row<T, ND, VEC>(a.q, me.token, me.head, me.valid, a.D, h, qf);
+        loaded(qf);
         floatx16 o[ND] = {};
         float m = -INFINITY, l = 0.f;
         bool bad = false;
