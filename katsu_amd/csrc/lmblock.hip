@@ -162,7 +162,7 @@ int rotary_table(float *table, int64_t length, int dim, double base, double fact
 }
 
 bool block_norm_ok(const katsu_block_norm &d) {
-    return dtype_ok(d.dtype) && d.gate_rows <= 2 && d.rows <= (uint64_t)kI32Max && d.cols > 0 &&
+    return dtype_ok(d.dtype) && d.gate_rows >= 0 && d.gate_rows <= 2 && d.rows <= (uint64_t)kI32Max && d.cols > 0 &&
            d.cols <= 16384 && std::isfinite(d.alpha) && d.eps >= 0.f && std::isfinite(d.eps);
 }
 
