@@ -73,10 +73,10 @@ AttnTensor tensor(const void *p, const int64_t (&stride)[2]) {
 // Channels of a row in LDS and in the parts.
 int width_of(const katsu_attention &d) { return d.head_dim <= 64 ? 64 : 128; }
 
-// Runs that an axis of `len` is split into: two blocks a CU, a run at least `least` long.
-int runs(int64_t blocks, int64_t len, int64_t least) {
+// Runs that an axis of `len` is split into: `want` blocks in all, a run at least `least` long.
+int runs(int64_t want, int64_t blocks, int64_t len, int64_t least) {
     return (int)std::max<int64_t>(
-        1, std::min(2 * kCUs / std::max<int64_t>(blocks, 1), cdiv(len, least)));
+        1, std::min(want / std::max<int64_t>(blocks, 1), cdiv(len, least)));
 }
 
 // The forward call's shape: tiles of 32 rows whose waves share the keys, or of 128.
@@ -92,10 +92,15 @@ FwdPlan fwd_plan(const katsu_attention &d) {
     p.bm = p.few ? 32 : 128;
     p.slots = (int)(rows / p.bm + B);
     const int64_t blocks = (int64_t)p.slots * (int64_t)d.kv_heads;
-    // A run's keys are worth more than the launch that joins the runs: in float32 two tiles
-    // (3.4 us each), in bfloat16 four.
-    p.splits = runs(blocks, cdiv((int64_t)d.tokens_k, B),
-                    d.dtype == KATSU_F32 ? (d.head_dim > 64 ? 64 : 128) : 256);
+    // A block a CU; a run's keys have to be worth the launch that joins the runs: single
+    // tokens 256 of them (32000 keys, 32/8 heads of 128: 34 us in 32 runs, 45 in 64; 4000: 15 in
+    // 16, 19 in 4), tiles of 128 rows 1024 in bfloat16 (1000 tokens, 16/4 heads of 128: 25 us in
+    // one run, 32 in four) and two tiles, 3.4 us each, in float32.
+    const int64_t keys = cdiv((int64_t)d.tokens_k, B);
+    if (d.dtype == KATSU_F32 && !p.few)
+        p.splits = runs(2 * kCUs, blocks, keys, d.head_dim > 64 ? 64 : 128);
+    else
+        p.splits = runs(kCUs, blocks, keys, p.few ? 256 : 1024);
     return p;
 }
 size_t part_floats(const katsu_attention &d, const FwdPlan &p) {
@@ -162,8 +167,8 @@ int launch_fwd(const AttnArgs &a, bool few, hipStream_t st) {
 
 // The backward call's shape.  dk and dv: blocks of one query head each, unless the key heads
 // alone give the card enough to do; in float32 always, as a sum over all of a group's rows
-// in one accumulator loses too much.  Both kernels: the other axis in runs of at least two
-// tiles where there are few blocks.
+// in one accumulator loses too much.  Both kernels: the other axis in runs where there are
+// few blocks.
 struct BwdPlan {
     int dq_slots, dq_splits, dkv_slots, dkv_splits, parts;
     bool each;
@@ -174,12 +179,12 @@ BwdPlan bwd_plan(const katsu_attention &d) {
     p.dq_slots = (int)((int64_t)d.tokens_q * group / 128 + B);
     p.dkv_slots = (int)((int64_t)d.tokens_k / 128 + B);
     p.each = group > 1 && (d.dtype == KATSU_F32 || p.dkv_slots * kv < 4 * kCUs);
-    // Keys of a run of dq, queries of one of dk and dv: two tiles.
-    const bool wide = d.head_dim > 64;
-    p.dq_splits = runs(p.dq_slots * kv, cdiv((int64_t)d.tokens_k, B),
-                       d.dtype == KATSU_F32 && wide ? 64 : 128);
-    p.dkv_splits = runs(p.dkv_slots * kv * (p.each ? group : 1),
-                        cdiv((int64_t)d.tokens_q, B) * (p.each ? 1 : group), wide ? 64 : 128);
+    // Keys of a run of dq, queries of one of dk and dv: two tiles in float32, 256 in bfloat16
+    // (1500 tokens, 8/8 heads of 64: 48 us; 51 with 512; 54 with one block a CU).
+    const int64_t least = d.dtype == KATSU_F32 ? d.head_dim > 64 ? 64 : 128 : 256;
+    p.dq_splits = runs(2 * kCUs, p.dq_slots * kv, cdiv((int64_t)d.tokens_k, B), least);
+    p.dkv_splits = runs(2 * kCUs, p.dkv_slots * kv * (p.each ? group : 1),
+                        cdiv((int64_t)d.tokens_q, B) * (p.each ? 1 : group), least);
     p.parts = (p.each ? (int)group : 1) * p.dkv_splits;
     return p;
 }
@@ -298,12 +303,18 @@ int attention_fwd(const katsu_attention &d, const void *q, const void *k, const 
         return launch_fwd<decltype(t), decltype(nd)::value, decltype(v)::value>(a, p.few, st);
     });
     if (rc != KATSU_OK || a.splits == 1) return rc;
-    const unsigned blocks = (unsigned)cdiv(a.Tq * a.H, 4);
-    if (d.dtype == KATSU_F32)
-        attention_join_kernel<float><<<blocks, 256, 0, st>>>(a, width);
-    else
-        attention_join_kernel<__bf16><<<blocks, 256, 0, st>>>(a, width);
-    return status_of(hipGetLastError());
+    // A wave a row, a block where there are parts enough for its waves.
+    const int64_t rows = a.Tq * a.H;
+    const bool many = a.splits >= 8;
+    auto join = [&](auto t) {
+        using T = decltype(t);
+        if (many)
+            attention_join_kernel<T, 4><<<dim3((unsigned)rows), 256, 0, st>>>(a, width);
+        else
+            attention_join_kernel<T, 1><<<dim3((unsigned)cdiv(rows, 4)), 256, 0, st>>>(a, width);
+        return status_of(hipGetLastError());
+    };
+    return d.dtype == KATSU_F32 ? join(float()) : join(__bf16());
 }
 
 size_t attention_bwd_bytes(const katsu_attention &d) {

@@ -262,27 +262,62 @@ __global__ void __launch_bounds__(64 * WM * WK, OCC) attention_fwd_kernel(const 
     AttnFwd<T, ND, WM, WK, BN, VEC>::run(a, lds);
 }
 
-// Joins the parts of the key axis: one wave a row, lane l channels l and l + 64.
-template <typename T>
+// Joins the parts of the key axis.  WPR waves a row, lane l channels l and l + 64: the lanes
+// hold the parts' weights, 64 of them at a time; each wave takes every WPR-th part, and the
+// waves' sums are added in order.
+template <typename T, int WPR>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, int W) {
-    const int lane = threadIdx.x & 63;
-    const int64_t rows = a.Tq * a.H, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    float M = -INFINITY, L = -1.f, x[2] = {0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s)
-        if (!(a.part_ml[(s * rows + row) * 2 + 1] < 0.f))
-            M = fmaxf(M, a.part_ml[(s * rows + row) * 2]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    for (int s = 0; s < a.splits; ++s) {
-        const float l = a.part_ml[(s * rows + row) * 2 + 1];
-        if (l < 0.f) continue;
-        const float by = __builtin_amdgcn_exp2f(a.part_ml[(s * rows + row) * 2] - ref);
-        L = (L < 0.f ? 0.f : L) + by * l;
+    __shared__ float sums[4][128];
+    const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
+    const int64_t rows = a.Tq * a.H;
+    const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
+    if (row >= rows) return;  // a whole wave, or (one row a block) never
+    const int first = WPR == 1 ? 0 : wave;
+    const float *ml = a.part_ml + row * 2;
+    float M = -INFINITY;
+    bool some = false;
+    for (int s = lane; s < a.splits; s += 64)
+        if (!(ml[s * rows * 2 + 1] < 0.f)) {  // no total is negative
+            M = fmaxf(M, ml[s * rows * 2]);
+            some = true;
+        }
+    some = __ballot(some) != 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (lane + 64 * i < a.D) x[i] += by * a.part[(s * rows + row) * W + lane + 64 * i];
+    for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+    const float ref = M == -INFINITY ? 0.f : M;
+    float L = 0.f, x[2] = {0.f, 0.f};
+    for (int s0 = 0; s0 < a.splits; s0 += 64) {
+        const int s = s0 + lane, n = min(a.splits - s0, 64);
+        float w = 0.f;
+        if (s < a.splits && !(ml[s * rows * 2 + 1] < 0.f)) {
+            w = __builtin_amdgcn_exp2f(ml[s * rows * 2] - ref);
+            L += w * ml[s * rows * 2 + 1];
+        }
+        const bool has = s < a.splits && !(ml[s * rows * 2 + 1] < 0.f);
+        const uint64_t there = __ballot(has);  // parts without a key hold nothing
+#pragma unroll 8
+        for (int i = first; i < n; i += WPR) {
+            if (!(there >> i & 1)) continue;
+            const float by = as_float(__builtin_amdgcn_readlane(as_bits(w), i));
+            const float *p = a.part + ((s0 + i) * rows + row) * W + lane;
+            if (lane < a.D) x[0] += by * p[0];
+            if (lane + 64 < a.D) x[1] += by * p[64];
+        }
     }
-    const bool some = !(L < 0.f);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) L += __shfl_xor(L, off, 64);
+    if constexpr (WPR > 1) {
+        sums[wave][lane] = x[0];
+        sums[wave][lane + 64] = x[1];
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[i] = sums[0][lane + 64 * i];
+#pragma unroll
+            for (int w = 1; w < WPR; ++w) x[i] += sums[w][lane + 64 * i];
+        }
+    }
     const int64_t token = row / a.H;
     const int head = (int)(row % a.H);
     T *p = plain_at<T>(a.out, token, head, 0);

@@ -258,9 +258,10 @@ def _dev_lm(first, *ts):
 
 def _heads(t, what):
     """A [tokens, heads, channels] tensor's strides; its channels must be adjacent."""
-    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+    s = t.stride()
+    if len(s) != 3 or (s[2] != 1 and t.shape[2] > 1):
         raise ValueError(f"{what} must be [tokens, heads, channels] with adjacent channels")
-    return t.stride(0), t.stride(1)
+    return s[:2]
 
 
 def _int32(t, n, dev, what):
@@ -312,7 +313,7 @@ def attention(q, k, v, cu_q=None, cu_k=None, k_lens=None, causal=True, scale=Non
     earlier one a key less.  A query that sees no key gives 0 and lse -inf.  scale: 1/sqrt(D)
     if None.  lse [H, Tq], float32, is what attention_backward takes.  `workspace`: an optional
     device tensor of attention_workspace_bytes(); without it the library's own buffer is used."""
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out is None else out
+    out = torch.empty_like(q) if out is None else out
     d = _attention(q, k, v, out, cu_q, cu_k, k_lens, causal, scale)
     lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32)
     check(lib().katsu_hip_attention_fwd_dev(ctypes.byref(d), _p(q), _p(k), _p(v), _p(cu_q),
@@ -327,9 +328,9 @@ def attention_backward(dout, q, k, v, out, lse, cu_q=None, cu_k=None, causal=Tru
     its out and lse.  Any token and head strides; `workspace` of
     attention_workspace_bytes(..., backward=True)."""
     d = _attention(q, k, v, out, cu_q, cu_k, None, causal, scale)
-    dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if dq is None else dq
-    dk = torch.empty(k.shape, device=q.device, dtype=q.dtype) if dk is None else dk
-    dv = torch.empty(v.shape, device=q.device, dtype=q.dtype) if dv is None else dv
+    dq = torch.empty_like(q) if dq is None else dq
+    dk = torch.empty_like(k) if dk is None else dk
+    dv = torch.empty_like(v) if dv is None else dv
     _dev_lm(q, dout, dq, dk, dv)
     if dout.shape != q.shape or dq.shape != q.shape or dk.shape != k.shape or dv.shape != k.shape:
         raise ValueError("gradients must have their operands' shapes")
@@ -363,9 +364,9 @@ def rotary(q, k, table, positions=None, interleaved=False, inverse=False, out_q=
     channels] (k may be None) turned by their tokens' positions, rows of `table` (int32; None:
     0, 1, ..).  Pairs are channels i and i + R/2, or neighbours with interleaved.  inverse turns
     back: the gradient of a turn.  The outputs may be the inputs."""
-    out_q = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out_q is None else out_q
+    out_q = torch.empty_like(q) if out_q is None else out_q
     if k is not None and out_k is None:
-        out_k = torch.empty(k.shape, device=q.device, dtype=q.dtype)
+        out_k = torch.empty_like(k)
     _dev_lm(q, k, out_q, out_k)
     tokens, heads, dim = q.shape if q.dim() == 3 else (0, 0, 0)
     strides = [(0, 0) if t is None else _heads(t, w)
