@@ -366,6 +366,20 @@ __device__ __forceinline__ uintx4 reg_frag(const floatx16 &x, int f) {
     }
     return u;
 }
+// What reg_frag leaves of x in bfloat16, rounded in turn: the two together hold 16 bits.
+__device__ __forceinline__ uintx4 reg_frag_rest(const floatx16 &x, int f, uintx4 hi) {
+    uintx4 u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t h = hi[i];
+        u[i] = __builtin_bit_cast(
+            uint32_t, __builtin_convertvector(floatx2{x[8 * f + 2 * i] - as_float(h << 16),
+                                                      x[8 * f + 2 * i + 1] -
+                                                          as_float(h & 0xffff0000u)},
+                                              bf16x2));
+    }
+    return u;
+}
 // The row of a result that register v of half h holds.
 __device__ __forceinline__ int reg_row(int v, int h) { return 8 * (v >> 2) + 4 * h + (v & 3); }
 
@@ -391,7 +405,8 @@ __device__ __forceinline__ ColFrags<ND> col_frags(lds_at col, int r0, int f) {
 }
 // acc[d] += (channels 32*d .. of the tile's rows r0 .. r0 + 31)^T x; `c` is the first step's
 // operand, read already.  `ahead` reads what follows the product during its last step.
-template <typename T, int ND, bool HARD, class F>
+// FINE: x in bfloat16 takes part with what the rounding leaves as well.
+template <typename T, int ND, bool HARD, bool FINE, class F>
 __device__ __forceinline__ void col_product(floatx16 (&acc)[ND], lds_at col, int r0,
                                             ColFrags<ND> c, const floatx16 &x, F ahead) {
     constexpr int NF = Rows<T, ND>::NF;
@@ -405,6 +420,11 @@ __device__ __forceinline__ void col_product(floatx16 (&acc)[ND], lds_at col, int
         const uintx4 p = reg_frag<T>(x, f);
 #pragma unroll
         for (int d = 0; d < ND; ++d) acc[d] = attn_mma<T>(c.x[d], p, acc[d]);
+        if constexpr (FINE) {
+            const uintx4 rest = reg_frag_rest(x, f, p);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) acc[d] = attn_mma<T>(c.x[d], rest, acc[d]);
+        }
         step_fence<HARD>();
         if (f + 1 < NF) c = n;
     }

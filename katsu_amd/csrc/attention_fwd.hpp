@@ -75,7 +75,7 @@ struct AttnFwd {
         l += sum;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
-            col_product<T, ND, true>(o, col, 32 * b, c, s[b], [&] {
+            col_product<T, ND, true, false>(o, col, 32 * b, c, s[b], [&] {
                 if (b + 1 < NB) c = col_frags<T, ND>(col, 32 * (b + 1), 0);
             });
     }
