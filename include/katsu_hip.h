@@ -32,7 +32,8 @@
  *
  * Library scratch: the *_dev entry points that need device scratch (the dW
  * split partials when no workspace is passed, the GEMM's split-K partials,
- * the sum's chunk partials, Grad-CAM's channel weights) take it from one
+ * the sum's chunk partials, Grad-CAM's channel weights, the language-model
+ * operators' partials) take it from one
  * buffer per purpose that the library keeps and shares across all streams
  * and graphs: an eager call sizes it, and a later capture of the same call
  * on any stream uses it without allocating.  Calls (or graph replays) that

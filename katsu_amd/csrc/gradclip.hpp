@@ -5,7 +5,8 @@
 // arguments: the first sums squares into one float64 part a block, the second has every
 // block add the parts in the same order and scale its share.  Squares are summed in
 // float64: they cannot overflow, and HBM is the bound either way (one fused
-// multiply-add for 2 or 4 bytes read).
+// multiply-add for 2 or 4 bytes read).  770 M bfloat16 values, not in place: 878 us, the sums
+// 278 (5.5 TB/s), the scaling 599 (5.1); 3.4 M float32 values in 26 tensors: 14 us of launches.
 #pragma once
 
 #include "lmvec.hpp"
@@ -62,8 +63,7 @@ __device__ __forceinline__ double squares(const T *p, int n) {
     return s[0] + s[1];
 }
 // Four pieces are read before the first is written: p and q may be the same memory, so the
-// compiler would wait for each in turn (770 M bfloat16 values, both launches: 1296 against
-// 1005 us).
+// compiler would wait for each in turn (770 M bfloat16 values: 903 us against 573).
 template <typename T>
 __device__ __forceinline__ void scale_chunk(const T *p, T *q, int n, float by) {
     constexpr int E = Piece<T>::E, U = 4;
