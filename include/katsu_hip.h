@@ -297,7 +297,7 @@ typedef enum katsu_dtype { KATSU_F32 = 0, KATSU_BF16 = 1 } katsu_dtype;
  * With causal set query i of Lq sees key j of Lk if j <= i + Lk - Lq: the last
  * query sees every key.  A query that sees none gives out 0 and lse -inf.
  * What masked places hold changes nothing, Inf and NaN included.
- * scale must be positive and finite. */
+ * scale must be positive and finite; an output's strides must not be zero. */
 typedef struct katsu_attention {
     int32_t dtype;  /* katsu_dtype of q, k, v, out */
     int32_t causal;

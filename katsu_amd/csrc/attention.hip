@@ -253,9 +253,14 @@ int launch_bwd(AttnArgs a, const BwdPlan &p, hipStream_t st) {
 
 }  // namespace
 
-bool attention_grads_ok(const katsu_attention_grads &g) {
-    return strides_ok(g.dout_stride) && strides_ok(g.dq_stride) && strides_ok(g.dk_stride) &&
-           strides_ok(g.dv_stride);
+// An output's places are its own: no broadcast strides.
+bool attention_out_ok(const int64_t (&s)[2], uint64_t tokens, uint64_t heads) {
+    return strides_ok(s) && (tokens < 2 || s[0] > 0) && (heads < 2 || s[1] > 0);
+}
+bool attention_grads_ok(const katsu_attention &d, const katsu_attention_grads &g) {
+    return strides_ok(g.dout_stride) && attention_out_ok(g.dq_stride, d.tokens_q, d.heads) &&
+           attention_out_ok(g.dk_stride, d.tokens_k, d.kv_heads) &&
+           attention_out_ok(g.dv_stride, d.tokens_k, d.kv_heads);
 }
 
 bool attention_ok(const katsu_attention &d) {
@@ -264,16 +269,16 @@ bool attention_ok(const katsu_attention &d) {
         return false;
     if (d.head_dim == 0 || d.head_dim > 128) return false;
     if (!(d.scale > 0.f) || !std::isfinite(d.scale)) return false;
-    if (d.tokens_q > (uint64_t)kI32Max || d.tokens_k > (uint64_t)kI32Max ||
-        d.seqs > (uint64_t)kI32Max)
-        return false;
+    // Tokens are counted in 32 bits, a tile beyond the last included.
+    const uint64_t most = (uint64_t)kI32Max - 65535;
+    if (d.tokens_q > most || d.tokens_k > most || d.seqs > most) return false;
     if (!strides_ok(d.q_stride) || !strides_ok(d.k_stride) || !strides_ok(d.v_stride) ||
         !strides_ok(d.out_stride))
         return false;
     // Tiles and blocks are counted in 32 bits.
     const uint64_t group = d.heads / d.kv_heads;
     const uint64_t rows = std::max(d.tokens_q * group, d.tokens_k * group);
-    return (rows / 32 + d.seqs) * d.kv_heads < (uint64_t)kI32Max / 4 &&
+    return (rows / 32 + d.seqs * group) * d.kv_heads < (uint64_t)kI32Max / 4 &&
            std::max(d.tokens_q, d.tokens_k) * d.heads < (uint64_t)kI32Max * 4;
 }
 

@@ -282,7 +282,10 @@ struct TileCopy {
         }
     }
 };
-__device__ __forceinline__ void attn_wait_dma() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Also for this wave's reads of LDS: the next loads go where the last tile was read.
+__device__ __forceinline__ void attn_wait_dma() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+}
 
 // ---- fragments and products ---------------------------------------------------
 

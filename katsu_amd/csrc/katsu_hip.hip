@@ -3254,7 +3254,8 @@ int katsu_hip_attention_fwd_dev(const katsu_attention *d, const void *q, const v
                                 const void *v, const int32_t *cu_q, const int32_t *cu_k,
                                 const int32_t *k_lens, void *out, float *lse, void *workspace,
                                 size_t workspace_bytes, void *stream) {
-    if (!d || !attention_ok(*d)) return KATSU_E_INVALID;
+    if (!d || !attention_ok(*d) || !attention_out_ok(d->out_stride, d->tokens_q, d->heads))
+        return KATSU_E_INVALID;
     if (d->seqs == 0 || d->tokens_q == 0) return KATSU_OK;
     if (!q || !out || (d->tokens_k > 0 && (!k || !v))) return KATSU_E_INVALID;
     if ((!cu_q || !cu_k) && (d->seqs != 1 || cu_q || cu_k)) return KATSU_E_INVALID;
@@ -3276,7 +3277,7 @@ int katsu_hip_attention_bwd_dev(const katsu_attention *d, const katsu_attention_
                                 const void *out, const float *lse, const int32_t *cu_q,
                                 const int32_t *cu_k, void *dq, void *dk, void *dv,
                                 void *workspace, size_t workspace_bytes, void *stream) {
-    if (!d || !g || !attention_ok(*d) || !attention_grads_ok(*g)) return KATSU_E_INVALID;
+    if (!d || !g || !attention_ok(*d) || !attention_grads_ok(*d, *g)) return KATSU_E_INVALID;
     if (d->seqs == 0 || (d->tokens_q == 0 && d->tokens_k == 0)) return KATSU_OK;
     if (d->tokens_q > 0 && (!dout || !q || !out || !lse || !dq)) return KATSU_E_INVALID;
     if (d->tokens_k > 0 && (!k || !v || !dk || !dv)) return KATSU_E_INVALID;

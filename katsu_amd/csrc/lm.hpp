@@ -20,7 +20,9 @@ int attention_fwd(const katsu_attention &d, const void *q, const void *k, const 
                   float *lse, void *ws, hipStream_t st);
 
 
-bool attention_grads_ok(const katsu_attention_grads &g);
+// Whether a tensor of these strides can be written; whether the gradients can.
+bool attention_out_ok(const int64_t (&stride)[2], uint64_t tokens, uint64_t heads);
+bool attention_grads_ok(const katsu_attention &d, const katsu_attention_grads &g);
 size_t attention_bwd_bytes(const katsu_attention &d);
 int attention_bwd(const katsu_attention &d, const katsu_attention_grads &g, const void *dout,
                   const void *q, const void *k, const void *v, const void *out, const float *lse,

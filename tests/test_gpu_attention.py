@@ -133,6 +133,27 @@ def test_masked_nonfinite(dev, dt, d, bad):
         math.isnan(bad) or torch.equal(out[50:], want))
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("lq,lk,d", [(3, 70, 64), (3, 3000, 128), (2, 40, 33), (300, 700, 128)])
+def test_masked_nonfinite_few_rows_and_runs(dev, dt, lq, lk, d):
+    """The same where few rows' waves share the keys, and where these are split into runs."""
+    for bad in (math.nan, math.inf):
+        q, k, v = _inputs(lq, lk, 2, 1, d, dt)
+        k[-1], v[-1] = bad, bad
+        out, lse = ops.attention(q.to(dev), k.to(dev), v.to(dev))
+        ro, rl, to, tl = forward(q[:-1], k[:-1], v[:-1], [lq - 1], [lk - 1], True, d ** -0.5)
+        assert_close(out[:-1], ro, to, "out")
+        assert_close(lse[:, :-1], rl, tl, "lse")
+        q, k, v = _inputs(lq, lk, 2, 1, d, dt)
+        v[lk - lq] = bad  # the last key that the first query sees: all see it
+        out, lse = ops.attention(q.to(dev), k.to(dev), v.to(dev))
+        want = torch.full_like(out, bad)
+        assert torch.equal(out.isnan(), want.isnan()) and (
+            math.isnan(bad) or torch.equal(out, want))
+        _, rl, _, tl = forward(q, k, torch.zeros_like(v), [lq], [lk], True, d ** -0.5)
+        assert_close(lse, rl, tl, "lse")
+
+
 def test_scores_that_are_all_minus_infinity(dev):
     """A row that sees keys, whose scores are all -inf: 0/0, as the formula has it."""
     q = torch.full((2, 1, 64), math.inf)

@@ -158,6 +158,51 @@ def test_masked_nonfinite(dev, dt, d, bad):
     assert_close(got[0][keep], want[0][keep], tol[0][keep], "dq")
 
 
+@pytest.mark.parametrize("dt", TYPES)
+def test_masked_nonfinite_runs(dev, dt):
+    """The same where the other axis is split into runs."""
+    t, d = 600, 128
+    q, k, v, do = _inputs(t, t, 2, 1, d, dt)
+    k[-1], v[-1], do[-1] = math.nan, math.nan, 0
+    got = _grads(dev, q, k, v, do, [t], [t])
+    want, tol = backward(do[:-1], q[:-1], k[:-1], v[:-1], [t - 1], [t - 1], True, d ** -0.5)
+    assert_close(got[0][:-1], want[0], tol[0], "dq")
+    q, k, v, do = _inputs(t, t, 2, 1, d, dt)
+    do[290] = math.nan
+    got = _grads(dev, q, k, v, do, [t], [t])
+    want, tol = backward(do[291:], q[291:], k, v, [t - 291], [t], True, d ** -0.5)
+    assert_close(got[1][291:], want[1][291:], tol[1][291:], "dk")
+    assert_close(got[2][291:], want[2][291:], tol[2][291:], "dv")
+    assert got[2][:291].isnan().all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_many_sequences(dev, dt):
+    """More than 64 sequences, of all lengths from none; and a long one among short ones."""
+    lens = [(7 * i) % 5 for i in range(200)]
+    _check(dev, lens, lens, 2, 2, 64, dt)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("lens", [[3, 700, 0, 64, 1500], [3, 1500, 0, 64, 130, 1400]])
+def test_orders_of_tiles(dev, dt, lens):
+    """Tiles enough that they go in pairs (256 to 512 of them), and by work (more): two
+    heads against the reference."""
+    t, heads, d = sum(lens), 24, 64
+    q, k, v, do = _inputs(t, t, heads, heads, d, dt)
+    out, lse = ops.attention(*(x.to(dev) for x in (q, k, v)), _cu(lens, dev), _cu(lens, dev))
+    got = _grads(dev, q, k, v, do, lens, lens)
+    for h in (0, 23):
+        one = [x[:, h:h + 1] for x in (q, k, v, do)]
+        ro, rl, to, tl = forward(*one[:3], lens, lens, True, d ** -0.5)
+        assert_close(out[:, h:h + 1], ro, to, "out")
+        assert_close(lse[h:h + 1], rl, tl, "lse")
+        want, tol = backward(one[3], *one[:3], lens, lens, True, d ** -0.5)
+        for a, b, c in zip(got, want, tol):
+            assert_close(a[:, h:h + 1], b, c, "gradient")
+    assert all(x.isfinite().all() for x in got) and out.isfinite().all()
+
+
 @pytest.mark.parametrize("kv", [1, 4])
 def test_same_bits_and_workspace(dev, kv):
     q, k, v, do = [x.to(dev) for x in _inputs(500, 500, 4, kv, 128, torch.bfloat16)]

@@ -55,6 +55,14 @@ def test_attention_pointers_and_starts():
     for gg, ptrs in ((bad, (P,) * 6), (g, (None,) + (P,) * 5), (g, (P,) * 5 + (None,))):
         assert L.katsu_hip_attention_bwd_dev(ctypes.byref(d), ctypes.byref(gg), *ptrs, None, None, P,
                                              P, P, P, 0, None) == _abi.E_INVALID
+    # Outputs whose places are not their own.
+    for kw in (dict(out_stride=(256, 0)), dict(out_stride=(0, 64))):
+        assert fwd(_attention(**kw)) == _abi.E_INVALID
+    for f in ("dq_stride", "dk_stride", "dv_stride"):
+        gg = _abi.AttentionGrads((256, 64), (256, 64), (128, 64), (128, 64))
+        setattr(gg, f, (ctypes.c_int64 * 2)(256, 0))
+        assert L.katsu_hip_attention_bwd_dev(ctypes.byref(d), ctypes.byref(gg), *(P,) * 6, None,
+                                             None, P, P, P, P, 0, None) == _abi.E_INVALID
     # A workspace that is too small.
     n = SZ(0)
     assert L.katsu_hip_attention_bwd_workspace(ctypes.byref(d), ctypes.byref(n)) == _abi.OK
