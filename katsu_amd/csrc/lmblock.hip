@@ -25,22 +25,27 @@ int status_of(hipError_t e) {
 
 bool dtype_ok(int t) { return t == KATSU_F32 || t == KATSU_BF16; }
 
-template <typename T>
-int launch_rotary(RotaryArgs a, bool inter, hipStream_t st) {
-    constexpr int E = Piece<T>::E;
-    const bool vec = (inter ? a.R : a.R / 2) % E == 0 && (a.D - a.R) % E == 0;
-    const int e = vec ? E : 1;
-    a.per_head = (inter ? (vec ? a.R / E : a.R / 2) : a.R / 2 / e);
+template <typename T, bool INTER, int E>
+int launch_rotary(RotaryArgs a, hipStream_t st) {
+    constexpr int P = !INTER ? E : E > 1 ? E / 2 : 1;
+    a.per_head = a.R / 2 / P;
     const bool in_place = a.t[0].in == a.t[0].out && (!a.t[1].heads || a.t[1].in == a.t[1].out);
-    if (!in_place) a.per_head += (a.D - a.R) / e;  // else the rest of each head is in its place
+    if (!in_place) a.per_head += (a.D - a.R) / E;  // else the rest of each head is in its place
     a.items = a.per_head * (a.t[0].heads + a.t[1].heads);
     a.inv_per_head = 1.f / (float)a.per_head;
-    const dim3 blocks((unsigned)std::min<int64_t>(a.tokens, 1 << 20));
-    if (inter && vec) rotary_kernel<T, true, true><<<blocks, 256, 0, st>>>(a);
-    if (inter && !vec) rotary_kernel<T, true, false><<<blocks, 256, 0, st>>>(a);
-    if (!inter && vec) rotary_kernel<T, false, true><<<blocks, 256, 0, st>>>(a);
-    if (!inter && !vec) rotary_kernel<T, false, false><<<blocks, 256, 0, st>>>(a);
+    rotary_kernel<T, INTER, E>
+        <<<dim3((unsigned)std::min<int64_t>(a.tokens, 1 << 20)), 256, 0, st>>>(a);
     return status_of(hipGetLastError());
+}
+// The widest accesses that the turning part, its halves and the rest are multiples of.
+template <typename T, bool INTER>
+int launch_rotary(const RotaryArgs &a, hipStream_t st) {
+    auto fits = [&](int e) { return (INTER ? a.R : a.R / 2) % e == 0 && (a.D - a.R) % e == 0; };
+    if constexpr (sizeof(T) == 2)
+        if (fits(8)) return launch_rotary<T, INTER, 8>(a, st);
+    if (fits(4)) return launch_rotary<T, INTER, 4>(a, st);
+    if (fits(2)) return launch_rotary<T, INTER, 2>(a, st);
+    return launch_rotary<T, INTER, 1>(a, st);
 }
 
 // Threads a row and 16-byte pieces a thread: a wave for rows of up to 128 pieces, so that
@@ -149,8 +154,11 @@ int rotary(const katsu_rotary &d, const void *q, const void *k, const float *tab
     a.D = (int)d.head_dim;
     a.R = (int)d.rotary_dim;
     a.sign = d.inverse ? -1.f : 1.f;
-    return d.dtype == KATSU_F32 ? launch_rotary<float>(a, d.interleaved != 0, st)
-                                : launch_rotary<__bf16>(a, d.interleaved != 0, st);
+    if (d.interleaved)
+        return d.dtype == KATSU_F32 ? launch_rotary<float, true>(a, st)
+                                    : launch_rotary<__bf16, true>(a, st);
+    return d.dtype == KATSU_F32 ? launch_rotary<float, false>(a, st)
+                                : launch_rotary<__bf16, false>(a, st);
 }
 
 int rotary_table(float *table, int64_t length, int dim, double base, double factor,

@@ -7,7 +7,8 @@
 // 128, half of each turning, float32: 66 us, 5.1 TB/s; a copy reaches 4.7).
 #pragma once
 
-#include "lmvec.hpp"
+#include <hip/hip_runtime.h>
+#include <stdint.h>
 
 namespace katsu {
 
@@ -26,14 +27,29 @@ struct RotaryArgs {
     float inv_per_head, sign;
 };
 
-// One block a token (grid-stride), a thread an item: E pairs in the half layout (two
-// pieces R/2 apart), E/2 pairs in the interleaved one, or a piece of the rest.  VEC: all
-// these are whole pieces; else an item is one pair or one channel.
-template <typename T, bool INTER, bool VEC>
+// N neighbouring values, of any alignment.
+template <typename T, int N>
+__device__ __forceinline__ void rotary_load(const T *p, float *x) {
+    T e[N];
+    __builtin_memcpy(e, p, sizeof e);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = (float)e[i];
+}
+template <typename T, int N>
+__device__ __forceinline__ void rotary_store(T *p, const float *x) {
+    T e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = (T)x[i];
+    __builtin_memcpy(p, e, sizeof e);
+}
+
+// One block a token (grid-stride), a thread an item: E pairs in the half layout (two pieces
+// of E channels R/2 apart), E/2 pairs (one at least) in the interleaved one, or E channels
+// of the rest.
+template <typename T, bool INTER, int E>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
-    constexpr int E = VEC ? Piece<T>::E : 1;
-    const int half = a.R / 2;
-    const int turning = INTER ? (VEC ? a.R / E : half) : half / E;  // items that turn
+    constexpr int P = !INTER ? E : E > 1 ? E / 2 : 1;  // pairs
+    const int half = a.R / 2, turning = half / P;      // items that turn
     for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
         int64_t pos = a.positions ? a.positions[token] : token;
         pos = pos < 0 ? 0 : pos < a.length ? pos : a.length - 1;  // stays inside the table
@@ -49,68 +65,44 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
             T *out = (T *)t.out + token * t.out_token + head * t.out_head;
             if (j >= turning) {
                 const int d = a.R + (j - turning) * E;
-                if constexpr (VEC) {
-                    lm_u4 u;
-                    __builtin_memcpy(&u, in + d, 16);
-                    __builtin_memcpy(out + d, &u, 16);
-                } else {
-                    out[d] = in[d];
-                }
+                T e[E];
+                __builtin_memcpy(e, in + d, sizeof e);
+                __builtin_memcpy(out + d, e, sizeof e);
                 continue;
             }
+            const int i = j * P;
+            float c[P], s[P], u[P], v[P];
+            rotary_load<float, P>(cs + i, c);
+            rotary_load<float, P>(cs + half + i, s);
             if constexpr (INTER) {
-                constexpr int P = VEC ? E / 2 : 1;  // pairs
-                const int i = j * P;
-                float c[P], s[P], x[2 * P];
-                if constexpr (VEC) {
-                    __builtin_memcpy(c, cs + i, sizeof c);
-                    __builtin_memcpy(s, cs + half + i, sizeof s);
-                    load_piece(in, 2 * i, a.D, x);
-                } else {
-                    c[0] = cs[i];
-                    s[0] = cs[half + i];
-                    x[0] = (float)in[2 * i];
-                    x[1] = (float)in[2 * i + 1];
-                }
+                float x[2 * P];
+                rotary_load<T, 2 * P>(in + 2 * i, x);
 #pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    const float u = x[2 * p], v = x[2 * p + 1], w = a.sign * s[p];
-                    x[2 * p] = u * c[p] - v * w;
-                    x[2 * p + 1] = u * w + v * c[p];
-                }
-                if constexpr (VEC) {
-                    store_piece(out, 2 * i, a.D, x);
-                } else {
-                    out[2 * i] = (T)x[0];
-                    out[2 * i + 1] = (T)x[1];
+                for (int e = 0; e < P; ++e) {
+                    u[e] = x[2 * e];
+                    v[e] = x[2 * e + 1];
                 }
             } else {
-                const int i = j * E;
-                float c[E], s[E], u[E], v[E];
-                if constexpr (VEC) {
-                    __builtin_memcpy(c, cs + i, sizeof c);
-                    __builtin_memcpy(s, cs + half + i, sizeof s);
-                    load_piece(in, i, a.D, u);
-                    load_piece(in, half + i, a.D, v);
-                } else {
-                    c[0] = cs[i];
-                    s[0] = cs[half + i];
-                    u[0] = (float)in[i];
-                    v[0] = (float)in[half + i];
-                }
+                rotary_load<T, P>(in + i, u);
+                rotary_load<T, P>(in + half + i, v);
+            }
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float x = u[e], y = v[e], w = a.sign * s[e];
-                    u[e] = x * c[e] - y * w;
-                    v[e] = x * w + y * c[e];
+            for (int e = 0; e < P; ++e) {
+                const float x = u[e], y = v[e], w = a.sign * s[e];
+                u[e] = x * c[e] - y * w;
+                v[e] = x * w + y * c[e];
+            }
+            if constexpr (INTER) {
+                float x[2 * P];
+#pragma unroll
+                for (int e = 0; e < P; ++e) {
+                    x[2 * e] = u[e];
+                    x[2 * e + 1] = v[e];
                 }
-                if constexpr (VEC) {
-                    store_piece(out, i, a.D, u);
-                    store_piece(out, half + i, a.D, v);
-                } else {
-                    out[i] = (T)u[0];
-                    out[half + i] = (T)v[0];
-                }
+                rotary_store<T, 2 * P>(out + 2 * i, x);
+            } else {
+                rotary_store<T, P>(out + i, u);
+                rotary_store<T, P>(out + half + i, v);
             }
         }
     }
