@@ -168,7 +168,8 @@ int launch_fwd(const AttnArgs &a, bool few, hipStream_t st) {
 // The backward call's shape.  dk and dv: blocks of one query head each, unless the key heads
 // alone give the card enough to do; in float32 always, and in runs of 2048 queries (up to
 // four runs, whose sums are memory), as a long sum in one accumulator loses too much (5110
-// tokens, heads of 16: dk 1.1e-6 off in one run, 8.4e-7 in four).  Both kernels: the other axis in runs where there are few blocks.
+// tokens, heads of 16: dk 1.1e-6 off in one run, 8.4e-7 in four).  Both kernels: the other
+// axis in runs where there are few blocks.
 struct BwdPlan {
     int dq_slots, dq_splits, dkv_slots, dkv_splits, parts;
     bool each;

@@ -19,7 +19,6 @@ int attention_fwd(const katsu_attention &d, const void *q, const void *k, const 
                   const int32_t *cu_q, const int32_t *cu_k, const int32_t *k_lens, void *out,
                   float *lse, void *ws, hipStream_t st);
 
-
 // Whether a tensor of these strides can be written; whether the gradients can.
 bool attention_out_ok(const int64_t (&stride)[2], uint64_t tokens, uint64_t heads);
 bool attention_grads_ok(const katsu_attention &d, const katsu_attention_grads &g);
