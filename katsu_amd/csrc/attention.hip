@@ -38,12 +38,14 @@ bool strides_ok(const int64_t (&s)[2]) {
 
 int elem(const katsu_attention &d) { return d.dtype == KATSU_F32 ? 4 : 2; }
 
-// 16-byte accesses: rows of whole 16-byte chunks at aligned places, and a tile's
-// 128 rows within the 32-bit offsets of a buffer load.
+// 16-byte accesses: rows of whole 16-byte chunks at aligned places, a tile's rows (64 at
+// most) within the 32-bit offsets of a buffer load, and rows that do not overlap unless all
+// are one: a buffer's end does not tell those past the last one.
 bool vec_ok(const katsu_attention &d, const void *p, const int64_t (&stride)[2]) {
     const int e = elem(d);
     return ((uintptr_t)p & 15) == 0 && d.head_dim * e % 16 == 0 && stride[0] * e % 16 == 0 &&
-           stride[1] * e % 16 == 0 && stride[0] * e < (1 << 23);
+           stride[1] * e % 16 == 0 && stride[0] * e < (1 << 23) &&
+           (stride[0] == 0 || stride[0] >= (int64_t)d.head_dim);
 }
 
 AttnArgs base_args(const katsu_attention &d, const int32_t *cu_q, const int32_t *cu_k,

@@ -229,8 +229,10 @@ __device__ __forceinline__ void dma_b32(uintx4 rs, int off, lds_at to) {
 // Copies a tile of ROWS rows to LDS, spread over NW waves, of which this is
 // wave w.  DMA: by loads that go to LDS directly, 16 bytes a lane, not waited
 // for here; rows and chunks that do not exist are out of the buffer's range and
-// arrive as zeros.  Else (rows that are not a multiple of 16 bytes, or not
-// aligned so) element by element.
+// arrive as zeros, but where all tokens share one row (a token stride of zero) the
+// rows past the last hold it too, so whoever reads a tile masks them.  Else (rows
+// that are not a multiple of 16 bytes, not aligned so, or overlap otherwise)
+// element by element.
 template <typename T, int ND, int ROWS, int NW, bool DMA>
 struct TileCopy {
     using R = Rows<T, ND>;

@@ -216,12 +216,12 @@ struct AttnDkv {
 
     // 32 queries (rows r0 .. of the tile) against the wave's keys.  row, col: this lane's
     // places in q's tile, followed by do's; vrow: in the block's v rows; stats: -lse / scale and
-    // -delta.
+    // -delta.  mask: only the tile's rows [ifirst, iend) take part.
     __device__ static __forceinline__ void block(lds_at row, lds_at col, lds_at stats, lds_at vrow,
                                                  const uintx4 (&kf)[NS], const uintx4 *vf,
                                                  floatx16 (&dk)[ND], floatx16 (&dv)[ND],
                                                  float scale2, int r0, bool mask, int ifirst,
-                                                 int h) {
+                                                 int iend, int h) {
         floatx16 sa[1], ga[1];
         floatx16 &s = sa[0], &g = ga[0];
 #pragma unroll
@@ -250,10 +250,12 @@ struct AttnDkv {
             s[v] = __builtin_amdgcn_exp2f(s[v] * scale2);
             g[v] *= s[v];
         }
-        if (mask) {
+        if (mask) {  // one comparison for both ends: below the first, the difference is large
+            asm volatile("" : "+v"(ifirst));  // computed here: no register for it in the loop
+            const uint32_t n = iend > ifirst ? iend - ifirst : 0;
 #pragma unroll
             for (int v = 0; v < 16; ++v)
-                if (r0 + reg_row(v, h) < ifirst) s[v] = g[v] = 0.f;
+                if ((uint32_t)(r0 + reg_row(v, h) - ifirst) >= n) s[v] = g[v] = 0.f;
         }
         col_product<T, ND, true, false>(dv, col + kTile, r0, c, s,
                            [&] { c = col_frags<T, ND>(col, r0, 0); });
@@ -293,7 +295,7 @@ struct AttnDkv {
         const char *gp =
             (const char *)a.dout.p + (sq.q0 * a.dout.token + head0 * a.dout.head) * sizeof(T);
         // The rows' starts of the sums are copied too, by the first wave, as zeros past the
-        // end: such rows have P = 1, and q, do and dS = 0, and add nothing.
+        // end.  Rows past the end are masked: their P would be 1 (or NaN, of a key with Inf).
         auto fetch = [&](int g, int t, int buf) {
             char *d = lds + kKeys + buf * kStage;
             const int64_t i = (int64_t)(t0 + t) * QT;
@@ -346,13 +348,13 @@ struct AttnDkv {
             asm("" : "+v"(vrow));  // no register for each of its places
 #pragma unroll
             for (int q = 0; q < NQ; ++q) {
-                if (i0 + 32 * q + 31 < wfirst) continue;
-                const bool mask = i0 + 32 * q < wall;
-                if (mask)
+                if (i0 + 32 * q + 31 < wfirst || i0 + 32 * q >= sq.lq) continue;
+                const bool cut = i0 + 32 * q < wall;  // by the causal mask
+                if (cut)
                     bad |= tile_nonfinite<T, ND, 32>(b + 32 * q * R::RB, lane) ||
                            tile_nonfinite<T, ND, 32>(b + kTile + 32 * q * R::RB, lane);
-                block(b + row, b + col, stats, vrow, kf, vf, dk, dv, a.scale2, 32 * q, mask,
-                      ifirst - i0, h);
+                block(b + row, b + col, stats, vrow, kf, vf, dk, dv, a.scale2, 32 * q,
+                      cut || i0 + 32 * q + 32 > sq.lq, ifirst - i0, sq.lq - i0, h);
             }
         }
         float *pk = a.part + ((int64_t)(kvh * a.parts + p) * a.Tk + token) * W;
