@@ -288,10 +288,10 @@ typedef enum katsu_dtype { KATSU_F32 = 0, KATSU_BF16 = 1 } katsu_dtype;
  * Strides are in elements, [0] between tokens and [1] between heads; channels
  * are adjacent.  Sequence s has queries cu_q[s] .. cu_q[s+1] and keys cu_k[s]
  * .. cu_k[s+1], or with k_lens the first k_lens[s] of those (slots of a cache);
- * cu_q and cu_k are device arrays of seqs + 1 int32 from 0 to the number of
- * tokens that do not fall, both NULL for one sequence of all tokens; values
- * outside the tensors are taken as their ends; what outputs hold for tokens
- * that no sequence holds is undefined.
+ * cu_q and cu_k are device arrays of seqs + 1 int32 that do not fall, both NULL
+ * for one sequence of all tokens; they may begin after 0 and end before the last
+ * token (a slice of a batch's starts); values outside the tensors are taken as
+ * their ends; what outputs hold for tokens that no sequence holds is undefined.
  *   S = scale q.k over the visible keys, P = softmax(S), out = P v,
  *   lse[head][token] = log sum exp S       (natural logarithm)
  * With causal set query i of Lq sees key j of Lk if j <= i + Lk - Lq: the last

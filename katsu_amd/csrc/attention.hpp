@@ -99,7 +99,8 @@ struct AttnTile {
     int at;
 };
 // By place, from the last: the last sequence whose first slot is not beyond it, 64
-// candidates a step.
+// candidates a step, of which the first always counts: slots before the first sequence's
+// (starts that begin after 0) find that one, and are no tile's.
 __device__ __forceinline__ bool tile_by_place(const AttnArgs &a, const int32_t *cu, int64_t total,
                                               int mult, int unit, int rank, int lane,
                                               AttnTile &t) {
@@ -108,15 +109,16 @@ __device__ __forceinline__ bool tile_by_place(const AttnArgs &a, const int32_t *
     if (cu) {
         while (n > 1) {
             const int step = (n + 63) >> 6, i = lane * step;
-            const bool ok = i < n && first_slot(cu, lo + i, total, mult, unit) <= slot;
-            const int at = max(__popcll(__ballot(ok)) - 1, 0) * step;
+            const bool ok =
+                lane == 0 || (i < n && first_slot(cu, lo + i, total, mult, unit) <= slot);
+            const int at = ((int)__popcll(__ballot(ok)) - 1) * step;
             lo += at;
             n = min(step, n - at);
         }
     }
     t.seq = seq_at(a, uni(lo));
     t.at = slot - uni(first_slot(cu, t.seq.s, total, mult, unit));
-    return true;
+    return t.at >= 0;
 }
 // By work, the longest first: with a causal mask tile j of a sequence has j + 1 tiles' work,
 // so the ranks go down the levels j, and at each through the sequences that have a tile

@@ -308,12 +308,13 @@ def attention(q, k, v, cu_q=None, cu_k=None, k_lens=None, causal=True, scale=Non
               workspace=None):
     """(out, lse) of softmax(scale q k^T) v over packed sequences: q [Tq, H, D], k and v
     [Tk, Hkv, D], channels adjacent, any token and head strides; cu_q and cu_k the int32 starts
-    of the sequences' queries and keys and the end (None: one sequence); k_lens how many of each
-    sequence's keys are in use (a cache's slots).  causal: the last query sees every key, each
-    earlier one a key less.  A query that sees no key gives 0 and lse -inf; the output of a token
-    that no sequence holds is undefined, its gradients too.  scale: 1/sqrt(D) if None.  lse
-    [H, Tq], float32, is what attention_backward takes.  `workspace`: an optional device tensor of
-    attention_workspace_bytes(); without it the library's own buffer is used."""
+    of the sequences' queries and keys and the end (None: one sequence; a slice of a batch's starts
+    gives those sequences); k_lens how many of each sequence's keys are in use (a cache's slots).
+    causal: the last query sees every key, each earlier one a key less.  A query that sees no key
+    gives 0 and lse -inf; the output of a token that no sequence holds is undefined, its gradients
+    too.  scale: 1/sqrt(D) if None.  lse [H, Tq], float32, is what attention_backward takes.
+    `workspace`: an optional device tensor of attention_workspace_bytes(); without it the library's
+    own buffer is used."""
     out = torch.empty_like(q) if out is None else out
     d = _attention(q, k, v, out, cu_q, cu_k, k_lens, causal, scale)
     lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32)
