@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(TPR == 64 ? 256 : TPR) block_norm_bwd_kernel(
 }
 
 // Column sums of the parts, in order within each of a block's 16 waves, then the waves'.
+// `sums` of w_pre, w_post (null if there is none) and, if it is one more, gate.
 template <typename T>
 __global__ void __launch_bounds__(1024) block_norm_sum_kernel(const float *part, int sets,
                                                              int64_t cols, int sums, T *w_pre,
@@ -216,7 +217,6 @@ __global__ void __launch_bounds__(1024) block_norm_sum_kernel(const float *part,
     v = s[0][lane];
 #pragma unroll
     for (int w = 1; w < 16; ++w) v += s[w][lane];
-    // Of the three, those that there are follow each other in this order.
     const int n = (w_pre != nullptr) + (w_post != nullptr);
     T *out = which == 0 && w_pre ? w_pre : which < n ? w_post : gate;
     out[c] = (T)v;

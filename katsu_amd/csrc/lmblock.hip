@@ -123,8 +123,8 @@ int launch_norm_bwd(const NormBwdArgs &a, void *dw_pre, void *dw_post, void *dga
     });
     if (rc != KATSU_OK || a.sums == 0) return rc;
     block_norm_sum_kernel<T><<<dim3((unsigned)cdiv(a.cols, 64), a.sums), 1024, 0, st>>>(
-        a.part, a.sets, a.cols, a.sums, (T *)dw_pre, (T *)dw_post,
-        a.gate && a.gate_row == 0 ? (T *)dgate : nullptr);
+        a.part, a.sets, a.cols, a.sums, a.w_pre ? (T *)dw_pre : nullptr,
+        a.w_post ? (T *)dw_post : nullptr, (T *)dgate);
     return status_of(hipGetLastError());
 }
 
