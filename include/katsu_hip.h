@@ -392,13 +392,21 @@ int katsu_hip_block_norm_bwd_dev(const katsu_block_norm *d, const void *dy, cons
 
 /* norm[0] = sqrt(sum over the n tensors of all squares), squares summed in
  * float64; out = in * min(1, max_norm / (norm + 1e-6)), tensor by tensor (out
- * may be in).  dtypes, in, out and counts are host arrays; the tensors are
- * contiguous device memory of katsu_dtype dtypes[i].  A norm that is NaN
+ * may be in; no two tensors that are written may share memory).  dtypes, in,
+ * out and counts are host arrays; the tensors are contiguous device memory of
+ * katsu_dtype dtypes[i].  A norm that is NaN
  * makes all outputs NaN, an infinite one zero (NaN where in is infinite).
- * max_norm must not be negative.  Partial sums are in library scratch. */
+ * max_norm must not be negative.  Partial sums go through a workspace as above,
+ * of katsu_hip_clip_grad_norm_workspace bytes for n tensors; the form without
+ * one takes the library's. */
+int katsu_hip_clip_grad_norm_workspace(size_t n, size_t *bytes);
 int katsu_hip_clip_grad_norm_dev(const int32_t *dtypes, const void *const *in, void *const *out,
                                  const size_t *counts, size_t n, float max_norm, float *norm,
                                  void *stream);
+int katsu_hip_clip_grad_norm_ws_dev(const int32_t *dtypes, const void *const *in,
+                                    void *const *out, const size_t *counts, size_t n,
+                                    float max_norm, float *norm, void *workspace,
+                                    size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -35,7 +35,8 @@ EXPORTS = (
     "katsu_hip_attention_bwd_workspace", "katsu_hip_attention_bwd_dev",
     "katsu_hip_rotary_dev", "katsu_hip_rotary_table_f32_dev",
     "katsu_hip_block_norm_dev", "katsu_hip_block_norm_bwd_workspace",
-    "katsu_hip_block_norm_bwd_dev", "katsu_hip_clip_grad_norm_dev",
+    "katsu_hip_block_norm_bwd_dev", "katsu_hip_clip_grad_norm_workspace",
+    "katsu_hip_clip_grad_norm_dev", "katsu_hip_clip_grad_norm_ws_dev",
 )
 
 
@@ -148,7 +149,9 @@ def lib():
         L.katsu_hip_block_norm_dev.argtypes = [bp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
         L.katsu_hip_block_norm_bwd_workspace.argtypes = [bp, ctypes.POINTER(sz)]
         L.katsu_hip_block_norm_bwd_dev.argtypes = [bp] + [vp] * 14 + [sz, vp]
+        L.katsu_hip_clip_grad_norm_workspace.argtypes = [sz, ctypes.POINTER(sz)]
         L.katsu_hip_clip_grad_norm_dev.argtypes = [vp, vp, vp, vp, sz, fp, vp, vp]
+        L.katsu_hip_clip_grad_norm_ws_dev.argtypes = [vp, vp, vp, vp, sz, fp, vp, vp, sz, vp]
         for name in EXPORTS:
             if name not in ("katsu_hip_version", "katsu_hip_strerror", "katsu_hip_shutdown",
                             "katsu_hip_noalloc_scratch_bytes",

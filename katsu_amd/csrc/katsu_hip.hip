@@ -3345,9 +3345,16 @@ int katsu_hip_block_norm_bwd_dev(const katsu_block_norm *d, const void *dy, cons
                           dw_pre, ws, st);
 }
 
-int katsu_hip_clip_grad_norm_dev(const int32_t *dtypes, const void *const *in, void *const *out,
-                                 const size_t *counts, size_t n, float max_norm, float *norm,
-                                 void *stream) {
+int katsu_hip_clip_grad_norm_workspace(size_t n, size_t *bytes) {
+    if (!bytes || n > (size_t)kI32Max) return KATSU_E_INVALID;
+    *bytes = clip_bytes(n);
+    return KATSU_OK;
+}
+
+int katsu_hip_clip_grad_norm_ws_dev(const int32_t *dtypes, const void *const *in,
+                                    void *const *out, const size_t *counts, size_t n,
+                                    float max_norm, float *norm, void *workspace,
+                                    size_t workspace_bytes, void *stream) {
     if (!norm || !(max_norm >= 0.f) || (n > 0 && (!dtypes || !in || !out || !counts)))
         return KATSU_E_INVALID;
     for (size_t i = 0; i < n; ++i) {
@@ -3357,9 +3364,16 @@ int katsu_hip_clip_grad_norm_dev(const int32_t *dtypes, const void *const *in, v
     }
     hipStream_t st = (hipStream_t)stream;
     void *ws = nullptr;
-    const int rc = lm_scratch(nullptr, 0, clip_bytes(n), st, &ws);
+    const int rc = lm_scratch(workspace, workspace_bytes, clip_bytes(n), st, &ws);
     if (rc) return rc;
     return clip_grad_norm(dtypes, in, out, counts, n, max_norm, norm, ws, st);
+}
+
+int katsu_hip_clip_grad_norm_dev(const int32_t *dtypes, const void *const *in, void *const *out,
+                                 const size_t *counts, size_t n, float max_norm, float *norm,
+                                 void *stream) {
+    return katsu_hip_clip_grad_norm_ws_dev(dtypes, in, out, counts, n, max_norm, norm, nullptr, 0,
+                                           stream);
 }
 
 }  // extern "C"

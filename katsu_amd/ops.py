@@ -453,10 +453,19 @@ def block_norm_workspace_bytes(dy):
     return nbytes.value
 
 
-def clip_grad_norm(grads, max_norm, out=None):
+def clip_workspace_bytes(n):
+    """Scratch that clip_grad_norm needs for n gradients."""
+    nbytes = ctypes.c_size_t(0)
+    check(lib().katsu_hip_clip_grad_norm_workspace(n, ctypes.byref(nbytes)), "clip_workspace")
+    return nbytes.value
+
+
+def clip_grad_norm(grads, max_norm, out=None, workspace=None):
     """The root of the sum of all squares of `grads` (a list of contiguous device tensors of
     either type), as a float32 device tensor [1]; each gradient times
-    min(1, max_norm / (norm + 1e-6)) is written to `out` (in place if None)."""
+    min(1, max_norm / (norm + 1e-6)) is written to `out` (in place if None).  No two of the tensors
+    written may share memory.  `workspace`: an optional device tensor of clip_workspace_bytes();
+    without it the library's own buffer is used."""
     n = len(grads)
     if n == 0:
         raise ValueError("no gradients")
@@ -477,7 +486,8 @@ def clip_grad_norm(grads, max_norm, out=None):
                          "one device, each output of its gradient's size and type")
     norm = torch.empty(1, device=grads[0].device, dtype=torch.float32)
     kinds, counts = array("i", [_DTYPE[t] for t in types]), array("Q", sizes)
-    check(lib().katsu_hip_clip_grad_norm_dev(
+    check(lib().katsu_hip_clip_grad_norm_ws_dev(
         kinds.buffer_info()[0], ptrs.buffer_info()[0], outs.buffer_info()[0],
-        counts.buffer_info()[0], n, max_norm, norm.data_ptr(), _stream()), "clip_grad_norm")
+        counts.buffer_info()[0], n, max_norm, norm.data_ptr(), *_workspace(workspace), _stream()),
+        "clip_grad_norm")
     return norm
