@@ -308,7 +308,7 @@ typedef struct katsu_attention {
 } katsu_attention;
 
 /* The forward pass; lse may be NULL.  `workspace` of
- * katsu_hip_attention_fwd_workspace bytes (device memory, 256-byte aligned)
+ * katsu_hip_attention_fwd_workspace bytes (device memory, 16-byte aligned)
  * holds the parts of a key axis split over workgroups; NULL uses a
  * library-owned buffer, allocated on first need and kept. */
 int katsu_hip_attention_fwd_workspace(const katsu_attention *d, size_t *bytes);

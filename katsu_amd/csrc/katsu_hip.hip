@@ -165,11 +165,12 @@ int ws_take(const WsSource &src, size_t need, hipStream_t st, float **out) {
     return scratch_get(ScratchKind::Dw, st, need, out);
 }
 
-// The caller's workspace if it passes one (checked), else the library's.
+// The caller's workspace if it passes one (checked: its values are read in 16-byte pieces, and
+// by buffer loads, which drop an address's lowest bits), else the library's.
 int lm_scratch(void *ws, size_t bytes, size_t need, hipStream_t st, void **out) {
     *out = ws;
     if (need == 0) return KATSU_OK;
-    if (ws) return bytes < need ? KATSU_E_INVALID : KATSU_OK;
+    if (ws) return bytes < need || ((uintptr_t)ws & 15) != 0 ? KATSU_E_INVALID : KATSU_OK;
     return scratch_get(ScratchKind::Lm, st, need, (float **)out);
 }
 

@@ -300,8 +300,13 @@ def attention_workspace_bytes(q, k, v, cu_q=None, cu_k=None, backward=False):
     return nbytes.value
 
 
-def _workspace(t):
-    return (0, 0) if t is None else (t.data_ptr(), t.numel() * t.element_size())
+def _workspace(t, dev):
+    """A workspace's address and bytes: the kernels write it, so it must be memory of theirs."""
+    if t is None:
+        return 0, 0
+    if t.device != dev or not t.is_contiguous():
+        raise ValueError("workspace must be contiguous and on the operands' device")
+    return t.data_ptr(), t.numel() * t.element_size()
 
 
 def attention(q, k, v, cu_q=None, cu_k=None, k_lens=None, causal=True, scale=None, out=None,
@@ -320,7 +325,8 @@ def attention(q, k, v, cu_q=None, cu_k=None, k_lens=None, causal=True, scale=Non
     lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32)
     check(lib().katsu_hip_attention_fwd_dev(ctypes.byref(d), _p(q), _p(k), _p(v), _p(cu_q),
                                             _p(cu_k), _p(k_lens), _p(out), _p(lse),
-                                            *_workspace(workspace), _stream()), "attention")
+                                            *_workspace(workspace, q.device), _stream()),
+          "attention")
     return out, lse
 
 
@@ -343,8 +349,9 @@ def attention_backward(dout, q, k, v, out, lse, cu_q=None, cu_k=None, causal=Tru
                                                    (dv, "dv"))))
     check(lib().katsu_hip_attention_bwd_dev(ctypes.byref(d), ctypes.byref(g), _p(dout), _p(q),
                                             _p(k), _p(v), _p(out), _p(lse), _p(cu_q), _p(cu_k),
-                                            _p(dq), _p(dk), _p(dv), *_workspace(workspace),
-                                            _stream()), "attention_backward")
+                                            _p(dq), _p(dk), _p(dv),
+                                            *_workspace(workspace, q.device), _stream()),
+          "attention_backward")
     return dq, dk, dv
 
 
@@ -439,8 +446,8 @@ def block_norm_backward(dy, dh, y, o, stats, gate=None, w_post=None, w_pre=None,
                               for t in (gate, w_post, w_pre))
     check(lib().katsu_hip_block_norm_bwd_dev(
         ctypes.byref(d), _p(dy), _p(dh), _p(y), _p(o), _p(stats), _p(gate), _p(w_post), _p(w_pre),
-        _p(dx), _p(do), _p(dgate), _p(dw_post), _p(dw_pre), *_workspace(workspace), _stream()),
-        "block_norm_backward")
+        _p(dx), _p(do), _p(dgate), _p(dw_post), _p(dw_pre), *_workspace(workspace, dy.device),
+        _stream()), "block_norm_backward")
     return dx, do, dgate, dw_post, dw_pre
 
 
@@ -488,6 +495,6 @@ def clip_grad_norm(grads, max_norm, out=None, workspace=None):
     kinds, counts = array("i", [_DTYPE[t] for t in types]), array("Q", sizes)
     check(lib().katsu_hip_clip_grad_norm_ws_dev(
         kinds.buffer_info()[0], ptrs.buffer_info()[0], outs.buffer_info()[0],
-        counts.buffer_info()[0], n, max_norm, norm.data_ptr(), *_workspace(workspace), _stream()),
-        "clip_grad_norm")
+        counts.buffer_info()[0], n, max_norm, norm.data_ptr(),
+        *_workspace(workspace, norm.device), _stream()), "clip_grad_norm")
     return norm
