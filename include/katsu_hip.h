@@ -341,7 +341,9 @@ int katsu_hip_attention_bwd_dev(const katsu_attention *d, const katsu_attention_
  * R/2 cosines, then R/2 sines; rows outside it are taken as its ends), or by
  * row t if positions is NULL.  inverse turns back: the gradient of a turn.
  * q and k ([tokens][heads][head_dim], strides in elements as above) go in one
- * launch; k may be NULL with k_heads 0.  Outputs may be the inputs. */
+ * launch; k may be NULL with k_heads 0.  Outputs may be the inputs, with the
+ * same strides; an output's strides must not be zero, none may be negative.
+ * At most 65535 heads each, fewer than 2^20 channels of a token in all. */
 typedef struct katsu_rotary {
     int32_t dtype, interleaved, inverse;
     uint64_t tokens, heads, k_heads, head_dim, rotary_dim, length;

@@ -130,6 +130,18 @@ int launch_norm_bwd(const NormBwdArgs &a, void *dw_pre, void *dw_post, void *dga
 
 }  // namespace
 
+// An output's places are its own, and if it is its input it is so value by value: a thread
+// may write before another has read.
+bool rotary_out_ok(const int64_t (&in)[2], const int64_t (&out)[2], bool same, uint64_t tokens,
+                   uint64_t heads) {
+    const uint64_t n[2] = {tokens, heads};
+    for (int i = 0; i < 2; ++i) {
+        if (in[i] < 0 || out[i] < 0) return false;
+        if (n[i] > 1 && (out[i] == 0 || (same && in[i] != out[i]))) return false;
+    }
+    return true;
+}
+
 bool rotary_ok(const katsu_rotary &d) {
     if (!dtype_ok(d.dtype) || d.heads > 65535 || d.k_heads > 65535) return false;
     if (d.head_dim == 0 || d.head_dim > 65536 || d.rotary_dim == 0 || d.rotary_dim % 2 != 0 ||
@@ -142,6 +154,10 @@ bool rotary_ok(const katsu_rotary &d) {
 
 int rotary(const katsu_rotary &d, const void *q, const void *k, const float *table,
            const int32_t *positions, void *q_out, void *k_out, hipStream_t st) {
+    if (d.heads && !rotary_out_ok(d.q_stride, d.q_out_stride, q == q_out, d.tokens, d.heads))
+        return KATSU_E_INVALID;
+    if (d.k_heads && !rotary_out_ok(d.k_stride, d.k_out_stride, k == k_out, d.tokens, d.k_heads))
+        return KATSU_E_INVALID;
     RotaryArgs a{};
     a.t[0] = {q, q_out, d.q_stride[0], d.q_stride[1], d.q_out_stride[0], d.q_out_stride[1],
               (int)d.heads};
