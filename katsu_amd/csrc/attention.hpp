@@ -42,7 +42,7 @@ enum AttnOrder { kByPlace, kByWork, kInPairs };
 struct AttnArgs {
     AttnTensor q, k, v, out, dout, dq, dk, dv;
     float *lse;                       // [H][Tq]
-    float *start;                     // backward, [2][H][Tq]: -lse / scale, -do.o
+    float *start;                     // backward, [2][H][Tq]: -log2(e) lse, -do.o
     const int32_t *cu_q, *cu_k, *k_lens;
     int64_t Tq, Tk;
     int B, H, Hkv, G, D, causal;

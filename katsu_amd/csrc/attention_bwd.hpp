@@ -27,7 +27,7 @@ namespace katsu {
 template <typename T, int ND>
 constexpr bool kFine = sizeof(T) == 2 && ND == 1;
 
-// ---- dq, and where the sums of dk and dv start --------------------------------------------------------
+// ---- dq, and what dk and dv take of a row ----------------------------------------
 // As the forward pass: a wave owns 32 rows (a row's scores in one lane and its partner),
 // the block's waves share the key tiles.
 template <typename T, int ND, int BN, bool VEC>
@@ -161,7 +161,7 @@ struct AttnDq {
             }
         }
         if (valid && h == 0 && split == 0) {
-            a.start[at] = -lse2 / a.scale2;
+            a.start[at] = -lse2;
             a.start[a.H * a.Tq + at] = -delta;
         }
         float *part = a.part + ((split * a.Tq + token) * a.H + head) * R::W;
@@ -212,27 +212,27 @@ struct AttnDkv {
     static constexpr int kTile = QT * R::RB, kStage = 2 * kTile + 512;
     static constexpr int kKeys = VLDS ? BK * R::RB : 0, kLds = kKeys + 2 * kStage;
     using Copy = TileCopy<T, ND, QT, 4, VEC>;
-    static_assert(QT <= 64, "a wave copies the rows' starts");
+    static_assert(QT <= 64, "a wave copies what there is of each row");
 
     // 32 queries (rows r0 .. of the tile) against the wave's keys.  row, col: this lane's
-    // places in q's tile, followed by do's; vrow: in the block's v rows; stats: -lse / scale and
+    // places in q's tile, followed by do's; vrow: in the block's v rows; stats: -lse2 and
     // -delta.  mask: only the tile's rows [ifirst, iend) take part.
+    //
+    // lse2 enters with the exponential's multiply-add: score sums that start from lse / scale
+    // are rounded to its size at each step (1047 tokens, heads of 80, float32: dk 1.0e-6 off
+    // so, 4.9e-7 from zero).  The sums of dP start from -delta, which is of their own size.
     __device__ static __forceinline__ void block(lds_at row, lds_at col, lds_at stats, lds_at vrow,
                                                  const uintx4 (&kf)[NS], const uintx4 *vf,
                                                  floatx16 (&dk)[ND], floatx16 (&dv)[ND],
                                                  float scale2, int r0, bool mask, int ifirst,
                                                  int iend, int h) {
-        floatx16 sa[1], ga[1];
+        floatx16 sa[1] = {}, ga[1];
         floatx16 &s = sa[0], &g = ga[0];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {  // sums that start from -lse / scale and -delta
-            const floatx4 x = lds_read<floatx4>(stats + (r0 + 8 * q + 4 * h) * 4);
+        for (int q = 0; q < 4; ++q) {  // sums of dP that start from -delta
             const floatx4 y = lds_read<floatx4>(stats + 256 + (r0 + 8 * q + 4 * h) * 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[4 * q + e] = x[e];
-                g[4 * q + e] = y[e];
-            }
+            for (int e = 0; e < 4; ++e) g[4 * q + e] = y[e];
         }
         ColFrags<ND> c;
         row_product<T, ND, 1, 2, R::W == 64>(sa, row, r0, [&](int st) { return kf[st]; }, [] {});
@@ -246,9 +246,14 @@ struct AttnDkv {
             },
             [&] { c = col_frags<T, ND>(col + kTile, r0, 0); });
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            s[v] = __builtin_amdgcn_exp2f(s[v] * scale2);
-            g[v] *= s[v];
+        for (int q = 0; q < 4; ++q) {
+            const floatx4 x = lds_read<floatx4>(stats + (r0 + 8 * q + 4 * h) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int v = 4 * q + e;
+                s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], scale2, x[e]));
+                g[v] *= s[v];
+            }
         }
         if (mask) {  // one comparison for both ends: below the first, the difference is large
             asm volatile("" : "+v"(ifirst));  // computed here: no register for it in the loop
@@ -294,7 +299,7 @@ struct AttnDkv {
         const char *qp = (const char *)a.q.p + (sq.q0 * a.q.token + head0 * a.q.head) * sizeof(T);
         const char *gp =
             (const char *)a.dout.p + (sq.q0 * a.dout.token + head0 * a.dout.head) * sizeof(T);
-        // The rows' starts of the sums are copied too, by the first wave, as zeros past the
+        // The rows' -lse2 and -delta are copied too, by the first wave, as zeros past the
         // end.  Rows past the end are masked: their P would be 1 (or NaN, of a key with Inf).
         auto fetch = [&](int g, int t, int buf) {
             char *d = lds + kKeys + buf * kStage;
@@ -372,7 +377,8 @@ struct AttnDkv {
                     const T *q = plain_at<T>(a.q, sq.q0 + i, gg, c0);
                     const T *d = plain_at<T>(a.dout, sq.q0 + i, gg, c0);
                     const float s = plain_dot(q, k, n), dp = plain_dot(d, v, n);
-                    const float w = __builtin_amdgcn_exp2f((s + a.start[at]) * a.scale2);
+                    const float w =
+                        __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.scale2, a.start[at]));
                     plain_add(av, w, d, n);
                     plain_add(ak, w * (dp + a.start[a.H * a.Tq + at]), q, n);
                 }
