@@ -169,9 +169,12 @@ int launch_fwd(const AttnArgs &a, bool few, hipStream_t st) {
 
 // The backward call's shape.  dk and dv: blocks of one query head each, unless the key heads
 // alone give the card enough to do; in float32 always, and in runs of 2048 queries (up to
-// four runs, whose sums are memory), as a long sum in one accumulator loses too much (5110
-// tokens, heads of 16: dk 1.1e-6 off in one run, 8.4e-7 in four).  Both kernels: the other
-// axis in runs where there are few blocks.
+// four runs, whose sums are memory), as a long sum in one accumulator loses more (5110
+// tokens, 8/4 heads of 16: dk 9.8e-7 off in three runs, 1.7e-6 in one, and 567 us against 717;
+// 4096, 16/16 heads of 64, all keys: 1.2e-6 in two, 1.4e-6 in one, and 1749 us against 1733).
+// That goes by the mean length, as the lengths are on the card: a sequence of 6000 among five
+// short ones is one run (8/8 heads of 64: 1.6e-6; plain float32 products 1.5e-6).  Both kernels:
+// the other axis in runs where there are few blocks.
 struct BwdPlan {
     int dq_slots, dq_splits, dkv_slots, dkv_splits, parts;
     bool each;
