@@ -32,8 +32,10 @@ int lds_optin(size_t bytes) {
     return status_of(e);
 }
 
+// Any in memory: places are computed in 64 bits.
 bool strides_ok(const int64_t (&s)[2]) {
-    return s[0] >= 0 && s[1] >= 0 && s[0] <= kI32Max && s[1] <= (int64_t)1 << 40;
+    const int64_t most = (int64_t)1 << 40;
+    return s[0] >= 0 && s[1] >= 0 && s[0] <= most && s[1] <= most;
 }
 
 int elem(const katsu_attention &d) { return d.dtype == KATSU_F32 ? 4 : 2; }

@@ -53,3 +53,34 @@ def test_rotary_single_places(dev, dt):
     assert torch.equal(a, c) and torch.equal(b, d)
     with pytest.raises(_abi.KatsuError):
         ops.rotary(q, None, table, out_q=x.expand(5, 3, 24))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 20])
+def test_attention_far_tokens(dev, dt, d):
+    """Tokens more than 2^31 values apart: all operands and outputs in one buffer of long rows."""
+    t, heads, kv = 3, 4, 2
+    step = (1 << 31) + 1024
+    n = {"q": heads, "k": kv, "v": kv, "do": heads, "out": heads, "dq": heads, "dk": kv, "dv": kv}
+    flat = torch.empty((t - 1) * step + sum(n.values()) * d, dtype=dt, device=dev)
+    far, at = {}, 0
+    for name, h in n.items():
+        far[name] = flat.as_strided((t, h, d), (step, d, 1), at)
+        at += h * d
+    g = torch.Generator().manual_seed(1)
+    near = {}
+    for name in ("q", "k", "v", "do"):
+        near[name] = torch.randn(t, n[name], d, generator=g).to(dt).to(dev)
+        far[name].copy_(near[name])
+    out, lse = ops.attention(near["q"], near["k"], near["v"])
+    want = ops.attention_backward(near["do"], near["q"], near["k"], near["v"], out, lse)
+    _, far_lse = ops.attention(far["q"], far["k"], far["v"], out=far["out"])
+    got = ops.attention_backward(far["do"], far["q"], far["k"], far["v"], far["out"], far_lse,
+                                 dq=far["dq"], dk=far["dk"], dv=far["dv"])
+    # The copy to LDS is another one, and with it the blocks of 32 channels and the order of the
+    # sums of at most 64 products: a few roundings. Rows of 40 bytes take the same copy near and far.
+    tol = 0 if d == 20 and dt is torch.bfloat16 else 64 * 2.0 ** -24 + (
+        0 if dt is torch.float32 else 2.0 ** -7)
+    for a, b in zip((far["out"], far_lse, *got), (out, lse, *want)):
+        assert ((a - b).abs() <= tol * (b.abs() + 1)).all()
