@@ -26,9 +26,10 @@ template <typename T, int TPR, int NV>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const NormArgs a) {
     constexpr int E = Piece<T>::E, RPB = TPR < 256 ? 256 / TPR : 1;
     __shared__ float part[2][16];
-    const int64_t row = (int64_t)blockIdx.x * RPB + (RPB > 1 ? threadIdx.x / TPR : 0);
+    const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    const int64_t row = block * RPB + (RPB > 1 ? threadIdx.x / TPR : 0);
     const int lane = threadIdx.x % TPR;
-    if (row >= a.rows) return;  // a whole wave, or never (one row a block)
+    if (row >= a.rows) return;  // a whole wave, or (one row a block) all of it
     const T *x = (const T *)a.x + row * a.cols, *o = (const T *)a.o + row * a.cols;
     const T *gate = a.gate ? (const T *)a.gate + row * a.gate_row : nullptr;
     float u[NV][E], v[NV][E];

@@ -68,13 +68,19 @@ int by_row_size(int64_t cols, F f) {
     return KATSU_E_INVALID;
 }
 
+// A launch has fewer than 2^32 threads along x: rows beyond that go along y.
+dim3 grid_of(int64_t blocks) {
+    const int64_t x = std::min<int64_t>(blocks, 1 << 20);
+    return dim3((unsigned)x, (unsigned)cdiv(blocks, x));
+}
+
 template <typename T>
 int launch_norm(const NormArgs &a, hipStream_t st) {
     return by_row_size<T>(a.cols, [&](auto tpr, auto nv) {
         constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
         constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
         block_norm_kernel<T, TPR, NV>
-            <<<dim3((unsigned)cdiv(a.rows, RPB)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(a);
+            <<<grid_of(cdiv(a.rows, RPB)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(a);
         return status_of(hipGetLastError());
     });
 }
