@@ -137,7 +137,9 @@ template <auto Kern>
 int launch(int64_t blocks, int threads, int lds, const AttnArgs &a, hipStream_t st) {
     const int rc = lds_optin<Kern>(lds);
     if (rc != KATSU_OK || blocks == 0) return rc;
-    Kern<<<dim3((unsigned)blocks), dim3(threads), lds, st>>>(a);
+    // A launch has fewer than 2^32 threads along x: blocks beyond that go along y.
+    const int64_t x = std::min<int64_t>(blocks, 1 << 20);
+    Kern<<<dim3((unsigned)x, (unsigned)cdiv(blocks, x)), dim3(threads), lds, st>>>(a);
     return status_of(hipGetLastError());
 }
 

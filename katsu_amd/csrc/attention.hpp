@@ -72,6 +72,8 @@ struct AttnSeq {
     int s, q0, lq, k0, lk;
 };
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// This block's number in a launch of rows of gridDim.x of them; those past the last have no tile.
+__device__ __forceinline__ unsigned block_id() { return blockIdx.y * gridDim.x + blockIdx.x; }
 
 __device__ __forceinline__ AttnSeq seq_at(const AttnArgs &a, int s) {
     AttnSeq r;

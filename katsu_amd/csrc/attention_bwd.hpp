@@ -72,7 +72,7 @@ struct AttnDq {
     __device__ static void run(const AttnArgs &a, char *lds) {
         const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
         const int l31 = lane & 31, h = lane >> 5;
-        const unsigned id = blockIdx.x;
+        const unsigned id = block_id();
         const int kvh = id % a.Hkv, split = id / a.Hkv % a.splits;
         AttnTile tl;
         if (!tile_by_work(a, a.cu_q, a.Tq, a.G, BM, (int)(id / a.Hkv / a.splits), lane, tl))
@@ -272,7 +272,7 @@ struct AttnDkv {
         const int l31 = lane & 31, h = lane >> 5;
         // A key head's queries are `parts` blocks' work: every head's tiles in `splits` runs,
         // or (!each) all heads' together.
-        const unsigned id = blockIdx.x;
+        const unsigned id = block_id();
         const int kvh = id % a.Hkv, p = id / a.Hkv % a.parts;
         const int split = p % a.splits;
         const int head0 = kvh * a.G + (a.each ? p / a.splits : 0), heads = a.each ? 1 : a.G;

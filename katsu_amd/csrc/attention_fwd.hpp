@@ -153,7 +153,7 @@ struct AttnFwd {
         const int wm = WK > 1 ? 0 : wave, wk = WK > 1 ? wave : 0;
         // Key heads innermost (blocks go round-robin over the 8 XCDs, so an XCD's L2
         // holds few heads' keys).
-        const unsigned id = blockIdx.x;
+        const unsigned id = block_id();
         const int kvh = id % a.Hkv, split = id / a.Hkv % a.splits;
         const int rank = (int)(id / a.Hkv / a.splits);
         AttnTile tl;

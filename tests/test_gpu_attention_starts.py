@@ -74,3 +74,27 @@ def test_slice_of_starts(dev, dt, d, heads, kv, case, causal):
     want, tol = backward(do[qs], *args)
     for name, a, b, c in zip(("dq", "dk", "dv"), (dq[qs], dk[ks], dv[ks]), want, tol):
         assert_close(a, b, c, name)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_most_sequences(dev, dt):
+    """So many sequences that a launch's first axis does not cover their tiles; most are empty."""
+    heads, d, n = 4, 16, (1 << 22) + 70
+    lens = torch.zeros(n, dtype=torch.int32)
+    lens[::1 << 17] = 3
+    some = [3] * int((lens > 0).sum())
+    cu = torch.cat([torch.zeros(1, dtype=torch.int32), lens.cumsum(0, dtype=torch.int32)]).to(dev)
+    t = sum(some)
+    g = torch.Generator().manual_seed(7)
+    q, k, v, do = (torch.randn(t, heads, d, generator=g).to(dt) for _ in range(4))
+    card = [x.to(dev) for x in (q, k, v)]
+    nan = [torch.full_like(x, float("nan")) for x in card]
+    out, lse = ops.attention(*card, cu, cu, out=nan[0].clone())
+    got = ops.attention_backward(do.to(dev), *card, out, lse, cu, cu, dq=nan[0], dk=nan[1],
+                                 dv=nan[2])
+    ro, rl, to, tl = forward(q, k, v, some, some, True, d ** -0.5)
+    assert_close(out, ro, to, "out")
+    assert_close(lse, rl, tl, "lse")
+    want, tol = backward(do, q, k, v, some, some, True, d ** -0.5)
+    for name, a, b, c in zip(("dq", "dk", "dv"), got, want, tol):
+        assert_close(a, b, c, name)
