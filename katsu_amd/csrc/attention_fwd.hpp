@@ -259,7 +259,7 @@ struct AttnFwd {
                 for (int w = 0; w < WK; ++w)
 #pragma unroll
                     for (int v = 0; v < 16; ++v)
-                        if (by[w] != 0.f) x[v] += by[w] * om[((w * ND + d) * 16 + v) * 64 + lane];
+                        x[v] += by[w] * om[((w * ND + d) * 16 + v) * 64 + lane];
                 finish(a, me, x, d, h, M, L);
             }
         }
