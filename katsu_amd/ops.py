@@ -274,8 +274,8 @@ def _attention(q, k, v, out, cu_q, cu_k, k_lens, causal, scale):
     _dev_lm(q, k, v, out)
     strides = [_heads(t, w) for t, w in ((q, "q"), (k, "k"), (v, "v"), (out, "out"))]
     tq, heads, dim = q.shape
-    if k.shape != v.shape or k.shape[2] != dim or out.shape != q.shape:
-        raise ValueError("k and v must have one shape, q's channels, and out q's shape")
+    if k.shape != v.shape or k.shape[2] != dim or dim == 0 or out.shape != q.shape:
+        raise ValueError("k and v must have one shape, q's channels (one at least), out q's shape")
     if k.shape[1] == 0 or heads % k.shape[1]:
         raise ValueError("query heads must be a multiple of key heads")
     if (cu_q is None) != (cu_k is None):

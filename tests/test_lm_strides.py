@@ -84,3 +84,13 @@ def test_attention_far_tokens(dev, dt, d):
         0 if dt is torch.float32 else 2.0 ** -7)
     for a, b in zip((far["out"], far_lse, *got), (out, lse, *want)):
         assert ((a - b).abs() <= tol * (b.abs() + 1)).all()
+
+
+@pytest.mark.gpu
+def test_no_channels(dev):
+    """A refusal of ops' own, not a division by zero."""
+    q = torch.empty(3, 2, 0, device=dev)
+    with pytest.raises(ValueError):
+        ops.attention(q, q, q)
+    with pytest.raises(ValueError):
+        ops.attention_workspace_bytes(q, q, q)
