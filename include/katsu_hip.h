@@ -297,7 +297,10 @@ typedef enum katsu_dtype { KATSU_F32 = 0, KATSU_BF16 = 1 } katsu_dtype;
  * With causal set query i of Lq sees key j of Lk if j <= i + Lk - Lq: the last
  * query sees every key.  A query that sees none gives out 0 and lse -inf.
  * What masked places hold changes nothing, Inf and NaN included.
- * scale must be positive and finite; an output's strides must not be zero. */
+ * scale must be positive and finite; heads at most 65535; an output's strides
+ * must not be zero, nor its memory an operand's.  In bfloat16 the products take
+ * P rounded to bfloat16, and the backward ones dS too (with 16 bits up to 32
+ * channels); sums are float32.  Float32 operands are not rounded. */
 typedef struct katsu_attention {
     int32_t dtype;  /* katsu_dtype of q, k, v, out */
     int32_t causal;
@@ -323,7 +326,9 @@ int katsu_hip_attention_fwd_dev(const katsu_attention *d, const void *q, const v
  *   dq = scale dS k,  dk = scale dS^T q and dv = P^T dout summed over the
  * query heads of a key head.  Outputs are overwritten.  A query that sees no
  * key gives no gradient, a key that no query sees gets zeros.
- * Workspace as above, of katsu_hip_attention_bwd_workspace bytes. */
+ * Workspace as above, of katsu_hip_attention_bwd_workspace bytes: in float32 dk
+ * and dv once more for each query head of a group and up to four runs (65536
+ * tokens, 32/8 heads of 128: 8.6 GB). */
 typedef struct katsu_attention_grads {
     int64_t dout_stride[2], dq_stride[2], dk_stride[2], dv_stride[2];
 } katsu_attention_grads;

@@ -11,10 +11,11 @@
 // in the registers of the wave that owns the row.  That computes the scores and dP twice,
 // seven products for five, and gives the same bits on every call.
 //
-// Bound by the matrix cores: 4096 tokens, 16/4 heads of 128, bfloat16, all keys 485 us (0.99
-// PFLOP/s of the seven products), 16384 tokens, 8 heads 3292 us (1.17); float32, 16/16 heads of
-// 64: 1735 us, 139 of the 154 TFLOP/s that a large library product reaches.  2711 + 1024 +
-// 1777 + 488 tokens packed, 16/4 heads, bfloat16: dq 100 us, dk and dv 144 and their sum 18.
+// Bound by the matrix cores: 4096 tokens, 16/4 heads of 128, bfloat16, all keys 447-474 us (1.0-1.1
+// PFLOP/s of the seven products), 16384 tokens, 8 heads 3400 us (1.13); float32, 16/16 heads of
+// 64: 1744 us, 138 TFLOP/s, of the 154 that a large product on the float32 instruction reaches.
+// 2711 + 1024 + 1777 + 488 tokens packed, 16/4 heads, bfloat16: dq 97 us, dk and dv 138 and their
+// sum 18.
 #pragma once
 
 #include "attention.hpp"

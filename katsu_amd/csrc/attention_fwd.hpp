@@ -12,11 +12,12 @@
 // them (each its own LDS, no barrier) and join at the end, for tiles of few rows.
 //
 // Bound: long prompts in bfloat16 by the matrix cores and, beside them, the exponentials
-// and conversions (8192 tokens, 16/4 heads of 128, causal: 274-294 us, 0.94-1.0 PFLOP/s, matrix
-// cores 55% busy, where a large library product reaches 1.23; 16384 tokens, 8 heads, all keys:
-// 1.09); in float32 by its matrix rate (4096 tokens, 16/4 heads of 128, all keys: 998 us, 138
-// TFLOP/s, of 154); single tokens by reading the cache (32 of 1500-7650 keys, 8 key heads of
-// 128: 129 us, 4.65 TB/s, where a copy reaches 4.74).  32 rows a wave, two waves a SIMD: the
+// and conversions (8192 tokens, 16/4 heads of 128, causal: 283-298 us, 0.92-0.97 PFLOP/s, matrix
+// cores 55% busy, where a large library product reaches 1.33; 16384 tokens, 8 heads, all keys:
+// 1.07); in float32 by the float32 instruction's rate (4096 tokens, 16/4 heads of 128, all keys:
+// 1000 us, 137 TFLOP/s, of 154); single tokens in bfloat16 by reading the cache (32 of 1500-7650
+// keys, 8 key heads of 128: 127-130 us, 4.6-4.7 TB/s, where a copy reaches 4.75), in float32 by
+// the two waves that a CU has of 512-byte rows (532 us, 2.26 TB/s; heads of 64 3.8).  32 rows a wave, two waves a SIMD: the
 // sums, q and one tile's scores fit 256 registers, and the one wave's exponentials run under
 // the other's products; tiles of 64 keys (32 of 512-byte rows), two of each in LDS, let two
 // blocks share a CU.

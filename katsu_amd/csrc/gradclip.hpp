@@ -6,7 +6,7 @@
 // block add the parts in the same order and scale its share.  Squares are summed in
 // float64: they cannot overflow, and HBM is the bound either way (one fused
 // multiply-add for 2 or 4 bytes read).  770 M bfloat16 values, not in place: 878 us, the sums
-// 278 (5.5 TB/s), the scaling 599 (5.1); 3.4 M float32 values in 26 tensors: 14 us of launches.
+// 274 (5.6 TB/s), the scaling 594 (5.2); 3.0 M float32 values in 26 tensors: 13.5 us of launches.
 #pragma once
 
 #include "lmvec.hpp"
