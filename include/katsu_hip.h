@@ -415,6 +415,101 @@ int katsu_hip_clip_grad_norm_ws_dev(const int32_t *dtypes, const void *const *in
                                     float max_norm, float *norm, void *workspace,
                                     size_t workspace_bytes, void *stream);
 
+/* Embedding: out[t] = scale * table[ids[t]], tokens x cols from vocab x cols;
+ * zeros where ids[t] (device int32) is not in [0, vocab): padding.  Strides are
+ * in elements between rows; columns are adjacent.  `accumulate` is the
+ * backward call's. */
+typedef struct katsu_embedding {
+    int32_t dtype;       /* katsu_dtype of the table and the output */
+    int32_t accumulate;  /* backward: add to dtable (1) or overwrite it (0) */
+    uint64_t tokens, vocab, cols;
+    int64_t table_stride, out_stride;
+    float scale;
+} katsu_embedding;
+int katsu_hip_embedding_dev(const katsu_embedding *d, const int32_t *ids, const void *table,
+                            void *out, void *stream);
+
+/* Its gradient: dtable[v] = (dtable[v] +) scale * sum of dout[t] over the
+ * tokens with ids[t] = v, summed in float32 in an order that the sizes and ids
+ * alone decide, and rounded once.  Rows without a token become zeros, or with
+ * `accumulate` stay as they are, bit by bit.  out_stride is dout's,
+ * table_stride dtable's.  Workspace as above, of
+ * katsu_hip_embedding_bwd_workspace bytes. */
+int katsu_hip_embedding_bwd_workspace(const katsu_embedding *d, size_t *bytes);
+int katsu_hip_embedding_bwd_dev(const katsu_embedding *d, const void *dout, const int32_t *ids,
+                                void *dtable, void *workspace, size_t workspace_bytes,
+                                void *stream);
+
+/* The norm of each query and key head, then rotary positions, in one pass:
+ *   n = x / sqrt(mean(x^2) + eps) * w,  y = n turned as katsu_hip_rotary_dev does
+ * with w_q and w_k of head_dim (1..512) values, or NULL for none; rotary_dim 0
+ * (and table NULL) leaves the turn out.  Operands, positions and strides are as
+ * in katsu_hip_rotary_dev; k may be NULL with k_heads 0.  Outputs may be the
+ * inputs, with the same strides.  n is not rounded before the turn. */
+typedef struct katsu_qk_norm_rotary {
+    int32_t dtype, interleaved;
+    uint64_t tokens, heads, k_heads, head_dim, rotary_dim, length;
+    int64_t q_stride[2], k_stride[2], q_out_stride[2], k_out_stride[2];
+    float eps;
+} katsu_qk_norm_rotary;
+int katsu_hip_qk_norm_rotary_dev(const katsu_qk_norm_rotary *d, const void *q, const void *k,
+                                 const void *w_q, const void *w_k, const float *table,
+                                 const int32_t *positions, void *q_out, void *k_out,
+                                 void *stream);
+
+/* Its gradient, from dq and dk, the gradients of the outputs, and the forward
+ * call's operands: dx_q and dx_k (strides q_out_stride and k_out_stride; they
+ * may be dq and dk, or q and k, with the same strides), dw_q and dw_k where
+ * w_q and w_k are given, summed over tokens and heads in float32 in a fixed
+ * order through a workspace as above. */
+typedef struct katsu_qk_norm_rotary_grads {
+    int64_t dq_stride[2], dk_stride[2];
+} katsu_qk_norm_rotary_grads;
+int katsu_hip_qk_norm_rotary_bwd_workspace(const katsu_qk_norm_rotary *d, size_t *bytes);
+int katsu_hip_qk_norm_rotary_bwd_dev(const katsu_qk_norm_rotary *d,
+                                     const katsu_qk_norm_rotary_grads *g, const void *dq,
+                                     const void *dk, const void *q, const void *k,
+                                     const void *w_q, const void *w_k, const float *table,
+                                     const int32_t *positions, void *dx_q, void *dx_k,
+                                     void *dw_q, void *dw_k, void *workspace,
+                                     size_t workspace_bytes, void *stream);
+
+/* The loss of rows x vocab logits z against a teacher's top logits t, `top`
+ * (0..1024) of them a row at the columns ids (both [rows][top], contiguous).
+ * Over a row's entries whose id is in [0, vocab), with tau the temperature:
+ *   p = softmax(t / tau),  P = softmax(z / tau) over all columns,
+ *   loss = tau^2 sum_k p_k (log p_k - log P[id_k]),
+ *   dlogits[v] = dloss tau (P[v] - sum of the p_k with id_k = v)
+ * With top 1 and tau 1 this is the cross entropy with labels.  An id may occur
+ * more than once.  A row without an entry, or with all of them at -inf, has
+ * loss 0 and gradient 0 whatever its logits, its other entries and its dloss
+ * hold.  p_k = 0 adds nothing.  A row of nothing but -inf, or with a NaN or
+ * +inf, has a loss of NaN, as the formula does.
+ * Strides are in elements between rows (columns are adjacent), of dloss
+ * between values (0: one for all rows).  stats [2][rows] (or NULL) receives
+ * each row's largest logit and 1 / sum exp((z - largest) / tau), 0 and 0 for a
+ * row without an entry: what the backward call reads. */
+typedef struct katsu_distillation {
+    int32_t dtype, teacher_dtype;  /* katsu_dtype of the logits, of the teacher's */
+    uint64_t rows, vocab, top;
+    int64_t stride, out_stride, dloss_stride;  /* of logits, dlogits, dloss */
+    float temperature;
+} katsu_distillation;
+int katsu_hip_distillation_workspace(const katsu_distillation *d, size_t *bytes);
+int katsu_hip_distillation_dev(const katsu_distillation *d, const void *logits,
+                               const int32_t *ids, const void *teacher, float *loss, float *stats,
+                               void *workspace, size_t workspace_bytes, void *stream);
+/* The gradient; dlogits may be logits, with the same stride. */
+int katsu_hip_distillation_bwd_dev(const katsu_distillation *d, const float *dloss,
+                                   const void *logits, const int32_t *ids, const void *teacher,
+                                   const float *stats, void *dlogits, void *stream);
+/* Both in one pass over the logits, where dloss is known before the loss is;
+ * dlogits may be logits, with the same stride. */
+int katsu_hip_distillation_step_dev(const katsu_distillation *d, const void *logits,
+                                    const int32_t *ids, const void *teacher, const float *dloss,
+                                    float *loss, void *dlogits, void *workspace,
+                                    size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

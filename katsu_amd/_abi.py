@@ -37,6 +37,11 @@ EXPORTS = (
     "katsu_hip_block_norm_dev", "katsu_hip_block_norm_bwd_workspace",
     "katsu_hip_block_norm_bwd_dev", "katsu_hip_clip_grad_norm_workspace",
     "katsu_hip_clip_grad_norm_dev", "katsu_hip_clip_grad_norm_ws_dev",
+    "katsu_hip_embedding_dev", "katsu_hip_embedding_bwd_workspace", "katsu_hip_embedding_bwd_dev",
+    "katsu_hip_qk_norm_rotary_dev", "katsu_hip_qk_norm_rotary_bwd_workspace",
+    "katsu_hip_qk_norm_rotary_bwd_dev", "katsu_hip_distillation_workspace",
+    "katsu_hip_distillation_dev", "katsu_hip_distillation_bwd_dev",
+    "katsu_hip_distillation_step_dev",
 )
 
 
@@ -83,6 +88,37 @@ class BlockNorm(ctypes.Structure):
     _fields_ = ([(f, ctypes.c_int32) for f in ("dtype", "gate_rows")] +
                 [(f, ctypes.c_uint64) for f in ("rows", "cols")] +
                 [(f, ctypes.c_float) for f in ("alpha", "eps")])
+
+
+class Embedding(ctypes.Structure):
+    """katsu_embedding: the shape, strides and scale of an embedding call."""
+    _fields_ = ([(f, ctypes.c_int32) for f in ("dtype", "accumulate")] +
+                [(f, ctypes.c_uint64) for f in ("tokens", "vocab", "cols")] +
+                [(f, ctypes.c_int64) for f in ("table_stride", "out_stride")] +
+                [("scale", ctypes.c_float)])
+
+
+class QkNormRotary(ctypes.Structure):
+    """katsu_qk_norm_rotary: the shapes and strides of a call on query and key heads."""
+    _fields_ = ([(f, ctypes.c_int32) for f in ("dtype", "interleaved")] +
+                [(f, ctypes.c_uint64) for f in ("tokens", "heads", "k_heads", "head_dim",
+                                                "rotary_dim", "length")] +
+                [(f, ctypes.c_int64 * 2) for f in ("q_stride", "k_stride", "q_out_stride",
+                                                   "k_out_stride")] +
+                [("eps", ctypes.c_float)])
+
+
+class QkNormRotaryGrads(ctypes.Structure):
+    """katsu_qk_norm_rotary_grads: the strides of a backward call's incoming gradients."""
+    _fields_ = [(f, ctypes.c_int64 * 2) for f in ("dq_stride", "dk_stride")]
+
+
+class Distillation(ctypes.Structure):
+    """katsu_distillation: the shapes and strides of a distillation call."""
+    _fields_ = ([(f, ctypes.c_int32) for f in ("dtype", "teacher_dtype")] +
+                [(f, ctypes.c_uint64) for f in ("rows", "vocab", "top")] +
+                [(f, ctypes.c_int64) for f in ("stride", "out_stride", "dloss_stride")] +
+                [("temperature", ctypes.c_float)])
 
 
 _lib = None
@@ -152,6 +188,20 @@ def lib():
         L.katsu_hip_clip_grad_norm_workspace.argtypes = [sz, ctypes.POINTER(sz)]
         L.katsu_hip_clip_grad_norm_dev.argtypes = [vp, vp, vp, vp, sz, fp, vp, vp]
         L.katsu_hip_clip_grad_norm_ws_dev.argtypes = [vp, vp, vp, vp, sz, fp, vp, vp, sz, vp]
+        ep, szp = ctypes.POINTER(Embedding), ctypes.POINTER(sz)
+        L.katsu_hip_embedding_dev.argtypes = [ep, vp, vp, vp, vp]
+        L.katsu_hip_embedding_bwd_workspace.argtypes = [ep, szp]
+        L.katsu_hip_embedding_bwd_dev.argtypes = [ep, vp, vp, vp, vp, sz, vp]
+        qp = ctypes.POINTER(QkNormRotary)
+        L.katsu_hip_qk_norm_rotary_dev.argtypes = [qp] + [vp] * 9
+        L.katsu_hip_qk_norm_rotary_bwd_workspace.argtypes = [qp, szp]
+        L.katsu_hip_qk_norm_rotary_bwd_dev.argtypes = ([qp, ctypes.POINTER(QkNormRotaryGrads)] +
+                                                       [vp] * 13 + [sz, vp])
+        dp = ctypes.POINTER(Distillation)
+        L.katsu_hip_distillation_workspace.argtypes = [dp, szp]
+        L.katsu_hip_distillation_dev.argtypes = [dp] + [vp] * 6 + [sz, vp]
+        L.katsu_hip_distillation_bwd_dev.argtypes = [dp] + [vp] * 7
+        L.katsu_hip_distillation_step_dev.argtypes = [dp] + [vp] * 7 + [sz, vp]
         for name in EXPORTS:
             if name not in ("katsu_hip_version", "katsu_hip_strerror", "katsu_hip_shutdown",
                             "katsu_hip_noalloc_scratch_bytes",

@@ -1,0 +1,303 @@
+// distill.hpp -- the loss of a row's logits z against a teacher's top logits t_k at ids
+// id_k, and its gradient.  Over the entries whose id is one of the V columns:
+//
+//   p = softmax(t / tau),  P = softmax(z / tau) over all V,
+//   loss = tau^2 sum_k p_k (log p_k - log P[id_k])
+//   dz_v = dloss tau (P_v - sum of the p_k with id_k = v)
+//
+// A row without such an entry, or with none above -inf, has loss and gradient 0, and its
+// logits are not read.  With M = max z and L = sum exp((z - M)/tau), log P_v is
+// (z_v - M)/tau - log L: differences of logits are taken first, so that large ones lose
+// nothing and the type's lowest value does not overflow.
+//
+// HBM-bound: one pass with each thread's running maximum and sum.
+#pragma once
+
+#include "lmvec.hpp"
+
+namespace katsu {
+
+struct DistillArgs {
+    const void *z, *teacher;
+    const int32_t *ids;
+    const float *dloss;
+    float *stats;       // [2][rows]: M, 1/L (0, 0 without an entry)
+    float *loss;
+    void *dz;
+    float *part;        // [rows][splits][2]: M and L of a run of columns
+    int64_t rows, vocab, z_row, dz_row, dloss_step, run;  // run: columns of a split
+    int top, splits, teacher_bf16;
+    float tau, scale2;  // scale2: log2(e) / tau
+};
+
+constexpr int kDistillTop = 1024;
+
+__device__ __forceinline__ float distill_exp(float x, float by) {  // exp((x)/tau)
+    return __builtin_amdgcn_exp2f(x * by);
+}
+
+// A block's sum or maximum; each call uses its own slot of `part`.
+template <int NT, class F>
+__device__ __forceinline__ float block_join(float v, float *part, F f) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = f(v, __shfl_xor(v, off, 64));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) v = f(v, part[w]);
+    return v;
+}
+struct JoinSum {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+struct JoinMax {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+
+// A thread's entries of a row: entry tid + NT i.
+template <int NT>
+struct DistillRow {
+    static constexpr int N = kDistillTop / NT;
+    int id[N];        // -1 where there is none
+    float t[N], p[N];
+    float largest, total;
+    bool some;
+
+    __device__ __forceinline__ void load(const DistillArgs &a, int64_t row) {
+        float m = -INFINITY;
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int k = threadIdx.x + NT * i;
+            id[i] = -1;
+            t[i] = -INFINITY;
+            if (k < a.top) {
+                const int v = a.ids[row * a.top + k];
+                if (v >= 0 && v < a.vocab) {
+                    id[i] = v;
+                    t[i] = a.teacher_bf16 ? (float)((const __bf16 *)a.teacher)[row * a.top + k]
+                                          : ((const float *)a.teacher)[row * a.top + k];
+                    any |= t[i] != -INFINITY;
+                    m = fmaxf(m, t[i]);
+                }
+            }
+        }
+        some = __syncthreads_or(any);
+        largest = m;
+    }
+    __device__ __forceinline__ void softmax(const DistillArgs &a, float *part_m, float *part_l) {
+        largest = block_join<NT>(largest, part_m, JoinMax());
+        float l = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            p[i] = t[i] == -INFINITY ? 0.f : distill_exp(t[i] - largest, a.scale2);
+            l += p[i];
+        }
+        total = block_join<NT>(l, part_l, JoinSum());
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] /= total;
+    }
+};
+
+// A running maximum and sum.
+struct DistillSum {
+    float m = -INFINITY, l = 0.f;
+    __device__ __forceinline__ static float ref(float m) { return m == -INFINITY ? 0.f : m; }
+    template <int N>
+    __device__ __forceinline__ void add(const float (&x)[N], float by) {
+        float top = x[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+        const float mn = fmaxf(m, top), r = ref(mn);
+        l *= distill_exp(m - r, by);
+#pragma unroll
+        for (int i = 0; i < N; ++i) l += distill_exp(x[i] - r, by);
+        m = mn;
+    }
+    __device__ __forceinline__ void join(float m2, float l2, float by) {
+        const float mn = fmaxf(m, m2), r = ref(mn);
+        l = l * distill_exp(m - r, by) + l2 * distill_exp(m2 - r, by);
+        m = mn;
+    }
+};
+
+// M and L of a row's columns [c0, c1), the same in every thread.
+template <typename T, int NT>
+__device__ __forceinline__ DistillSum distill_columns(const T *z, int64_t c0, int64_t c1, float by,
+                                                      float *part) {
+    constexpr int E = Piece<T>::E;
+    DistillSum s;
+    int64_t i = c0 + threadIdx.x * E;
+    for (; i + E <= c1; i += NT * E) {
+        float x[E];
+        load_piece(z, i, c1, x);
+        s.add(x, by);
+    }
+    for (; i < c1; ++i) {  // this thread's piece is the last one, cut short
+        const float x[1] = {(float)z[i]};
+        s.add(x, by);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+        s.join(__shfl_xor(s.m, off, 64), __shfl_xor(s.l, off, 64), by);
+    if ((threadIdx.x & 63) == 0) {
+        part[2 * (threadIdx.x >> 6)] = s.m;
+        part[2 * (threadIdx.x >> 6) + 1] = s.l;
+    }
+    __syncthreads();
+    DistillSum all;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) all.join(part[2 * w], part[2 * w + 1], by);
+    return all;
+}
+
+template <typename T, int NT>
+__device__ __forceinline__ void distill_loss(const DistillArgs &a, int64_t row,
+                                             const DistillRow<NT> &d, const DistillSum &s,
+                                             float *part) {
+    const T *z = (const T *)a.z + row * a.z_row;
+    const float inv_tau = 1.f / a.tau, lt = logf(d.total), ls = logf(s.l);
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < DistillRow<NT>::N; ++i)
+        if (d.id[i] >= 0 && d.p[i] != 0.f)
+            v += d.p[i] * (((d.t[i] - d.largest) - ((float)z[d.id[i]] - s.m)) * inv_tau - lt + ls);
+    v = block_join<NT>(v, part, JoinSum());
+    if (threadIdx.x == 0) a.loss[row] = a.tau * a.tau * v;
+}
+
+// The gradient of columns [c0, c1): all of them as if there were no teacher, then the
+// teacher's, of which the first of equal ids takes their sum.
+template <typename T, int NT>
+__device__ __forceinline__ void distill_grad(const DistillArgs &a, int64_t row, int64_t c0,
+                                             int64_t c1, const DistillRow<NT> &d, float m,
+                                             float inv, int *ids, float *ps) {
+    constexpr int E = Piece<T>::E, N = DistillRow<NT>::N;
+    const T *z = (const T *)a.z + row * a.z_row;
+    T *dz = (T *)a.dz + row * a.dz_row;
+    const float g = a.dloss[row * a.dloss_step] * a.tau, by = inv * g;
+    float fix[N];
+    bool own[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int k = threadIdx.x + NT * i;
+        ids[k] = d.id[i];
+        ps[k] = d.p[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int k = threadIdx.x + NT * i;
+        own[i] = d.id[i] >= c0 && d.id[i] < c1;
+        if (!own[i]) continue;
+        float p = 0.f;
+        for (int j = 0; j < a.top; ++j) {
+            if (ids[j] != d.id[i]) continue;
+            p += ps[j];
+            if (j < k) own[i] = false;
+        }
+        if (own[i]) fix[i] = (distill_exp((float)z[d.id[i]] - m, a.scale2) * inv - p) * g;
+    }
+    __syncthreads();  // dz may be z: all of the teacher's logits are read
+    for (int64_t i = c0 + threadIdx.x * E; i < c1; i += NT * E) {
+        float x[E];
+        load_piece(z, i, c1, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = distill_exp(x[e] - m, a.scale2) * by;
+        store_piece(dz, i, c1, x);
+    }
+    __syncthreads();  // and all others written
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (own[i]) dz[d.id[i]] = (T)fix[i];
+}
+
+template <typename T, int NT>
+__device__ __forceinline__ void distill_zero(const DistillArgs &a, int64_t row, int64_t c0,
+                                             int64_t c1) {
+    constexpr int E = Piece<T>::E;
+    const float x[E] = {};
+    for (int64_t i = c0 + threadIdx.x * E; i < c1; i += NT * E)
+        store_piece((T *)a.dz + row * a.dz_row, i, c1, x);
+}
+
+// Loss, gradient or both of whole rows: a block a row.
+template <typename T, int NT, bool LOSS, bool GRAD>
+__global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
+    __shared__ float part[5][2 * NT / 64];
+    __shared__ int ids[GRAD ? kDistillTop : 1];
+    __shared__ float ps[GRAD ? kDistillTop : 1];
+    const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (row >= a.rows) return;
+    const int64_t c0 = LOSS ? 0 : blockIdx.z * a.run;
+    const int64_t c1 = LOSS ? a.vocab : min(c0 + a.run, a.vocab);
+    DistillRow<NT> d;
+    d.load(a, row);
+    if (!d.some) {
+        if (LOSS && threadIdx.x == 0) {
+            a.loss[row] = 0.f;
+            if (a.stats) a.stats[row] = a.stats[a.rows + row] = 0.f;
+        }
+        if (GRAD) distill_zero<T, NT>(a, row, c0, c1);
+        return;
+    }
+    d.softmax(a, part[0], part[1]);
+    float m, inv;
+    if constexpr (LOSS) {
+        const DistillSum s = distill_columns<T, NT>((const T *)a.z + row * a.z_row, 0, a.vocab,
+                                                    a.scale2, part[2]);
+        distill_loss<T, NT>(a, row, d, s, part[3]);
+        m = s.m;
+        inv = 1.f / s.l;
+        if (a.stats && threadIdx.x == 0) {
+            a.stats[row] = m;
+            a.stats[a.rows + row] = inv;
+        }
+    } else {
+        m = a.stats[row];
+        inv = a.stats[a.rows + row];
+    }
+    if constexpr (GRAD) distill_grad<T, NT>(a, row, c0, c1, d, m, inv, ids, ps);
+}
+
+// Few rows: M and L of runs of a row's columns, then the loss from them.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
+    __shared__ float part[2 * NT / 64];
+    const int64_t row = blockIdx.x, c0 = blockIdx.z * a.run;
+    const DistillSum s = distill_columns<T, NT>((const T *)a.z + row * a.z_row, c0,
+                                                min(c0 + a.run, a.vocab), a.scale2, part);
+    if (threadIdx.x == 0) {
+        float *p = a.part + (row * a.splits + blockIdx.z) * 2;
+        p[0] = s.m;
+        p[1] = s.l;
+    }
+}
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) distill_join_kernel(const DistillArgs a) {
+    __shared__ float part[3][2 * NT / 64];
+    const int64_t row = blockIdx.x;
+    DistillRow<NT> d;
+    d.load(a, row);
+    float m = 0.f, inv = 0.f;
+    if (d.some) {
+        d.softmax(a, part[0], part[1]);
+        DistillSum s;
+        for (int i = 0; i < a.splits; ++i) {
+            const float *p = a.part + (row * a.splits + i) * 2;
+            s.join(p[0], p[1], a.scale2);
+        }
+        distill_loss<T, NT>(a, row, d, s, part[2]);
+        m = s.m;
+        inv = 1.f / s.l;
+    } else if (threadIdx.x == 0) {
+        a.loss[row] = 0.f;
+    }
+    if (threadIdx.x == 0) {
+        a.stats[row] = m;
+        a.stats[a.rows + row] = inv;
+    }
+}
+
+}  // namespace katsu

@@ -1,0 +1,274 @@
+// headnorm.hpp -- each query and key head divided by its root mean square, times a weight
+// for each channel, and its first R channels turned by the token's position, in one pass:
+//
+//   r = 1/sqrt(mean(x^2) + eps),  n = x r w,  y = turn(n)       (the turn as in rotary.hpp)
+//
+// and its gradient, with g = the gradient of y turned back:
+//   dw = sum over tokens and heads of g x r,  dx = r g w - x r^3 mean(g w x)
+// where both of a head's sums are taken at once.
+//
+// HBM-bound: a head stays in its lanes' registers, so each operand is read once and each
+// result written once.
+#pragma once
+
+#include "lmvec.hpp"
+
+namespace katsu {
+
+// One of q and k.
+struct HeadTensor {
+    const void *x, *w, *dy;  // dy: the gradient of the output (backward)
+    void *out;               // output, or the gradient of x
+    int64_t x_token, x_head, dy_token, dy_head, out_token, out_head;
+    int heads;
+};
+struct HeadArgs {
+    HeadTensor t[2];  // q and k
+    const float *table;
+    const int32_t *positions;  // NULL: 0, 1, ..
+    int64_t tokens, length;
+    int D, R, units;           // units of 2E channels of a head
+    float eps, inv_d;
+    float *part;               // backward, [blocks][D]: sums of dw, q's blocks first
+    int blocks[2];             // backward: blocks of q, of k
+};
+
+// A head is units of 2E channels: E pairs (R/2 apart, or 2E neighbours with INTER) for the
+// part that turns, then two pieces of E neighbours of the rest.  E divides R/2 and the rest,
+// whose last unit may have one piece only.
+template <typename T, bool INTER, int E>
+struct HeadUnit {
+    int c[2];      // its pieces' first channels
+    bool has[2];
+    bool turns;
+    int angle;     // its first pair
+
+    __device__ __forceinline__ void init(const HeadArgs &a, int u) {
+        const int half = a.R / 2, turning = half / E;
+        turns = u < turning;
+        angle = u * E;
+        if (turns) {
+            c[0] = INTER ? 2 * u * E : u * E;
+            c[1] = INTER ? c[0] + E : half + u * E;
+        } else {
+            c[0] = a.R + (u - turning) * 2 * E;
+            c[1] = c[0] + E;
+        }
+        has[0] = u < a.units;
+        has[1] = has[0] && c[1] < a.D;
+    }
+    __device__ __forceinline__ void load(const void *p, int64_t at, float (&x)[2][E]) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (has[i])
+                rotary_load<T, E>((const T *)p + at + c[i], x[i]);
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+    }
+    __device__ __forceinline__ void store(void *p, int64_t at, const float (&x)[2][E]) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (has[i]) rotary_store<T, E>((T *)p + at + c[i], x[i]);
+    }
+    __device__ __forceinline__ void angles(const float *row, int R, float (&cs)[2][E]) const {
+        if (!turns) return;
+        rotary_load<float, E>(row + angle, cs[0]);
+        rotary_load<float, E>(row + R / 2 + angle, cs[1]);
+    }
+    // sign: -1 turns back.
+    __device__ __forceinline__ void turn(float (&x)[2][E], const float (&cs)[2][E],
+                                         float sign) const {
+        if (!turns) return;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            // INTER: pair e is the unit's channels 2e and 2e + 1.
+            const int i0 = INTER ? (2 * e) / E : 0, e0 = INTER ? (2 * e) % E : e;
+            const int i1 = INTER ? (2 * e + 1) / E : 1, e1 = INTER ? (2 * e + 1) % E : e;
+            const float u = x[i0][e0], v = x[i1][e1], c = cs[0][e], s = sign * cs[1][e];
+            x[i0][e0] = u * c - v * s;
+            x[i1][e1] = u * s + v * c;
+        }
+    }
+};
+
+__device__ __forceinline__ const float *head_angles(const HeadArgs &a, int64_t token) {
+    int64_t pos = a.positions ? a.positions[token] : token;
+    pos = pos < 0 ? 0 : pos < a.length ? pos : a.length - 1;  // stays inside the table
+    return a.table + pos * a.R;
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int off = G / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+// The token and the head of the item that lies `local` after the base-th of a token's n: local
+// below 2^20, so that the quotient is exact.
+__device__ __forceinline__ int head_split(int local, int n, float inv_n, int &token) {
+    const int q = (int)(((float)local + 0.5f) * inv_n);
+    token = q;
+    return local - q * n;
+}
+
+// G lanes a head, NU units a lane.
+template <typename T, bool INTER, int E, int G, int NU>
+__global__ void __launch_bounds__(256) head_norm_kernel(const HeadArgs a) {
+    constexpr int PER = 256 / G;
+    const int n = a.t[0].heads + a.t[1].heads, lane = threadIdx.x % G;
+    const int64_t base = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * PER;
+    const int64_t token0 = base / n;
+    int more;
+    int head = head_split((int)(base - token0 * n) + threadIdx.x / G, n, 1.f / (float)n, more);
+    const int64_t token = token0 + more;
+    if (token >= a.tokens) return;  // a whole group
+    const bool second = head >= a.t[0].heads;
+    const HeadTensor &t = a.t[second];
+    if (second) head -= a.t[0].heads;
+    const int64_t in = token * t.x_token + head * t.x_head;
+    HeadUnit<T, INTER, E> u[NU];
+    float x[NU][2][E], cs[NU][2][E], w[NU][2][E];
+    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < NU; ++k) {
+        u[k].init(a, k * G + lane);
+        u[k].load(t.x, in, x[k]);
+    }
+    if (a.R) {
+        const float *row = head_angles(a, token);
+#pragma unroll
+        for (int k = 0; k < NU; ++k) u[k].angles(row, a.R, cs[k]);
+    }
+    if (t.w) {
+#pragma unroll
+        for (int k = 0; k < NU; ++k) u[k].load(t.w, 0, w[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < NU; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) ss += x[k][i][e] * x[k][i][e];
+    const float r = rsqrtf(group_sum<G>(ss) * a.inv_d + a.eps);
+#pragma unroll
+    for (int k = 0; k < NU; ++k) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[k][i][e] *= t.w ? r * w[k][i][e] : r;
+        u[k].turn(x[k], cs[k], 1.f);
+        u[k].store(t.out, token * t.out_token + head * t.out_head, x[k]);
+    }
+}
+
+// The gradient.  A block takes heads of q or of k, so that a lane's channels, and with them
+// its sums of dw, stay the same; the blocks' sums are added by head_norm_sum_kernel.
+template <typename T, bool INTER, int E, int G, int NU>
+__global__ void __launch_bounds__(256) head_norm_bwd_kernel(const HeadArgs a) {
+    constexpr int PER = 256 / G;
+    __shared__ float part[4][G * NU * 2 * E];
+    const bool second = (int)blockIdx.x >= a.blocks[0];
+    const HeadTensor &t = a.t[second];
+    const int block = (int)blockIdx.x - (second ? a.blocks[0] : 0);
+    const int lane = threadIdx.x % G, group = threadIdx.x / G;
+    const int64_t items = a.tokens * t.heads, step = (int64_t)a.blocks[second] * PER;
+    const float inv_n = 1.f / (float)t.heads;
+    HeadUnit<T, INTER, E> u[NU];
+    float w[NU][2][E], dw[NU][2][E] = {};
+#pragma unroll
+    for (int k = 0; k < NU; ++k) {
+        u[k].init(a, k * G + lane);
+        if (t.w) u[k].load(t.w, 0, w[k]);
+    }
+    for (int64_t base = (int64_t)block * PER; base < items; base += step) {
+        const int64_t token0 = base / t.heads;
+        int more;
+        const int head =
+            head_split((int)(base - token0 * t.heads) + group, t.heads, inv_n, more);
+        const int64_t token = token0 + more;
+        if (token >= a.tokens) break;  // a whole group, at its last item
+        float x[NU][2][E], g[NU][2][E], cs[NU][2][E];
+#pragma unroll
+        for (int k = 0; k < NU; ++k) {
+            u[k].load(t.x, token * t.x_token + head * t.x_head, x[k]);
+            u[k].load(t.dy, token * t.dy_token + head * t.dy_head, g[k]);
+        }
+        if (a.R) {
+            const float *row = head_angles(a, token);
+#pragma unroll
+            for (int k = 0; k < NU; ++k) u[k].angles(row, a.R, cs[k]);
+        }
+        float ss = 0.f, sg = 0.f;
+#pragma unroll
+        for (int k = 0; k < NU; ++k) {
+            u[k].turn(g[k], cs[k], -1.f);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    ss += x[k][i][e] * x[k][i][e];
+                    sg += (t.w ? g[k][i][e] * w[k][i][e] : g[k][i][e]) * x[k][i][e];
+                }
+        }
+        ss = group_sum<G>(ss);
+        sg = group_sum<G>(sg);
+        const float r = rsqrtf(ss * a.inv_d + a.eps), c = r * r * (sg * a.inv_d);
+#pragma unroll
+        for (int k = 0; k < NU; ++k) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    dw[k][i][e] += g[k][i][e] * (x[k][i][e] * r);
+                    const float gw = t.w ? g[k][i][e] * w[k][i][e] : g[k][i][e];
+                    x[k][i][e] = r * (gw - x[k][i][e] * c);
+                }
+            u[k].store(t.out, token * t.out_token + head * t.out_head, x[k]);
+        }
+    }
+    if (!t.w) return;
+    // The wave's groups, then the waves.
+#pragma unroll
+    for (int k = 0; k < NU; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                float v = dw[k][i][e];
+#pragma unroll
+                for (int off = 32; off >= G; off >>= 1) v += __shfl_xor(v, off, 64);
+                if ((threadIdx.x & 63) < G && u[k].has[i])
+                    part[threadIdx.x >> 6][u[k].c[i] + e] = v;
+            }
+    __syncthreads();
+    for (int d = threadIdx.x; d < a.D; d += 256)
+        a.part[(int64_t)blockIdx.x * a.D + d] =
+            part[0][d] + part[1][d] + part[2][d] + part[3][d];
+}
+
+// dw: the blocks' sums, in order within each of 16 rows of threads, then the rows'.
+// blockIdx.y: q or k.
+template <typename T>
+__global__ void __launch_bounds__(1024) head_norm_sum_kernel(const float *part, int n_q, int n_k,
+                                                            int D, T *dw_q, T *dw_k) {
+    __shared__ float s[16][64];
+    const bool second = blockIdx.y != 0;
+    T *out = second ? dw_k : dw_q;
+    if (!out) return;
+    const float *p = part + (second ? (int64_t)n_q * D : 0);
+    const int n = second ? n_k : n_q, lane = threadIdx.x & 63, row = threadIdx.x >> 6;
+    const int d = blockIdx.x * 64 + lane;
+    float v = 0.f;
+    if (d < D) {
+#pragma unroll 8
+        for (int i = row; i < n; i += 16) v += p[(int64_t)i * D + d];
+    }
+    s[row][lane] = v;
+    __syncthreads();
+    if (row != 0 || d >= D) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) v += s[i][lane];
+    out[d] = (T)v;
+}
+
+}  // namespace katsu

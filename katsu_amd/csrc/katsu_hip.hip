@@ -3377,4 +3377,141 @@ int katsu_hip_clip_grad_norm_dev(const int32_t *dtypes, const void *const *in, v
                                            stream);
 }
 
+int katsu_hip_embedding_dev(const katsu_embedding *d, const int32_t *ids, const void *table,
+                            void *out, void *stream) {
+    if (!d || !embedding_ok(*d) || !embedding_out_ok(d->tokens, d->cols, d->out_stride))
+        return KATSU_E_INVALID;
+    if (d->tokens == 0) return KATSU_OK;
+    if (!ids || !out || (d->vocab > 0 && !table)) return KATSU_E_INVALID;
+    return embedding(*d, ids, table, out, (hipStream_t)stream);
+}
+
+int katsu_hip_embedding_bwd_workspace(const katsu_embedding *d, size_t *bytes) {
+    if (!d || !bytes || !embedding_ok(*d)) return KATSU_E_INVALID;
+    *bytes = embedding_bwd_bytes(*d);
+    return KATSU_OK;
+}
+
+int katsu_hip_embedding_bwd_dev(const katsu_embedding *d, const void *dout, const int32_t *ids,
+                                void *dtable, void *workspace, size_t workspace_bytes,
+                                void *stream) {
+    if (!d || !embedding_ok(*d) || !embedding_out_ok(d->vocab, d->cols, d->table_stride))
+        return KATSU_E_INVALID;
+    if (d->vocab == 0 || (d->tokens == 0 && d->accumulate)) return KATSU_OK;
+    if (!dtable || (d->tokens > 0 && (!dout || !ids))) return KATSU_E_INVALID;
+    hipStream_t st = (hipStream_t)stream;
+    void *ws = nullptr;
+    const int rc = lm_scratch(workspace, workspace_bytes, embedding_bwd_bytes(*d), st, &ws);
+    if (rc) return rc;
+    return embedding_bwd(*d, dout, ids, dtable, ws, st);
+}
+
+int katsu_hip_qk_norm_rotary_dev(const katsu_qk_norm_rotary *d, const void *q, const void *k,
+                                 const void *w_q, const void *w_k, const float *table,
+                                 const int32_t *positions, void *q_out, void *k_out,
+                                 void *stream) {
+    if (!d || !qk_norm_rotary_ok(*d)) return KATSU_E_INVALID;
+    if (d->tokens == 0 || d->heads + d->k_heads == 0) return KATSU_OK;
+    if ((d->rotary_dim > 0 && !table) || (d->heads && (!q || !q_out)) ||
+        (d->k_heads && (!k || !k_out)))
+        return KATSU_E_INVALID;
+    if ((d->heads && !rotary_out_ok(d->q_stride, d->q_out_stride, q == q_out, d->tokens,
+                                    d->heads)) ||
+        (d->k_heads && !rotary_out_ok(d->k_stride, d->k_out_stride, k == k_out, d->tokens,
+                                      d->k_heads)))
+        return KATSU_E_INVALID;
+    return qk_norm_rotary(*d, q, k, w_q, w_k, table, positions, q_out, k_out,
+                          (hipStream_t)stream);
+}
+
+int katsu_hip_qk_norm_rotary_bwd_workspace(const katsu_qk_norm_rotary *d, size_t *bytes) {
+    if (!d || !bytes || !qk_norm_rotary_ok(*d)) return KATSU_E_INVALID;
+    *bytes = qk_norm_rotary_bwd_bytes(*d);
+    return KATSU_OK;
+}
+
+int katsu_hip_qk_norm_rotary_bwd_dev(const katsu_qk_norm_rotary *d,
+                                     const katsu_qk_norm_rotary_grads *g, const void *dq,
+                                     const void *dk, const void *q, const void *k,
+                                     const void *w_q, const void *w_k, const float *table,
+                                     const int32_t *positions, void *dx_q, void *dx_k,
+                                     void *dw_q, void *dw_k, void *workspace,
+                                     size_t workspace_bytes, void *stream) {
+    if (!d || !g || !qk_norm_rotary_ok(*d)) return KATSU_E_INVALID;
+    if ((w_q && !dw_q) || (w_k && !dw_k)) return KATSU_E_INVALID;
+    if (d->tokens > 0) {
+        if ((d->rotary_dim > 0 && !table && d->heads + d->k_heads > 0) ||
+            (d->heads && (!q || !dq || !dx_q)) || (d->k_heads && (!k || !dk || !dx_k)))
+            return KATSU_E_INVALID;
+        // Each of the two that an output may be.
+        if (d->heads &&
+            (!rotary_out_ok(d->q_stride, d->q_out_stride, q == dx_q, d->tokens, d->heads) ||
+             !rotary_out_ok(g->dq_stride, d->q_out_stride, dq == dx_q, d->tokens, d->heads)))
+            return KATSU_E_INVALID;
+        if (d->k_heads &&
+            (!rotary_out_ok(d->k_stride, d->k_out_stride, k == dx_k, d->tokens, d->k_heads) ||
+             !rotary_out_ok(g->dk_stride, d->k_out_stride, dk == dx_k, d->tokens, d->k_heads)))
+            return KATSU_E_INVALID;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    void *ws = nullptr;
+    const int rc = lm_scratch(workspace, workspace_bytes, qk_norm_rotary_bwd_bytes(*d), st, &ws);
+    if (rc) return rc;
+    return qk_norm_rotary_bwd(*d, *g, dq, dk, q, k, w_q, w_k, table, positions, dx_q, dx_k, dw_q,
+                              dw_k, ws, st);
+}
+
+int katsu_hip_distillation_workspace(const katsu_distillation *d, size_t *bytes) {
+    if (!d || !bytes || !distillation_ok(*d)) return KATSU_E_INVALID;
+    *bytes = distillation_bytes(*d);
+    return KATSU_OK;
+}
+
+int katsu_hip_distillation_dev(const katsu_distillation *d, const void *logits,
+                               const int32_t *ids, const void *teacher, float *loss, float *stats,
+                               void *workspace, size_t workspace_bytes, void *stream) {
+    if (!d || !distillation_ok(*d)) return KATSU_E_INVALID;
+    if (d->rows == 0) return KATSU_OK;
+    if (!loss || (d->vocab > 0 && !logits) || (d->top > 0 && (!ids || !teacher)))
+        return KATSU_E_INVALID;
+    hipStream_t st = (hipStream_t)stream;
+    void *ws = nullptr;
+    const int rc = lm_scratch(workspace, workspace_bytes, distillation_bytes(*d), st, &ws);
+    if (rc) return rc;
+    return distillation(*d, logits, ids, teacher, loss, stats, ws, st);
+}
+
+// An output of the logits' shape: rows of its own, and where it is the logits, row by row.
+static bool dlogits_ok(const katsu_distillation &d, const void *logits, const void *dlogits) {
+    return embedding_out_ok(d.rows, d.vocab, d.out_stride) &&
+           (logits != dlogits || d.rows < 2 || d.stride == d.out_stride);
+}
+
+int katsu_hip_distillation_bwd_dev(const katsu_distillation *d, const float *dloss,
+                                   const void *logits, const int32_t *ids, const void *teacher,
+                                   const float *stats, void *dlogits, void *stream) {
+    if (!d || !distillation_ok(*d) || !dlogits_ok(*d, logits, dlogits)) return KATSU_E_INVALID;
+    if (d->rows == 0 || d->vocab == 0) return KATSU_OK;
+    if (!logits || !dlogits || !dloss || !stats || (d->top > 0 && (!ids || !teacher)))
+        return KATSU_E_INVALID;
+    return distillation_bwd(*d, dloss, logits, ids, teacher, stats, dlogits,
+                            (hipStream_t)stream);
+}
+
+int katsu_hip_distillation_step_dev(const katsu_distillation *d, const void *logits,
+                                    const int32_t *ids, const void *teacher, const float *dloss,
+                                    float *loss, void *dlogits, void *workspace,
+                                    size_t workspace_bytes, void *stream) {
+    if (!d || !distillation_ok(*d) || !dlogits_ok(*d, logits, dlogits)) return KATSU_E_INVALID;
+    if (d->rows == 0) return KATSU_OK;
+    if (!loss || !dloss || (d->vocab > 0 && (!logits || !dlogits)) ||
+        (d->top > 0 && (!ids || !teacher)))
+        return KATSU_E_INVALID;
+    hipStream_t st = (hipStream_t)stream;
+    void *ws = nullptr;
+    const int rc = lm_scratch(workspace, workspace_bytes, distillation_bytes(*d), st, &ws);
+    if (rc) return rc;
+    return distillation_step(*d, logits, ids, teacher, dloss, loss, dlogits, ws, st);
+}
+
 }  // extern "C"

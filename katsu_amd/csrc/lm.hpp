@@ -1,5 +1,5 @@
 // lm.hpp -- what the C ABI (katsu_hip.hip) calls of the language-model operators,
-// which are compiled apart from it (attention.hip, lmblock.hip).  Each returns a katsu_status;
+// which are compiled apart from it (attention.hip, lmblock.hip, lmends.hip).  Each returns a katsu_status;
 // argument checks are done here too, before any launch.
 #pragma once
 
@@ -28,6 +28,9 @@ int attention_bwd(const katsu_attention &d, const katsu_attention_grads &g, cons
                   const int32_t *cu_q, const int32_t *cu_k, void *dq, void *dk, void *dv, void *ws,
                   hipStream_t st);
 
+// Whether a tensor of these strides can be written, also where it is the input.
+bool rotary_out_ok(const int64_t (&in)[2], const int64_t (&out)[2], bool same, uint64_t tokens,
+                   uint64_t heads);
 bool rotary_ok(const katsu_rotary &d);
 int rotary(const katsu_rotary &d, const void *q, const void *k, const float *table,
            const int32_t *positions, void *q_out, void *k_out, hipStream_t st);
@@ -49,5 +52,37 @@ size_t clip_bytes(size_t n);
 int clip_grad_norm(const int32_t *dtypes, const void *const *in, void *const *out,
                    const size_t *counts, size_t n, float max_norm, float *norm, void *ws,
                    hipStream_t st);
+
+bool embedding_ok(const katsu_embedding &d);
+// Whether rows of these columns can be written with this stride.
+bool embedding_out_ok(uint64_t rows, uint64_t cols, int64_t stride);
+int embedding(const katsu_embedding &d, const int32_t *ids, const void *table, void *out,
+              hipStream_t st);
+size_t embedding_bwd_bytes(const katsu_embedding &d);
+int embedding_bwd(const katsu_embedding &d, const void *dout, const int32_t *ids, void *dtable,
+                  void *ws, hipStream_t st);
+
+bool qk_norm_rotary_ok(const katsu_qk_norm_rotary &d);
+int qk_norm_rotary(const katsu_qk_norm_rotary &d, const void *q, const void *k, const void *w_q,
+                   const void *w_k, const float *table, const int32_t *positions, void *q_out,
+                   void *k_out, hipStream_t st);
+size_t qk_norm_rotary_bwd_bytes(const katsu_qk_norm_rotary &d);
+int qk_norm_rotary_bwd(const katsu_qk_norm_rotary &d, const katsu_qk_norm_rotary_grads &g,
+                       const void *dq, const void *dk, const void *q, const void *k,
+                       const void *w_q, const void *w_k, const float *table,
+                       const int32_t *positions, void *dq_out, void *dk_out, void *dw_q,
+                       void *dw_k, void *ws, hipStream_t st);
+
+bool distillation_ok(const katsu_distillation &d);
+// Scratch bytes of a forward call or a step.
+size_t distillation_bytes(const katsu_distillation &d);
+int distillation(const katsu_distillation &d, const void *logits, const int32_t *ids,
+                 const void *teacher, float *loss, float *stats, void *ws, hipStream_t st);
+int distillation_bwd(const katsu_distillation &d, const float *dloss, const void *logits,
+                     const int32_t *ids, const void *teacher, const float *stats, void *dlogits,
+                     hipStream_t st);
+int distillation_step(const katsu_distillation &d, const void *logits, const int32_t *ids,
+                      const void *teacher, const float *dloss, float *loss, void *dlogits,
+                      void *ws, hipStream_t st);
 
 }  // namespace katsu

@@ -1,0 +1,368 @@
+// lmends.hip -- launches of the kernels at the ends of a language model and before its
+// attention: embedding, the norms of query and key heads with their turn, distillation.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "distill.hpp"
+#include "embedding.hpp"
+#include "headnorm.hpp"
+#include "lm.hpp"
+
+namespace katsu {
+namespace {
+
+constexpr int64_t kI32Max = 0x7fffffff, kStrideMax = (int64_t)1 << 40;
+constexpr int kCUs = 256;
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int status_of(hipError_t e) {
+    if (e == hipSuccess) return KATSU_OK;
+    return e == hipErrorNoDevice || e == hipErrorInvalidDevice ? KATSU_E_NODEVICE : KATSU_E_LAUNCH;
+}
+
+bool dtype_ok(int t) { return t == KATSU_F32 || t == KATSU_BF16; }
+bool stride_ok(int64_t s) { return s >= 0 && s <= kStrideMax; }
+
+// A launch has fewer than 2^32 threads along x: blocks beyond that go along y.
+dim3 grid_of(int64_t blocks, int z = 1) {
+    const int64_t x = std::min<int64_t>(blocks, 1 << 20);
+    return dim3((unsigned)x, (unsigned)cdiv(blocks, x), (unsigned)z);
+}
+
+// ---- embedding ----
+
+EmbedArgs embed_args(const katsu_embedding &d, const int32_t *ids) {
+    EmbedArgs a{};
+    a.ids = ids;
+    a.tokens = (int64_t)d.tokens;
+    a.vocab = (int64_t)d.vocab;
+    a.cols = (int64_t)d.cols;
+    a.scale = d.scale;
+    const int64_t wide = 64 * kEmbedPieces * (d.dtype == KATSU_F32 ? 4 : 8);
+    a.chunks = (int)cdiv(a.cols, wide);
+    return a;
+}
+
+// ---- heads ----
+
+// The widest accesses that half of the turning part and the rest are multiples of, the
+// lanes of a head, and the units of a lane.
+template <typename T, bool INTER, class F>
+int by_head(const HeadArgs &a, F f) {
+    auto with = [&](auto e) {
+        constexpr int E = decltype(e)::value;
+        const int units = a.R / 2 / E + (int)cdiv(a.D - a.R, 2 * E);
+        auto lanes = [&](auto g, auto nu) { return f(e, g, nu, units); };
+        std::integral_constant<int, 1> one;
+        if constexpr (E >= 4) {
+            if (units <= 4) return lanes(std::integral_constant<int, 4>(), one);
+            if (units <= 8) return lanes(std::integral_constant<int, 8>(), one);
+        }
+        if (units <= 16) return lanes(std::integral_constant<int, 16>(), one);
+        if (units <= 32) return lanes(std::integral_constant<int, 32>(), one);
+        if constexpr (E <= 4)
+            if (units <= 64) return lanes(std::integral_constant<int, 64>(), one);
+        if constexpr (E <= 2)
+            if (units <= 128)
+                return lanes(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+        if constexpr (E == 1)
+            if (units <= 256)
+                return lanes(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+        return (int)KATSU_E_INVALID;
+    };
+    auto fits = [&](int e) { return a.R / 2 % e == 0 && (a.D - a.R) % e == 0; };
+    if constexpr (sizeof(T) == 2)
+        if (fits(8)) return with(std::integral_constant<int, 8>());
+    if (fits(4)) return with(std::integral_constant<int, 4>());
+    if (fits(2)) return with(std::integral_constant<int, 2>());
+    return with(std::integral_constant<int, 1>());
+}
+template <class F>
+int by_head_type(const katsu_qk_norm_rotary &d, F f) {
+    auto with = [&](auto t) {
+        return d.interleaved ? f(t, std::true_type()) : f(t, std::false_type());
+    };
+    return d.dtype == KATSU_F32 ? with(float()) : with(__bf16());
+}
+
+HeadArgs head_args(const katsu_qk_norm_rotary &d, const float *table, const int32_t *positions) {
+    HeadArgs a{};
+    for (int i = 0; i < 2; ++i) {
+        HeadTensor &t = a.t[i];
+        const int64_t(&in)[2] = i ? d.k_stride : d.q_stride;
+        const int64_t(&out)[2] = i ? d.k_out_stride : d.q_out_stride;
+        t.x_token = in[0];
+        t.x_head = in[1];
+        t.out_token = out[0];
+        t.out_head = out[1];
+        t.heads = (int)(i ? d.k_heads : d.heads);
+    }
+    a.table = table;
+    a.positions = positions;
+    a.tokens = (int64_t)d.tokens;
+    a.length = (int64_t)d.length;
+    a.D = (int)d.head_dim;
+    a.R = (int)d.rotary_dim;
+    a.eps = d.eps;
+    a.inv_d = 1.f / (float)d.head_dim;
+    return a;
+}
+
+// Blocks of the gradient's launch: of q, of k; each block's sums of dw are a part.
+void head_blocks(const katsu_qk_norm_rotary &d, int (&blocks)[2]) {
+    const int64_t most = 4 * kCUs, n = (int64_t)(d.heads + d.k_heads);
+    const int64_t heads[2] = {(int64_t)d.heads, (int64_t)d.k_heads};
+    for (int i = 0; i < 2; ++i) {
+        const int64_t items = heads[i] * (int64_t)d.tokens;
+        blocks[i] = items == 0 ? 0
+                               : (int)std::min(cdiv(items, 16),
+                                               std::max<int64_t>(1, most * heads[i] / n));
+    }
+}
+
+// ---- distillation ----
+
+struct DistillPlan {
+    int splits;
+    int64_t run;
+};
+// Runs of columns: whole rows where there are enough of them.
+DistillPlan distill_plan(const katsu_distillation &d) {
+    DistillPlan p = {1, (int64_t)d.vocab};
+    const int64_t rows = (int64_t)d.rows, V = (int64_t)d.vocab;
+    const int64_t want = std::min(cdiv(4 * kCUs, std::max<int64_t>(rows, 1)), cdiv(V, 4096));
+    if (rows >= kCUs || want <= 1) return p;
+    p.run = cdiv(cdiv(V, want), 512) * 512;
+    p.splits = (int)cdiv(V, p.run);
+    return p;
+}
+DistillArgs distill_args(const katsu_distillation &d, const void *logits, const int32_t *ids,
+                         const void *teacher) {
+    DistillArgs a{};
+    const DistillPlan p = distill_plan(d);
+    a.z = logits;
+    a.teacher = teacher;
+    a.ids = ids;
+    a.rows = (int64_t)d.rows;
+    a.vocab = (int64_t)d.vocab;
+    a.z_row = d.stride;
+    a.dz_row = d.out_stride;
+    a.dloss_step = d.dloss_stride;
+    a.run = p.run;
+    a.splits = p.splits;
+    a.top = (int)d.top;
+    a.teacher_bf16 = d.teacher_dtype == KATSU_BF16;
+    a.tau = d.temperature;
+    a.scale2 = (float)(1.4426950408889634 / (double)d.temperature);
+    return a;
+}
+template <typename T, bool LOSS, bool GRAD>
+int launch_distill(const DistillArgs &a, int splits, hipStream_t st) {
+    distill_kernel<T, 256, LOSS, GRAD><<<grid_of(a.rows, splits), 256, 0, st>>>(a);
+    return status_of(hipGetLastError());
+}
+// The loss and the statistics of few rows, in two launches.
+template <typename T>
+int launch_parts(const DistillArgs &a, hipStream_t st) {
+    distill_part_kernel<T, 256>
+        <<<dim3((unsigned)a.rows, 1, (unsigned)a.splits), 256, 0, st>>>(a);
+    distill_join_kernel<T, 256><<<dim3((unsigned)a.rows), 256, 0, st>>>(a);
+    return status_of(hipGetLastError());
+}
+
+}  // namespace
+
+bool embedding_ok(const katsu_embedding &d) {
+    return dtype_ok(d.dtype) && (d.accumulate == 0 || d.accumulate == 1) &&
+           d.tokens <= (uint64_t)kI32Max && d.vocab <= (uint64_t)kI32Max && d.cols > 0 &&
+           d.cols <= (uint64_t)kI32Max && stride_ok(d.table_stride) && stride_ok(d.out_stride) &&
+           std::isfinite(d.scale);
+}
+bool embedding_out_ok(uint64_t rows, uint64_t cols, int64_t stride) {
+    return rows < 2 || stride >= (int64_t)cols;
+}
+
+int embedding(const katsu_embedding &d, const int32_t *ids, const void *table, void *out,
+              hipStream_t st) {
+    EmbedArgs a = embed_args(d, ids);
+    a.in = table;
+    a.out = out;
+    a.in_row = d.table_stride;
+    a.out_row = d.out_stride;
+    const unsigned blocks =
+        (unsigned)std::min<int64_t>(cdiv(a.tokens * a.chunks, 4), 1 << 20);
+    if (d.dtype == KATSU_F32)
+        embed_kernel<float><<<blocks, 256, 0, st>>>(a);
+    else
+        embed_kernel<__bf16><<<blocks, 256, 0, st>>>(a);
+    return status_of(hipGetLastError());
+}
+
+size_t embedding_bwd_bytes(const katsu_embedding &) { return 0; }
+
+int embedding_bwd(const katsu_embedding &d, const void *dout, const int32_t *ids, void *dtable,
+                  void *, hipStream_t st) {
+    EmbedArgs a = embed_args(d, ids);
+    a.in = dout;
+    a.out = dtable;
+    a.in_row = d.out_stride;
+    a.out_row = d.table_stride;
+    a.add = d.accumulate;
+    const unsigned blocks = (unsigned)std::min<int64_t>(cdiv(a.vocab, 4), 1 << 20);
+    if (d.dtype == KATSU_F32)
+        embed_grad_few_kernel<float><<<blocks, 256, 0, st>>>(a);
+    else
+        embed_grad_few_kernel<__bf16><<<blocks, 256, 0, st>>>(a);
+    return status_of(hipGetLastError());
+}
+
+bool qk_norm_rotary_ok(const katsu_qk_norm_rotary &d) {
+    if (!dtype_ok(d.dtype) || d.heads > 65535 || d.k_heads > 65535) return false;
+    if (d.head_dim == 0 || d.head_dim > 512 || d.rotary_dim % 2 != 0 ||
+        d.rotary_dim > d.head_dim)
+        return false;
+    if (d.tokens > (uint64_t)kI32Max || d.length > (uint64_t)kI32Max) return false;
+    if (d.rotary_dim > 0 && d.length == 0) return false;
+    for (const auto &s : {d.q_stride, d.k_stride, d.q_out_stride, d.k_out_stride})
+        if (!stride_ok(s[0]) || !stride_ok(s[1])) return false;
+    return d.eps >= 0.f && std::isfinite(d.eps);
+}
+
+int qk_norm_rotary(const katsu_qk_norm_rotary &d, const void *q, const void *k, const void *w_q,
+                   const void *w_k, const float *table, const int32_t *positions, void *q_out,
+                   void *k_out, hipStream_t st) {
+    HeadArgs a = head_args(d, table, positions);
+    a.t[0].x = q;
+    a.t[0].w = w_q;
+    a.t[0].out = q_out;
+    a.t[1].x = k;
+    a.t[1].w = w_k;
+    a.t[1].out = k_out;
+    return by_head_type(d, [&](auto t, auto inter) {
+        using T = decltype(t);
+        constexpr bool INTER = decltype(inter)::value;
+        return by_head<T, INTER>(a, [&](auto e, auto g, auto nu, int units) {
+            constexpr int G = decltype(g)::value;
+            a.units = units;
+            const int64_t items = a.tokens * (a.t[0].heads + a.t[1].heads);
+            head_norm_kernel<T, INTER, decltype(e)::value, G, decltype(nu)::value>
+                <<<grid_of(cdiv(items, 256 / G)), 256, 0, st>>>(a);
+            return status_of(hipGetLastError());
+        });
+    });
+}
+
+size_t qk_norm_rotary_bwd_bytes(const katsu_qk_norm_rotary &d) {
+    int blocks[2];
+    head_blocks(d, blocks);
+    return (size_t)(blocks[0] + blocks[1]) * d.head_dim * sizeof(float);
+}
+
+int qk_norm_rotary_bwd(const katsu_qk_norm_rotary &d, const katsu_qk_norm_rotary_grads &g,
+                       const void *dq, const void *dk, const void *q, const void *k,
+                       const void *w_q, const void *w_k, const float *table,
+                       const int32_t *positions, void *dq_out, void *dk_out, void *dw_q,
+                       void *dw_k, void *ws, hipStream_t st) {
+    HeadArgs a = head_args(d, table, positions);
+    head_blocks(d, a.blocks);
+    a.part = (float *)ws;
+    a.t[0].x = q;
+    a.t[0].w = w_q;
+    a.t[0].dy = dq;
+    a.t[0].out = dq_out;
+    a.t[0].dy_token = g.dq_stride[0];
+    a.t[0].dy_head = g.dq_stride[1];
+    a.t[1].x = k;
+    a.t[1].w = w_k;
+    a.t[1].dy = dk;
+    a.t[1].out = dk_out;
+    a.t[1].dy_token = g.dk_stride[0];
+    a.t[1].dy_head = g.dk_stride[1];
+    const int blocks = a.blocks[0] + a.blocks[1];
+    int rc = KATSU_OK;
+    if (blocks > 0)
+        rc = by_head_type(d, [&](auto t, auto inter) {
+            using T = decltype(t);
+            constexpr bool INTER = decltype(inter)::value;
+            return by_head<T, INTER>(a, [&](auto e, auto g, auto nu, int units) {
+                a.units = units;
+                head_norm_bwd_kernel<T, INTER, decltype(e)::value, decltype(g)::value,
+                                     decltype(nu)::value>
+                    <<<dim3((unsigned)blocks), 256, 0, st>>>(a);
+                return status_of(hipGetLastError());
+            });
+        });
+    if (rc != KATSU_OK || (!w_q && !w_k)) return rc;
+    const dim3 grid((unsigned)cdiv(a.D, 64), 2);
+    if (!w_q) dw_q = nullptr;
+    if (!w_k) dw_k = nullptr;
+    if (d.dtype == KATSU_F32)
+        head_norm_sum_kernel<float><<<grid, 1024, 0, st>>>(a.part, a.blocks[0], a.blocks[1], a.D,
+                                                           (float *)dw_q, (float *)dw_k);
+    else
+        head_norm_sum_kernel<__bf16><<<grid, 1024, 0, st>>>(a.part, a.blocks[0], a.blocks[1],
+                                                            a.D, (__bf16 *)dw_q, (__bf16 *)dw_k);
+    return status_of(hipGetLastError());
+}
+
+bool distillation_ok(const katsu_distillation &d) {
+    return dtype_ok(d.dtype) && dtype_ok(d.teacher_dtype) && d.rows <= (uint64_t)kI32Max &&
+           d.vocab <= (uint64_t)kI32Max && d.top <= kDistillTop && stride_ok(d.stride) &&
+           stride_ok(d.out_stride) && stride_ok(d.dloss_stride) && d.temperature > 0.f &&
+           std::isfinite(d.temperature) && std::isfinite(1.f / d.temperature);
+}
+
+size_t distillation_bytes(const katsu_distillation &d) {
+    const DistillPlan p = distill_plan(d);
+    return p.splits > 1 ? (size_t)d.rows * (2 * p.splits + 2) * sizeof(float) : 0;
+}
+
+int distillation(const katsu_distillation &d, const void *logits, const int32_t *ids,
+                 const void *teacher, float *loss, float *stats, void *ws, hipStream_t st) {
+    DistillArgs a = distill_args(d, logits, ids, teacher);
+    a.loss = loss;
+    a.part = (float *)ws;
+    a.stats = stats;
+    auto run = [&](auto t) {
+        using T = decltype(t);
+        if (a.splits == 1) return launch_distill<T, true, false>(a, 1, st);
+        if (!a.stats) a.stats = a.part + 2 * a.rows * a.splits;
+        return launch_parts<T>(a, st);
+    };
+    return d.dtype == KATSU_F32 ? run(float()) : run(__bf16());
+}
+
+int distillation_bwd(const katsu_distillation &d, const float *dloss, const void *logits,
+                     const int32_t *ids, const void *teacher, const float *stats, void *dlogits,
+                     hipStream_t st) {
+    DistillArgs a = distill_args(d, logits, ids, teacher);
+    a.dloss = dloss;
+    a.stats = const_cast<float *>(stats);
+    a.dz = dlogits;
+    return d.dtype == KATSU_F32 ? launch_distill<float, false, true>(a, a.splits, st)
+                                : launch_distill<__bf16, false, true>(a, a.splits, st);
+}
+
+int distillation_step(const katsu_distillation &d, const void *logits, const int32_t *ids,
+                      const void *teacher, const float *dloss, float *loss, void *dlogits,
+                      void *ws, hipStream_t st) {
+    DistillArgs a = distill_args(d, logits, ids, teacher);
+    a.loss = loss;
+    a.dloss = dloss;
+    a.dz = dlogits;
+    a.part = (float *)ws;
+    auto run = [&](auto t) {
+        using T = decltype(t);
+        if (a.splits == 1) return launch_distill<T, true, true>(a, 1, st);
+        a.stats = a.part + 2 * a.rows * a.splits;
+        const int rc = launch_parts<T>(a, st);
+        return rc != KATSU_OK ? rc : launch_distill<T, false, true>(a, a.splits, st);
+    };
+    return d.dtype == KATSU_F32 ? run(float()) : run(__bf16());
+}
+
+}  // namespace katsu

@@ -44,6 +44,22 @@ __device__ __forceinline__ void store_piece(T *p, int64_t i, int64_t n, const fl
     }
 }
 
+// N neighbouring values, of any alignment.
+template <typename T, int N>
+__device__ __forceinline__ void rotary_load(const T *p, float *x) {
+    T e[N];
+    __builtin_memcpy(e, p, sizeof e);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = (float)e[i];
+}
+template <typename T, int N>
+__device__ __forceinline__ void rotary_store(T *p, const float *x) {
+    T e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = (T)x[i];
+    __builtin_memcpy(p, e, sizeof e);
+}
+
 // The sum over a row's TPR threads (a wave, or a whole block), the same in each: a
 // fixed tree.  Each call of a block uses its own slot of `part`.
 template <int TPR>

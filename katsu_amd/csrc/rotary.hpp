@@ -7,8 +7,7 @@
 // 128, half of each turning, float32: 66 us, 5.1 TB/s; a copy reaches 4.7).
 #pragma once
 
-#include <hip/hip_runtime.h>
-#include <stdint.h>
+#include "lmvec.hpp"
 
 namespace katsu {
 
@@ -26,22 +25,6 @@ struct RotaryArgs {
     int D, R, items, per_head;  // items of a token, of a head
     float inv_per_head, sign;
 };
-
-// N neighbouring values, of any alignment.
-template <typename T, int N>
-__device__ __forceinline__ void rotary_load(const T *p, float *x) {
-    T e[N];
-    __builtin_memcpy(e, p, sizeof e);
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = (float)e[i];
-}
-template <typename T, int N>
-__device__ __forceinline__ void rotary_store(T *p, const float *x) {
-    T e[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) e[i] = (T)x[i];
-    __builtin_memcpy(p, e, sizeof e);
-}
 
 // One block a token (grid-stride), a thread an item: E pairs in the half layout (two pieces
 // of E channels R/2 apart), E/2 pairs (one at least) in the interleaved one, or E channels

@@ -10,8 +10,8 @@ from array import array
 
 import torch
 
-from ._abi import (BF16, F32, Attention, AttentionGrads, BlockNorm, Rotary, check, geometry,
-                   lib)
+from ._abi import (BF16, F32, Attention, AttentionGrads, BlockNorm, Distillation, Embedding,
+                   QkNormRotary, QkNormRotaryGrads, Rotary, check, geometry, lib)
 
 
 # A small call's time is its host side (a pass of four 48 x 56 products and
@@ -498,3 +498,229 @@ def clip_grad_norm(grads, max_norm, out=None, workspace=None):
         counts.buffer_info()[0], n, max_norm, norm.data_ptr(),
         *_workspace(workspace, norm.device), _stream()), "clip_grad_norm")
     return norm
+
+
+# ---- the ends of a language model, and the heads before its attention ----
+
+def _here(t):
+    """The launches go to the current device's current stream: the operands must be there."""
+    if t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError("operands must be on the current device")
+
+
+def _scratch(workspace, dev, size_fn, d):
+    """The caller's workspace, or one of torch's for this call: unlike the library's own buffer it
+    belongs to the stream, or to the graph that is captured."""
+    if workspace is None:
+        nbytes = ctypes.c_size_t(0)
+        check(size_fn(ctypes.byref(d), ctypes.byref(nbytes)), "workspace")
+        if nbytes.value == 0:
+            return None, 0, 0
+        workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
+    return (workspace, *_workspace(workspace, dev))
+
+
+def _rows(t, what):
+    """A [rows, cols] tensor's row stride; its columns must be adjacent."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what} must be [rows, cols] with adjacent columns")
+    return t.stride(0)
+
+
+def _embedding(table, out, ids, scale, beta):
+    _dev_lm(table, out)
+    _here(table)
+    strides = _rows(table, "the table"), _rows(out, "out")
+    if out.shape[1] != table.shape[1] or table.shape[1] == 0:
+        raise ValueError("out must have the table's columns, one at least")
+    if beta not in (0.0, 1.0):
+        raise ValueError("beta must be 0 or 1")
+    _int32(ids, out.shape[0], table.device, "ids")
+    return Embedding(_DTYPE[table.dtype], int(beta), out.shape[0], *table.shape, *strides, scale)
+
+
+def embedding(ids, table, scale=1.0, out=None):
+    """[T, C]: scale times the rows of table [V, C] that ids (int32 [T]) name; zeros where an id is
+    not in [0, V), as for padding.  Rows of table and out may have any stride."""
+    if out is None:
+        out = torch.empty((ids.numel(), table.shape[-1]), dtype=table.dtype, device=table.device)
+    d = _embedding(table, out, ids, scale, 0.0)
+    check(lib().katsu_hip_embedding_dev(ctypes.byref(d), _p(ids), _p(table), _p(out), _stream()),
+          "embedding")
+    return out
+
+
+def embedding_backward(dout, ids, vocab, scale=1.0, out=None, beta=0.0, workspace=None):
+    """The gradient of embedding's table [vocab, C] from dout [T, C]: each row the sum of its
+    tokens' gradients, times scale; tokens with an id that is no row add nothing.  beta=1
+    accumulates into `out` and leaves rows without a token as they are.  The same call gives the
+    same bits.  `workspace`: an optional device tensor of embedding_workspace_bytes()."""
+    if out is None:
+        if beta != 0.0:
+            raise ValueError("beta=1 needs the gradient that it accumulates into")
+        out = torch.empty((vocab, dout.shape[-1]), dtype=dout.dtype, device=dout.device)
+    if out.shape[0] != vocab:
+        raise ValueError("out must have a row for each of the vocabulary")
+    d = _embedding(out, dout, ids, scale, beta)
+    keep, *ws = _scratch(workspace, dout.device, lib().katsu_hip_embedding_bwd_workspace, d)
+    check(lib().katsu_hip_embedding_bwd_dev(ctypes.byref(d), _p(dout), _p(ids), _p(out), *ws,
+                                            _stream()), "embedding_backward")
+    return out
+
+
+def embedding_workspace_bytes(tokens, vocab, cols, dtype):
+    """Scratch that embedding_backward needs."""
+    d = Embedding(_DTYPE[dtype], 0, tokens, vocab, cols, cols, cols, 1.0)
+    nbytes = ctypes.c_size_t(0)
+    check(lib().katsu_hip_embedding_bwd_workspace(ctypes.byref(d), ctypes.byref(nbytes)),
+          "embedding_workspace")
+    return nbytes.value
+
+
+def _qk_norm_rotary(q, k, out_q, out_k, table, positions, w_q, w_k, eps, interleaved):
+    _dev_lm(q, k, out_q, out_k, w_q, w_k)
+    _here(q)
+    strides = [(0, 0) if t is None else _heads(t, w)
+               for t, w in ((q, "q"), (k, "k"), (out_q, "out_q"), (out_k, "out_k"))]
+    tokens, heads, dim = q.shape
+    if out_q.shape != q.shape or (k is None) != (out_k is None) or (k is not None and (
+            out_k.shape != k.shape or k.shape[0] != tokens or k.shape[2] != dim)):
+        raise ValueError("q and k must have the same tokens and channels, outputs their shapes")
+    for w in (w_q, w_k):
+        if w is not None and (w.shape != (dim,) or not w.is_contiguous()):
+            raise ValueError("weights must be contiguous [channels]")
+    if w_k is not None and k is None:
+        raise ValueError("w_k goes with k")
+    if table is not None and (table.dim() != 2 or table.dtype is not torch.float32
+                              or table.device != q.device or not table.is_contiguous()
+                              or table.shape[1] == 0):
+        raise ValueError("table must be contiguous float32 [length, channels that turn]")
+    if table is None and positions is not None:
+        raise ValueError("positions go with a table")
+    _int32(positions, tokens, q.device, "positions")
+    length, rot = (0, 0) if table is None else table.shape
+    return QkNormRotary(_DTYPE[q.dtype], bool(interleaved), tokens, heads,
+                        0 if k is None else k.shape[1], dim, rot, length, *strides, eps)
+
+
+def qk_norm_rotary(q, k, table=None, positions=None, w_q=None, w_k=None, eps=1e-6,
+                   interleaved=False, out_q=None, out_k=None):
+    """(q', k'): each head of q and k [tokens, heads, channels] (k may be None) divided by its
+    channels' root mean square, times w_q or w_k ([channels], None: no weight), then turned as
+    rotary does by rows of `table` (None: not turned), in one pass and rounded once.  At most 512
+    channels, adjacent; any token and head strides.  The outputs may be the inputs."""
+    out_q = torch.empty_like(q) if out_q is None else out_q
+    if k is not None and out_k is None:
+        out_k = torch.empty_like(k)
+    d = _qk_norm_rotary(q, k, out_q, out_k, table, positions, w_q, w_k, eps, interleaved)
+    check(lib().katsu_hip_qk_norm_rotary_dev(ctypes.byref(d), _p(q), _p(k), _p(w_q), _p(w_k),
+                                             _p(table), _p(positions), _p(out_q), _p(out_k),
+                                             _stream()), "qk_norm_rotary")
+    return out_q, out_k
+
+
+def qk_norm_rotary_backward(dq, dk, q, k, table=None, positions=None, w_q=None, w_k=None,
+                            eps=1e-6, interleaved=False, out_q=None, out_k=None, workspace=None):
+    """(dx_q, dx_k, dw_q, dw_k) from dq and dk, the gradients of qk_norm_rotary's outputs, and its
+    operands; None for those that were not given.  out_q and out_k receive dx_q and dx_k and may be
+    dq and dk.  `workspace`: an optional device tensor of qk_norm_rotary_workspace_bytes()."""
+    out_q = torch.empty_like(q) if out_q is None else out_q
+    if k is not None and out_k is None:
+        out_k = torch.empty_like(k)
+    d = _qk_norm_rotary(q, k, out_q, out_k, table, positions, w_q, w_k, eps, interleaved)
+    _dev_lm(q, dq, dk)
+    if dq.shape != q.shape or (dk is None) != (k is None) or (k is not None
+                                                              and dk.shape != k.shape):
+        raise ValueError("gradients must have their operands' shapes")
+    g = QkNormRotaryGrads(_heads(dq, "dq"), (0, 0) if dk is None else _heads(dk, "dk"))
+    dw_q, dw_k = (None if w is None else torch.empty_like(w) for w in (w_q, w_k))
+    keep, *ws = _scratch(workspace, q.device, lib().katsu_hip_qk_norm_rotary_bwd_workspace, d)
+    check(lib().katsu_hip_qk_norm_rotary_bwd_dev(
+        ctypes.byref(d), ctypes.byref(g), _p(dq), _p(dk), _p(q), _p(k), _p(w_q), _p(w_k),
+        _p(table), _p(positions), _p(out_q), _p(out_k), _p(dw_q), _p(dw_k), *ws, _stream()),
+        "qk_norm_rotary_backward")
+    return out_q, out_k, dw_q, dw_k
+
+
+def qk_norm_rotary_workspace_bytes(q, k):
+    """Scratch that qk_norm_rotary_backward needs for operands of these shapes (k may be None)."""
+    d = _qk_norm_rotary(q, k, q, k, None, None, None, None, 0.0, False)
+    nbytes = ctypes.c_size_t(0)
+    check(lib().katsu_hip_qk_norm_rotary_bwd_workspace(ctypes.byref(d), ctypes.byref(nbytes)),
+          "qk_norm_rotary_workspace")
+    return nbytes.value
+
+
+def _distillation(logits, ids, teacher, temperature, out=None, dloss=None):
+    _dev_lm(logits, out)
+    _here(logits)
+    strides = _rows(logits, "logits"), 0 if out is None else _rows(out, "out")
+    rows, vocab = logits.shape
+    if out is not None and out.shape != logits.shape:
+        raise ValueError("out must have the logits' shape")
+    if (ids.dim() != 2 or ids.shape[0] != rows or teacher.shape != ids.shape
+            or ids.dtype is not torch.int32 or teacher.dtype not in _DTYPE
+            or not ids.is_contiguous() or not teacher.is_contiguous()
+            or ids.device != logits.device or teacher.device != logits.device):
+        raise ValueError("ids (int32) and teacher (float32 or bfloat16) must be contiguous "
+                         "[rows, top] on the logits' device")
+    if dloss is not None and (dloss.dtype is not torch.float32 or dloss.device != logits.device
+                              or dloss.shape != (rows,)):
+        raise ValueError("dloss must be float32 [rows] on the logits' device")
+    return Distillation(_DTYPE[logits.dtype], _DTYPE[teacher.dtype], rows, vocab, ids.shape[1],
+                        *strides, 0 if dloss is None else dloss.stride(0), temperature)
+
+
+def distillation(logits, ids, teacher, temperature=1.0, workspace=None):
+    """(loss, stats): for each row of logits [rows, V] temperature^2 times the divergence of
+    softmax(logits / temperature) from the teacher's softmax(teacher / temperature) over its top
+    logits, teacher [rows, K] at the columns ids (int32 [rows, K], K at most 1024); entries with an
+    id that is no column do not count.  loss [rows], float32.  K = 1 and temperature 1: the cross
+    entropy with labels.  A row without an entry has loss 0.  stats [2, rows] float32 is for
+    distillation_backward.  `workspace`: an optional device tensor of
+    distillation_workspace_bytes()."""
+    d = _distillation(logits, ids, teacher, temperature)
+    dev = logits.device
+    loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
+    stats = torch.empty((2, d.rows), dtype=torch.float32, device=dev)
+    keep, *ws = _scratch(workspace, dev, lib().katsu_hip_distillation_workspace, d)
+    check(lib().katsu_hip_distillation_dev(ctypes.byref(d), _p(logits), _p(ids), _p(teacher),
+                                           _p(loss), _p(stats), *ws, _stream()), "distillation")
+    return loss, stats
+
+
+def distillation_backward(dloss, logits, ids, teacher, stats, temperature=1.0, out=None):
+    """The gradient of the logits from dloss (float32 [rows], any stride) and distillation's operands
+    and stats; zeros in rows without an entry.  `out` may be the logits."""
+    out = torch.empty_like(logits) if out is None else out
+    d = _distillation(logits, ids, teacher, temperature, out, dloss)
+    if (stats.dtype is not torch.float32 or stats.device != logits.device
+            or stats.shape != (2, d.rows) or not stats.is_contiguous()):
+        raise ValueError("stats must be what distillation returned")
+    check(lib().katsu_hip_distillation_bwd_dev(ctypes.byref(d), _p(dloss), _p(logits), _p(ids),
+                                               _p(teacher), _p(stats), _p(out), _stream()),
+          "distillation_backward")
+    return out
+
+
+def distillation_step(logits, ids, teacher, dloss, temperature=1.0, out=None, workspace=None):
+    """(loss, gradient of the logits) in one pass over them, where dloss (float32 [rows], any
+    stride: what the sum or the mean of the losses gives each) is known beforehand.  `out`, the
+    gradient, may be the logits."""
+    out = torch.empty_like(logits) if out is None else out
+    d = _distillation(logits, ids, teacher, temperature, out, dloss)
+    loss = torch.empty(d.rows, dtype=torch.float32, device=logits.device)
+    keep, *ws = _scratch(workspace, logits.device, lib().katsu_hip_distillation_workspace, d)
+    check(lib().katsu_hip_distillation_step_dev(ctypes.byref(d), _p(logits), _p(ids), _p(teacher),
+                                                _p(dloss), _p(loss), _p(out), *ws, _stream()),
+          "distillation_step")
+    return loss, out
+
+
+def distillation_workspace_bytes(logits, ids, teacher):
+    """Scratch that distillation or distillation_step needs for operands of these shapes."""
+    d = _distillation(logits, ids, teacher, 1.0)
+    nbytes = ctypes.c_size_t(0)
+    check(lib().katsu_hip_distillation_workspace(ctypes.byref(d), ctypes.byref(nbytes)),
+          "distillation_workspace")
+    return nbytes.value
