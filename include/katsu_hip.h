@@ -417,7 +417,7 @@ int katsu_hip_clip_grad_norm_ws_dev(const int32_t *dtypes, const void *const *in
 
 /* Embedding: out[t] = scale * table[ids[t]], tokens x cols from vocab x cols;
  * zeros where ids[t] (device int32) is not in [0, vocab): padding.  Strides are
- * in elements between rows; columns are adjacent.  `accumulate` is the
+ * in elements between rows; columns (2^20 at most) are adjacent.  `accumulate` is the
  * backward call's. */
 typedef struct katsu_embedding {
     int32_t dtype;       /* katsu_dtype of the table and the output */

@@ -85,4 +85,370 @@ __global__ void __launch_bounds__(256) embed_grad_few_kernel(const EmbedArgs a) 
     }
 }
 
+// ---- the gradient of more tokens: sorted by id, then summed ----------------------
+// Sorting is stable, so that a row's tokens stay in order, and ids that are no row go last
+// as `vocab`.  The sorted tokens are cut into tiles of `tile`, whatever rows they belong to,
+// so that a frequent token is the work of many waves: a run of equal ids inside a tile is a
+// row's sum, what a tile's ends cut off goes to `part` and is joined.
+
+struct EmbedSort {
+    const int32_t *ids;
+    int32_t *key, *at;        // sorted ids, and their tokens
+    const int32_t *key_in, *at_in;  // NULL: ids themselves
+    int32_t *counts;          // [blocks][1 << bits]
+    uint32_t *there;          // a bit for each row of the table
+    int64_t tokens, vocab;
+    int shift, bits, blocks, per;  // per: tokens of a block, a multiple of 1024
+};
+struct EmbedTiles {
+    EmbedArgs a;
+    const int32_t *key, *at;
+    const uint32_t *there;    // NULL: rows without a token are zeros already
+    float *part;              // [tiles][2][cols]: what belongs to the tile before, after
+    int64_t tiles;
+    int tile, chunks;         // chunks: of 64 pieces
+    int64_t tile_blocks;      // blocks beyond these set rows to zero
+};
+
+constexpr int kEmbedSortMax = 16384, kEmbedSortBits = 9, kEmbedBits = 10;
+
+__device__ __forceinline__ int embed_key(const int32_t *ids, int64_t t, int64_t vocab) {
+    const int v = ids[t];
+    return v >= 0 && v < vocab ? v : (int)vocab;
+}
+// Which lanes have the same digit, among those of `live`.
+__device__ __forceinline__ uint64_t same_digit(int d, int bits, uint64_t live) {
+    uint64_t m = live;
+    for (int b = 0; b < bits; ++b) {
+        const bool bit = d >> b & 1;
+        const uint64_t on = __ballot(bit);
+        m &= bit ? on : ~on;
+    }
+    return m;
+}
+// What a wave's lanes have read and written before is before what they do after.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+// This lane's place among its wave's equal digits so far; count[d] is the wave's.
+__device__ __forceinline__ int digit_rank(int *count, int d, int bits, bool live, int lane) {
+    const uint64_t m = same_digit(d, bits, __ballot(live));
+    const int before = __popcll(m & (((uint64_t)1 << lane) - 1));
+    int at = 0;
+    if (live) at = count[d] + before;
+    wave_sync();
+    if (live && before == 0) count[d] += __popcll(m);
+    wave_sync();
+    return at;
+}
+// The exclusive sum over a block of 1024 threads; part: 16 values.
+__device__ __forceinline__ int block_scan(int v, int *part) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int s = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int up = __shfl_up(s, off, 64);
+        if (lane >= off) s += up;
+    }
+    if (lane == 63) part[wave] = s;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < wave; ++w) before += part[w];
+    return before + s - v;
+}
+template <typename T>
+__device__ __forceinline__ void embed_zero_row(const EmbedArgs &a, int64_t v, int lane) {
+    constexpr int E = Piece<T>::E;
+    const float x[E] = {};
+    for (int64_t i = (int64_t)lane * E; i < a.cols; i += 64 * E)
+        store_piece((T *)a.out + v * a.out_row, i, a.cols, x);
+}
+
+// Up to kEmbedSortMax tokens: block 0 sorts them in LDS; the other blocks meanwhile look
+// which of their rows have a token, and set those without to zero.
+template <typename T>
+__global__ void __launch_bounds__(1024) embed_sort_kernel(const EmbedSort s, const EmbedArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = (int)s.tokens;
+    if (blockIdx.x > 0) {
+        uint32_t *there = (uint32_t *)lds;
+        const int64_t per = (s.vocab + gridDim.x - 2) / (gridDim.x - 1);
+        const int64_t end = min(per * blockIdx.x, s.vocab);
+        for (int64_t v0 = per * (blockIdx.x - 1); v0 < end; v0 += 1 << 18) {
+            const int rows = (int)min(end - v0, (int64_t)1 << 18), words = (rows + 31) / 32;
+            for (int i = threadIdx.x; i < words; i += 1024) there[i] = 0;
+            __syncthreads();
+            for (int t = threadIdx.x; t < n; t += 1024) {
+                const int64_t v = s.ids[t] - v0;
+                if (v >= 0 && v < rows) atomicOr(there + (v >> 5), 1u << (v & 31));
+            }
+            __syncthreads();
+            for (int i = wave; i < rows; i += 16)
+                if (!(there[i >> 5] >> (i & 31) & 1)) embed_zero_row<T>(a, v0 + i, lane);
+            __syncthreads();
+        }
+        return;
+    }
+    constexpr int N = kEmbedSortMax / 1024, D = 1 << kEmbedSortBits;
+    int *keys = (int *)lds;
+    uint16_t *ats = (uint16_t *)(keys + kEmbedSortMax);
+    int *count = (int *)(ats + kEmbedSortMax), *part = count + 16 * D;
+    int *mine = count + wave * D;
+    const int per = (n + 1023) / 1024 * 64, t0 = wave * per;  // tokens of a wave
+    int key[N], at[N], rank[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int t = t0 + i * 64 + lane;
+        key[i] = i * 64 < per && t < n ? embed_key(s.ids, t, s.vocab) : 0;
+        at[i] = t;
+    }
+    const int bits = s.bits, mask = (1 << bits) - 1;
+    for (int shift = 0; shift < s.shift; shift += bits) {  // s.shift: all bits
+        for (int i = lane; i <= mask; i += 64) mine[i] = 0;
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i * 64 < per)
+                rank[i] = digit_rank(mine, key[i] >> shift & mask, bits, t0 + i * 64 + lane < n,
+                                     lane);
+        __syncthreads();
+        int total = 0;
+        if ((int)threadIdx.x <= mask)
+            for (int w = 0; w < 16; ++w) {
+                const int c = count[w * D + threadIdx.x];
+                count[w * D + threadIdx.x] = total;
+                total += c;
+            }
+        const int first = block_scan(total, part);
+        if ((int)threadIdx.x <= mask)
+            for (int w = 0; w < 16; ++w) count[w * D + threadIdx.x] += first;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i * 64 < per && t0 + i * 64 + lane < n) {
+                const int to = mine[key[i] >> shift & mask] + rank[i];
+                keys[to] = key[i];
+                ats[to] = (uint16_t)at[i];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i * 64 < per && t0 + i * 64 + lane < n) {
+                key[i] = keys[t0 + i * 64 + lane];
+                at[i] = ats[t0 + i * 64 + lane];
+            }
+        // The next pass's places are written after two more barriers.
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (i * 64 < per && t0 + i * 64 + lane < n) {
+            s.key[t0 + i * 64 + lane] = key[i];
+            s.at[t0 + i * 64 + lane] = at[i];
+        }
+}
+
+// More tokens: a pass for each digit of `bits` from `shift` on, in two launches.  How many of
+// each digit every block has;
+__global__ void __launch_bounds__(1024) embed_count_kernel(const EmbedSort s) {
+    __shared__ int count[1 << kEmbedBits];
+    const int mask = (1 << s.bits) - 1;
+    if (!s.key_in)  // the first launch: no row has a token yet
+        for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < (s.vocab + 31) / 32;
+             i += (int64_t)gridDim.x * 1024)
+            s.there[i] = 0;
+    if ((int)threadIdx.x <= mask) count[threadIdx.x] = 0;
+    __syncthreads();
+    const int64_t t0 = (int64_t)blockIdx.x * s.per, t1 = min(t0 + s.per, s.tokens);
+    for (int64_t t = t0 + threadIdx.x; t < t1; t += 1024) {
+        const int k = s.key_in ? s.key_in[t] : embed_key(s.ids, t, s.vocab);
+        atomicAdd(count + (k >> s.shift & mask), 1);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x <= mask)
+        s.counts[((int64_t)blockIdx.x << s.bits) + threadIdx.x] = count[threadIdx.x];
+}
+// then each block's places, after those of all smaller digits and of the blocks before it.
+__global__ void __launch_bounds__(1024) embed_scatter_kernel(const EmbedSort s) {
+    constexpr int D = 1 << kEmbedBits;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    int *count = (int *)lds, *part = count + 16 * D;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mask = (1 << s.bits) - 1;
+    int *mine = count + wave * D;
+    int total = 0, before = 0;
+    if ((int)threadIdx.x <= mask) {
+#pragma unroll 8
+        for (int b = 0; b < s.blocks; ++b) {
+            const int c = s.counts[((int64_t)b << s.bits) + threadIdx.x];
+            total += c;
+            before += b < (int)blockIdx.x ? c : 0;
+        }
+    }
+    const int first = block_scan(total, part) + before;
+    for (int i = lane; i <= mask; i += 64) mine[i] = 0;
+    wave_sync();
+    // Each wave's tokens follow those of the wave before.
+    const int64_t per = s.per / 16, t0 = (int64_t)blockIdx.x * s.per + wave * per;
+    const int64_t t1 = min(t0 + per, s.tokens);
+    for (int64_t t = t0 + lane; t < t1; t += 64) {
+        const int k = s.key_in ? s.key_in[t] : embed_key(s.ids, t, s.vocab);
+        atomicAdd(mine + (k >> s.shift & mask), 1);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x <= mask) {
+        int at = first;
+        for (int w = 0; w < 16; ++w) {
+            const int c = count[w * D + threadIdx.x];
+            count[w * D + threadIdx.x] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    for (int64_t r = t0; r < t1; r += 64) {
+        const int64_t t = r + lane;
+        const bool live = t < t1;
+        int k = 0, at = 0;
+        if (live) {
+            k = s.key_in ? s.key_in[t] : embed_key(s.ids, t, s.vocab);
+            at = s.at_in ? s.at_in[t] : (int)t;
+        }
+        const int to = digit_rank(mine, k >> s.shift & mask, s.bits, live, lane);
+        if (!live) continue;
+        s.key[to] = k;
+        s.at[to] = at;
+        if (!s.key_in && k < s.vocab) {
+            const uint32_t bit = 1u << (k & 31);
+            if (!(s.there[k >> 5] & bit)) atomicOr(s.there + (k >> 5), bit);
+        }
+    }
+}
+
+// dtable[v] = (dtable[v] +) scale x, of a lane's piece.
+template <typename T>
+__device__ __forceinline__ void embed_write(const EmbedArgs &a, int64_t v, int64_t i, float *x) {
+    constexpr int E = Piece<T>::E;
+    T *out = (T *)a.out + v * a.out_row;
+    float old[E] = {};
+    if (a.add) load_piece(out, i, a.cols, old);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = x[e] * a.scale + old[e];
+    store_piece(out, i, a.cols, x);
+}
+
+// A wave a tile's chunk of 64 pieces, eight tokens' rows in flight.
+template <typename T>
+__global__ void __launch_bounds__(256) embed_tile_kernel(const EmbedTiles t) {
+    constexpr int E = Piece<T>::E, U = 8;
+    const EmbedArgs &a = t.a;
+    const int lane = threadIdx.x & 63;
+    const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (block >= t.tile_blocks) {
+        if (!t.there) return;
+        const int64_t step =
+            ((int64_t)gridDim.y * gridDim.x - t.tile_blocks) * 4;
+        for (int64_t v = (block - t.tile_blocks) * 4 + (threadIdx.x >> 6); v < a.vocab; v += step)
+            if (!(t.there[v >> 5] >> (v & 31) & 1)) embed_zero_row<T>(a, v, lane);
+        return;
+    }
+    const int64_t item = block * 4 + (threadIdx.x >> 6), j = item / t.chunks;
+    if (j >= t.tiles) return;
+    const int64_t i = (item - j * t.chunks) * (64 * E) + lane * E;
+    const int64_t t0 = j * t.tile, t1 = min(t0 + t.tile, a.tokens);
+    int cur = t.key[t0];
+    if (cur >= a.vocab) return;
+    bool before = t0 > 0 && t.key[t0 - 1] == cur;
+    float x[E] = {};
+    auto flush = [&](bool after) {
+        if (i >= a.cols) return;
+        if (!before && !after) {
+            embed_write<T>(a, cur, i, x);
+        } else {
+            float *p = t.part + (2 * j + (before ? 0 : 1)) * a.cols;
+#pragma unroll
+            for (int e = 0; e < E; e += 4) store_piece<float>(p, i + e, a.cols, x + e);
+        }
+    };
+    for (int64_t b = t0; b < t1; b += 64) {
+        const bool in = b + lane < t1;
+        const int key = in ? t.key[b + lane] : (int)a.vocab, at = in ? t.at[b + lane] : 0;
+        const int n = __popcll(__ballot(key < a.vocab));  // the rest is no row's
+        for (int r = 0; r < n; r += U) {
+            float y[U][E];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (r + u < n && i < a.cols)
+                    load_piece((const T *)a.in +
+                                   __builtin_amdgcn_readlane(at, r + u) * a.in_row,
+                               i, a.cols, y[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (r + u >= n) break;
+                const int k = __builtin_amdgcn_readlane(key, r + u);
+                if (k != cur) {
+                    flush(false);
+                    before = false;
+                    cur = k;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[e] = 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] += y[u][e];
+            }
+        }
+        if (n < 64) break;
+    }
+    flush(t1 < a.tokens && t.key[t1] == cur);
+}
+
+// A block a tile and 256 columns: the run that begins in the tile and does not end there, with
+// what the next tiles have of it, each wave every fourth of them.
+template <typename T>
+__global__ void __launch_bounds__(256) embed_join_kernel(const EmbedTiles t) {
+    __shared__ float sums[3][64][4];
+    const EmbedArgs &a = t.a;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t j = blockIdx.x, t0 = j * t.tile, t1 = t0 + t.tile;
+    if (t1 >= a.tokens) return;
+    const int cur = t.key[t1];
+    if (cur >= a.vocab || t.key[t1 - 1] != cur) return;
+    if (t.key[t0] == cur && t0 > 0 && t.key[t0 - 1] == cur) return;  // began before
+    const int64_t i = (int64_t)blockIdx.y * 256 + lane * 4;
+    // The tiles that begin with it.
+    int64_t n = 0;
+    for (;;) {
+        const int64_t b = (j + 1 + n + lane) * t.tile;
+        const uint64_t other = __ballot(!(b < a.tokens && t.key[b] == cur));
+        n += other ? __builtin_ctzll(other) : 64;
+        if (other) break;
+    }
+    float x[4] = {};
+    if (i < a.cols) {
+        if (wave == 0) load_piece<float>(t.part + (2 * j + 1) * a.cols, i, a.cols, x);
+#pragma unroll 4
+        for (int64_t k = wave; k < n; k += 4) {
+            float y[4];
+            load_piece<float>(t.part + 2 * (j + 1 + k) * a.cols, i, a.cols, y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] += y[e];
+        }
+    }
+    if (wave > 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[wave - 1][lane][e] = x[e];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 0; w < 3; ++w)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += sums[w][lane][e];
+    if (i >= a.cols) return;
+    T *out = (T *)a.out + cur * a.out_row;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e < a.cols)
+            out[i + e] = (T)(x[e] * a.scale + (a.add ? (float)out[i + e] : 0.f));
+}
+
 }  // namespace katsu

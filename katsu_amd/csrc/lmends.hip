@@ -27,6 +27,15 @@ int status_of(hipError_t e) {
 bool dtype_ok(int t) { return t == KATSU_F32 || t == KATSU_BF16; }
 bool stride_ok(int64_t s) { return s >= 0 && s <= kStrideMax; }
 
+// Dynamic LDS above 64 KiB must be opted into, once per kernel function.
+template <auto Kern>
+int lds_optin(size_t bytes) {
+    if (bytes <= 65536) return KATSU_OK;
+    static const hipError_t e = hipFuncSetAttribute(
+        (const void *)Kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    return status_of(e);
+}
+
 // A launch has fewer than 2^32 threads along x: blocks beyond that go along y.
 dim3 grid_of(int64_t blocks, int z = 1) {
     const int64_t x = std::min<int64_t>(blocks, 1 << 20);
@@ -34,6 +43,8 @@ dim3 grid_of(int64_t blocks, int z = 1) {
 }
 
 // ---- embedding ----
+
+constexpr uint64_t kEmbedCols = 1 << 20;
 
 EmbedArgs embed_args(const katsu_embedding &d, const int32_t *ids) {
     EmbedArgs a{};
@@ -45,6 +56,104 @@ EmbedArgs embed_args(const katsu_embedding &d, const int32_t *ids) {
     const int64_t wide = 64 * kEmbedPieces * (d.dtype == KATSU_F32 ? 4 : 8);
     a.chunks = (int)cdiv(a.cols, wide);
     return a;
+}
+
+// The gradient's shape.
+enum EmbedPath { kEmbedFew, kEmbedOneBlock, kEmbedPasses };
+struct EmbedPlan {
+    EmbedPath path;
+    int bits, passes, blocks, per, tile;
+    int64_t tiles;
+    size_t keys, counts, there, part, bytes;  // bytes of each, of all
+};
+size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+EmbedPlan embed_plan(const katsu_embedding &d) {
+    EmbedPlan p{};
+    const int64_t T = (int64_t)d.tokens;
+    p.path = T <= 256 ? kEmbedFew : T <= kEmbedSortMax ? kEmbedOneBlock : kEmbedPasses;
+    if (p.path == kEmbedFew) return p;
+    int all = 1;  // bits of the keys 0 .. vocab
+    while (d.vocab >> all) ++all;
+    p.passes = (int)cdiv(all, p.path == kEmbedOneBlock ? kEmbedSortBits : kEmbedBits);
+    p.bits = (int)cdiv(all, p.passes);
+    const int chunks = (int)cdiv((int64_t)d.cols, 64 * (d.dtype == KATSU_F32 ? 4 : 8));
+    p.tile = 32;
+    while (cdiv(T, p.tile) * chunks > 16384 && p.tile < 1024) p.tile *= 2;
+    p.tiles = cdiv(T, p.tile);
+    p.keys = up16((size_t)T * 4);
+    p.part = p.tiles > 1 ? up16((size_t)p.tiles * 2 * d.cols * 4) : 0;
+    p.bytes = 2 * p.keys + p.part;
+    if (p.path == kEmbedPasses) {
+        p.per = (int)(cdiv(T, 256 * 1024) * 1024);
+        p.per = std::max(p.per, 4096);
+        p.blocks = (int)cdiv(T, p.per);
+        p.counts = up16(((size_t)p.blocks << p.bits) * 4);
+        p.there = up16((size_t)cdiv((int64_t)d.vocab, 32) * 4);
+        p.bytes += 2 * p.keys + p.counts + p.there;
+    }
+    return p;
+}
+template <typename T>
+int embed_grad(const katsu_embedding &d, const EmbedArgs &a, char *ws, hipStream_t st) {
+    const EmbedPlan p = embed_plan(d);
+    if (p.path == kEmbedFew) {
+        embed_grad_few_kernel<T><<<(unsigned)std::min<int64_t>(cdiv(a.vocab, 4), 1 << 20), 256, 0,
+                                   st>>>(a);
+        return status_of(hipGetLastError());
+    }
+    auto take = [&](size_t n) {
+        char *at = ws;
+        ws += n;
+        return at;
+    };
+    EmbedTiles t{};
+    t.a = a;
+    t.part = (float *)take(p.part);
+    EmbedSort s{};
+    s.ids = a.ids;
+    s.tokens = a.tokens;
+    s.vocab = a.vocab;
+    s.bits = p.bits;
+    s.key = (int32_t *)take(p.keys);
+    s.at = (int32_t *)take(p.keys);
+    if (p.path == kEmbedOneBlock) {
+        constexpr size_t lds = kEmbedSortMax * 6 + (16 * 4 << kEmbedSortBits) + 64;
+        const int rc = lds_optin<embed_sort_kernel<T>>(lds);
+        if (rc != KATSU_OK) return rc;
+        s.shift = p.bits * p.passes;
+        const int64_t zero = a.add ? 0 : std::min<int64_t>(2 * kCUs - 1, cdiv(a.vocab, 16));
+        embed_sort_kernel<T><<<(unsigned)(1 + zero), 1024, lds, st>>>(s, a);
+    } else {
+        constexpr size_t lds = (16 * 4 << kEmbedBits) + 64;
+        const int rc = lds_optin<embed_scatter_kernel>(lds);
+        if (rc != KATSU_OK) return rc;
+        int32_t *key[2] = {(int32_t *)take(p.keys), s.key}, *at[2] = {(int32_t *)take(p.keys), s.at};
+        s.counts = (int32_t *)take(p.counts);
+        s.there = (uint32_t *)take(p.there);
+        s.blocks = p.blocks;
+        s.per = p.per;
+        for (int i = 0; i < p.passes; ++i) {
+            s.shift = i * p.bits;
+            s.key = key[i & 1];
+            s.at = at[i & 1];
+            embed_count_kernel<<<(unsigned)p.blocks, 1024, 0, st>>>(s);
+            embed_scatter_kernel<<<(unsigned)p.blocks, 1024, lds, st>>>(s);
+            s.key_in = s.key;
+            s.at_in = s.at;
+        }
+        if (!a.add) t.there = s.there;
+    }
+    t.key = s.key;
+    t.at = s.at;
+    t.tile = p.tile;
+    t.tiles = p.tiles;
+    t.chunks = (int)cdiv(a.cols, 64 * Piece<T>::E);
+    t.tile_blocks = cdiv(t.tiles * t.chunks, 4);
+    embed_tile_kernel<T><<<grid_of(t.tile_blocks + (t.there ? 4 * kCUs : 0)), 256, 0, st>>>(t);
+    if (t.tiles > 1)
+        embed_join_kernel<T><<<dim3((unsigned)t.tiles, (unsigned)cdiv(a.cols, 256)), 256, 0,
+                               st>>>(t);
+    return status_of(hipGetLastError());
 }
 
 // ---- heads ----
@@ -179,7 +288,7 @@ int launch_parts(const DistillArgs &a, hipStream_t st) {
 bool embedding_ok(const katsu_embedding &d) {
     return dtype_ok(d.dtype) && (d.accumulate == 0 || d.accumulate == 1) &&
            d.tokens <= (uint64_t)kI32Max && d.vocab <= (uint64_t)kI32Max && d.cols > 0 &&
-           d.cols <= (uint64_t)kI32Max && stride_ok(d.table_stride) && stride_ok(d.out_stride) &&
+           d.cols <= kEmbedCols && stride_ok(d.table_stride) && stride_ok(d.out_stride) &&
            std::isfinite(d.scale);
 }
 bool embedding_out_ok(uint64_t rows, uint64_t cols, int64_t stride) {
@@ -202,22 +311,18 @@ int embedding(const katsu_embedding &d, const int32_t *ids, const void *table, v
     return status_of(hipGetLastError());
 }
 
-size_t embedding_bwd_bytes(const katsu_embedding &) { return 0; }
+size_t embedding_bwd_bytes(const katsu_embedding &d) { return embed_plan(d).bytes; }
 
 int embedding_bwd(const katsu_embedding &d, const void *dout, const int32_t *ids, void *dtable,
-                  void *, hipStream_t st) {
+                  void *ws, hipStream_t st) {
     EmbedArgs a = embed_args(d, ids);
     a.in = dout;
     a.out = dtable;
     a.in_row = d.out_stride;
     a.out_row = d.table_stride;
     a.add = d.accumulate;
-    const unsigned blocks = (unsigned)std::min<int64_t>(cdiv(a.vocab, 4), 1 << 20);
-    if (d.dtype == KATSU_F32)
-        embed_grad_few_kernel<float><<<blocks, 256, 0, st>>>(a);
-    else
-        embed_grad_few_kernel<__bf16><<<blocks, 256, 0, st>>>(a);
-    return status_of(hipGetLastError());
+    return d.dtype == KATSU_F32 ? embed_grad<float>(d, a, (char *)ws, st)
+                                : embed_grad<__bf16>(d, a, (char *)ws, st);
 }
 
 bool qk_norm_rotary_ok(const katsu_qk_norm_rotary &d) {
