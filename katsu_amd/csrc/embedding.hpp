@@ -98,27 +98,39 @@ struct EmbedSort {
     int32_t *counts;          // [blocks][1 << bits]
     uint32_t *there;          // a bit for each row of the table
     int64_t tokens, vocab;
-    int shift, bits, blocks, per;  // per: tokens of a block, a multiple of 1024
+    int shift, bits, blocks;
+    int per;                  // tokens of a block, a multiple of 1024; rows of a slab
 };
 struct EmbedTiles {
     EmbedArgs a;
     const int32_t *key, *at;
-    const uint32_t *there;    // NULL: rows without a token are zeros already
+    const uint32_t *there;    // NULL: rows without a token stay as they are
     float *part;              // [tiles][2][cols]: what belongs to the tile before, after
     int64_t tiles;
     int tile, chunks;         // chunks: of 64 pieces
-    int64_t tile_blocks;      // blocks beyond these set rows to zero
+    int64_t tile_blocks, zero_blocks;  // blocks that add tokens; that set rows to zero
 };
 
-constexpr int kEmbedSortMax = 16384, kEmbedSortBits = 9, kEmbedBits = 10;
+constexpr int kEmbedSlab = 512, kEmbedSlabTokens = 1 << 19, kEmbedBits = 10;
+constexpr int kEmbedAhead = 16;  // rows in flight
 
 __device__ __forceinline__ int embed_key(const int32_t *ids, int64_t t, int64_t vocab) {
     const int v = ids[t];
     return v >= 0 && v < vocab ? v : (int)vocab;
 }
-// Which lanes have the same digit, among those of `live`.
+// Which lanes have the same digit, among those of `live`: few of them one digit after the other,
+// else bit by bit.
 __device__ __forceinline__ uint64_t same_digit(int d, int bits, uint64_t live) {
     uint64_t m = live;
+    if (__popcll(live) <= 8) {
+        for (uint64_t rest = live; rest;) {
+            const int v = __builtin_amdgcn_readlane(d, __builtin_ctzll(rest));
+            const uint64_t same = __ballot(d == v) & live;
+            if (d == v) m = same;
+            rest &= ~same;
+        }
+        return m;
+    }
     for (int b = 0; b < bits; ++b) {
         const bool bit = d >> b & 1;
         const uint64_t on = __ballot(bit);
@@ -166,87 +178,97 @@ __device__ __forceinline__ void embed_zero_row(const EmbedArgs &a, int64_t v, in
         store_piece((T *)a.out + v * a.out_row, i, a.cols, x);
 }
 
-// Up to kEmbedSortMax tokens: block 0 sorts them in LDS; the other blocks meanwhile look
-// which of their rows have a token, and set those without to zero.
-template <typename T>
-__global__ void __launch_bounds__(1024) embed_sort_kernel(const EmbedSort s, const EmbedArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+// A block sorts the tokens of a slab of rows: all blocks look through all ids, count those of
+// smaller rows, which are before the slab's, and each wave's of every row of the slab; then each
+// wave places its tokens, of which it looks only at the batches that had some.
+__global__ void __launch_bounds__(1024) embed_slab_kernel(const EmbedSort s) {
+    __shared__ int count[16][kEmbedSlab], part[16], below[16], end;
+    constexpr int U = 8;  // rounds of 64 tokens in a batch, of which a wave has 64 at most
+    static_assert(kEmbedSlabTokens == 16 * 64 * 64 * U, "a bit a batch");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = (int)s.tokens;
-    if (blockIdx.x > 0) {
-        uint32_t *there = (uint32_t *)lds;
-        const int64_t per = (s.vocab + gridDim.x - 2) / (gridDim.x - 1);
-        const int64_t end = min(per * blockIdx.x, s.vocab);
-        for (int64_t v0 = per * (blockIdx.x - 1); v0 < end; v0 += 1 << 18) {
-            const int rows = (int)min(end - v0, (int64_t)1 << 18), words = (rows + 31) / 32;
-            for (int i = threadIdx.x; i < words; i += 1024) there[i] = 0;
-            __syncthreads();
-            for (int t = threadIdx.x; t < n; t += 1024) {
-                const int64_t v = s.ids[t] - v0;
-                if (v >= 0 && v < rows) atomicOr(there + (v >> 5), 1u << (v & 31));
-            }
-            __syncthreads();
-            for (int i = wave; i < rows; i += 16)
-                if (!(there[i >> 5] >> (i & 31) & 1)) embed_zero_row<T>(a, v0 + i, lane);
-            __syncthreads();
-        }
-        return;
-    }
-    constexpr int N = kEmbedSortMax / 1024, D = 1 << kEmbedSortBits;
-    int *keys = (int *)lds;
-    uint16_t *ats = (uint16_t *)(keys + kEmbedSortMax);
-    int *count = (int *)(ats + kEmbedSortMax), *part = count + 16 * D;
-    int *mine = count + wave * D;
-    const int per = (n + 1023) / 1024 * 64, t0 = wave * per;  // tokens of a wave
-    int key[N], at[N], rank[N];
+    const int per = (n + 1023) / 1024 * 64;  // tokens of a wave
+    const int t0 = min(wave * per, n), t1 = min(t0 + per, n);
+    const int64_t slabs = (s.vocab + s.per - 1) / s.per;
+    int *mine = count[wave];
+    for (int64_t slab = blockIdx.x; slab < slabs; slab += gridDim.x) {
+        const uint32_t v0 = (uint32_t)(slab * s.per);
+        const uint32_t rows = (uint32_t)min((int64_t)s.per, s.vocab - v0);
+        auto batch = [&](int r, uint32_t (&id)[U]) {
+            const int32_t *p = s.ids + r;
+            if (r + 64 * U <= t1) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int t = t0 + i * 64 + lane;
-        key[i] = i * 64 < per && t < n ? embed_key(s.ids, t, s.vocab) : 0;
-        at[i] = t;
-    }
-    const int bits = s.bits, mask = (1 << bits) - 1;
-    for (int shift = 0; shift < s.shift; shift += bits) {  // s.shift: all bits
-        for (int i = lane; i <= mask; i += 64) mine[i] = 0;
+                for (int u = 0; u < U; ++u) id[u] = (uint32_t)p[u * 64 + lane];
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    id[u] = r + u * 64 + lane < t1 ? (uint32_t)p[u * 64 + lane] : 0xffffffffu;
+            }
+        };
+        for (uint32_t i = lane; i < rows; i += 64) mine[i] = 0;
         wave_sync();
+        int less = 0;
+        uint64_t some = 0;
+        for (int r = t0, b = 0; r < t1; r += 64 * U, ++b) {
+            uint32_t id[U];
+            batch(r, id);
+            bool any = false;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i * 64 < per)
-                rank[i] = digit_rank(mine, key[i] >> shift & mask, bits, t0 + i * 64 + lane < n,
-                                     lane);
-        __syncthreads();
-        int total = 0;
-        if ((int)threadIdx.x <= mask)
-            for (int w = 0; w < 16; ++w) {
-                const int c = count[w * D + threadIdx.x];
-                count[w * D + threadIdx.x] = total;
-                total += c;
+            for (int u = 0; u < U; ++u) {
+                less += id[u] < v0;
+                any |= id[u] - v0 < rows;
             }
-        const int first = block_scan(total, part);
-        if ((int)threadIdx.x <= mask)
-            for (int w = 0; w < 16; ++w) count[w * D + threadIdx.x] += first;
-        __syncthreads();
+            if (!__ballot(any)) continue;
+            some |= (uint64_t)1 << b;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i * 64 < per && t0 + i * 64 + lane < n) {
-                const int to = mine[key[i] >> shift & mask] + rank[i];
-                keys[to] = key[i];
-                ats[to] = (uint16_t)at[i];
-            }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i * 64 < per && t0 + i * 64 + lane < n) {
-                key[i] = keys[t0 + i * 64 + lane];
-                at[i] = ats[t0 + i * 64 + lane];
-            }
-        // The next pass's places are written after two more barriers.
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (i * 64 < per && t0 + i * 64 + lane < n) {
-            s.key[t0 + i * 64 + lane] = key[i];
-            s.at[t0 + i * 64 + lane] = at[i];
+            for (int u = 0; u < U; ++u)
+                if (id[u] - v0 < rows) atomicAdd(mine + (id[u] - v0), 1);
         }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) less += __shfl_xor(less, off, 64);
+        if (lane == 0) below[wave] = less;
+        __syncthreads();
+        int sum = 0;
+        if (threadIdx.x < rows) {
+#pragma unroll
+            for (int w = 0; w < 16; ++w) sum += count[w][threadIdx.x];
+        }
+        // The slab's rows are whole words of bits.
+        const uint64_t there = __ballot(sum > 0);
+        if ((lane & 31) == 0 && threadIdx.x < rows)
+            s.there[(v0 + threadIdx.x) >> 5] = (uint32_t)(there >> lane);
+        int first = block_scan(sum, part);
+#pragma unroll
+        for (int w = 0; w < 16; ++w) first += below[w];
+        if (threadIdx.x < rows) {
+            int at = first;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) {
+                const int c = count[w][threadIdx.x];
+                count[w][threadIdx.x] = at;
+                at += c;
+            }
+            if (threadIdx.x + 1 == rows) end = at;
+        }
+        __syncthreads();
+        for (; some; some &= some - 1) {
+            const int r = t0 + __builtin_ctzll(some) * (64 * U);
+            uint32_t id[U];
+            batch(r, id);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool has = id[u] - v0 < rows;
+                if (!__ballot(has)) continue;
+                const int to = digit_rank(mine, has ? (int)(id[u] - v0) : 0, s.bits, has, lane);
+                if (has) {
+                    s.key[to] = (int)id[u];
+                    s.at[to] = r + u * 64 + lane;
+                }
+            }
+        }
+        if (slab + 1 == slabs)  // behind the last row's tokens
+            for (int t = end + (int)threadIdx.x; t < n; t += 1024) s.key[t] = (int)s.vocab;
+        __syncthreads();
+    }
 }
 
 // More tokens: a pass for each digit of `bits` from `shift` on, in two launches.  How many of
@@ -336,19 +358,25 @@ __device__ __forceinline__ void embed_write(const EmbedArgs &a, int64_t v, int64
     store_piece(out, i, a.cols, x);
 }
 
-// A wave a tile's chunk of 64 pieces, eight tokens' rows in flight.
+// A wave a tile's chunk of 64 pieces, kEmbedAhead tokens' rows in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) embed_tile_kernel(const EmbedTiles t) {
-    constexpr int E = Piece<T>::E, U = 8;
+    constexpr int E = Piece<T>::E, U = kEmbedAhead;
     const EmbedArgs &a = t.a;
     const int lane = threadIdx.x & 63;
-    const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    const int64_t id = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    // One of each kind by turns, so that zeros are written while rows are awaited.
+    const int64_t both = min(t.tile_blocks, t.zero_blocks);
+    if (id >= t.tile_blocks + t.zero_blocks) return;
+    const int64_t block = id < 2 * both ? (id & 1 ? t.tile_blocks : 0) + id / 2
+                          : id - both + (t.zero_blocks > both ? t.tile_blocks : 0);
     if (block >= t.tile_blocks) {
-        if (!t.there) return;
-        const int64_t step =
-            ((int64_t)gridDim.y * gridDim.x - t.tile_blocks) * 4;
-        for (int64_t v = (block - t.tile_blocks) * 4 + (threadIdx.x >> 6); v < a.vocab; v += step)
-            if (!(t.there[v >> 5] >> (v & 31) & 1)) embed_zero_row<T>(a, v, lane);
+        const int64_t v = (block - t.tile_blocks) * 32 + (threadIdx.x >> 6) * 8;
+        if (!t.there || v >= a.vocab) return;
+        // Eight rows a wave; their bits are read before the first store.
+        const uint32_t bits = __builtin_amdgcn_readfirstlane(t.there[v >> 5] >> (v & 31));
+        for (int i = 0; i < 8; ++i)
+            if (!(bits >> i & 1) && v + i < a.vocab) embed_zero_row<T>(a, v + i, lane);
         return;
     }
     const int64_t item = block * 4 + (threadIdx.x >> 6), j = item / t.chunks;
@@ -374,13 +402,12 @@ __global__ void __launch_bounds__(256) embed_tile_kernel(const EmbedTiles t) {
         const int key = in ? t.key[b + lane] : (int)a.vocab, at = in ? t.at[b + lane] : 0;
         const int n = __popcll(__ballot(key < a.vocab));  // the rest is no row's
         for (int r = 0; r < n; r += U) {
-            float y[U][E];
+            RawPiece<T> y[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (r + u < n && i < a.cols)
-                    load_piece((const T *)a.in +
-                                   __builtin_amdgcn_readlane(at, r + u) * a.in_row,
-                               i, a.cols, y[u]);
+                    y[u].load((const T *)a.in + __builtin_amdgcn_readlane(at, r + u) * a.in_row,
+                              i, a.cols);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (r + u >= n) break;
@@ -393,7 +420,7 @@ __global__ void __launch_bounds__(256) embed_tile_kernel(const EmbedTiles t) {
                     for (int e = 0; e < E; ++e) x[e] = 0.f;
                 }
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] += y[u][e];
+                for (int e = 0; e < E; ++e) x[e] += y[u].at(e);
             }
         }
         if (n < 64) break;

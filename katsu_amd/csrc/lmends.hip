@@ -59,7 +59,7 @@ EmbedArgs embed_args(const katsu_embedding &d, const int32_t *ids) {
 }
 
 // The gradient's shape.
-enum EmbedPath { kEmbedFew, kEmbedOneBlock, kEmbedPasses };
+enum EmbedPath { kEmbedFew, kEmbedSlabs, kEmbedPasses };
 struct EmbedPlan {
     EmbedPath path;
     int bits, passes, blocks, per, tile;
@@ -70,26 +70,38 @@ size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 EmbedPlan embed_plan(const katsu_embedding &d) {
     EmbedPlan p{};
     const int64_t T = (int64_t)d.tokens;
-    p.path = T <= 256 ? kEmbedFew : T <= kEmbedSortMax ? kEmbedOneBlock : kEmbedPasses;
+    const int64_t V = (int64_t)d.vocab;
+    auto bits = [](int64_t n) {  // of numbers up to n
+        int b = 1;
+        while (n >> b) ++b;
+        return b;
+    };
+    // Slabs: two a CU.  Their blocks read all ids twice, so with more tokens the passes.
+    p.per = (int)std::min<int64_t>(cdiv(V, kCUs * 32) * 32, kEmbedSlab);
+    const int64_t slabs = cdiv(V, p.per);
+    p.path = T <= 256 ? kEmbedFew : T <= kEmbedSlabTokens && slabs * T <= 1 << 25 ? kEmbedSlabs : kEmbedPasses;
     if (p.path == kEmbedFew) return p;
-    int all = 1;  // bits of the keys 0 .. vocab
-    while (d.vocab >> all) ++all;
-    p.passes = (int)cdiv(all, p.path == kEmbedOneBlock ? kEmbedSortBits : kEmbedBits);
-    p.bits = (int)cdiv(all, p.passes);
+    if (p.path == kEmbedSlabs) {
+        p.blocks = (int)slabs;
+        p.bits = bits(p.per - 1);
+    } else {
+        p.passes = (int)cdiv(bits(V), kEmbedBits);
+        p.bits = (int)cdiv(bits(V), p.passes);
+    }
     const int chunks = (int)cdiv((int64_t)d.cols, 64 * (d.dtype == KATSU_F32 ? 4 : 8));
-    p.tile = 32;
-    while (cdiv(T, p.tile) * chunks > 16384 && p.tile < 1024) p.tile *= 2;
+    p.tile = 8;
+    while (cdiv(T, p.tile) * chunks > 1024 && p.tile < 1024) p.tile *= 2;
     p.tiles = cdiv(T, p.tile);
     p.keys = up16((size_t)T * 4);
     p.part = p.tiles > 1 ? up16((size_t)p.tiles * 2 * d.cols * 4) : 0;
-    p.bytes = 2 * p.keys + p.part;
+    p.there = up16((size_t)cdiv(V, 32) * 4);
+    p.bytes = 2 * p.keys + p.part + p.there;
     if (p.path == kEmbedPasses) {
         p.per = (int)(cdiv(T, 256 * 1024) * 1024);
         p.per = std::max(p.per, 4096);
         p.blocks = (int)cdiv(T, p.per);
         p.counts = up16(((size_t)p.blocks << p.bits) * 4);
-        p.there = up16((size_t)cdiv((int64_t)d.vocab, 32) * 4);
-        p.bytes += 2 * p.keys + p.counts + p.there;
+        p.bytes += 2 * p.keys + p.counts;
     }
     return p;
 }
@@ -116,20 +128,16 @@ int embed_grad(const katsu_embedding &d, const EmbedArgs &a, char *ws, hipStream
     s.bits = p.bits;
     s.key = (int32_t *)take(p.keys);
     s.at = (int32_t *)take(p.keys);
-    if (p.path == kEmbedOneBlock) {
-        constexpr size_t lds = kEmbedSortMax * 6 + (16 * 4 << kEmbedSortBits) + 64;
-        const int rc = lds_optin<embed_sort_kernel<T>>(lds);
-        if (rc != KATSU_OK) return rc;
-        s.shift = p.bits * p.passes;
-        const int64_t zero = a.add ? 0 : std::min<int64_t>(2 * kCUs - 1, cdiv(a.vocab, 16));
-        embed_sort_kernel<T><<<(unsigned)(1 + zero), 1024, lds, st>>>(s, a);
+    s.there = (uint32_t *)take(p.there);
+    if (p.path == kEmbedSlabs) {
+        s.per = p.per;
+        embed_slab_kernel<<<(unsigned)p.blocks, 1024, 0, st>>>(s);
     } else {
         constexpr size_t lds = (16 * 4 << kEmbedBits) + 64;
         const int rc = lds_optin<embed_scatter_kernel>(lds);
         if (rc != KATSU_OK) return rc;
         int32_t *key[2] = {(int32_t *)take(p.keys), s.key}, *at[2] = {(int32_t *)take(p.keys), s.at};
         s.counts = (int32_t *)take(p.counts);
-        s.there = (uint32_t *)take(p.there);
         s.blocks = p.blocks;
         s.per = p.per;
         for (int i = 0; i < p.passes; ++i) {
@@ -141,15 +149,16 @@ int embed_grad(const katsu_embedding &d, const EmbedArgs &a, char *ws, hipStream
             s.key_in = s.key;
             s.at_in = s.at;
         }
-        if (!a.add) t.there = s.there;
     }
+    if (!a.add) t.there = s.there;
     t.key = s.key;
     t.at = s.at;
     t.tile = p.tile;
     t.tiles = p.tiles;
     t.chunks = (int)cdiv(a.cols, 64 * Piece<T>::E);
     t.tile_blocks = cdiv(t.tiles * t.chunks, 4);
-    embed_tile_kernel<T><<<grid_of(t.tile_blocks + (t.there ? 4 * kCUs : 0)), 256, 0, st>>>(t);
+    t.zero_blocks = t.there ? cdiv(a.vocab, 32) : 0;
+    embed_tile_kernel<T><<<grid_of(t.tile_blocks + t.zero_blocks), 256, 0, st>>>(t);
     if (t.tiles > 1)
         embed_join_kernel<T><<<dim3((unsigned)t.tiles, (unsigned)cdiv(a.cols, 256)), 256, 0,
                                st>>>(t);

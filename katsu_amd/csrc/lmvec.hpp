@@ -29,6 +29,26 @@ __device__ __forceinline__ void load_piece(const T *p, int64_t i, int64_t n, flo
 #pragma unroll
     for (int j = 0; j < E; ++j) x[j] = (float)e[j];
 }
+// The same in four registers, for pieces that wait: an array of bfloat16 takes one for each value.
+template <typename T>
+struct RawPiece {
+    static constexpr int E = Piece<T>::E;
+    lm_u4 v;
+    __device__ __forceinline__ void load(const T *p, int64_t i, int64_t n) {
+        if (i + E <= n) {
+            __builtin_memcpy(&v, p + i, 16);
+        } else {
+            T e[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) e[j] = i + j < n ? p[i + j] : (T)0.f;
+            __builtin_memcpy(&v, e, 16);
+        }
+    }
+    __device__ __forceinline__ float at(int j) const {
+        const uint32_t u = v[j * (int)sizeof(T) / 4];
+        return __builtin_bit_cast(float, sizeof(T) == 4 ? u : j & 1 ? u & 0xffff0000u : u << 16);
+    }
+};
 template <typename T>
 __device__ __forceinline__ void store_piece(T *p, int64_t i, int64_t n, const float *x) {
     constexpr int E = Piece<T>::E;
