@@ -437,9 +437,10 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedTiles t) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t j = blockIdx.x, t0 = j * t.tile, t1 = t0 + t.tile;
     if (t1 >= a.tokens) return;
-    const int cur = t.key[t1];
-    if (cur >= a.vocab || t.key[t1 - 1] != cur) return;
-    if (t.key[t0] == cur && t0 > 0 && t.key[t0 - 1] == cur) return;  // began before
+    // Read together; most blocks end here.
+    const int cur = t.key[t1], last = t.key[t1 - 1], head = t.key[t0], before = t.key[max(t0, (int64_t)1) - 1];
+    if (cur >= a.vocab || last != cur) return;
+    if (head == cur && t0 > 0 && before == cur) return;  // began before the tile
     const int64_t i = (int64_t)blockIdx.y * 256 + lane * 4;
     // The tiles that begin with it.
     int64_t n = 0;
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedTiles t) {
     float x[4] = {};
     if (i < a.cols) {
         if (wave == 0) load_piece<float>(t.part + (2 * j + 1) * a.cols, i, a.cols, x);
-#pragma unroll 4
+#pragma unroll 8
         for (int64_t k = wave; k < n; k += 4) {
             float y[4];
             load_piece<float>(t.part + 2 * (j + 1 + k) * a.cols, i, a.cols, y);

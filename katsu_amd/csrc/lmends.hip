@@ -90,7 +90,7 @@ EmbedPlan embed_plan(const katsu_embedding &d) {
     }
     const int chunks = (int)cdiv((int64_t)d.cols, 64 * (d.dtype == KATSU_F32 ? 4 : 8));
     p.tile = 8;
-    while (cdiv(T, p.tile) * chunks > 1024 && p.tile < 1024) p.tile *= 2;
+    while (cdiv(T, p.tile) * chunks > 2048 && p.tile < 1024) p.tile *= 2;
     p.tiles = cdiv(T, p.tile);
     p.keys = up16((size_t)T * 4);
     p.part = p.tiles > 1 ? up16((size_t)p.tiles * 2 * d.cols * 4) : 0;
