@@ -13,6 +13,8 @@
 // HBM-bound: one pass with each thread's running maximum and sum.
 #pragma once
 
+#include <type_traits>
+
 #include "lmvec.hpp"
 
 namespace katsu {
@@ -30,7 +32,13 @@ struct DistillArgs {
     float tau, scale2;  // scale2: log2(e) / tau
 };
 
-constexpr int kDistillTop = 1024;
+constexpr int kDistillTop = 1024, kDistillBits = 1 << 16;
+
+struct DistillIds {
+    int id[kDistillTop];
+    float p[kDistillTop];
+    uint32_t bits[kDistillBits / 32];
+};
 
 __device__ __forceinline__ float distill_exp(float x, float by) {  // exp((x)/tau)
     return __builtin_amdgcn_exp2f(x * by);
@@ -167,38 +175,71 @@ __device__ __forceinline__ void distill_loss(const DistillArgs &a, int64_t row,
     if (threadIdx.x == 0) a.loss[row] = a.tau * a.tau * v;
 }
 
+// The teacher's columns among [c0, c1): an entry's value, of which the first of equal ids takes the
+// sum, and whether the thread writes it.  A set of bits tells whether any id occurs twice (ids that
+// share the last 16 bits count as well): only then they are compared with each other.
+template <int NT>
+struct DistillFix {
+    static constexpr int N = DistillRow<NT>::N;
+    float v[N];
+    bool own[N];
+
+    template <typename T>
+    __device__ __forceinline__ void find(const DistillArgs &a, const T *z, int64_t c0, int64_t c1,
+                                         const DistillRow<NT> &d, float m, float inv, float g,
+                                         DistillIds &s) {
+        for (int i = threadIdx.x; i < kDistillBits / 32; i += NT) s.bits[i] = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s.id[threadIdx.x + NT * i] = d.id[i];
+            s.p[threadIdx.x + NT * i] = d.p[i];
+        }
+        __syncthreads();
+        bool twice = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            own[i] = d.id[i] >= c0 && d.id[i] < c1;
+            if (!own[i]) continue;
+            const uint32_t bit = 1u << (d.id[i] & 31);
+            twice |= atomicOr(s.bits + (d.id[i] % kDistillBits >> 5), bit) & bit;
+        }
+        twice = __syncthreads_or(twice);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (!own[i]) continue;
+            const int k = threadIdx.x + NT * i;
+            float p = d.p[i];
+            if (twice) {
+                p = 0.f;
+                for (int j = 0; j < a.top; ++j) {
+                    if (s.id[j] != d.id[i]) continue;
+                    p += s.p[j];
+                    if (j < k) own[i] = false;
+                }
+            }
+            if (own[i]) v[i] = (distill_exp((float)z[d.id[i]] - m, a.scale2) * inv - p) * g;
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void write(const DistillRow<NT> &d, T *dz) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (own[i]) dz[d.id[i]] = (T)v[i];
+    }
+};
+
 // The gradient of columns [c0, c1): all of them as if there were no teacher, then the
-// teacher's, of which the first of equal ids takes their sum.
+// teacher's.
 template <typename T, int NT>
 __device__ __forceinline__ void distill_grad(const DistillArgs &a, int64_t row, int64_t c0,
                                              int64_t c1, const DistillRow<NT> &d, float m,
-                                             float inv, int *ids, float *ps) {
-    constexpr int E = Piece<T>::E, N = DistillRow<NT>::N;
+                                             float inv, DistillIds &s) {
+    constexpr int E = Piece<T>::E;
     const T *z = (const T *)a.z + row * a.z_row;
     T *dz = (T *)a.dz + row * a.dz_row;
     const float g = a.dloss[row * a.dloss_step] * a.tau, by = inv * g;
-    float fix[N];
-    bool own[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int k = threadIdx.x + NT * i;
-        ids[k] = d.id[i];
-        ps[k] = d.p[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int k = threadIdx.x + NT * i;
-        own[i] = d.id[i] >= c0 && d.id[i] < c1;
-        if (!own[i]) continue;
-        float p = 0.f;
-        for (int j = 0; j < a.top; ++j) {
-            if (ids[j] != d.id[i]) continue;
-            p += ps[j];
-            if (j < k) own[i] = false;
-        }
-        if (own[i]) fix[i] = (distill_exp((float)z[d.id[i]] - m, a.scale2) * inv - p) * g;
-    }
+    DistillFix<NT> fix;
+    fix.find(a, z, c0, c1, d, m, inv, g, s);
     __syncthreads();  // dz may be z: all of the teacher's logits are read
     for (int64_t i = c0 + threadIdx.x * E; i < c1; i += NT * E) {
         float x[E];
@@ -208,9 +249,7 @@ __device__ __forceinline__ void distill_grad(const DistillArgs &a, int64_t row, 
         store_piece(dz, i, c1, x);
     }
     __syncthreads();  // and all others written
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (own[i]) dz[d.id[i]] = (T)fix[i];
+    fix.write(d, dz);
 }
 
 template <typename T, int NT>
@@ -226,8 +265,7 @@ __device__ __forceinline__ void distill_zero(const DistillArgs &a, int64_t row, 
 template <typename T, int NT, bool LOSS, bool GRAD>
 __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
     __shared__ float part[5][2 * NT / 64];
-    __shared__ int ids[GRAD ? kDistillTop : 1];
-    __shared__ float ps[GRAD ? kDistillTop : 1];
+    __shared__ std::conditional_t<GRAD, DistillIds, int> ids;
     const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     if (row >= a.rows) return;
     const int64_t c0 = LOSS ? 0 : blockIdx.z * a.run;
@@ -258,7 +296,72 @@ __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
         m = a.stats[row];
         inv = a.stats[a.rows + row];
     }
-    if constexpr (GRAD) distill_grad<T, NT>(a, row, c0, c1, d, m, inv, ids, ps);
+    if constexpr (GRAD) distill_grad<T, NT>(a, row, c0, c1, d, m, inv, ids);
+}
+
+// Loss and gradient of rows of up to NT * NP pieces, which stay in the block's registers between
+// the two: the logits are read once.
+template <typename T, int NT, int NP>
+__global__ void __launch_bounds__(NT) distill_step_kernel(const DistillArgs a) {
+    constexpr int E = Piece<T>::E;
+    __shared__ float part[5][NT / 64];
+    __shared__ DistillIds ids;
+    const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (row >= a.rows) return;
+    const T *z = (const T *)a.z + row * a.z_row;
+    T *dz = (T *)a.dz + row * a.dz_row;
+    const int V = (int)a.vocab;
+    DistillRow<NT> d;
+    d.load(a, row);
+    if (!d.some) {
+        if (threadIdx.x == 0) a.loss[row] = 0.f;
+        distill_zero<T, NT>(a, row, 0, V);
+        return;
+    }
+    RawPiece<T> x[NP];
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+        const T *at = z + k * NT * E;
+        if ((k + 1) * NT * E <= V)  // the whole block's pieces
+            __builtin_memcpy(&x[k].v, at + threadIdx.x * E, 16);
+        else
+            x[k].load(at, threadIdx.x * E, V - k * NT * E, -INFINITY);
+    }
+    d.softmax(a, part[0], part[1]);
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) m = fmaxf(m, x[k].at(e));
+    m = block_join<NT>(m, part[2], JoinMax());
+    float l = 0.f;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) x[k].packed();
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) l += distill_exp(x[k].at(e) - m, a.scale2);
+    DistillSum s;
+    s.m = m;
+    s.l = block_join<NT>(l, part[3], JoinSum());
+    distill_loss<T, NT>(a, row, d, s, part[4]);
+    const float inv = 1.f / s.l, g = a.dloss[row * a.dloss_step] * a.tau, by = inv * g;
+    DistillFix<NT> fix;
+    fix.find(a, z, 0, V, d, m, inv, g, ids);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) x[k].packed();
+    __syncthreads();  // dz may be z: all of the teacher's logits are read
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+        const int i = (k * NT + (int)threadIdx.x) * E;
+        if (i >= V) break;
+        float y[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = distill_exp(x[k].at(e) - m, a.scale2) * by;
+        store_piece(dz, i, V, y);
+    }
+    __syncthreads();  // and all others written
+    fix.write(d, dz);
 }
 
 // Few rows: M and L of runs of a row's columns, then the loss from them.

@@ -283,6 +283,21 @@ int launch_distill(const DistillArgs &a, int splits, hipStream_t st) {
     distill_kernel<T, 256, LOSS, GRAD><<<grid_of(a.rows, splits), 256, 0, st>>>(a);
     return status_of(hipGetLastError());
 }
+// Loss and gradient with the rows in registers: threads of a row, and its pieces a thread.
+template <typename T, class F>
+bool by_row_pieces(const DistillArgs &a, F f) {
+    const int64_t pieces = cdiv(a.vocab, Piece<T>::E);
+    std::integral_constant<int, 256> few;
+    if (pieces <= 256) return f(few, std::integral_constant<int, 1>());
+    if (pieces <= 1024) return f(few, std::integral_constant<int, 4>());
+    if (pieces <= 2048) return f(few, std::integral_constant<int, 8>());
+    if (pieces <= 4096) return f(few, std::integral_constant<int, 16>());
+    if (pieces <= 8192)
+        return f(std::integral_constant<int, 512>(), std::integral_constant<int, 16>());
+    if (pieces <= 16384)
+        return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 16>());
+    return false;
+}
 // The loss and the statistics of few rows, in two launches.
 template <typename T>
 int launch_parts(const DistillArgs &a, hipStream_t st) {
@@ -471,6 +486,12 @@ int distillation_step(const katsu_distillation &d, const void *logits, const int
     a.part = (float *)ws;
     auto run = [&](auto t) {
         using T = decltype(t);
+        if (by_row_pieces<T>(a, [&](auto nt, auto np) {
+                constexpr int NT = decltype(nt)::value, NP = decltype(np)::value;
+                distill_step_kernel<T, NT, NP><<<grid_of(a.rows), NT, 0, st>>>(a);
+                return true;
+            }))
+            return status_of(hipGetLastError());
         if (a.splits == 1) return launch_distill<T, true, true>(a, 1, st);
         a.stats = a.part + 2 * a.rows * a.splits;
         const int rc = launch_parts<T>(a, st);

@@ -34,16 +34,19 @@ template <typename T>
 struct RawPiece {
     static constexpr int E = Piece<T>::E;
     lm_u4 v;
-    __device__ __forceinline__ void load(const T *p, int64_t i, int64_t n) {
+    // Those past the row's end are `none`.
+    __device__ __forceinline__ void load(const T *p, int64_t i, int64_t n, float none = 0.f) {
         if (i + E <= n) {
             __builtin_memcpy(&v, p + i, 16);
         } else {
             T e[E];
 #pragma unroll
-            for (int j = 0; j < E; ++j) e[j] = i + j < n ? p[i + j] : (T)0.f;
+            for (int j = 0; j < E; ++j) e[j] = i + j < n ? p[i + j] : (T)none;
             __builtin_memcpy(&v, e, 16);
         }
     }
+    // Its values are converted again after this: held as float32 they take twice the registers.
+    __device__ __forceinline__ void packed() { asm volatile("" : "+v"(v)); }
     __device__ __forceinline__ float at(int j) const {
         const uint32_t u = v[j * (int)sizeof(T) / 4];
         return __builtin_bit_cast(float, sizeof(T) == 4 ? u : j & 1 ? u & 0xffff0000u : u << 16);
