@@ -495,10 +495,9 @@ typedef struct katsu_distillation {
     int64_t stride, out_stride, dloss_stride;  /* of logits, dlogits, dloss */
     float temperature;
 } katsu_distillation;
-int katsu_hip_distillation_workspace(const katsu_distillation *d, size_t *bytes);
 int katsu_hip_distillation_dev(const katsu_distillation *d, const void *logits,
                                const int32_t *ids, const void *teacher, float *loss, float *stats,
-                               void *workspace, size_t workspace_bytes, void *stream);
+                               void *stream);
 /* The gradient; dlogits may be logits, with the same stride. */
 int katsu_hip_distillation_bwd_dev(const katsu_distillation *d, const float *dloss,
                                    const void *logits, const int32_t *ids, const void *teacher,
@@ -507,8 +506,7 @@ int katsu_hip_distillation_bwd_dev(const katsu_distillation *d, const float *dlo
  * dlogits may be logits, with the same stride. */
 int katsu_hip_distillation_step_dev(const katsu_distillation *d, const void *logits,
                                     const int32_t *ids, const void *teacher, const float *dloss,
-                                    float *loss, void *dlogits, void *workspace,
-                                    size_t workspace_bytes, void *stream);
+                                    float *loss, void *dlogits, void *stream);
 
 #ifdef __cplusplus
 }

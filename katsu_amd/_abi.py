@@ -39,9 +39,8 @@ EXPORTS = (
     "katsu_hip_clip_grad_norm_dev", "katsu_hip_clip_grad_norm_ws_dev",
     "katsu_hip_embedding_dev", "katsu_hip_embedding_bwd_workspace", "katsu_hip_embedding_bwd_dev",
     "katsu_hip_qk_norm_rotary_dev", "katsu_hip_qk_norm_rotary_bwd_workspace",
-    "katsu_hip_qk_norm_rotary_bwd_dev", "katsu_hip_distillation_workspace",
-    "katsu_hip_distillation_dev", "katsu_hip_distillation_bwd_dev",
-    "katsu_hip_distillation_step_dev",
+    "katsu_hip_qk_norm_rotary_bwd_dev", "katsu_hip_distillation_dev",
+    "katsu_hip_distillation_bwd_dev", "katsu_hip_distillation_step_dev",
 )
 
 
@@ -198,10 +197,9 @@ def lib():
         L.katsu_hip_qk_norm_rotary_bwd_dev.argtypes = ([qp, ctypes.POINTER(QkNormRotaryGrads)] +
                                                        [vp] * 13 + [sz, vp])
         dp = ctypes.POINTER(Distillation)
-        L.katsu_hip_distillation_workspace.argtypes = [dp, szp]
-        L.katsu_hip_distillation_dev.argtypes = [dp] + [vp] * 6 + [sz, vp]
+        L.katsu_hip_distillation_dev.argtypes = [dp] + [vp] * 6
         L.katsu_hip_distillation_bwd_dev.argtypes = [dp] + [vp] * 7
-        L.katsu_hip_distillation_step_dev.argtypes = [dp] + [vp] * 7 + [sz, vp]
+        L.katsu_hip_distillation_step_dev.argtypes = [dp] + [vp] * 7
         for name in EXPORTS:
             if name not in ("katsu_hip_version", "katsu_hip_strerror", "katsu_hip_shutdown",
                             "katsu_hip_noalloc_scratch_bytes",

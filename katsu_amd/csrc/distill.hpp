@@ -26,9 +26,8 @@ struct DistillArgs {
     float *stats;       // [2][rows]: M, 1/L (0, 0 without an entry)
     float *loss;
     void *dz;
-    float *part;        // [rows][splits][2]: M and L of a run of columns
-    int64_t rows, vocab, z_row, dz_row, dloss_step, run;  // run: columns of a split
-    int top, splits, teacher_bf16;
+    int64_t rows, vocab, z_row, dz_row, dloss_step, run;  // run: columns of a block's gradient
+    int top, teacher_bf16;
     float tau, scale2;  // scale2: log2(e) / tau
 };
 
@@ -82,10 +81,12 @@ struct DistillRow {
             t[i] = -INFINITY;
             if (k < a.top) {
                 const int v = a.ids[row * a.top + k];
+                const float x = a.teacher_bf16
+                                    ? (float)((const __bf16 *)a.teacher)[row * a.top + k]
+                                    : ((const float *)a.teacher)[row * a.top + k];
                 if (v >= 0 && v < a.vocab) {
                     id[i] = v;
-                    t[i] = a.teacher_bf16 ? (float)((const __bf16 *)a.teacher)[row * a.top + k]
-                                          : ((const float *)a.teacher)[row * a.top + k];
+                    t[i] = x;
                     any |= t[i] != -INFINITY;
                     m = fmaxf(m, t[i]);
                 }
@@ -128,6 +129,11 @@ struct DistillSum {
         l = l * distill_exp(m - r, by) + l2 * distill_exp(m2 - r, by);
         m = mn;
     }
+    __device__ __forceinline__ void wave(float by) {  // of all lanes, in each
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1)
+            join(__shfl_xor(m, off, 64), __shfl_xor(l, off, 64), by);
+    }
 };
 
 // M and L of a row's columns [c0, c1), the same in every thread.
@@ -135,20 +141,27 @@ template <typename T, int NT>
 __device__ __forceinline__ DistillSum distill_columns(const T *z, int64_t c0, int64_t c1, float by,
                                                       float *part) {
     constexpr int E = Piece<T>::E;
+    constexpr int U = 4;  // pieces in flight
     DistillSum s;
     int64_t i = c0 + threadIdx.x * E;
-    for (; i + E <= c1; i += NT * E) {
-        float x[E];
-        load_piece(z, i, c1, x);
-        s.add(x, by);
-    }
-    for (; i < c1; ++i) {  // this thread's piece is the last one, cut short
-        const float x[1] = {(float)z[i]};
-        s.add(x, by);
-    }
+    for (; i + ((U - 1) * NT + 1) * E <= c1; i += U * NT * E) {
+        RawPiece<T> r[U];
+        float x[U * E];
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1)
-        s.join(__shfl_xor(s.m, off, 64), __shfl_xor(s.l, off, 64), by);
+        for (int u = 0; u < U; ++u) __builtin_memcpy(&r[u].v, z + i + u * NT * E, 16);
+#pragma unroll
+        for (int e = 0; e < U * E; ++e) x[e] = r[e / E].at(e % E);
+        s.add(x, by);
+    }
+    for (; i < c1; i += NT * E) {
+        RawPiece<T> r;
+        float x[E];
+        r.load(z, i, c1, -INFINITY);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = r.at(e);
+        s.add(x, by);
+    }
+    s.wave(by);
     if ((threadIdx.x & 63) == 0) {
         part[2 * (threadIdx.x >> 6)] = s.m;
         part[2 * (threadIdx.x >> 6) + 1] = s.l;
@@ -362,45 +375,6 @@ __global__ void __launch_bounds__(NT) distill_step_kernel(const DistillArgs a) {
     }
     __syncthreads();  // and all others written
     fix.write(d, dz);
-}
-
-// Few rows: M and L of runs of a row's columns, then the loss from them.
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
-    __shared__ float part[2 * NT / 64];
-    const int64_t row = blockIdx.x, c0 = blockIdx.z * a.run;
-    const DistillSum s = distill_columns<T, NT>((const T *)a.z + row * a.z_row, c0,
-                                                min(c0 + a.run, a.vocab), a.scale2, part);
-    if (threadIdx.x == 0) {
-        float *p = a.part + (row * a.splits + blockIdx.z) * 2;
-        p[0] = s.m;
-        p[1] = s.l;
-    }
-}
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT) distill_join_kernel(const DistillArgs a) {
-    __shared__ float part[3][2 * NT / 64];
-    const int64_t row = blockIdx.x;
-    DistillRow<NT> d;
-    d.load(a, row);
-    float m = 0.f, inv = 0.f;
-    if (d.some) {
-        d.softmax(a, part[0], part[1]);
-        DistillSum s;
-        for (int i = 0; i < a.splits; ++i) {
-            const float *p = a.part + (row * a.splits + i) * 2;
-            s.join(p[0], p[1], a.scale2);
-        }
-        distill_loss<T, NT>(a, row, d, s, part[2]);
-        m = s.m;
-        inv = 1.f / s.l;
-    } else if (threadIdx.x == 0) {
-        a.loss[row] = 0.f;
-    }
-    if (threadIdx.x == 0) {
-        a.stats[row] = m;
-        a.stats[a.rows + row] = inv;
-    }
 }
 
 }  // namespace katsu

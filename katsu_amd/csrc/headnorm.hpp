@@ -246,28 +246,28 @@ __global__ void __launch_bounds__(256) head_norm_bwd_kernel(const HeadArgs a) {
             part[0][d] + part[1][d] + part[2][d] + part[3][d];
 }
 
-// dw: the blocks' sums, in order within each of 16 rows of threads, then the rows'.
+// dw: the blocks' sums, in order within each of 32 rows of threads, then the rows'.
 // blockIdx.y: q or k.
 template <typename T>
 __global__ void __launch_bounds__(1024) head_norm_sum_kernel(const float *part, int n_q, int n_k,
                                                             int D, T *dw_q, T *dw_k) {
-    __shared__ float s[16][64];
+    __shared__ float s[32][33];
     const bool second = blockIdx.y != 0;
     T *out = second ? dw_k : dw_q;
     if (!out) return;
     const float *p = part + (second ? (int64_t)n_q * D : 0);
-    const int n = second ? n_k : n_q, lane = threadIdx.x & 63, row = threadIdx.x >> 6;
-    const int d = blockIdx.x * 64 + lane;
+    const int n = second ? n_k : n_q, col = threadIdx.x & 31, row = threadIdx.x >> 5;
+    const int d = blockIdx.x * 32 + col;
     float v = 0.f;
     if (d < D) {
-#pragma unroll 8
-        for (int i = row; i < n; i += 16) v += p[(int64_t)i * D + d];
+#pragma unroll 16
+        for (int i = row; i < n; i += 32) v += p[(int64_t)i * D + d];
     }
-    s[row][lane] = v;
+    s[row][col] = v;
     __syncthreads();
     if (row != 0 || d >= D) return;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += s[i][lane];
+    for (int i = 1; i < 32; ++i) v += s[i][col];
     out[d] = (T)v;
 }
 

@@ -3461,24 +3461,14 @@ int katsu_hip_qk_norm_rotary_bwd_dev(const katsu_qk_norm_rotary *d,
                               dw_k, ws, st);
 }
 
-int katsu_hip_distillation_workspace(const katsu_distillation *d, size_t *bytes) {
-    if (!d || !bytes || !distillation_ok(*d)) return KATSU_E_INVALID;
-    *bytes = distillation_bytes(*d);
-    return KATSU_OK;
-}
-
 int katsu_hip_distillation_dev(const katsu_distillation *d, const void *logits,
                                const int32_t *ids, const void *teacher, float *loss, float *stats,
-                               void *workspace, size_t workspace_bytes, void *stream) {
+                               void *stream) {
     if (!d || !distillation_ok(*d)) return KATSU_E_INVALID;
     if (d->rows == 0) return KATSU_OK;
     if (!loss || (d->vocab > 0 && !logits) || (d->top > 0 && (!ids || !teacher)))
         return KATSU_E_INVALID;
-    hipStream_t st = (hipStream_t)stream;
-    void *ws = nullptr;
-    const int rc = lm_scratch(workspace, workspace_bytes, distillation_bytes(*d), st, &ws);
-    if (rc) return rc;
-    return distillation(*d, logits, ids, teacher, loss, stats, ws, st);
+    return distillation(*d, logits, ids, teacher, loss, stats, (hipStream_t)stream);
 }
 
 // An output of the logits' shape: rows of its own, and where it is the logits, row by row.
@@ -3500,18 +3490,13 @@ int katsu_hip_distillation_bwd_dev(const katsu_distillation *d, const float *dlo
 
 int katsu_hip_distillation_step_dev(const katsu_distillation *d, const void *logits,
                                     const int32_t *ids, const void *teacher, const float *dloss,
-                                    float *loss, void *dlogits, void *workspace,
-                                    size_t workspace_bytes, void *stream) {
+                                    float *loss, void *dlogits, void *stream) {
     if (!d || !distillation_ok(*d) || !dlogits_ok(*d, logits, dlogits)) return KATSU_E_INVALID;
     if (d->rows == 0) return KATSU_OK;
     if (!loss || !dloss || (d->vocab > 0 && (!logits || !dlogits)) ||
         (d->top > 0 && (!ids || !teacher)))
         return KATSU_E_INVALID;
-    hipStream_t st = (hipStream_t)stream;
-    void *ws = nullptr;
-    const int rc = lm_scratch(workspace, workspace_bytes, distillation_bytes(*d), st, &ws);
-    if (rc) return rc;
-    return distillation_step(*d, logits, ids, teacher, dloss, loss, dlogits, ws, st);
+    return distillation_step(*d, logits, ids, teacher, dloss, loss, dlogits, (hipStream_t)stream);
 }
 
 }  // extern "C"

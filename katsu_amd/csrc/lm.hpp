@@ -74,15 +74,13 @@ int qk_norm_rotary_bwd(const katsu_qk_norm_rotary &d, const katsu_qk_norm_rotary
                        void *dw_k, void *ws, hipStream_t st);
 
 bool distillation_ok(const katsu_distillation &d);
-// Scratch bytes of a forward call or a step.
-size_t distillation_bytes(const katsu_distillation &d);
 int distillation(const katsu_distillation &d, const void *logits, const int32_t *ids,
-                 const void *teacher, float *loss, float *stats, void *ws, hipStream_t st);
+                 const void *teacher, float *loss, float *stats, hipStream_t st);
 int distillation_bwd(const katsu_distillation &d, const float *dloss, const void *logits,
                      const int32_t *ids, const void *teacher, const float *stats, void *dlogits,
                      hipStream_t st);
 int distillation_step(const katsu_distillation &d, const void *logits, const int32_t *ids,
                       const void *teacher, const float *dloss, float *loss, void *dlogits,
-                      void *ws, hipStream_t st);
+                      hipStream_t st);
 
 }  // namespace katsu

@@ -244,24 +244,9 @@ void head_blocks(const katsu_qk_norm_rotary &d, int (&blocks)[2]) {
 
 // ---- distillation ----
 
-struct DistillPlan {
-    int splits;
-    int64_t run;
-};
-// Runs of columns: whole rows where there are enough of them.
-DistillPlan distill_plan(const katsu_distillation &d) {
-    DistillPlan p = {1, (int64_t)d.vocab};
-    const int64_t rows = (int64_t)d.rows, V = (int64_t)d.vocab;
-    const int64_t want = std::min(cdiv(4 * kCUs, std::max<int64_t>(rows, 1)), cdiv(V, 4096));
-    if (rows >= kCUs || want <= 1) return p;
-    p.run = cdiv(cdiv(V, want), 512) * 512;
-    p.splits = (int)cdiv(V, p.run);
-    return p;
-}
 DistillArgs distill_args(const katsu_distillation &d, const void *logits, const int32_t *ids,
                          const void *teacher) {
     DistillArgs a{};
-    const DistillPlan p = distill_plan(d);
     a.z = logits;
     a.teacher = teacher;
     a.ids = ids;
@@ -270,17 +255,22 @@ DistillArgs distill_args(const katsu_distillation &d, const void *logits, const 
     a.z_row = d.stride;
     a.dz_row = d.out_stride;
     a.dloss_step = d.dloss_stride;
-    a.run = p.run;
-    a.splits = p.splits;
+    a.run = a.vocab;
     a.top = (int)d.top;
     a.teacher_bf16 = d.teacher_dtype == KATSU_BF16;
     a.tau = d.temperature;
     a.scale2 = (float)(1.4426950408889634 / (double)d.temperature);
     return a;
 }
-template <typename T, bool LOSS, bool GRAD>
-int launch_distill(const DistillArgs &a, int splits, hipStream_t st) {
-    distill_kernel<T, 256, LOSS, GRAD><<<grid_of(a.rows, splits), 256, 0, st>>>(a);
+// A block a row: of 16 waves where there are few rows and long ones (250 x 130000 float32: 31 us, 40
+// in blocks of 4), else of 4 (1000 x 32000 bfloat16: 16 us, 32 in blocks of 16).  Rows that are
+// read twice, for the gradient as well, fill the card with fewer (400 x 100000 float32: 115, 128).
+template <typename T, bool GRAD>
+int launch_loss(const DistillArgs &a, hipStream_t st) {
+    if (GRAD ? a.rows < 4 * kCUs : a.rows < kCUs && a.vocab > 8192)
+        distill_kernel<T, 1024, true, GRAD><<<grid_of(a.rows), 1024, 0, st>>>(a);
+    else
+        distill_kernel<T, 256, true, GRAD><<<grid_of(a.rows), 256, 0, st>>>(a);
     return status_of(hipGetLastError());
 }
 // Loss and gradient with the rows in registers: threads of a row, and its pieces a thread.
@@ -298,15 +288,6 @@ bool by_row_pieces(const DistillArgs &a, F f) {
         return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 16>());
     return false;
 }
-// The loss and the statistics of few rows, in two launches.
-template <typename T>
-int launch_parts(const DistillArgs &a, hipStream_t st) {
-    distill_part_kernel<T, 256>
-        <<<dim3((unsigned)a.rows, 1, (unsigned)a.splits), 256, 0, st>>>(a);
-    distill_join_kernel<T, 256><<<dim3((unsigned)a.rows), 256, 0, st>>>(a);
-    return status_of(hipGetLastError());
-}
-
 }  // namespace
 
 bool embedding_ok(const katsu_embedding &d) {
@@ -426,7 +407,7 @@ int qk_norm_rotary_bwd(const katsu_qk_norm_rotary &d, const katsu_qk_norm_rotary
             });
         });
     if (rc != KATSU_OK || (!w_q && !w_k)) return rc;
-    const dim3 grid((unsigned)cdiv(a.D, 64), 2);
+    const dim3 grid((unsigned)cdiv(a.D, 32), 2);
     if (!w_q) dw_q = nullptr;
     if (!w_k) dw_k = nullptr;
     if (d.dtype == KATSU_F32)
@@ -445,24 +426,13 @@ bool distillation_ok(const katsu_distillation &d) {
            std::isfinite(d.temperature) && std::isfinite(1.f / d.temperature);
 }
 
-size_t distillation_bytes(const katsu_distillation &d) {
-    const DistillPlan p = distill_plan(d);
-    return p.splits > 1 ? (size_t)d.rows * (2 * p.splits + 2) * sizeof(float) : 0;
-}
-
 int distillation(const katsu_distillation &d, const void *logits, const int32_t *ids,
-                 const void *teacher, float *loss, float *stats, void *ws, hipStream_t st) {
+                 const void *teacher, float *loss, float *stats, hipStream_t st) {
     DistillArgs a = distill_args(d, logits, ids, teacher);
     a.loss = loss;
-    a.part = (float *)ws;
     a.stats = stats;
-    auto run = [&](auto t) {
-        using T = decltype(t);
-        if (a.splits == 1) return launch_distill<T, true, false>(a, 1, st);
-        if (!a.stats) a.stats = a.part + 2 * a.rows * a.splits;
-        return launch_parts<T>(a, st);
-    };
-    return d.dtype == KATSU_F32 ? run(float()) : run(__bf16());
+    return d.dtype == KATSU_F32 ? launch_loss<float, false>(a, st)
+                                : launch_loss<__bf16, false>(a, st);
 }
 
 int distillation_bwd(const katsu_distillation &d, const float *dloss, const void *logits,
@@ -472,18 +442,24 @@ int distillation_bwd(const katsu_distillation &d, const float *dloss, const void
     a.dloss = dloss;
     a.stats = const_cast<float *>(stats);
     a.dz = dlogits;
-    return d.dtype == KATSU_F32 ? launch_distill<float, false, true>(a, a.splits, st)
-                                : launch_distill<__bf16, false, true>(a, a.splits, st);
+    // Few rows: runs of columns, four blocks a CU.
+    const int64_t want = std::min(cdiv(4 * kCUs, a.rows), cdiv(a.vocab, 4096));
+    a.run = cdiv(cdiv(a.vocab, want), 2048) * 2048;
+    const dim3 grid = grid_of(a.rows, (int)cdiv(a.vocab, a.run));
+    if (d.dtype == KATSU_F32)
+        distill_kernel<float, 256, false, true><<<grid, 256, 0, st>>>(a);
+    else
+        distill_kernel<__bf16, 256, false, true><<<grid, 256, 0, st>>>(a);
+    return status_of(hipGetLastError());
 }
 
 int distillation_step(const katsu_distillation &d, const void *logits, const int32_t *ids,
                       const void *teacher, const float *dloss, float *loss, void *dlogits,
-                      void *ws, hipStream_t st) {
+                      hipStream_t st) {
     DistillArgs a = distill_args(d, logits, ids, teacher);
     a.loss = loss;
     a.dloss = dloss;
     a.dz = dlogits;
-    a.part = (float *)ws;
     auto run = [&](auto t) {
         using T = decltype(t);
         if (by_row_pieces<T>(a, [&](auto nt, auto np) {
@@ -492,10 +468,7 @@ int distillation_step(const katsu_distillation &d, const void *logits, const int
                 return true;
             }))
             return status_of(hipGetLastError());
-        if (a.splits == 1) return launch_distill<T, true, true>(a, 1, st);
-        a.stats = a.part + 2 * a.rows * a.splits;
-        const int rc = launch_parts<T>(a, st);
-        return rc != KATSU_OK ? rc : launch_distill<T, false, true>(a, a.splits, st);
+        return launch_loss<T, true>(a, st);  // rows that the registers do not hold
     };
     return d.dtype == KATSU_F32 ? run(float()) : run(__bf16());
 }

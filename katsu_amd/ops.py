@@ -502,13 +502,21 @@ def clip_grad_norm(grads, max_norm, out=None, workspace=None):
 
 # ---- the ends of a language model, and the heads before its attention ----
 
-def _here(t):
-    """The launches go to the current device's current stream: the operands must be there."""
-    if t.get_device() != torch._C._cuda_getDevice():
+def _operands(first, *ts):
+    """float32 or bfloat16, all of the first one's type, on the current device: the launches go to its
+    current stream.  (Type and device number are compared: a device object takes 0.1 us to make.)"""
+    dt, dev = first.dtype, first.get_device()
+    if dt not in _DTYPE or dev < 0:
+        raise ValueError("float32 or bfloat16 device tensors expected")
+    if dev != torch._C._cuda_getDevice():
         raise ValueError("operands must be on the current device")
+    for t in ts:
+        if t is not None and (t.dtype is not dt or t.get_device() != dev):
+            raise ValueError("all operands must have one type and device")
+    return _DTYPE[dt]
 
 
-def _scratch(workspace, dev, size_fn, d):
+def _scratch(workspace, first, size_fn, d):
     """The caller's workspace, or one of torch's for this call: unlike the library's own buffer it
     belongs to the stream, or to the graph that is captured."""
     if workspace is None:
@@ -516,8 +524,9 @@ def _scratch(workspace, dev, size_fn, d):
         check(size_fn(ctypes.byref(d), ctypes.byref(nbytes)), "workspace")
         if nbytes.value == 0:
             return None, 0, 0
-        workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
-    return (workspace, *_workspace(workspace, dev))
+        workspace = first.new_empty(nbytes.value, dtype=torch.uint8)
+        return workspace, workspace.data_ptr(), nbytes.value
+    return (workspace, *_workspace(workspace, first.device))
 
 
 def _rows(t, what):
@@ -528,22 +537,21 @@ def _rows(t, what):
 
 
 def _embedding(table, out, ids, scale, beta):
-    _dev_lm(table, out)
-    _here(table)
+    kind = _operands(table, out)
     strides = _rows(table, "the table"), _rows(out, "out")
     if out.shape[1] != table.shape[1] or table.shape[1] == 0:
         raise ValueError("out must have the table's columns, one at least")
     if beta not in (0.0, 1.0):
         raise ValueError("beta must be 0 or 1")
     _int32(ids, out.shape[0], table.device, "ids")
-    return Embedding(_DTYPE[table.dtype], int(beta), out.shape[0], *table.shape, *strides, scale)
+    return Embedding(kind, int(beta), out.shape[0], *table.shape, *strides, scale)
 
 
 def embedding(ids, table, scale=1.0, out=None):
     """[T, C]: scale times the rows of table [V, C] that ids (int32 [T]) name; zeros where an id is
     not in [0, V), as for padding.  Rows of table and out may have any stride."""
     if out is None:
-        out = torch.empty((ids.numel(), table.shape[-1]), dtype=table.dtype, device=table.device)
+        out = table.new_empty((ids.numel(), table.shape[-1]))
     d = _embedding(table, out, ids, scale, 0.0)
     check(lib().katsu_hip_embedding_dev(ctypes.byref(d), _p(ids), _p(table), _p(out), _stream()),
           "embedding")
@@ -558,11 +566,11 @@ def embedding_backward(dout, ids, vocab, scale=1.0, out=None, beta=0.0, workspac
     if out is None:
         if beta != 0.0:
             raise ValueError("beta=1 needs the gradient that it accumulates into")
-        out = torch.empty((vocab, dout.shape[-1]), dtype=dout.dtype, device=dout.device)
+        out = dout.new_empty((vocab, dout.shape[-1]))
     if out.shape[0] != vocab:
         raise ValueError("out must have a row for each of the vocabulary")
     d = _embedding(out, dout, ids, scale, beta)
-    keep, *ws = _scratch(workspace, dout.device, lib().katsu_hip_embedding_bwd_workspace, d)
+    keep, *ws = _scratch(workspace, dout, lib().katsu_hip_embedding_bwd_workspace, d)
     check(lib().katsu_hip_embedding_bwd_dev(ctypes.byref(d), _p(dout), _p(ids), _p(out), *ws,
                                             _stream()), "embedding_backward")
     return out
@@ -577,30 +585,32 @@ def embedding_workspace_bytes(tokens, vocab, cols, dtype):
     return nbytes.value
 
 
-def _qk_norm_rotary(q, k, out_q, out_k, table, positions, w_q, w_k, eps, interleaved):
-    _dev_lm(q, k, out_q, out_k, w_q, w_k)
-    _here(q)
-    strides = [(0, 0) if t is None else _heads(t, w)
-               for t, w in ((q, "q"), (k, "k"), (out_q, "out_q"), (out_k, "out_k"))]
-    tokens, heads, dim = q.shape
-    if out_q.shape != q.shape or (k is None) != (out_k is None) or (k is not None and (
-            out_k.shape != k.shape or k.shape[0] != tokens or k.shape[2] != dim)):
-        raise ValueError("q and k must have the same tokens and channels, outputs their shapes")
+def _qk_norm_rotary(q, k, out_q, out_k, table, positions, w_q, w_k, eps, interleaved, *more):
+    kind = _operands(q, k, out_q, out_k, w_q, w_k, *more)
+    tokens, heads, dim = q.shape if q.dim() == 3 else (0, 0, 0)
+    strides = [_heads(q, "q"), (0, 0), _heads(out_q, "out_q"), (0, 0)]
+    if out_q.shape != q.shape or (k is None) != (out_k is None):
+        raise ValueError("outputs must have the operands' shapes")
+    if k is not None:
+        strides[1::2] = _heads(k, "k"), _heads(out_k, "out_k")
+        if out_k.shape != k.shape or k.shape[0] != tokens or k.shape[2] != dim:
+            raise ValueError("q and k must have the same tokens and channels, outputs their shapes")
+    elif w_k is not None:
+        raise ValueError("w_k goes with k")
     for w in (w_q, w_k):
         if w is not None and (w.shape != (dim,) or not w.is_contiguous()):
             raise ValueError("weights must be contiguous [channels]")
-    if w_k is not None and k is None:
-        raise ValueError("w_k goes with k")
-    if table is not None and (table.dim() != 2 or table.dtype is not torch.float32
-                              or table.device != q.device or not table.is_contiguous()
-                              or table.shape[1] == 0):
-        raise ValueError("table must be contiguous float32 [length, channels that turn]")
-    if table is None and positions is not None:
+    length = rot = 0
+    if table is not None:
+        if (table.dim() != 2 or table.dtype is not torch.float32 or not table.is_contiguous()
+                or table.get_device() != q.get_device() or table.shape[1] == 0):
+            raise ValueError("table must be contiguous float32 [length, channels that turn]")
+        length, rot = table.shape
+    elif positions is not None:
         raise ValueError("positions go with a table")
     _int32(positions, tokens, q.device, "positions")
-    length, rot = (0, 0) if table is None else table.shape
-    return QkNormRotary(_DTYPE[q.dtype], bool(interleaved), tokens, heads,
-                        0 if k is None else k.shape[1], dim, rot, length, *strides, eps)
+    return QkNormRotary(kind, bool(interleaved), tokens, heads, 0 if k is None else k.shape[1], dim,
+                        rot, length, *strides, eps)
 
 
 def qk_norm_rotary(q, k, table=None, positions=None, w_q=None, w_k=None, eps=1e-6,
@@ -627,14 +637,13 @@ def qk_norm_rotary_backward(dq, dk, q, k, table=None, positions=None, w_q=None, 
     out_q = torch.empty_like(q) if out_q is None else out_q
     if k is not None and out_k is None:
         out_k = torch.empty_like(k)
-    d = _qk_norm_rotary(q, k, out_q, out_k, table, positions, w_q, w_k, eps, interleaved)
-    _dev_lm(q, dq, dk)
+    d = _qk_norm_rotary(q, k, out_q, out_k, table, positions, w_q, w_k, eps, interleaved, dq, dk)
     if dq.shape != q.shape or (dk is None) != (k is None) or (k is not None
                                                               and dk.shape != k.shape):
         raise ValueError("gradients must have their operands' shapes")
     g = QkNormRotaryGrads(_heads(dq, "dq"), (0, 0) if dk is None else _heads(dk, "dk"))
     dw_q, dw_k = (None if w is None else torch.empty_like(w) for w in (w_q, w_k))
-    keep, *ws = _scratch(workspace, q.device, lib().katsu_hip_qk_norm_rotary_bwd_workspace, d)
+    keep, *ws = _scratch(workspace, q, lib().katsu_hip_qk_norm_rotary_bwd_workspace, d)
     check(lib().katsu_hip_qk_norm_rotary_bwd_dev(
         ctypes.byref(d), ctypes.byref(g), _p(dq), _p(dk), _p(q), _p(k), _p(w_q), _p(w_k),
         _p(table), _p(positions), _p(out_q), _p(out_k), _p(dw_q), _p(dw_k), *ws, _stream()),
@@ -652,8 +661,7 @@ def qk_norm_rotary_workspace_bytes(q, k):
 
 
 def _distillation(logits, ids, teacher, temperature, out=None, dloss=None):
-    _dev_lm(logits, out)
-    _here(logits)
+    kind = _operands(logits, out)
     strides = _rows(logits, "logits"), 0 if out is None else _rows(out, "out")
     rows, vocab = logits.shape
     if out is not None and out.shape != logits.shape:
@@ -661,31 +669,28 @@ def _distillation(logits, ids, teacher, temperature, out=None, dloss=None):
     if (ids.dim() != 2 or ids.shape[0] != rows or teacher.shape != ids.shape
             or ids.dtype is not torch.int32 or teacher.dtype not in _DTYPE
             or not ids.is_contiguous() or not teacher.is_contiguous()
-            or ids.device != logits.device or teacher.device != logits.device):
+            or not ids.get_device() == teacher.get_device() == logits.get_device()):
         raise ValueError("ids (int32) and teacher (float32 or bfloat16) must be contiguous "
                          "[rows, top] on the logits' device")
     if dloss is not None and (dloss.dtype is not torch.float32 or dloss.device != logits.device
                               or dloss.shape != (rows,)):
         raise ValueError("dloss must be float32 [rows] on the logits' device")
-    return Distillation(_DTYPE[logits.dtype], _DTYPE[teacher.dtype], rows, vocab, ids.shape[1],
+    return Distillation(kind, _DTYPE[teacher.dtype], rows, vocab, ids.shape[1],
                         *strides, 0 if dloss is None else dloss.stride(0), temperature)
 
 
-def distillation(logits, ids, teacher, temperature=1.0, workspace=None):
+def distillation(logits, ids, teacher, temperature=1.0):
     """(loss, stats): for each row of logits [rows, V] temperature^2 times the divergence of
     softmax(logits / temperature) from the teacher's softmax(teacher / temperature) over its top
     logits, teacher [rows, K] at the columns ids (int32 [rows, K], K at most 1024); entries with an
     id that is no column do not count.  loss [rows], float32.  K = 1 and temperature 1: the cross
     entropy with labels.  A row without an entry has loss 0.  stats [2, rows] float32 is for
-    distillation_backward.  `workspace`: an optional device tensor of
-    distillation_workspace_bytes()."""
+    distillation_backward."""
     d = _distillation(logits, ids, teacher, temperature)
-    dev = logits.device
-    loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
-    stats = torch.empty((2, d.rows), dtype=torch.float32, device=dev)
-    keep, *ws = _scratch(workspace, dev, lib().katsu_hip_distillation_workspace, d)
+    loss = logits.new_empty(d.rows, dtype=torch.float32)
+    stats = logits.new_empty((2, d.rows), dtype=torch.float32)
     check(lib().katsu_hip_distillation_dev(ctypes.byref(d), _p(logits), _p(ids), _p(teacher),
-                                           _p(loss), _p(stats), *ws, _stream()), "distillation")
+                                           _p(loss), _p(stats), _stream()), "distillation")
     return loss, stats
 
 
@@ -703,24 +708,14 @@ def distillation_backward(dloss, logits, ids, teacher, stats, temperature=1.0, o
     return out
 
 
-def distillation_step(logits, ids, teacher, dloss, temperature=1.0, out=None, workspace=None):
+def distillation_step(logits, ids, teacher, dloss, temperature=1.0, out=None):
     """(loss, gradient of the logits) in one pass over them, where dloss (float32 [rows], any
     stride: what the sum or the mean of the losses gives each) is known beforehand.  `out`, the
     gradient, may be the logits."""
     out = torch.empty_like(logits) if out is None else out
     d = _distillation(logits, ids, teacher, temperature, out, dloss)
-    loss = torch.empty(d.rows, dtype=torch.float32, device=logits.device)
-    keep, *ws = _scratch(workspace, logits.device, lib().katsu_hip_distillation_workspace, d)
+    loss = logits.new_empty(d.rows, dtype=torch.float32)
     check(lib().katsu_hip_distillation_step_dev(ctypes.byref(d), _p(logits), _p(ids), _p(teacher),
-                                                _p(dloss), _p(loss), _p(out), *ws, _stream()),
+                                                _p(dloss), _p(loss), _p(out), _stream()),
           "distillation_step")
     return loss, out
-
-
-def distillation_workspace_bytes(logits, ids, teacher):
-    """Scratch that distillation or distillation_step needs for operands of these shapes."""
-    d = _distillation(logits, ids, teacher, 1.0)
-    nbytes = ctypes.c_size_t(0)
-    check(lib().katsu_hip_distillation_workspace(ctypes.byref(d), ctypes.byref(nbytes)),
-          "distillation_workspace")
-    return nbytes.value

@@ -130,41 +130,33 @@ def _distill(**kw):
     dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=NAN), dict(temperature=INF),
     dict(temperature=1e-42)])
 def test_distillation_refuses(kw):
-    n = SZ(0)
-    for rc in (L.katsu_hip_distillation_workspace(_distill(**kw), ctypes.byref(n)),
-               L.katsu_hip_distillation_dev(_distill(**kw), *[P] * 6, 1 << 30, None),
+    for rc in (L.katsu_hip_distillation_dev(_distill(**kw), *[P] * 5, None),
                L.katsu_hip_distillation_bwd_dev(_distill(**kw), *[P] * 6, None),
-               L.katsu_hip_distillation_step_dev(_distill(**kw), *[P] * 7, 1 << 30, None)):
+               L.katsu_hip_distillation_step_dev(_distill(**kw), *[P] * 6, None)):
         assert rc == _abi.E_INVALID
 
 
 def test_distillation_pointers():
     fwd, bwd, step = (L.katsu_hip_distillation_dev, L.katsu_hip_distillation_bwd_dev,
                       L.katsu_hip_distillation_step_dev)
-    n = SZ(0)
     for i in range(4):  # logits, ids, teacher, loss; stats may be missing
         some = [None if j == i else P for j in range(4)]
-        assert fwd(_distill(), *some, P, P, 1 << 30, None) == _abi.E_INVALID
+        assert fwd(_distill(), *some, P, None) == _abi.E_INVALID
     for i in range(6):
         some = [None if j == i else P for j in range(6)]
         assert bwd(_distill(), *some, None) == _abi.E_INVALID
-        assert step(_distill(), *some, P, 1 << 30, None) == _abi.E_INVALID
+        assert step(_distill(), *some, None) == _abi.E_INVALID
     # Rows that share memory; in place with another stride.
     other = ctypes.c_void_p(P.value + 64)
     for kw, out in ((dict(out_stride=7), other), (dict(stride=16), P)):
-        assert bwd(_distill(**kw), *[P] * 5, out, None) == _abi.E_INVALID
-        assert step(_distill(**kw), *[P] * 5, out, P, 1 << 30, None) == _abi.E_INVALID
-    assert fwd(_distill(rows=0), *[None] * 6, 0, None) == _abi.OK
+        assert bwd(_distill(**kw), P, P, P, P, P, out, None) == _abi.E_INVALID
+        assert step(_distill(**kw), P, P, P, P, P, out, None) == _abi.E_INVALID
+    for fn in (fwd, bwd, step):
+        assert fn(None, *[P] * (5 if fn is fwd else 6), None) == _abi.E_INVALID
+    assert fwd(_distill(rows=0), *[None] * 5, None) == _abi.OK
     assert bwd(_distill(rows=0), *[None] * 6, None) == _abi.OK
     assert bwd(_distill(vocab=0), *[None] * 6, None) == _abi.OK
-    assert step(_distill(rows=0), *[None] * 7, 0, None) == _abi.OK
-    # Few long rows take scratch.
-    big = dict(rows=2, vocab=100000, stride=100000, out_stride=100000)
-    assert L.katsu_hip_distillation_workspace(_distill(**big), ctypes.byref(n)) == _abi.OK
-    assert n.value > 0
-    for ws, size in ((P, n.value - 1), (ctypes.c_void_p(P.value + 4), 1 << 30)):
-        assert fwd(_distill(**big), *[P] * 5, ws, size, None) == _abi.E_INVALID
-        assert step(_distill(**big), *[P] * 5, other, ws, size, None) == _abi.E_INVALID
+    assert step(_distill(rows=0), *[None] * 6, None) == _abi.OK
 
 
 def _bad(*calls):
@@ -250,12 +242,10 @@ def test_memory(dev):
     g, size = torch.Generator().manual_seed(1), 1 << 22
     x, ids = torch.zeros(6000, 8, device=dev), torch.zeros(6000, dtype=torch.int32, device=dev)
     q, w = torch.zeros(50, 2, 64, device=dev), torch.ones(64, device=dev)
-    z, i, t = (torch.zeros(2, 50000, device=dev), torch.zeros(2, 1, dtype=torch.int32, device=dev),
+    z, i, t = (torch.zeros(2, 50, device=dev), torch.zeros(2, 1, dtype=torch.int32, device=dev),
                torch.zeros(2, 1, device=dev))
     calls = (lambda ws: ops.embedding_backward(x, ids, 6000, workspace=ws),
-             lambda ws: ops.qk_norm_rotary_backward(q, None, q, None, w_q=w, workspace=ws),
-             lambda ws: ops.distillation(z, i, t, workspace=ws),
-             lambda ws: ops.distillation_step(z, i, t, t[:, 0], workspace=ws))
+             lambda ws: ops.qk_norm_rotary_backward(q, None, q, None, w_q=w, workspace=ws))
     for ws in (torch.empty(size, dtype=torch.uint8),
                torch.empty(1, dtype=torch.uint8, device=dev).expand(size),
                torch.empty(2 * size, dtype=torch.uint8, device=dev)[::2]):
@@ -267,6 +257,7 @@ def test_memory(dev):
     torch._C._cuda_getDevice = lambda: 1  # as if another device were the current one
     try:
         _bad(lambda: ops.embedding(ids, x), lambda: ops.qk_norm_rotary(q, None),
-             lambda: ops.distillation(z, i, t), *(lambda c=c: c(None) for c in calls))
+             lambda: ops.distillation(z, i, t), lambda: ops.distillation_step(z, i, t, t[:, 0]),
+             *(lambda c=c: c(None) for c in calls))
     finally:
         torch._C._cuda_getDevice = now
