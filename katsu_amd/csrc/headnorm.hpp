@@ -15,6 +15,8 @@
 
 namespace katsu {
 
+constexpr int kHeadThreads = 256;  // of a block of the gradient
+
 // One of q and k.
 struct HeadTensor {
     const void *x, *w, *dy;  // dy: the gradient of the output (backward)
@@ -28,6 +30,7 @@ struct HeadArgs {
     const int32_t *positions;  // NULL: 0, 1, ..
     int64_t tokens, length;
     int D, R, units;           // units of 2E channels of a head
+    uint64_t inv[3];           // head_inv of q's heads, k's, both
     float eps, inv_d;
     float *part;               // backward, [blocks][D]: sums of dw, q's blocks first
     int blocks[2];             // backward: blocks of q, of k
@@ -103,12 +106,18 @@ __device__ __forceinline__ float group_sum(float v) {
     for (int off = G / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
     return v;
 }
-// The token and the head of the item that lies `local` after the base-th of a token's n: local
-// below 2^20, so that the quotient is exact.
-__device__ __forceinline__ int head_split(int local, int n, float inv_n, int &token) {
-    const int q = (int)(((float)local + 0.5f) * inv_n);
-    token = q;
-    return local - q * n;
+// floor(i / n) for i n below 2^64: a product's upper half, as a division of 64 bits takes as many
+// instructions as the rest of a head.
+struct HeadPlace {
+    int64_t token;
+    int head;
+};
+__device__ __forceinline__ HeadPlace head_place(int64_t base, int local, int n, uint64_t inv) {
+    const int64_t t = inv ? (int64_t)__umul64hi((uint64_t)base, inv) : base;
+    // `local` after the base-th: below 2^20, so that the quotient is exact.
+    local += (int)(base - t * n);
+    const int q = (int)(((float)local + 0.5f) * (1.f / (float)n));
+    return {t + q, local - q * n};
 }
 
 // G lanes a head, NU units a lane.
@@ -117,10 +126,9 @@ __global__ void __launch_bounds__(256) head_norm_kernel(const HeadArgs a) {
     constexpr int PER = 256 / G;
     const int n = a.t[0].heads + a.t[1].heads, lane = threadIdx.x % G;
     const int64_t base = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * PER;
-    const int64_t token0 = base / n;
-    int more;
-    int head = head_split((int)(base - token0 * n) + threadIdx.x / G, n, 1.f / (float)n, more);
-    const int64_t token = token0 + more;
+    const HeadPlace at = head_place(base, threadIdx.x / G, n, a.inv[2]);
+    const int64_t token = at.token;
+    int head = at.head;
     if (token >= a.tokens) return;  // a whole group
     const bool second = head >= a.t[0].heads;
     const HeadTensor &t = a.t[second];
@@ -164,15 +172,14 @@ __global__ void __launch_bounds__(256) head_norm_kernel(const HeadArgs a) {
 // The gradient.  A block takes heads of q or of k, so that a lane's channels, and with them
 // its sums of dw, stay the same; the blocks' sums are added by head_norm_sum_kernel.
 template <typename T, bool INTER, int E, int G, int NU>
-__global__ void __launch_bounds__(256) head_norm_bwd_kernel(const HeadArgs a) {
-    constexpr int PER = 256 / G;
-    __shared__ float part[4][G * NU * 2 * E];
+__global__ void __launch_bounds__(kHeadThreads) head_norm_bwd_kernel(const HeadArgs a) {
+    constexpr int PER = kHeadThreads / G, W = kHeadThreads / 64;
+    __shared__ float part[W][G * NU * 2 * E];
     const bool second = (int)blockIdx.x >= a.blocks[0];
     const HeadTensor &t = a.t[second];
     const int block = (int)blockIdx.x - (second ? a.blocks[0] : 0);
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const int64_t items = a.tokens * t.heads, step = (int64_t)a.blocks[second] * PER;
-    const float inv_n = 1.f / (float)t.heads;
     HeadUnit<T, INTER, E> u[NU];
     float w[NU][2][E], dw[NU][2][E] = {};
 #pragma unroll
@@ -181,11 +188,9 @@ __global__ void __launch_bounds__(256) head_norm_bwd_kernel(const HeadArgs a) {
         if (t.w) u[k].load(t.w, 0, w[k]);
     }
     for (int64_t base = (int64_t)block * PER; base < items; base += step) {
-        const int64_t token0 = base / t.heads;
-        int more;
-        const int head =
-            head_split((int)(base - token0 * t.heads) + group, t.heads, inv_n, more);
-        const int64_t token = token0 + more;
+        const HeadPlace p = head_place(base, group, t.heads, a.inv[second]);
+        const int64_t token = p.token;
+        const int head = p.head;
         if (token >= a.tokens) break;  // a whole group, at its last item
         float x[NU][2][E], g[NU][2][E], cs[NU][2][E];
 #pragma unroll
@@ -241,9 +246,12 @@ __global__ void __launch_bounds__(256) head_norm_bwd_kernel(const HeadArgs a) {
                     part[threadIdx.x >> 6][u[k].c[i] + e] = v;
             }
     __syncthreads();
-    for (int d = threadIdx.x; d < a.D; d += 256)
-        a.part[(int64_t)blockIdx.x * a.D + d] =
-            part[0][d] + part[1][d] + part[2][d] + part[3][d];
+    for (int d = threadIdx.x; d < a.D; d += kHeadThreads) {
+        float v = part[0][d];
+#pragma unroll
+        for (int i = 1; i < W; ++i) v += part[i][d];
+        a.part[(int64_t)blockIdx.x * a.D + d] = v;
+    }
 }
 
 // dw: the blocks' sums, in order within each of 32 rows of threads, then the rows'.

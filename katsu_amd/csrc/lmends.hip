@@ -169,7 +169,7 @@ int embed_grad(const katsu_embedding &d, const EmbedArgs &a, char *ws, hipStream
 
 // The widest accesses that half of the turning part and the rest are multiples of, the
 // lanes of a head, and the units of a lane.
-template <typename T, bool INTER, class F>
+template <typename T, bool INTER, int MAX, class F>
 int by_head(const HeadArgs &a, F f) {
     auto with = [&](auto e) {
         constexpr int E = decltype(e)::value;
@@ -193,7 +193,7 @@ int by_head(const HeadArgs &a, F f) {
         return (int)KATSU_E_INVALID;
     };
     auto fits = [&](int e) { return a.R / 2 % e == 0 && (a.D - a.R) % e == 0; };
-    if constexpr (sizeof(T) == 2)
+    if constexpr (MAX == 8)
         if (fits(8)) return with(std::integral_constant<int, 8>());
     if (fits(4)) return with(std::integral_constant<int, 4>());
     if (fits(2)) return with(std::integral_constant<int, 2>());
@@ -219,6 +219,10 @@ HeadArgs head_args(const katsu_qk_norm_rotary &d, const float *table, const int3
         t.out_head = out[1];
         t.heads = (int)(i ? d.k_heads : d.heads);
     }
+    auto inverse = [](uint64_t n) { return n > 1 ? ~(uint64_t)0 / n + 1 : 0; };
+    a.inv[0] = inverse(d.heads);
+    a.inv[1] = inverse(d.k_heads);
+    a.inv[2] = inverse(d.heads + d.k_heads);
     a.table = table;
     a.positions = positions;
     a.tokens = (int64_t)d.tokens;
@@ -337,6 +341,8 @@ bool qk_norm_rotary_ok(const katsu_qk_norm_rotary &d) {
         return false;
     if (d.tokens > (uint64_t)kI32Max || d.length > (uint64_t)kI32Max) return false;
     if (d.rotary_dim > 0 && d.length == 0) return false;
+    // Items are divided by the heads with a product of 64 bits (head_place).
+    if (d.tokens * (d.heads + d.k_heads) > (uint64_t)1 << 46) return false;
     for (const auto &s : {d.q_stride, d.k_stride, d.q_out_stride, d.k_out_stride})
         if (!stride_ok(s[0]) || !stride_ok(s[1])) return false;
     return d.eps >= 0.f && std::isfinite(d.eps);
@@ -355,7 +361,7 @@ int qk_norm_rotary(const katsu_qk_norm_rotary &d, const void *q, const void *k, 
     return by_head_type(d, [&](auto t, auto inter) {
         using T = decltype(t);
         constexpr bool INTER = decltype(inter)::value;
-        return by_head<T, INTER>(a, [&](auto e, auto g, auto nu, int units) {
+        return by_head<T, INTER, 16 / sizeof(T)>(a, [&](auto e, auto g, auto nu, int units) {
             constexpr int G = decltype(g)::value;
             a.units = units;
             const int64_t items = a.tokens * (a.t[0].heads + a.t[1].heads);
@@ -398,11 +404,11 @@ int qk_norm_rotary_bwd(const katsu_qk_norm_rotary &d, const katsu_qk_norm_rotary
         rc = by_head_type(d, [&](auto t, auto inter) {
             using T = decltype(t);
             constexpr bool INTER = decltype(inter)::value;
-            return by_head<T, INTER>(a, [&](auto e, auto g, auto nu, int units) {
+            return by_head<T, INTER, 4>(a, [&](auto e, auto g, auto nu, int units) {
                 a.units = units;
                 head_norm_bwd_kernel<T, INTER, decltype(e)::value, decltype(g)::value,
                                      decltype(nu)::value>
-                    <<<dim3((unsigned)blocks), 256, 0, st>>>(a);
+                    <<<dim3((unsigned)blocks), kHeadThreads, 0, st>>>(a);
                 return status_of(hipGetLastError());
             });
         });
