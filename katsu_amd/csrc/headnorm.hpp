@@ -36,6 +36,17 @@ struct HeadArgs {
     int blocks[2];             // backward: blocks of q, of k
 };
 
+// E neighbouring values as they are in memory.
+template <typename T, int E>
+struct HeadPacked {
+    uint32_t w[(E * sizeof(T) + 3) / 4] = {};
+    __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(w, p, E * sizeof(T)); }
+    __device__ __forceinline__ float at(int e) const {
+        const uint32_t u = w[e * (int)sizeof(T) / 4];
+        return __builtin_bit_cast(float, sizeof(T) == 4 ? u : e & 1 ? u & 0xffff0000u : u << 16);
+    }
+};
+
 // A head is units of 2E channels: E pairs (R/2 apart, or 2E neighbours with INTER) for the
 // part that turns, then two pieces of E neighbours of the rest.  E divides R/2 and the rest,
 // whose last unit may have one piece only.
@@ -68,6 +79,12 @@ struct HeadUnit {
             else
 #pragma unroll
                 for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+    }
+    // As it is in memory, for heads that wait.
+    __device__ __forceinline__ void load(const void *p, int64_t at, HeadPacked<T, E> (&x)[2]) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (has[i]) x[i].load((const T *)p + at + c[i]);
     }
     __device__ __forceinline__ void store(void *p, int64_t at, const float (&x)[2][E]) const {
 #pragma unroll
@@ -179,7 +196,7 @@ __global__ void __launch_bounds__(kHeadThreads) head_norm_bwd_kernel(const HeadA
     const HeadTensor &t = a.t[second];
     const int block = (int)blockIdx.x - (second ? a.blocks[0] : 0);
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
-    const int64_t items = a.tokens * t.heads, step = (int64_t)a.blocks[second] * PER;
+    const int64_t step = (int64_t)a.blocks[second] * PER;
     HeadUnit<T, INTER, E> u[NU];
     float w[NU][2][E], dw[NU][2][E] = {};
 #pragma unroll
@@ -187,22 +204,40 @@ __global__ void __launch_bounds__(kHeadThreads) head_norm_bwd_kernel(const HeadA
         u[k].init(a, k * G + lane);
         if (t.w) u[k].load(t.w, 0, w[k]);
     }
-    for (int64_t base = (int64_t)block * PER; base < items; base += step) {
+    HeadPacked<T, E> px[NU][2], pg[NU][2];
+    const float *row = a.table;
+    int64_t out = 0;
+    auto fetch = [&](int64_t base) {  // whether this group has a head there
         const HeadPlace p = head_place(base, group, t.heads, a.inv[second]);
-        const int64_t token = p.token;
-        const int head = p.head;
-        if (token >= a.tokens) break;  // a whole group, at its last item
-        float x[NU][2][E], g[NU][2][E], cs[NU][2][E];
+        if (p.token >= a.tokens) return false;
 #pragma unroll
         for (int k = 0; k < NU; ++k) {
-            u[k].load(t.x, token * t.x_token + head * t.x_head, x[k]);
-            u[k].load(t.dy, token * t.dy_token + head * t.dy_head, g[k]);
+            u[k].load(t.x, p.token * t.x_token + p.head * t.x_head, px[k]);
+            u[k].load(t.dy, p.token * t.dy_token + p.head * t.dy_head, pg[k]);
         }
+        if (a.R) row = head_angles(a, p.token);
+        out = p.token * t.out_token + p.head * t.out_head;
+        return true;
+    };
+    int64_t base = (int64_t)block * PER;
+    for (bool has = fetch(base); has;) {  // the same for all of a group's lanes
+        float x[NU][2][E], g[NU][2][E], cs[NU][2][E];
         if (a.R) {
-            const float *row = head_angles(a, token);
 #pragma unroll
             for (int k = 0; k < NU; ++k) u[k].angles(row, a.R, cs[k]);
         }
+#pragma unroll
+        for (int k = 0; k < NU; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    x[k][i][e] = u[k].has[i] ? px[k][i].at(e) : 0.f;
+                    g[k][i][e] = u[k].has[i] ? pg[k][i].at(e) : 0.f;
+                }
+        const int64_t to = out;
+        base += step;
+        has = fetch(base);
         float ss = 0.f, sg = 0.f;
 #pragma unroll
         for (int k = 0; k < NU; ++k) {
@@ -228,7 +263,7 @@ __global__ void __launch_bounds__(kHeadThreads) head_norm_bwd_kernel(const HeadA
                     const float gw = t.w ? g[k][i][e] * w[k][i][e] : g[k][i][e];
                     x[k][i][e] = r * (gw - x[k][i][e] * c);
                 }
-            u[k].store(t.out, token * t.out_token + head * t.out_head, x[k]);
+            u[k].store(t.out, to, x[k]);
         }
     }
     if (!t.w) return;
@@ -267,9 +302,12 @@ __global__ void __launch_bounds__(1024) head_norm_sum_kernel(const float *part, 
     const int n = second ? n_k : n_q, col = threadIdx.x & 31, row = threadIdx.x >> 5;
     const int d = blockIdx.x * 32 + col;
     float v = 0.f;
-    if (d < D) {
-#pragma unroll 16
-        for (int i = row; i < n; i += 32) v += p[(int64_t)i * D + d];
+    for (int i = row; d < D && i < n; i += 32 * 16) {  // 16 in flight
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = i + 32 * j < n ? p[(int64_t)(i + 32 * j) * D + d] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v += x[j];
     }
     s[row][col] = v;
     __syncthreads();

@@ -236,7 +236,7 @@ HeadArgs head_args(const katsu_qk_norm_rotary &d, const float *table, const int3
 
 // Blocks of the gradient's launch: of q, of k; each block's sums of dw are a part.
 void head_blocks(const katsu_qk_norm_rotary &d, int (&blocks)[2]) {
-    const int64_t most = 4 * kCUs, n = (int64_t)(d.heads + d.k_heads);
+    const int64_t most = 5 * kCUs, n = (int64_t)(d.heads + d.k_heads);
     const int64_t heads[2] = {(int64_t)d.heads, (int64_t)d.k_heads};
     for (int i = 0; i < 2; ++i) {
         const int64_t items = heads[i] * (int64_t)d.tokens;
