@@ -59,7 +59,7 @@ EmbedArgs embed_args(const katsu_embedding &d, const int32_t *ids) {
 }
 
 // The gradient's shape.
-enum EmbedPath { kEmbedFew, kEmbedSlabs, kEmbedPasses };
+enum EmbedPath { kByRows, kBySlabs, kByPasses };
 struct EmbedPlan {
     EmbedPath path;
     int bits, passes, blocks, per, tile;
@@ -79,9 +79,9 @@ EmbedPlan embed_plan(const katsu_embedding &d) {
     // Slabs: two a CU.  Their blocks read all ids twice, so with more tokens the passes.
     p.per = (int)std::min<int64_t>(cdiv(V, kCUs * 32) * 32, kEmbedSlab);
     const int64_t slabs = cdiv(V, p.per);
-    p.path = T <= 256 ? kEmbedFew : T <= kEmbedSlabTokens && slabs * T <= 1 << 25 ? kEmbedSlabs : kEmbedPasses;
-    if (p.path == kEmbedFew) return p;
-    if (p.path == kEmbedSlabs) {
+    p.path = T <= kEmbedFew ? kByRows : T <= kEmbedSlabTokens && slabs * T <= 1 << 25 ? kBySlabs : kByPasses;
+    if (p.path == kByRows) return p;
+    if (p.path == kBySlabs) {
         p.blocks = (int)slabs;
         p.bits = bits(p.per - 1);
     } else {
@@ -96,7 +96,7 @@ EmbedPlan embed_plan(const katsu_embedding &d) {
     p.part = p.tiles > 1 ? up16((size_t)p.tiles * 2 * d.cols * 4) : 0;
     p.there = up16((size_t)cdiv(V, 32) * 4);
     p.bytes = 2 * p.keys + p.part + p.there;
-    if (p.path == kEmbedPasses) {
+    if (p.path == kByPasses) {
         p.per = (int)(cdiv(T, 256 * 1024) * 1024);
         p.per = std::max(p.per, 4096);
         p.blocks = (int)cdiv(T, p.per);
@@ -108,9 +108,9 @@ EmbedPlan embed_plan(const katsu_embedding &d) {
 template <typename T>
 int embed_grad(const katsu_embedding &d, const EmbedArgs &a, char *ws, hipStream_t st) {
     const EmbedPlan p = embed_plan(d);
-    if (p.path == kEmbedFew) {
-        embed_grad_few_kernel<T><<<(unsigned)std::min<int64_t>(cdiv(a.vocab, 4), 1 << 20), 256, 0,
-                                   st>>>(a);
+    if (p.path == kByRows) {
+        const int rows = (int)std::min<int64_t>(std::max<int64_t>(a.vocab / 8192, 1), 1 << 12);
+        embed_grad_few_kernel<T><<<(unsigned)cdiv(a.vocab, 4 * rows), 256, 0, st>>>(a, rows);
         return status_of(hipGetLastError());
     }
     auto take = [&](size_t n) {
@@ -129,7 +129,7 @@ int embed_grad(const katsu_embedding &d, const EmbedArgs &a, char *ws, hipStream
     s.key = (int32_t *)take(p.keys);
     s.at = (int32_t *)take(p.keys);
     s.there = (uint32_t *)take(p.there);
-    if (p.path == kEmbedSlabs) {
+    if (p.path == kBySlabs) {
         s.per = p.per;
         embed_slab_kernel<<<(unsigned)p.blocks, 1024, 0, st>>>(s);
     } else {
@@ -157,7 +157,7 @@ int embed_grad(const katsu_embedding &d, const EmbedArgs &a, char *ws, hipStream
     t.tiles = p.tiles;
     t.chunks = (int)cdiv(a.cols, 64 * Piece<T>::E);
     t.tile_blocks = cdiv(t.tiles * t.chunks, 4);
-    t.zero_blocks = t.there ? cdiv(a.vocab, 32) : 0;
+    t.zero_blocks = t.there ? cdiv(a.vocab, 8 * 4) : 0;  // eight rows a wave
     embed_tile_kernel<T><<<grid_of(t.tile_blocks + t.zero_blocks), 256, 0, st>>>(t);
     if (t.tiles > 1)
         embed_join_kernel<T><<<dim3((unsigned)t.tiles, (unsigned)cdiv(a.cols, 256)), 256, 0,
