@@ -256,10 +256,10 @@ __device__ __forceinline__ void distill_grad(const DistillArgs &a, int64_t row, 
     __syncthreads();  // dz may be z: all of the teacher's logits are read
     for (int64_t i = c0 + threadIdx.x * E; i < c1; i += NT * E) {
         float x[E];
-        load_piece(z, i, c1, x);
+        load_whole(z, i, c1, x);
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] = distill_exp(x[e] - m, a.scale2) * by;
-        store_piece(dz, i, c1, x);
+        store_whole(dz, i, c1, x);
     }
     __syncthreads();  // and all others written
     fix.write(d, dz);
@@ -271,7 +271,7 @@ __device__ __forceinline__ void distill_zero(const DistillArgs &a, int64_t row, 
     constexpr int E = Piece<T>::E;
     const float x[E] = {};
     for (int64_t i = c0 + threadIdx.x * E; i < c1; i += NT * E)
-        store_piece((T *)a.dz + row * a.dz_row, i, c1, x);
+        store_whole((T *)a.dz + row * a.dz_row, i, c1, x);
 }
 
 // Loss, gradient or both of whole rows: a block a row.
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(NT) distill_step_kernel(const DistillArgs a) {
         float y[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] = distill_exp(x[k].at(e) - m, a.scale2) * by;
-        store_piece(dz, i, V, y);
+        store_whole(dz, i, V, y);
     }
     __syncthreads();  // and all others written
     fix.write(d, dz);

@@ -37,30 +37,24 @@ __global__ void __launch_bounds__(256) embed_kernel(const EmbedArgs a) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int64_t i = c0 + (k * 64 + lane) * E;
-            if (has && i < a.cols) load_piece(in, i, a.cols, x[k]);
+            if (has && i < a.cols) load_whole(in, i, a.cols, x[k]);
         }
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int64_t i = c0 + (k * 64 + lane) * E;
 #pragma unroll
             for (int e = 0; e < E; ++e) x[k][e] = has ? x[k][e] * a.scale : 0.f;
-            if (i < a.cols) store_piece(out, i, a.cols, x[k]);
+            if (i < a.cols) store_whole(out, i, a.cols, x[k]);
         }
     }
 }
 
-// Whole pieces and the rest apart: in one loop the compiler stores what both have in common first, and
-// a piece of bfloat16 in three parts (130000 rows of 2 KB: 66 us, XX so).
 template <typename T>
 __device__ __forceinline__ void embed_zero_row(const EmbedArgs &a, int64_t v, int lane) {
     constexpr int E = Piece<T>::E;
-    T *out = (T *)a.out + v * a.out_row;
-    const int64_t whole = a.cols / E * E;
-    for (int64_t i = (int64_t)lane * E; i < whole; i += 64 * E) {
-        const lm_u4 zero = {0, 0, 0, 0};
-        __builtin_memcpy(out + i, &zero, 16);
-    }
-    for (int64_t i = whole + lane; i < a.cols; i += 64) out[i] = (T)0.f;
+    const float x[E] = {};
+    for (int64_t i = (int64_t)lane * E; i < a.cols; i += 64 * E)
+        store_whole((T *)a.out + v * a.out_row, i, a.cols, x);
 }
 // dtable[v] = (dtable[v] +) scale x, of a lane's piece.
 template <typename T>
@@ -68,10 +62,10 @@ __device__ __forceinline__ void embed_write(const EmbedArgs &a, int64_t v, int64
     constexpr int E = Piece<T>::E;
     T *out = (T *)a.out + v * a.out_row;
     float old[E] = {};
-    if (a.add) load_piece(out, i, a.cols, old);
+    if (a.add) load_whole(out, i, a.cols, old);
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = x[e] * a.scale + old[e];
-    store_piece(out, i, a.cols, x);
+    store_whole(out, i, a.cols, x);
 }
 
 // The gradient of up to kEmbedFew tokens: a wave a row of the table, which it compares with all
@@ -410,7 +404,7 @@ __global__ void __launch_bounds__(256) embed_tile_kernel(const EmbedTiles t) {
         } else {
             float *p = t.part + (2 * j + (before ? 0 : 1)) * a.cols;
 #pragma unroll
-            for (int e = 0; e < E; e += 4) store_piece<float>(p, i + e, a.cols, x + e);
+            for (int e = 0; e < E; e += 4) store_whole<float>(p, i + e, a.cols, x + e);
         }
     };
     for (int64_t b = t0; b < t1; b += 64) {
@@ -468,11 +462,11 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedTiles t) {
     }
     float x[4] = {};
     if (i < a.cols) {
-        if (wave == 0) load_piece<float>(t.part + (2 * j + 1) * a.cols, i, a.cols, x);
+        if (wave == 0) load_whole<float>(t.part + (2 * j + 1) * a.cols, i, a.cols, x);
 #pragma unroll 8
         for (int64_t k = wave; k < n; k += 4) {
             float y[4];
-            load_piece<float>(t.part + 2 * (j + 1 + k) * a.cols, i, a.cols, y);
+            load_whole<float>(t.part + 2 * (j + 1 + k) * a.cols, i, a.cols, y);
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] += y[e];
         }

@@ -8,6 +8,8 @@
 namespace katsu {
 
 typedef uint32_t lm_u4 __attribute__((ext_vector_type(4)));
+typedef float lm_f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 lm_b2 __attribute__((ext_vector_type(2)));
 
 // E neighbouring values as float32.
 template <typename T>
@@ -29,7 +31,25 @@ __device__ __forceinline__ void load_piece(const T *p, int64_t i, int64_t n, flo
 #pragma unroll
     for (int j = 0; j < E; ++j) x[j] = (float)e[j];
 }
-// The same in four registers, for pieces that wait: an array of bfloat16 takes one for each value.
+template <typename T>
+__device__ __forceinline__ void store_piece(T *p, int64_t i, int64_t n, const float *x) {
+    constexpr int E = Piece<T>::E;
+    T e[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) e[j] = (T)x[j];
+    if (i + E <= n) {
+        __builtin_memcpy(p + i, e, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (i + j < n) p[i + j] = e[j];
+    }
+}
+// The same as it is in memory, in four registers.  From an array of values, as above, the compiler
+// makes three accesses, one of which the one at a row's end, value by value, shares, and holds a
+// register for each value of bfloat16.  Whole accesses are faster where the memory is all
+// (130000 rows of 2 KB set to zero: 66 and 38 us; 16384 rows of 8 KB looked up: 47 and 35), not in
+// the norms' gradient, which has no registers for what is then loaded early (114 and 136 us).
 template <typename T>
 struct RawPiece {
     static constexpr int E = Piece<T>::E;
@@ -45,26 +65,48 @@ struct RawPiece {
             __builtin_memcpy(&v, e, 16);
         }
     }
+    __device__ __forceinline__ void store(T *p, int64_t i, int64_t n) const {
+        if (i + E <= n) {
+            __builtin_memcpy(p + i, &v, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (i + j < n) p[i + j] = (T)at(j);
+        }
+    }
     // Its values are converted again after this: held as float32 they take twice the registers.
     __device__ __forceinline__ void packed() { asm volatile("" : "+v"(v)); }
     __device__ __forceinline__ float at(int j) const {
         const uint32_t u = v[j * (int)sizeof(T) / 4];
         return __builtin_bit_cast(float, sizeof(T) == 4 ? u : j & 1 ? u & 0xffff0000u : u << 16);
     }
+    __device__ __forceinline__ void set(const float *x) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            uint32_t u;
+            if constexpr (sizeof(T) == 4) {
+                const float f = x[k];
+                u = __builtin_bit_cast(uint32_t, f);
+            } else {
+                u = __builtin_bit_cast(
+                    uint32_t, __builtin_convertvector(lm_f2{x[2 * k], x[2 * k + 1]}, lm_b2));
+            }
+            v[k] = u;
+        }
+    }
 };
 template <typename T>
-__device__ __forceinline__ void store_piece(T *p, int64_t i, int64_t n, const float *x) {
-    constexpr int E = Piece<T>::E;
-    T e[E];
+__device__ __forceinline__ void load_whole(const T *p, int64_t i, int64_t n, float *x) {
+    RawPiece<T> r;
+    r.load(p, i, n);
 #pragma unroll
-    for (int j = 0; j < E; ++j) e[j] = (T)x[j];
-    if (i + E <= n) {
-        __builtin_memcpy(p + i, e, 16);
-    } else {
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-            if (i + j < n) p[i + j] = e[j];
-    }
+    for (int j = 0; j < Piece<T>::E; ++j) x[j] = r.at(j);
+}
+template <typename T>
+__device__ __forceinline__ void store_whole(T *p, int64_t i, int64_t n, const float *x) {
+    RawPiece<T> r;
+    r.set(x);
+    r.store(p, i, n);
 }
 
 // N neighbouring values, of any alignment.
