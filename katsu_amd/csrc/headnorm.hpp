@@ -112,10 +112,13 @@ struct HeadUnit {
     }
 };
 
-__device__ __forceinline__ const float *head_angles(const HeadArgs &a, int64_t token) {
-    int64_t pos = a.positions ? a.positions[token] : token;
-    pos = pos < 0 ? 0 : pos < a.length ? pos : a.length - 1;  // stays inside the table
-    return a.table + pos * a.R;
+// A token's position as it is given; 0 beyond the last token.
+__device__ __forceinline__ int64_t head_position(const HeadArgs &a, int64_t token) {
+    return !a.positions ? token : token < a.tokens ? a.positions[token] : 0;
+}
+// Where its angles begin: inside the table.
+__device__ __forceinline__ int64_t head_row(const HeadArgs &a, int64_t pos) {
+    return (pos < 0 ? 0 : pos < a.length ? pos : a.length - 1) * a.R;
 }
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(256) head_norm_kernel(const HeadArgs a) {
         u[k].load(t.x, in, x[k]);
     }
     if (a.R) {
-        const float *row = head_angles(a, token);
+        const float *row = a.table + head_row(a, head_position(a, token));
 #pragma unroll
         for (int k = 0; k < NU; ++k) u[k].angles(row, a.R, cs[k]);
     }
@@ -205,27 +208,34 @@ __global__ void __launch_bounds__(kHeadThreads) head_norm_bwd_kernel(const HeadA
         if (t.w) u[k].load(t.w, 0, w[k]);
     }
     HeadPacked<T, E> px[NU][2], pg[NU][2];
-    const float *row = a.table;
+    float pcs[NU][2][E];
     int64_t out = 0;
+    // A head's angles lie where its token's position says, which is read a head earlier still.
+    auto place = [&](int64_t base) { return head_place(base, group, t.heads, a.inv[second]); };
+    int64_t pos = head_position(a, place((int64_t)block * PER).token);
     auto fetch = [&](int64_t base) {  // whether this group has a head there
-        const HeadPlace p = head_place(base, group, t.heads, a.inv[second]);
+        const HeadPlace p = place(base);
         if (p.token >= a.tokens) return false;
+        const float *row = a.table + head_row(a, pos);
 #pragma unroll
         for (int k = 0; k < NU; ++k) {
             u[k].load(t.x, p.token * t.x_token + p.head * t.x_head, px[k]);
             u[k].load(t.dy, p.token * t.dy_token + p.head * t.dy_head, pg[k]);
+            if (a.R) u[k].angles(row, a.R, pcs[k]);
         }
-        if (a.R) row = head_angles(a, p.token);
+        pos = head_position(a, place(base + step).token);
         out = p.token * t.out_token + p.head * t.out_head;
         return true;
     };
     int64_t base = (int64_t)block * PER;
     for (bool has = fetch(base); has;) {  // the same for all of a group's lanes
         float x[NU][2][E], g[NU][2][E], cs[NU][2][E];
-        if (a.R) {
 #pragma unroll
-            for (int k = 0; k < NU; ++k) u[k].angles(row, a.R, cs[k]);
-        }
+        for (int k = 0; k < NU; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e) cs[k][i][e] = pcs[k][i][e];
 #pragma unroll
         for (int k = 0; k < NU; ++k)
 #pragma unroll
