@@ -16,7 +16,7 @@ struct EmbedArgs {
     void *out;        // out or dtable
     int64_t tokens, vocab, cols, in_row, out_row;
     float scale;
-    int chunks, add;  // pieces of a row, 64 * kEmbedPieces of 16 bytes; whether dtable is added to
+    int add;          // whether dtable is added to
 };
 
 constexpr int kEmbedPieces = 4;
@@ -26,9 +26,9 @@ template <typename T>
 __global__ void __launch_bounds__(256) embed_kernel(const EmbedArgs a) {
     constexpr int E = Piece<T>::E, N = kEmbedPieces;
     const int lane = threadIdx.x & 63;
-    const int64_t step = (int64_t)gridDim.x * 4, items = a.tokens * a.chunks;
-    for (int64_t it = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += step) {
-        const int64_t t = it / a.chunks, c0 = (it - t * a.chunks) * (64 * N * E);
+    const int64_t c0 = (int64_t)blockIdx.y * (64 * N * E);
+    for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < a.tokens;
+         t += (int64_t)gridDim.x * 4) {
         const int64_t id = a.ids[t];
         const T *in = (const T *)a.in + id * a.in_row;
         T *out = (T *)a.out + t * a.out_row;
@@ -140,7 +140,7 @@ struct EmbedTiles {
     int64_t tile_blocks, zero_blocks;  // blocks that add tokens; that set rows to zero
 };
 
-constexpr int kEmbedSlab = 512, kEmbedSlabTokens = 1 << 19, kEmbedBits = 10;
+constexpr int kEmbedSlab = 512, kEmbedSlabTokens = 1 << 16, kEmbedBits = 10;
 constexpr int kEmbedAhead = 16;  // rows in flight
 
 __device__ __forceinline__ int embed_key(const int32_t *ids, int64_t t, int64_t vocab) {
@@ -205,7 +205,7 @@ __device__ __forceinline__ int block_scan(int v, int *part) {
 __global__ void __launch_bounds__(1024) embed_slab_kernel(const EmbedSort s) {
     __shared__ int count[16][kEmbedSlab], part[16], below[16], end;
     constexpr int U = 8;  // rounds of 64 tokens in a batch, of which a wave has 64 at most
-    static_assert(kEmbedSlabTokens == 16 * 64 * 64 * U, "a bit a batch");
+    static_assert(kEmbedSlabTokens <= 16 * 64 * 64 * U, "a bit a batch");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = (int)s.tokens;
     const int per = (n + 1023) / 1024 * 64;  // tokens of a wave
     const int t0 = min(wave * per, n), t1 = min(t0 + per, n);
@@ -360,11 +360,15 @@ __global__ void __launch_bounds__(1024) embed_scatter_kernel(const EmbedSort s) 
         if (!live) continue;
         s.key[to] = k;
         s.at[to] = at;
-        if (!s.key_in && k < s.vocab) {
-            const uint32_t bit = 1u << (k & 31);
-            if (!(s.there[k >> 5] & bit)) atomicOr(s.there + (k >> 5), bit);
-        }
     }
+}
+// Which rows have a token: the first of each run of the sorted ids says so (a bit set for every
+// token took 80 us of 262144 tokens' 165).
+__global__ void __launch_bounds__(256) embed_there_kernel(const EmbedSort s) {
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t >= s.tokens) return;
+    const int k = s.key_in[t], before = t > 0 ? s.key_in[t - 1] : -1;
+    if (k < s.vocab && k != before) atomicOr(s.there + (k >> 5), 1u << (k & 31));
 }
 
 // A wave a tile's chunk of 64 pieces, kEmbedAhead tokens' rows in flight.

@@ -53,8 +53,6 @@ EmbedArgs embed_args(const katsu_embedding &d, const int32_t *ids) {
     a.vocab = (int64_t)d.vocab;
     a.cols = (int64_t)d.cols;
     a.scale = d.scale;
-    const int64_t wide = 64 * kEmbedPieces * (d.dtype == KATSU_F32 ? 4 : 8);
-    a.chunks = (int)cdiv(a.cols, wide);
     return a;
 }
 
@@ -76,19 +74,27 @@ EmbedPlan embed_plan(const katsu_embedding &d) {
         while (n >> b) ++b;
         return b;
     };
-    // Slabs: two a CU.  Their blocks read all ids twice, so with more tokens the passes.
+    // By rows: 256 tokens 14 us, 18 by slabs; 500 tokens 19 and 18 (32000 x 256 float32).  Slabs: one a
+    // CU, more where a block's LDS does not hold its rows' counts.  Their blocks all read all
+    // ids, so with more tokens or rows the passes: 65536 tokens 54 us, 57 in passes, 131072 tokens 90
+    // and 73 (32000 x 256 bfloat16); 20000 tokens, 10^6 rows 112 and 96; where one pass is enough,
+    // 32768 tokens 36 and 36, 65536 tokens 55 and 40 (1001 rows).
     p.per = (int)std::min<int64_t>(cdiv(V, kCUs * 32) * 32, kEmbedSlab);
     const int64_t slabs = cdiv(V, p.per);
-    p.path = T <= kEmbedFew ? kByRows : T <= kEmbedSlabTokens && slabs * T <= 1 << 25 ? kBySlabs : kByPasses;
+    p.passes = (int)cdiv(bits(V), kEmbedBits);
+    const bool few = T <= (p.passes == 1 ? kEmbedSlabTokens / 2 : kEmbedSlabTokens) &&
+                     T * std::max<int64_t>(slabs, kCUs) <= kEmbedSlabTokens * kCUs;
+    p.path = T <= kEmbedFew ? kByRows : few ? kBySlabs : kByPasses;
     if (p.path == kByRows) return p;
     if (p.path == kBySlabs) {
         p.blocks = (int)slabs;
         p.bits = bits(p.per - 1);
     } else {
-        p.passes = (int)cdiv(bits(V), kEmbedBits);
         p.bits = (int)cdiv(bits(V), p.passes);
     }
     const int chunks = (int)cdiv((int64_t)d.cols, 64 * (d.dtype == KATSU_F32 ? 4 : 8));
+    // Tiles of 8 tokens, more where that makes enough waves: longer tiles leave fewer parts (16384
+    // tokens, 32000 x 2048 bfloat16: 70 us in tiles of 64, 66 of 32, 77 of 16).
     p.tile = 8;
     while (cdiv(T, p.tile) * chunks > 2048 && p.tile < 1024) p.tile *= 2;
     p.tiles = cdiv(T, p.tile);
@@ -149,6 +155,7 @@ int embed_grad(const katsu_embedding &d, const EmbedArgs &a, char *ws, hipStream
             s.key_in = s.key;
             s.at_in = s.at;
         }
+        if (!a.add) embed_there_kernel<<<(unsigned)cdiv(s.tokens, 256), 256, 0, st>>>(s);
     }
     if (!a.add) t.there = s.there;
     t.key = s.key;
@@ -311,8 +318,9 @@ int embedding(const katsu_embedding &d, const int32_t *ids, const void *table, v
     a.out = out;
     a.in_row = d.table_stride;
     a.out_row = d.out_stride;
-    const unsigned blocks =
-        (unsigned)std::min<int64_t>(cdiv(a.tokens * a.chunks, 4), 1 << 20);
+    const int64_t wide = 64 * kEmbedPieces * (d.dtype == KATSU_F32 ? 4 : 8);
+    const dim3 blocks((unsigned)std::min<int64_t>(cdiv(a.tokens, 4), 1 << 20),
+                      (unsigned)cdiv(a.cols, wide));
     if (d.dtype == KATSU_F32)
         embed_kernel<float><<<blocks, 256, 0, st>>>(a);
     else

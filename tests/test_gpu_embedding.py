@@ -93,7 +93,8 @@ def test_lookup_strides(dev, dt):
                                                (129, 1001, 256), (255, 70, 1030),
                                                (1000, 5000, 64), (1500, 31, 100),
                                                (5000, 3000, 72), (20000, 700, 33),
-                                               (9000, 100000, 8)])
+                                               (9000, 100000, 8), (150000, 100000, 8),
+                                               (6000, 3000000, 3), (530000, 700, 5)])
 def test_gradient(dev, dt, kind, tokens, vocab, cols):
     print(dt, kind, tokens, vocab, cols, flush=True)
     g = torch.Generator().manual_seed(5)
@@ -145,14 +146,14 @@ def test_padding_holds_anything(dev, tokens):
     assert torch.equal(got[keep.to(dev)], clean[keep.to(dev)])
 
 
-@pytest.mark.parametrize("tokens", [200, 3000, 30000])
+@pytest.mark.parametrize("tokens", [200, 3000, 30000, 530000])
 def test_same_bits(dev, tokens):
     """Calls, replays of a graph with other tokens between, another stream, an own workspace."""
     g = torch.Generator().manual_seed(10)
-    dout = torch.randn(tokens, 136, generator=g).to(dev)
+    dout = torch.randn(tokens, 36, generator=g).to(dev)
     a, b = (_ids(tokens, 2000, s).to(dev) for s in (11, 12))
     want = [ops.embedding_backward(dout, i, 2000, 0.5) for i in (a, b)]
-    ws = torch.empty(ops.embedding_workspace_bytes(tokens, 2000, 136, torch.float32),
+    ws = torch.empty(ops.embedding_workspace_bytes(tokens, 2000, 36, torch.float32),
                      dtype=torch.uint8, device=dev)
     ids = a.clone()
     side = torch.cuda.Stream()
