@@ -97,19 +97,24 @@ class Embedding(ctypes.Structure):
                 [("scale", ctypes.c_float)])
 
 
+def _strides(*names):
+    """Two int64 fields for each of the header's int64_t name[2]: ctypes takes 0.3 us to convert
+    an array."""
+    return [(f"{n}{i}", ctypes.c_int64) for n in names for i in range(2)]
+
+
 class QkNormRotary(ctypes.Structure):
     """katsu_qk_norm_rotary: the shapes and strides of a call on query and key heads."""
     _fields_ = ([(f, ctypes.c_int32) for f in ("dtype", "interleaved")] +
                 [(f, ctypes.c_uint64) for f in ("tokens", "heads", "k_heads", "head_dim",
                                                 "rotary_dim", "length")] +
-                [(f, ctypes.c_int64 * 2) for f in ("q_stride", "k_stride", "q_out_stride",
-                                                   "k_out_stride")] +
+                _strides("q_stride", "k_stride", "q_out_stride", "k_out_stride") +
                 [("eps", ctypes.c_float)])
 
 
 class QkNormRotaryGrads(ctypes.Structure):
     """katsu_qk_norm_rotary_grads: the strides of a backward call's incoming gradients."""
-    _fields_ = [(f, ctypes.c_int64 * 2) for f in ("dq_stride", "dk_stride")]
+    _fields_ = _strides("dq_stride", "dk_stride")
 
 
 class Distillation(ctypes.Structure):

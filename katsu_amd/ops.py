@@ -502,6 +502,10 @@ def clip_grad_norm(grads, max_norm, out=None, workspace=None):
 
 # ---- the ends of a language model, and the heads before its attention ----
 
+def _at(t):
+    return 0 if t is None else t.data_ptr()
+
+
 def _operands(first, *ts):
     """float32 or bfloat16, all of the first one's type, on the current device: the launches go to its
     current stream.  (Type and device number are compared: a device object takes 0.1 us to make.)"""
@@ -521,7 +525,7 @@ def _scratch(workspace, first, size_fn, d):
     belongs to the stream, or to the graph that is captured."""
     if workspace is None:
         nbytes = ctypes.c_size_t(0)
-        check(size_fn(ctypes.byref(d), ctypes.byref(nbytes)), "workspace")
+        check(size_fn(d, nbytes), "workspace")
         if nbytes.value == 0:
             return None, 0, 0
         workspace = first.new_empty(nbytes.value, dtype=torch.uint8)
@@ -553,7 +557,7 @@ def embedding(ids, table, scale=1.0, out=None):
     if out is None:
         out = table.new_empty((ids.numel(), table.shape[-1]))
     d = _embedding(table, out, ids, scale, 0.0)
-    check(lib().katsu_hip_embedding_dev(ctypes.byref(d), _p(ids), _p(table), _p(out), _stream()),
+    check(lib().katsu_hip_embedding_dev(d, _at(ids), _at(table), _at(out), _stream()),
           "embedding")
     return out
 
@@ -571,7 +575,7 @@ def embedding_backward(dout, ids, vocab, scale=1.0, out=None, beta=0.0, workspac
         raise ValueError("out must have a row for each of the vocabulary")
     d = _embedding(out, dout, ids, scale, beta)
     keep, *ws = _scratch(workspace, dout, lib().katsu_hip_embedding_bwd_workspace, d)
-    check(lib().katsu_hip_embedding_bwd_dev(ctypes.byref(d), _p(dout), _p(ids), _p(out), *ws,
+    check(lib().katsu_hip_embedding_bwd_dev(d, _at(dout), _at(ids), _at(out), *ws,
                                             _stream()), "embedding_backward")
     return out
 
@@ -587,20 +591,22 @@ def embedding_workspace_bytes(tokens, vocab, cols, dtype):
 
 def _qk_norm_rotary(q, k, out_q, out_k, table, positions, w_q, w_k, eps, interleaved, *more):
     kind = _operands(q, k, out_q, out_k, w_q, w_k, *more)
-    tokens, heads, dim = q.shape if q.dim() == 3 else (0, 0, 0)
-    strides = [_heads(q, "q"), (0, 0), _heads(out_q, "out_q"), (0, 0)]
-    if out_q.shape != q.shape or (k is None) != (out_k is None):
+    (q0, q1), (o0, o1) = _heads(q, "q"), _heads(out_q, "out_q")
+    k0 = k1 = p0 = p1 = k_heads = length = rot = 0
+    shape = q.shape
+    tokens, heads, dim = shape
+    if out_q.shape != shape or (k is None) != (out_k is None):
         raise ValueError("outputs must have the operands' shapes")
     if k is not None:
-        strides[1::2] = _heads(k, "k"), _heads(out_k, "out_k")
-        if out_k.shape != k.shape or k.shape[0] != tokens or k.shape[2] != dim:
+        (k0, k1), (p0, p1) = _heads(k, "k"), _heads(out_k, "out_k")
+        k_tokens, k_heads, k_dim = shape = k.shape
+        if out_k.shape != shape or k_tokens != tokens or k_dim != dim:
             raise ValueError("q and k must have the same tokens and channels, outputs their shapes")
     elif w_k is not None:
         raise ValueError("w_k goes with k")
     for w in (w_q, w_k):
         if w is not None and (w.shape != (dim,) or not w.is_contiguous()):
             raise ValueError("weights must be contiguous [channels]")
-    length = rot = 0
     if table is not None:
         if (table.dim() != 2 or table.dtype is not torch.float32 or not table.is_contiguous()
                 or table.get_device() != q.get_device() or table.shape[1] == 0):
@@ -608,9 +614,10 @@ def _qk_norm_rotary(q, k, out_q, out_k, table, positions, w_q, w_k, eps, interle
         length, rot = table.shape
     elif positions is not None:
         raise ValueError("positions go with a table")
-    _int32(positions, tokens, q.device, "positions")
-    return QkNormRotary(kind, bool(interleaved), tokens, heads, 0 if k is None else k.shape[1], dim,
-                        rot, length, *strides, eps)
+    if positions is not None:
+        _int32(positions, tokens, q.device, "positions")
+    return QkNormRotary(kind, bool(interleaved), tokens, heads, k_heads, dim, rot, length, q0, q1,
+                        k0, k1, o0, o1, p0, p1, eps)
 
 
 def qk_norm_rotary(q, k, table=None, positions=None, w_q=None, w_k=None, eps=1e-6,
@@ -623,9 +630,9 @@ def qk_norm_rotary(q, k, table=None, positions=None, w_q=None, w_k=None, eps=1e-
     if k is not None and out_k is None:
         out_k = torch.empty_like(k)
     d = _qk_norm_rotary(q, k, out_q, out_k, table, positions, w_q, w_k, eps, interleaved)
-    check(lib().katsu_hip_qk_norm_rotary_dev(ctypes.byref(d), _p(q), _p(k), _p(w_q), _p(w_k),
-                                             _p(table), _p(positions), _p(out_q), _p(out_k),
-                                             _stream()), "qk_norm_rotary")
+    check(lib().katsu_hip_qk_norm_rotary_dev(d, _at(q), _at(k), _at(w_q), _at(w_k), _at(table),
+                                             _at(positions), _at(out_q), _at(out_k), _stream()),
+          "qk_norm_rotary")
     return out_q, out_k
 
 
@@ -641,13 +648,12 @@ def qk_norm_rotary_backward(dq, dk, q, k, table=None, positions=None, w_q=None, 
     if dq.shape != q.shape or (dk is None) != (k is None) or (k is not None
                                                               and dk.shape != k.shape):
         raise ValueError("gradients must have their operands' shapes")
-    g = QkNormRotaryGrads(_heads(dq, "dq"), (0, 0) if dk is None else _heads(dk, "dk"))
+    g = QkNormRotaryGrads(*_heads(dq, "dq"), *((0, 0) if dk is None else _heads(dk, "dk")))
     dw_q, dw_k = (None if w is None else torch.empty_like(w) for w in (w_q, w_k))
     keep, *ws = _scratch(workspace, q, lib().katsu_hip_qk_norm_rotary_bwd_workspace, d)
     check(lib().katsu_hip_qk_norm_rotary_bwd_dev(
-        ctypes.byref(d), ctypes.byref(g), _p(dq), _p(dk), _p(q), _p(k), _p(w_q), _p(w_k),
-        _p(table), _p(positions), _p(out_q), _p(out_k), _p(dw_q), _p(dw_k), *ws, _stream()),
-        "qk_norm_rotary_backward")
+        d, g, _at(dq), _at(dk), _at(q), _at(k), _at(w_q), _at(w_k), _at(table), _at(positions),
+        _at(out_q), _at(out_k), _at(dw_q), _at(dw_k), *ws, _stream()), "qk_norm_rotary_backward")
     return out_q, out_k, dw_q, dw_k
 
 
@@ -689,8 +695,8 @@ def distillation(logits, ids, teacher, temperature=1.0):
     d = _distillation(logits, ids, teacher, temperature)
     loss = logits.new_empty(d.rows, dtype=torch.float32)
     stats = logits.new_empty((2, d.rows), dtype=torch.float32)
-    check(lib().katsu_hip_distillation_dev(ctypes.byref(d), _p(logits), _p(ids), _p(teacher),
-                                           _p(loss), _p(stats), _stream()), "distillation")
+    check(lib().katsu_hip_distillation_dev(d, _at(logits), _at(ids), _at(teacher), _at(loss),
+                                           _at(stats), _stream()), "distillation")
     return loss, stats
 
 
@@ -702,8 +708,8 @@ def distillation_backward(dloss, logits, ids, teacher, stats, temperature=1.0, o
     if (stats.dtype is not torch.float32 or stats.device != logits.device
             or stats.shape != (2, d.rows) or not stats.is_contiguous()):
         raise ValueError("stats must be what distillation returned")
-    check(lib().katsu_hip_distillation_bwd_dev(ctypes.byref(d), _p(dloss), _p(logits), _p(ids),
-                                               _p(teacher), _p(stats), _p(out), _stream()),
+    check(lib().katsu_hip_distillation_bwd_dev(d, _at(dloss), _at(logits), _at(ids), _at(teacher),
+                                               _at(stats), _at(out), _stream()),
           "distillation_backward")
     return out
 
@@ -715,7 +721,7 @@ def distillation_step(logits, ids, teacher, dloss, temperature=1.0, out=None):
     out = torch.empty_like(logits) if out is None else out
     d = _distillation(logits, ids, teacher, temperature, out, dloss)
     loss = logits.new_empty(d.rows, dtype=torch.float32)
-    check(lib().katsu_hip_distillation_step_dev(ctypes.byref(d), _p(logits), _p(ids), _p(teacher),
-                                                _p(dloss), _p(loss), _p(out), _stream()),
+    check(lib().katsu_hip_distillation_step_dev(d, _at(logits), _at(ids), _at(teacher), _at(dloss),
+                                                _at(loss), _at(out), _stream()),
           "distillation_step")
     return loss, out

@@ -66,10 +66,13 @@ def _heads(**kw):
     d = dict(dtype=_abi.F32, interleaved=0, tokens=2, heads=2, k_heads=0, head_dim=8, rotary_dim=8,
              length=4, q_stride=(16, 8), q_out_stride=(16, 8), k_stride=(8, 8),
              k_out_stride=(8, 8), eps=1e-6)
-    return ctypes.byref(_abi.QkNormRotary(**{**d, **kw}))
+    flat = {}
+    for name, v in {**d, **kw}.items():
+        flat.update({name + "0": v[0], name + "1": v[1]} if isinstance(v, tuple) else {name: v})
+    return ctypes.byref(_abi.QkNormRotary(**flat))
 
 
-GRADS = ctypes.byref(_abi.QkNormRotaryGrads((16, 8), (8, 8)))
+GRADS = ctypes.byref(_abi.QkNormRotaryGrads(16, 8, 8, 8))
 
 
 @pytest.mark.parametrize("kw", [
@@ -107,8 +110,8 @@ def test_heads_pointers():
     for name in ("dq", "dk", "q", "k", "table", "dx_q", "dx_k", "dw_q", "dw_k"):
         assert bwd(**{name: None}) == _abi.E_INVALID, name
     assert bwd(grads=None) == _abi.E_INVALID
-    assert bwd(grads=ctypes.byref(_abi.QkNormRotaryGrads((32, 8), (8, 8)))) == _abi.E_INVALID
-    assert bwd(grads=ctypes.byref(_abi.QkNormRotaryGrads((-16, 8), (8, 8)))) == _abi.E_INVALID
+    assert bwd(grads=ctypes.byref(_abi.QkNormRotaryGrads(32, 8, 8, 8))) == _abi.E_INVALID
+    assert bwd(grads=ctypes.byref(_abi.QkNormRotaryGrads(-16, 8, 8, 8))) == _abi.E_INVALID
     n = SZ(0)
     assert L.katsu_hip_qk_norm_rotary_bwd_workspace(_heads(k_heads=1),
                                                     ctypes.byref(n)) == _abi.OK
