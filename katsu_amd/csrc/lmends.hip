@@ -273,32 +273,45 @@ DistillArgs distill_args(const katsu_distillation &d, const void *logits, const 
     a.scale2 = (float)(1.4426950408889634 / (double)d.temperature);
     return a;
 }
-// A block a row: of 16 waves where there are few rows and long ones (250 x 130000 float32: 31 us, 40
-// in blocks of 4), else of 4 (1000 x 32000 bfloat16: 16 us, 32 in blocks of 16).  Rows that are
-// read twice, for the gradient as well, fill the card with fewer (400 x 100000 float32: 115, 128).
+// A block a row.  16 waves where there are few rows and long ones (250 x 130000 float32: 31 us, 40
+// with 4); else 4 (1000 x 32000 bfloat16: 16 us, 32 with 16), or 2 for short rows, whose time is
+// the block's joins (8000 x 1000: 16 us, 22 with 4; 8000 x 16000 54 and 57; 4096 x 32000 54 and
+// 52).  Rows that are read twice, for the gradient as well, fill the card with fewer (400 x
+// 100000 float32: 115 us with 16 waves, 128 with 4).
+template <typename T, int NT, bool GRAD>
+int launch_loss(const DistillArgs &a, hipStream_t st) {
+    distill_kernel<T, NT, true, GRAD><<<grid_of(a.rows), NT, 0, st>>>(a);
+    return status_of(hipGetLastError());
+}
 template <typename T, bool GRAD>
 int launch_loss(const DistillArgs &a, hipStream_t st) {
     if (GRAD ? a.rows < 4 * kCUs : a.rows < kCUs && a.vocab > 8192)
-        distill_kernel<T, 1024, true, GRAD><<<grid_of(a.rows), 1024, 0, st>>>(a);
-    else
-        distill_kernel<T, 256, true, GRAD><<<grid_of(a.rows), 256, 0, st>>>(a);
-    return status_of(hipGetLastError());
+        return launch_loss<T, 1024, GRAD>(a, st);
+    if constexpr (!GRAD)
+        if (a.vocab <= 16384) return launch_loss<T, 128, GRAD>(a, st);
+    return launch_loss<T, 256, GRAD>(a, st);
 }
-// Loss and gradient with the rows in registers: threads of a row, and its pieces a thread.
+// Loss and gradient with the rows in registers: threads of a row, and its pieces a thread.  Two
+// waves up to 512 pieces (8000 x 3000 bfloat16: 36 us, 40 with four; 8000 x 8000 59 and 54), then
+// four as long as 16 pieces a thread hold the row (8192 x 32000 bfloat16: 201 us, 226 with
+// eight waves, 337 with 16).
 template <typename T, class F>
 bool by_row_pieces(const DistillArgs &a, F f) {
     const int64_t pieces = cdiv(a.vocab, Piece<T>::E);
-    std::integral_constant<int, 256> few;
-    if (pieces <= 256) return f(few, std::integral_constant<int, 1>());
-    if (pieces <= 1024) return f(few, std::integral_constant<int, 4>());
-    if (pieces <= 2048) return f(few, std::integral_constant<int, 8>());
-    if (pieces <= 4096) return f(few, std::integral_constant<int, 16>());
+    std::integral_constant<int, 128> two;
+    std::integral_constant<int, 256> four;
+    if (pieces <= 128) return f(two, std::integral_constant<int, 1>());
+    if (pieces <= 512) return f(two, std::integral_constant<int, 4>());
+    if (pieces <= 1024) return f(four, std::integral_constant<int, 4>());
+    if (pieces <= 2048) return f(four, std::integral_constant<int, 8>());
+    if (pieces <= 4096) return f(four, std::integral_constant<int, 16>());
     if (pieces <= 8192)
         return f(std::integral_constant<int, 512>(), std::integral_constant<int, 16>());
     if (pieces <= 16384)
         return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 16>());
     return false;
 }
+
 }  // namespace
 
 bool embedding_ok(const katsu_embedding &d) {
