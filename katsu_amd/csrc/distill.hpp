@@ -136,15 +136,31 @@ struct DistillSum {
     }
 };
 
-// M and L of a row's columns [c0, c1), the same in every thread.
+// How many values a row begins after a 16-byte boundary.  Its pieces begin that much before it, so
+// that they lie on such boundaries: loads of 16 bytes that begin in the middle of 4 take longer
+// (2000 rows of 32001 bfloat16: the loss XX us instead of 34, with its gradient XX instead of 66).
+template <typename T>
+__device__ __forceinline__ int row_shift(const T *p) {
+    return (int)((uintptr_t)p / sizeof(T) % Piece<T>::E);
+}
+
+// M and L of a row, the same in every thread.
 template <typename T, int NT>
-__device__ __forceinline__ DistillSum distill_columns(const T *z, int64_t c0, int64_t c1, float by,
-                                                      float *part) {
-    constexpr int E = Piece<T>::E;
-    constexpr int U = 4;  // pieces in flight
+__device__ __forceinline__ DistillSum distill_row(const T *z, int64_t n, float by, float *part) {
+    constexpr int E = Piece<T>::E, U = 4;  // pieces in flight
     DistillSum s;
-    int64_t i = c0 + threadIdx.x * E;
-    for (; i + ((U - 1) * NT + 1) * E <= c1; i += U * NT * E) {
+    int64_t i = (int)threadIdx.x * E - row_shift(z);
+    auto one = [&] {
+        RawPiece<T> r;
+        float x[E];
+        r.load(z, i, n, -INFINITY, 0);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = r.at(e);
+        s.add(x, by);
+        i += NT * E;
+    };
+    if (i < 0) one();
+    for (; i + ((U - 1) * NT + 1) * E <= n; i += U * NT * E) {
         RawPiece<T> r[U];
         float x[U * E];
 #pragma unroll
@@ -153,14 +169,7 @@ __device__ __forceinline__ DistillSum distill_columns(const T *z, int64_t c0, in
         for (int e = 0; e < U * E; ++e) x[e] = r[e / E].at(e % E);
         s.add(x, by);
     }
-    for (; i < c1; i += NT * E) {
-        RawPiece<T> r;
-        float x[E];
-        r.load(z, i, c1, -INFINITY);
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = r.at(e);
-        s.add(x, by);
-    }
+    while (i < n) one();
     s.wave(by);
     if ((threadIdx.x & 63) == 0) {
         part[2 * (threadIdx.x >> 6)] = s.m;
@@ -254,13 +263,33 @@ __device__ __forceinline__ void distill_grad(const DistillArgs &a, int64_t row, 
     DistillFix<NT> fix;
     fix.find(a, z, c0, c1, d, m, inv, g, s);
     __syncthreads();  // dz may be z: all of the teacher's logits are read
-    for (int64_t i = c0 + threadIdx.x * E; i < c1; i += NT * E) {
+    constexpr int U = 4;  // pieces in flight
+    int64_t i = c0 + (int)threadIdx.x * E - (c0 == 0 ? row_shift(z) : 0);
+    auto value = [&](RawPiece<T> &r) {
         float x[E];
-        load_whole(z, i, c1, x);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = distill_exp(x[e] - m, a.scale2) * by;
-        store_whole(dz, i, c1, x);
+        for (int e = 0; e < E; ++e) x[e] = distill_exp(r.at(e) - m, a.scale2) * by;
+        r.set(x);
+    };
+    auto one = [&] {
+        RawPiece<T> r;
+        r.load(z, i, c1, 0.f, 0);
+        value(r);
+        r.store(dz, i, c1, 0);
+        i += NT * E;
+    };
+    if (i < c0) one();
+    for (; i + ((U - 1) * NT + 1) * E <= c1; i += U * NT * E) {
+        RawPiece<T> r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) __builtin_memcpy(&r[u].v, z + i + u * NT * E, 16);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            value(r[u]);
+            __builtin_memcpy(dz + i + u * NT * E, &r[u].v, 16);
+        }
     }
+    while (i < c1) one();
     __syncthreads();  // and all others written
     fix.write(d, dz);
 }
@@ -269,9 +298,11 @@ template <typename T, int NT>
 __device__ __forceinline__ void distill_zero(const DistillArgs &a, int64_t row, int64_t c0,
                                              int64_t c1) {
     constexpr int E = Piece<T>::E;
-    const float x[E] = {};
-    for (int64_t i = c0 + threadIdx.x * E; i < c1; i += NT * E)
-        store_whole((T *)a.dz + row * a.dz_row, i, c1, x);
+    T *dz = (T *)a.dz + row * a.dz_row;
+    const RawPiece<T> zero = {};
+    for (int64_t i = c0 + (int)threadIdx.x * E - (c0 == 0 ? row_shift(dz) : 0); i < c1;
+         i += NT * E)
+        zero.store(dz, i, c1, 0);
 }
 
 // Loss, gradient or both of whole rows: a block a row.
@@ -281,8 +312,12 @@ __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
     __shared__ std::conditional_t<GRAD, DistillIds, int> ids;
     const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     if (row >= a.rows) return;
-    const int64_t c0 = LOSS ? 0 : blockIdx.z * a.run;
-    const int64_t c1 = LOSS ? a.vocab : min(c0 + a.run, a.vocab);
+    int64_t c0 = 0, c1 = a.vocab;
+    if (!LOSS) {  // runs of pieces
+        const int shift = row_shift((const T *)a.z + row * a.z_row);
+        if (blockIdx.z > 0) c0 = blockIdx.z * a.run - shift;
+        if (blockIdx.z + 1 < gridDim.z) c1 = (blockIdx.z + 1) * a.run - shift;
+    }
     DistillRow<NT> d;
     d.load(a, row);
     if (!d.some) {
@@ -296,8 +331,8 @@ __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
     d.softmax(a, part[0], part[1]);
     float m, inv;
     if constexpr (LOSS) {
-        const DistillSum s = distill_columns<T, NT>((const T *)a.z + row * a.z_row, 0, a.vocab,
-                                                    a.scale2, part[2]);
+        const DistillSum s =
+            distill_row<T, NT>((const T *)a.z + row * a.z_row, a.vocab, a.scale2, part[2]);
         distill_loss<T, NT>(a, row, d, s, part[3]);
         m = s.m;
         inv = 1.f / s.l;
@@ -331,14 +366,16 @@ __global__ void __launch_bounds__(NT) distill_step_kernel(const DistillArgs a) {
         distill_zero<T, NT>(a, row, 0, V);
         return;
     }
+    const int shift = V + E <= NT * NP * E ? row_shift(z) : 0;
     RawPiece<T> x[NP];
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-        const T *at = z + k * NT * E;
-        if ((k + 1) * NT * E <= V)  // the whole block's pieces
+        const int first = k * NT * E - shift;  // of the block's pieces
+        const T *at = z + first;
+        if (first >= 0 && first + NT * E <= V)
             __builtin_memcpy(&x[k].v, at + threadIdx.x * E, 16);
         else
-            x[k].load(at, threadIdx.x * E, V - k * NT * E, -INFINITY);
+            x[k].load(at, threadIdx.x * E, V - first, -INFINITY, -first);
     }
     d.softmax(a, part[0], part[1]);
     float m = -INFINITY;
@@ -366,12 +403,13 @@ __global__ void __launch_bounds__(NT) distill_step_kernel(const DistillArgs a) {
     __syncthreads();  // dz may be z: all of the teacher's logits are read
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-        const int i = (k * NT + (int)threadIdx.x) * E;
+        const int i = (k * NT + (int)threadIdx.x) * E - shift;
         if (i >= V) break;
         float y[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] = distill_exp(x[k].at(e) - m, a.scale2) * by;
-        store_whole(dz, i, V, y);
+        x[k].set(y);
+        x[k].store(dz, i, V, 0);
     }
     __syncthreads();  // and all others written
     fix.write(d, dz);

@@ -54,24 +54,27 @@ template <typename T>
 struct RawPiece {
     static constexpr int E = Piece<T>::E;
     lm_u4 v;
-    // Those past the row's end are `none`.
-    __device__ __forceinline__ void load(const T *p, int64_t i, int64_t n, float none = 0.f) {
-        if (i + E <= n) {
+    // Those outside the row's [first, n) are `none`, and not written.
+    __device__ __forceinline__ void load(const T *p, int64_t i, int64_t n, float none = 0.f,
+                                         int64_t first = INT64_MIN) {
+        if (i >= first && i + E <= n) {
             __builtin_memcpy(&v, p + i, 16);
         } else {
             T e[E];
 #pragma unroll
-            for (int j = 0; j < E; ++j) e[j] = i + j < n ? p[i + j] : (T)none;
+            for (int j = 0; j < E; ++j)
+                e[j] = i + j >= first && i + j < n ? p[i + j] : (T)none;
             __builtin_memcpy(&v, e, 16);
         }
     }
-    __device__ __forceinline__ void store(T *p, int64_t i, int64_t n) const {
-        if (i + E <= n) {
+    __device__ __forceinline__ void store(T *p, int64_t i, int64_t n,
+                                          int64_t first = INT64_MIN) const {
+        if (i >= first && i + E <= n) {
             __builtin_memcpy(p + i, &v, 16);
         } else {
 #pragma unroll
             for (int j = 0; j < E; ++j)
-                if (i + j < n) p[i + j] = (T)at(j);
+                if (i + j >= first && i + j < n) p[i + j] = (T)at(j);
         }
     }
     // Its values are converted again after this: held as float32 they take twice the registers.
