@@ -137,39 +137,37 @@ struct DistillSum {
 };
 
 // How many values a row begins after a 16-byte boundary.  Its pieces begin that much before it, so
-// that they lie on such boundaries: loads of 16 bytes that begin in the middle of 4 take longer
-// (2000 rows of 32001 bfloat16: the loss XX us instead of 34, with its gradient XX instead of 66).
+// that they lie on such boundaries: accesses of 16 bytes that begin in the middle of 4 take longer
+// (2000 rows of 32001 bfloat16: the loss 34 us so, 30 with the shift, the gradient 67 and 62).
 template <typename T>
 __device__ __forceinline__ int row_shift(const T *p) {
     return (int)((uintptr_t)p / sizeof(T) % Piece<T>::E);
 }
 
-// M and L of a row, the same in every thread.
-template <typename T, int NT>
-__device__ __forceinline__ DistillSum distill_row(const T *z, int64_t n, float by, float *part) {
-    constexpr int E = Piece<T>::E, U = 4;  // pieces in flight
+// M and L of a thread's pieces of a row, U of them in flight.
+template <typename T, int NT, int U>
+__device__ __forceinline__ DistillSum distill_pieces(const T *z, int64_t n, float by) {
+    constexpr int E = Piece<T>::E;
     DistillSum s;
-    int64_t i = (int)threadIdx.x * E - row_shift(z);
-    auto one = [&] {
-        RawPiece<T> r;
-        float x[E];
-        r.load(z, i, n, -INFINITY, 0);
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = r.at(e);
-        s.add(x, by);
-        i += NT * E;
-    };
-    if (i < 0) one();
-    for (; i + ((U - 1) * NT + 1) * E <= n; i += U * NT * E) {
+    for (int64_t i = (int)threadIdx.x * E - row_shift(z); i < n; i += U * NT * E) {
         RawPiece<T> r[U];
         float x[U * E];
 #pragma unroll
-        for (int u = 0; u < U; ++u) __builtin_memcpy(&r[u].v, z + i + u * NT * E, 16);
+        for (int u = 0; u < U; ++u)
+            if (u == 0 || i + u * NT * E < n)
+                r[u].load(z, i + u * NT * E, n, -INFINITY, 0);
+            else
+                r[u].fill(-INFINITY);
 #pragma unroll
         for (int e = 0; e < U * E; ++e) x[e] = r[e / E].at(e % E);
         s.add(x, by);
     }
-    while (i < n) one();
+    return s;
+}
+// M and L of a row, the same in every thread.
+template <typename T, int NT, int U>
+__device__ __forceinline__ DistillSum distill_row(const T *z, int64_t n, float by, float *part) {
+    DistillSum s = distill_pieces<T, NT, U>(z, n, by);
     s.wave(by);
     if ((threadIdx.x & 63) == 0) {
         part[2 * (threadIdx.x >> 6)] = s.m;
@@ -250,46 +248,42 @@ struct DistillFix {
     }
 };
 
+// A thread's pieces of columns [c0, c1) as if there were no teacher, U of them in flight.
+template <typename T, int NT, int U>
+__device__ __forceinline__ void grad_pieces(const T *z, T *dz, int64_t c0, int64_t c1, float m,
+                                            float scale2, float by) {
+    constexpr int E = Piece<T>::E;
+    for (int64_t i = c0 + (int)threadIdx.x * E - (c0 == 0 ? row_shift(z) : 0); i < c1;
+         i += U * NT * E) {
+        RawPiece<T> r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (u == 0 || i + u * NT * E < c1) r[u].load(z, i + u * NT * E, c1, 0.f, 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u > 0 && i + u * NT * E >= c1) break;
+            float x[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = distill_exp(r[u].at(e) - m, scale2) * by;
+            r[u].set(x);
+            r[u].store(dz, i + u * NT * E, c1, 0);
+        }
+    }
+}
+
 // The gradient of columns [c0, c1): all of them as if there were no teacher, then the
 // teacher's.
-template <typename T, int NT>
+template <typename T, int NT, int U>
 __device__ __forceinline__ void distill_grad(const DistillArgs &a, int64_t row, int64_t c0,
                                              int64_t c1, const DistillRow<NT> &d, float m,
                                              float inv, DistillIds &s) {
-    constexpr int E = Piece<T>::E;
     const T *z = (const T *)a.z + row * a.z_row;
     T *dz = (T *)a.dz + row * a.dz_row;
     const float g = a.dloss[row * a.dloss_step] * a.tau, by = inv * g;
     DistillFix<NT> fix;
     fix.find(a, z, c0, c1, d, m, inv, g, s);
     __syncthreads();  // dz may be z: all of the teacher's logits are read
-    constexpr int U = 4;  // pieces in flight
-    int64_t i = c0 + (int)threadIdx.x * E - (c0 == 0 ? row_shift(z) : 0);
-    auto value = [&](RawPiece<T> &r) {
-        float x[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = distill_exp(r.at(e) - m, a.scale2) * by;
-        r.set(x);
-    };
-    auto one = [&] {
-        RawPiece<T> r;
-        r.load(z, i, c1, 0.f, 0);
-        value(r);
-        r.store(dz, i, c1, 0);
-        i += NT * E;
-    };
-    if (i < c0) one();
-    for (; i + ((U - 1) * NT + 1) * E <= c1; i += U * NT * E) {
-        RawPiece<T> r[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) __builtin_memcpy(&r[u].v, z + i + u * NT * E, 16);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            value(r[u]);
-            __builtin_memcpy(dz + i + u * NT * E, &r[u].v, 16);
-        }
-    }
-    while (i < c1) one();
+    grad_pieces<T, NT, U>(z, dz, c0, c1, m, a.scale2, by);
     __syncthreads();  // and all others written
     fix.write(d, dz);
 }
@@ -305,8 +299,8 @@ __device__ __forceinline__ void distill_zero(const DistillArgs &a, int64_t row, 
         zero.store(dz, i, c1, 0);
 }
 
-// Loss, gradient or both of whole rows: a block a row.
-template <typename T, int NT, bool LOSS, bool GRAD>
+// Loss, gradient or both of whole rows: a block a row, U of a thread's pieces in flight.
+template <typename T, int NT, bool LOSS, bool GRAD, int U>
 __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
     __shared__ float part[5][2 * NT / 64];
     __shared__ std::conditional_t<GRAD, DistillIds, int> ids;
@@ -332,7 +326,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
     float m, inv;
     if constexpr (LOSS) {
         const DistillSum s =
-            distill_row<T, NT>((const T *)a.z + row * a.z_row, a.vocab, a.scale2, part[2]);
+            distill_row<T, NT, U>((const T *)a.z + row * a.z_row, a.vocab, a.scale2, part[2]);
         distill_loss<T, NT>(a, row, d, s, part[3]);
         m = s.m;
         inv = 1.f / s.l;
@@ -344,7 +338,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
         m = a.stats[row];
         inv = a.stats[a.rows + row];
     }
-    if constexpr (GRAD) distill_grad<T, NT>(a, row, c0, c1, d, m, inv, ids);
+    if constexpr (GRAD) distill_grad<T, NT, U>(a, row, c0, c1, d, m, inv, ids);
 }
 
 // Loss and gradient of rows of up to NT * NP pieces, which stay in the block's registers between

@@ -273,6 +273,14 @@ DistillArgs distill_args(const katsu_distillation &d, const void *logits, const 
     a.scale2 = (float)(1.4426950408889634 / (double)d.temperature);
     return a;
 }
+// Four of a thread's pieces in flight where it has as many; where it has not, the look at each
+// costs more than it gives (the loss of 8000 x 1000 bfloat16: 16 us with one, 20 with four; of
+// 8000 x 8000: 34 and 32).
+template <typename T, int NT, class F>
+int by_pieces(int64_t cols, F f) {
+    if (cols < 4 * NT * Piece<T>::E) return f(std::integral_constant<int, 1>());
+    return f(std::integral_constant<int, 4>());
+}
 // A block a row.  16 waves where there are few rows and long ones (250 x 130000 float32: 31 us, 40
 // with 4); else 4 (1000 x 32000 bfloat16: 16 us, 32 with 16), or 2 for short rows, whose time is
 // the block's joins (8000 x 1000: 16 us, 22 with 4; 8000 x 16000 54 and 57; 4096 x 32000 54 and
@@ -280,8 +288,10 @@ DistillArgs distill_args(const katsu_distillation &d, const void *logits, const 
 // 100000 float32: 115 us with 16 waves, 128 with 4).
 template <typename T, int NT, bool GRAD>
 int launch_loss(const DistillArgs &a, hipStream_t st) {
-    distill_kernel<T, NT, true, GRAD><<<grid_of(a.rows), NT, 0, st>>>(a);
-    return status_of(hipGetLastError());
+    return by_pieces<T, NT>(a.vocab, [&](auto u) {
+        distill_kernel<T, NT, true, GRAD, decltype(u)::value><<<grid_of(a.rows), NT, 0, st>>>(a);
+        return status_of(hipGetLastError());
+    });
 }
 template <typename T, bool GRAD>
 int launch_loss(const DistillArgs &a, hipStream_t st) {
@@ -473,11 +483,14 @@ int distillation_bwd(const katsu_distillation &d, const float *dloss, const void
     const int64_t want = std::min(cdiv(4 * kCUs, a.rows), cdiv(a.vocab, 4096));
     a.run = cdiv(cdiv(a.vocab, want), 2048) * 2048;
     const dim3 grid = grid_of(a.rows, (int)cdiv(a.vocab, a.run));
-    if (d.dtype == KATSU_F32)
-        distill_kernel<float, 256, false, true><<<grid, 256, 0, st>>>(a);
-    else
-        distill_kernel<__bf16, 256, false, true><<<grid, 256, 0, st>>>(a);
-    return status_of(hipGetLastError());
+    auto run = [&](auto t) {
+        using T = decltype(t);
+        return by_pieces<T, 256>(a.run, [&](auto u) {
+            distill_kernel<T, 256, false, true, decltype(u)::value><<<grid, 256, 0, st>>>(a);
+            return status_of(hipGetLastError());
+        });
+    };
+    return d.dtype == KATSU_F32 ? run(float()) : run(__bf16());
 }
 
 int distillation_step(const katsu_distillation &d, const void *logits, const int32_t *ids,

@@ -83,6 +83,12 @@ struct RawPiece {
         const uint32_t u = v[j * (int)sizeof(T) / 4];
         return __builtin_bit_cast(float, sizeof(T) == 4 ? u : j & 1 ? u & 0xffff0000u : u << 16);
     }
+    __device__ __forceinline__ void fill(float x) {
+        float y[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) y[j] = x;
+        set(y);
+    }
     __device__ __forceinline__ void set(const float *x) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
