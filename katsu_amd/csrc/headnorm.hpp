@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kHeadThreads) head_norm_bwd_kernel(const HeadA
         u[k].init(a, k * G + lane);
         if (t.w) u[k].load(t.w, 0, w[k]);
     }
-    HeadPacked<T, E> px[NU][2], pg[NU][2];
+    HeadPacked<T, E> px[NU][2], pg[NU][2];  // zeros where the lane has no piece
     float pcs[NU][2][E];
     int64_t out = 0;
     // A head's angles lie where its token's position says, which is read a head earlier still.
@@ -242,8 +242,8 @@ __global__ void __launch_bounds__(kHeadThreads) head_norm_bwd_kernel(const HeadA
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    x[k][i][e] = u[k].has[i] ? px[k][i].at(e) : 0.f;
-                    g[k][i][e] = u[k].has[i] ? pg[k][i].at(e) : 0.f;
+                    x[k][i][e] = px[k][i].at(e);
+                    g[k][i][e] = pg[k][i].at(e);
                 }
         const int64_t to = out;
         base += step;
