@@ -488,7 +488,8 @@ int katsu_hip_qk_norm_rotary_bwd_dev(const katsu_qk_norm_rotary *d,
  * Strides are in elements between rows (columns are adjacent), of dloss
  * between values (0: one for all rows).  stats [2][rows] (or NULL) receives
  * each row's largest logit and 1 / sum exp((z - largest) / tau), 0 and 0 for a
- * row without an entry: what the backward call reads. */
+ * row without an entry: what the backward call reads.  The order of a row's
+ * sums depends on where it begins within 16 bytes. */
 typedef struct katsu_distillation {
     int32_t dtype, teacher_dtype;  /* katsu_dtype of the logits, of the teacher's */
     uint64_t rows, vocab, top;

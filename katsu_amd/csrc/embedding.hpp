@@ -3,7 +3,9 @@
 //   out[t] = scale table[ids[t]]                       (zeros where ids[t] is no row)
 //   dtable[v] = (dtable[v] +) scale sum over t with ids[t] = v of dout[t], t rising
 //
-// HBM-bound: each row is read and written once.
+// HBM-bound: each row is read and written once (16384 tokens of 32000 x 2048 float32: 40 us, 212 MB
+// moved, 5.3 TB/s; the gradient in bfloat16, 200 MB: 64 us, of which adding and writing zeros 47,
+// 4.3 TB/s, the sort before it 11, the join behind it 6; a copy reaches 4.7).
 #pragma once
 
 #include "lmvec.hpp"
@@ -21,7 +23,7 @@ struct EmbedArgs {
 
 constexpr int kEmbedPieces = 4;
 
-// A wave a row's chunk: 4 KB in flight.
+// A wave a token's chunk of 4 KB, all of it in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) embed_kernel(const EmbedArgs a) {
     constexpr int E = Piece<T>::E, N = kEmbedPieces;
@@ -201,7 +203,9 @@ __device__ __forceinline__ int block_scan(int v, int *part) {
 }
 // A block sorts the tokens of a slab of rows: all blocks look through all ids, count those of
 // smaller rows, which are before the slab's, and each wave's of every row of the slab; then each
-// wave places its tokens, of which it looks only at the batches that had some.
+// wave places its tokens, of which it looks only at the batches that had some.  Bound by latency and,
+// where a frequent token makes one block's waves place most of theirs, by that block's
+// instructions (16384 tokens: 11 us; 23 with every match by bits, one at a time where they are few).
 __global__ void __launch_bounds__(1024) embed_slab_kernel(const EmbedSort s) {
     __shared__ int count[16][kEmbedSlab], part[16], below[16], end;
     constexpr int U = 8;  // rounds of 64 tokens in a batch, of which a wave has 64 at most
@@ -371,7 +375,8 @@ __global__ void __launch_bounds__(256) embed_there_kernel(const EmbedSort s) {
     if (k < s.vocab && k != before) atomicOr(s.there + (k >> 5), 1u << (k & 31));
 }
 
-// A wave a tile's chunk of 64 pieces, kEmbedAhead tokens' rows in flight.
+// A wave a tile's chunk of 64 pieces, kEmbedAhead tokens' rows in flight (16: 66 us in tiles of 32 rows
+// of 4 KB; 8: 68).
 template <typename T>
 __global__ void __launch_bounds__(256) embed_tile_kernel(const EmbedTiles t) {
     constexpr int E = Piece<T>::E, U = kEmbedAhead;
@@ -452,7 +457,8 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedTiles t) {
     const int64_t j = blockIdx.x, t0 = j * t.tile, t1 = t0 + t.tile;
     if (t1 >= a.tokens) return;
     // Read together; most blocks end here.
-    const int cur = t.key[t1], last = t.key[t1 - 1], head = t.key[t0], before = t.key[max(t0, (int64_t)1) - 1];
+    const int cur = t.key[t1], last = t.key[t1 - 1], head = t.key[t0];
+    const int before = t.key[max(t0, (int64_t)1) - 1];
     if (cur >= a.vocab || last != cur) return;
     if (head == cur && t0 > 0 && before == cur) return;  // began before the tile
     const int64_t i = (int64_t)blockIdx.y * 256 + lane * 4;

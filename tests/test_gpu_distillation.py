@@ -223,6 +223,37 @@ def test_extremes(dev, dt, rows):
         assert torch.equal(a[4:], base[4:])
 
 
+@pytest.mark.parametrize("rows", [4, 400])
+def test_row_of_minus_infinity(dev, rows):
+    """Logits of nothing but -inf, as the formula has it: NaN where a teacher speaks, else zeros."""
+    z, ids, t, dloss = _inputs(rows, 300, 4, torch.float32, pad=False)
+    clean = _all(dev, z, ids, t, dloss, 1.0)
+    z[1:3], ids[2] = -math.inf, -1
+    loss, _, grad, loss2, grad2 = _all(dev, z, ids, t, dloss, 1.0)
+    for a, b, was, gwas in ((loss, grad, clean[0], clean[2]), (loss2, grad2, clean[3], clean[4])):
+        assert a[1].isnan() and b[1].isnan().all() and a[2] == 0 and not b[2].any()
+        assert torch.equal(a[3:], was[3:]) and torch.equal(b[3:], gwas[3:])
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_many_long_rows(dev, dt):
+    """Rows that no block's registers hold, more than 1024 of them: one row of logits, read by all."""
+    rows, vocab = 1030, 140001
+    g = torch.Generator().manual_seed(7)
+    z = (torch.randn(1, vocab, generator=g) * 2.5).to(dt)
+    ids = torch.randint(0, vocab, (4, 6), generator=g, dtype=torch.int32)
+    t = torch.randn(4, 6, generator=g).to(dt)
+    want, dz, ltol, gtol = _ref(z.expand(4, vocab), ids, t, 2.0, torch.ones(4))
+    loss, grad = ops.distillation_step(
+        z.to(dev).expand(rows, vocab), ids.repeat(258, 1)[:rows].to(dev),
+        t.repeat(258, 1)[:rows].to(dev), torch.ones(1, device=dev).expand(rows), 2.0)
+    _close(loss[:4], want, ltol)
+    _close(grad[:4], dz, gtol)
+    for i in range(4, rows, 4):
+        n = min(4, rows - i)
+        assert torch.equal(loss[i:i + n], loss[:n]) and torch.equal(grad[i:i + n], grad[:n]), i
+
+
 def test_cross_entropy(dev):
     """One entry at temperature 1 is the cross entropy with labels, -1 for rows that do not count."""
     g = torch.Generator().manual_seed(3)

@@ -175,6 +175,23 @@ def test_same_bits(dev, tokens):
         assert torch.equal(ops.embedding_backward(dout, a, 2000, 0.5), want[0])
 
 
+def test_two_streams_at_once(dev):
+    """Calls that overlap, each with memory of its own."""
+    g = torch.Generator().manual_seed(13)
+    dout = torch.randn(5000, 300, generator=g).to(dev)
+    ids = [_ids(5000, 900, s).to(dev) for s in (14, 15)]
+    want = [ops.embedding_backward(dout, i, 900) for i in ids]
+    streams = [torch.cuda.Stream() for _ in ids]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for n, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[n].append(ops.embedding_backward(dout, ids[n], 900))
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want[n]) for n in (0, 1) for t in got[n])
+
+
 def test_large_offsets(dev):
     """Rows of a table and of its gradient that lie beyond 2^32 bytes and 2^31 elements."""
     vocab, cols = 1_100_000, 2048

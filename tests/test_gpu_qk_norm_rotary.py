@@ -257,3 +257,39 @@ def test_same_bits(dev):
                                                                               **how)
         assert all(torch.equal(a, b) for a, b in zip(got, now))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_no_tokens_and_no_heads(dev):
+    """Nothing to turn: the weights' gradients are zeros."""
+    w = torch.ones(16, device=dev)
+    for q, k in ((torch.zeros(0, 3, 16, device=dev), torch.zeros(0, 1, 16, device=dev)),
+                 (torch.zeros(5, 0, 16, device=dev), torch.ones(5, 2, 16, device=dev))):
+        a, b = ops.qk_norm_rotary(q, k, w_q=w, w_k=w)
+        assert a.shape == q.shape and b.shape == k.shape
+        dq, dk, dw_q, dw_k = ops.qk_norm_rotary_backward(q, k, q, k, w_q=w, w_k=w)
+        assert dq.shape == q.shape and dk.shape == k.shape and not dw_q.any()
+        assert dw_k.any() == (k.numel() > 0)
+
+
+def test_large_offsets(dev):
+    """Heads beyond 2^31 elements."""
+    tokens, heads, d = 70_000, 248, 128
+    x = torch.zeros(tokens, heads, d, dtype=torch.bfloat16, device=dev)
+    g = torch.Generator().manual_seed(8)
+    host, grad = (torch.randn(2, heads, d, generator=g).bfloat16() for _ in range(2))
+    x[-2:] = host.to(dev)
+    dy = torch.zeros_like(x)
+    dy[-2:] = grad.to(dev)
+    table = ops.rotary_table(tokens, 64, device=dev)
+    w = torch.randn(d, generator=g).bfloat16()
+    pos = torch.arange(tokens - 2, tokens)
+    y, _ = ops.qk_norm_rotary(x, None, table, w_q=w.to(dev), eps=EPS)
+    _close(y[-2:], *_forward(host, w, table.cpu(), pos, False))
+    assert not y[:-2].any()
+    dx, _, dw, _ = ops.qk_norm_rotary_backward(dy, None, x, None, table, w_q=w.to(dev), eps=EPS,
+                                               out_q=dy)
+    want, dwant, tol, wtol = _backward(grad, host, w, table.cpu(), pos, False)
+    _close(dx[-2:], want, tol)
+    # The sum runs over all tokens, of which the others add zeros.
+    _close(dw, dwant, wtol)
+    assert not dx[:-2].any()
