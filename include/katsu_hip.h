@@ -444,8 +444,8 @@ int katsu_hip_embedding_bwd_dev(const katsu_embedding *d, const void *dout, cons
  *   n = x / sqrt(mean(x^2) + eps) * w,  y = n turned as katsu_hip_rotary_dev does
  * with w_q and w_k of head_dim (1..512) values, or NULL for none; rotary_dim 0
  * (and table NULL) leaves the turn out.  Operands, positions and strides are as
- * in katsu_hip_rotary_dev; k may be NULL with k_heads 0.  Outputs may be the
- * inputs, with the same strides.  n is not rounded before the turn. */
+ * in katsu_hip_rotary_dev; k may be NULL with k_heads 0.  q_out may be q, and
+ * k_out k, with the same strides.  n is not rounded before the turn. */
 typedef struct katsu_qk_norm_rotary {
     int32_t dtype, interleaved;
     uint64_t tokens, heads, k_heads, head_dim, rotary_dim, length;

@@ -625,7 +625,7 @@ def qk_norm_rotary(q, k, table=None, positions=None, w_q=None, w_k=None, eps=1e-
     """(q', k'): each head of q and k [tokens, heads, channels] (k may be None) divided by its
     channels' root mean square, times w_q or w_k ([channels], None: no weight), then turned as
     rotary does by rows of `table` (None: not turned), in one pass and rounded once.  At most 512
-    channels, adjacent; any token and head strides.  The outputs may be the inputs."""
+    channels, adjacent; any token and head strides.  out_q may be q, and out_k k."""
     out_q = torch.empty_like(q) if out_q is None else out_q
     if k is not None and out_k is None:
         out_k = torch.empty_like(k)
