@@ -476,7 +476,9 @@ int katsu_hip_qk_norm_rotary_bwd_dev(const katsu_qk_norm_rotary *d,
 
 /* The loss of rows x vocab logits z against a teacher's top logits t, `top`
  * (0..1024) of them a row at the columns ids (both [rows][top], contiguous).
- * Over a row's entries whose id is in [0, vocab), with tau the temperature:
+ * The temperature is positive and finite, and so is log2(e) / temperature in
+ * float32 (4.23e-39 is too small).  Over a row's entries whose id is in
+ * [0, vocab), with tau the temperature:
  *   p = softmax(t / tau),  P = softmax(z / tau) over all columns,
  *   loss = tau^2 sum_k p_k (log p_k - log P[id_k]),
  *   dlogits[v] = dloss tau (P[v] - sum of the p_k with id_k = v)

@@ -260,6 +260,9 @@ void head_blocks(const katsu_qk_norm_rotary &d, int (&blocks)[2]) {
 
 // ---- distillation ----
 
+// log2(e) / tau: what the kernels multiply differences of logits with.
+float exponent_scale(float tau) { return (float)(1.4426950408889634 / (double)tau); }
+
 DistillArgs distill_args(const katsu_distillation &d, const void *logits, const int32_t *ids,
                          const void *teacher) {
     DistillArgs a{};
@@ -275,7 +278,7 @@ DistillArgs distill_args(const katsu_distillation &d, const void *logits, const 
     a.top = (int)d.top;
     a.teacher_bf16 = d.teacher_dtype == KATSU_BF16;
     a.tau = d.temperature;
-    a.scale2 = (float)(1.4426950408889634 / (double)d.temperature);
+    a.scale2 = exponent_scale(d.temperature);
     return a;
 }
 // Four of a thread's pieces in flight where it has as many; where it has not, the look at each
@@ -465,7 +468,7 @@ bool distillation_ok(const katsu_distillation &d) {
     return dtype_ok(d.dtype) && dtype_ok(d.teacher_dtype) && d.rows <= (uint64_t)kI32Max &&
            d.vocab <= (uint64_t)kI32Max && d.top <= kDistillTop && stride_ok(d.stride) &&
            stride_ok(d.out_stride) && stride_ok(d.dloss_stride) && d.temperature > 0.f &&
-           std::isfinite(d.temperature) && std::isfinite(1.f / d.temperature);
+           std::isfinite(d.temperature) && std::isfinite(exponent_scale(d.temperature));
 }
 
 int distillation(const katsu_distillation &d, const void *logits, const int32_t *ids,
