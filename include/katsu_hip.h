@@ -347,7 +347,8 @@ int katsu_hip_attention_bwd_dev(const katsu_attention *d, const katsu_attention_
  * row t if positions is NULL.  inverse turns back: the gradient of a turn.
  * q and k ([tokens][heads][head_dim], strides in elements as above) go in one
  * launch; k may be NULL with k_heads 0.  Outputs may be the inputs, with the
- * same strides; an output's strides must not be zero, none may be negative.
+ * same strides; no two heads of an output may share memory, no stride may be
+ * negative.
  * At most 65535 heads each, fewer than 2^20 channels of a token in all. */
 typedef struct katsu_rotary {
     int32_t dtype, interleaved, inverse;

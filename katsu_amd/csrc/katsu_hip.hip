@@ -3416,9 +3416,9 @@ int katsu_hip_qk_norm_rotary_dev(const katsu_qk_norm_rotary *d, const void *q, c
         (d->k_heads && (!k || !k_out)))
         return KATSU_E_INVALID;
     if ((d->heads && !rotary_out_ok(d->q_stride, d->q_out_stride, q == q_out, d->tokens,
-                                    d->heads)) ||
+                                    d->heads, d->head_dim)) ||
         (d->k_heads && !rotary_out_ok(d->k_stride, d->k_out_stride, k == k_out, d->tokens,
-                                      d->k_heads)))
+                                      d->k_heads, d->head_dim)))
         return KATSU_E_INVALID;
     return qk_norm_rotary(*d, q, k, w_q, w_k, table, positions, q_out, k_out,
                           (hipStream_t)stream);
@@ -3445,12 +3445,16 @@ int katsu_hip_qk_norm_rotary_bwd_dev(const katsu_qk_norm_rotary *d,
             return KATSU_E_INVALID;
         // Each of the two that an output may be.
         if (d->heads &&
-            (!rotary_out_ok(d->q_stride, d->q_out_stride, q == dx_q, d->tokens, d->heads) ||
-             !rotary_out_ok(g->dq_stride, d->q_out_stride, dq == dx_q, d->tokens, d->heads)))
+            (!rotary_out_ok(d->q_stride, d->q_out_stride, q == dx_q, d->tokens, d->heads,
+                            d->head_dim) ||
+             !rotary_out_ok(g->dq_stride, d->q_out_stride, dq == dx_q, d->tokens, d->heads,
+                            d->head_dim)))
             return KATSU_E_INVALID;
         if (d->k_heads &&
-            (!rotary_out_ok(d->k_stride, d->k_out_stride, k == dx_k, d->tokens, d->k_heads) ||
-             !rotary_out_ok(g->dk_stride, d->k_out_stride, dk == dx_k, d->tokens, d->k_heads)))
+            (!rotary_out_ok(d->k_stride, d->k_out_stride, k == dx_k, d->tokens, d->k_heads,
+                            d->head_dim) ||
+             !rotary_out_ok(g->dk_stride, d->k_out_stride, dk == dx_k, d->tokens, d->k_heads,
+                            d->head_dim)))
             return KATSU_E_INVALID;
     }
     hipStream_t st = (hipStream_t)stream;

@@ -28,9 +28,10 @@ int attention_bwd(const katsu_attention &d, const katsu_attention_grads &g, cons
                   const int32_t *cu_q, const int32_t *cu_k, void *dq, void *dk, void *dv, void *ws,
                   hipStream_t st);
 
-// Whether a tensor of these strides can be written, also where it is the input.
+// Whether a tensor of these strides can be written: no two of its heads share memory, and where it
+// is the input (`same`), each is in its place.
 bool rotary_out_ok(const int64_t (&in)[2], const int64_t (&out)[2], bool same, uint64_t tokens,
-                   uint64_t heads);
+                   uint64_t heads, uint64_t dim);
 bool rotary_ok(const katsu_rotary &d);
 int rotary(const katsu_rotary &d, const void *q, const void *k, const float *table,
            const int32_t *positions, void *q_out, void *k_out, hipStream_t st);

@@ -139,11 +139,23 @@ int launch_norm_bwd(const NormBwdArgs &a, void *dw_pre, void *dw_post, void *dga
 // An output's places are its own, and if it is its input it is so value by value: a thread
 // may write before another has read.
 bool rotary_out_ok(const int64_t (&in)[2], const int64_t (&out)[2], bool same, uint64_t tokens,
-                   uint64_t heads) {
+                   uint64_t heads, uint64_t dim) {
     const uint64_t n[2] = {tokens, heads};
     for (int i = 0; i < 2; ++i) {
         if (in[i] < 0 || out[i] < 0) return false;
-        if (n[i] > 1 && (out[i] == 0 || (same && in[i] != out[i]))) return false;
+        if (n[i] > 1 && (out[i] < (int64_t)dim || (same && in[i] != out[i]))) return false;
+    }
+    if (tokens < 2 || heads < 2) return true;
+    // One of the two within a step of the other, as almost always;
+    const int inner = out[0] < out[1] ? 0 : 1;
+    const int64_t step = out[1 - inner];
+    if ((__int128)(n[inner] - 1) * out[inner] + (int64_t)dim <= step) return true;
+    // else no number of heads' steps may come closer than `dim` to one of tokens' steps.
+    for (uint64_t j = 1; j < heads; ++j) {
+        const __int128 at = (__int128)j * out[1];
+        const __int128 i = at / out[0], left = at - i * out[0];
+        if (i < (__int128)tokens && left < (__int128)dim) return false;
+        if (i + 1 < (__int128)tokens && out[0] - left < (__int128)dim) return false;
     }
     return true;
 }
@@ -160,9 +172,11 @@ bool rotary_ok(const katsu_rotary &d) {
 
 int rotary(const katsu_rotary &d, const void *q, const void *k, const float *table,
            const int32_t *positions, void *q_out, void *k_out, hipStream_t st) {
-    if (d.heads && !rotary_out_ok(d.q_stride, d.q_out_stride, q == q_out, d.tokens, d.heads))
+    if (d.heads && !rotary_out_ok(d.q_stride, d.q_out_stride, q == q_out, d.tokens, d.heads,
+                                  d.head_dim))
         return KATSU_E_INVALID;
-    if (d.k_heads && !rotary_out_ok(d.k_stride, d.k_out_stride, k == k_out, d.tokens, d.k_heads))
+    if (d.k_heads && !rotary_out_ok(d.k_stride, d.k_out_stride, k == k_out, d.tokens, d.k_heads,
+                                    d.head_dim))
         return KATSU_E_INVALID;
     RotaryArgs a{};
     a.t[0] = {q, q_out, d.q_stride[0], d.q_stride[1], d.q_out_stride[0], d.q_out_stride[1],
