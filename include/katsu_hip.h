@@ -418,8 +418,8 @@ int katsu_hip_clip_grad_norm_ws_dev(const int32_t *dtypes, const void *const *in
 
 /* Embedding: out[t] = scale * table[ids[t]], tokens x cols from vocab x cols;
  * zeros where ids[t] (device int32) is not in [0, vocab): padding.  Strides are
- * in elements between rows; columns (2^20 at most) are adjacent.  `accumulate` is the
- * backward call's. */
+ * in elements between rows; columns (2^20 at most) are adjacent.  The output
+ * shares no memory with the table.  `accumulate` is the backward call's. */
 typedef struct katsu_embedding {
     int32_t dtype;       /* katsu_dtype of the table and the output */
     int32_t accumulate;  /* backward: add to dtable (1) or overwrite it (0) */
@@ -434,7 +434,7 @@ int katsu_hip_embedding_dev(const katsu_embedding *d, const int32_t *ids, const 
  * tokens with ids[t] = v, summed in float32 in an order that the sizes and ids
  * alone decide, and rounded once.  Rows without a token become zeros, or with
  * `accumulate` stay as they are, bit by bit.  out_stride is dout's,
- * table_stride dtable's.  Workspace as above, of
+ * table_stride dtable's; they share no memory.  Workspace as above, of
  * katsu_hip_embedding_bwd_workspace bytes. */
 int katsu_hip_embedding_bwd_workspace(const katsu_embedding *d, size_t *bytes);
 int katsu_hip_embedding_bwd_dev(const katsu_embedding *d, const void *dout, const int32_t *ids,

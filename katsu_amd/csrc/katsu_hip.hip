@@ -3383,6 +3383,9 @@ int katsu_hip_embedding_dev(const katsu_embedding *d, const int32_t *ids, const 
         return KATSU_E_INVALID;
     if (d->tokens == 0) return KATSU_OK;
     if (!ids || !out || (d->vocab > 0 && !table)) return KATSU_E_INVALID;
+    if (rows_share(table, d->vocab, d->table_stride, out, d->tokens, d->out_stride, d->cols,
+                   d->dtype))
+        return KATSU_E_INVALID;
     return embedding(*d, ids, table, out, (hipStream_t)stream);
 }
 
@@ -3399,6 +3402,9 @@ int katsu_hip_embedding_bwd_dev(const katsu_embedding *d, const void *dout, cons
         return KATSU_E_INVALID;
     if (d->vocab == 0 || (d->tokens == 0 && d->accumulate)) return KATSU_OK;
     if (!dtable || (d->tokens > 0 && (!dout || !ids))) return KATSU_E_INVALID;
+    if (rows_share(dout, d->tokens, d->out_stride, dtable, d->vocab, d->table_stride, d->cols,
+                   d->dtype))
+        return KATSU_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
     void *ws = nullptr;
     const int rc = lm_scratch(workspace, workspace_bytes, embedding_bwd_bytes(*d), st, &ws);

@@ -57,6 +57,9 @@ int clip_grad_norm(const int32_t *dtypes, const void *const *in, void *const *ou
 bool embedding_ok(const katsu_embedding &d);
 // Whether rows of these columns can be written with this stride.
 bool embedding_out_ok(uint64_t rows, uint64_t cols, int64_t stride);
+// Whether any of n_a rows of a and n_b rows of b share memory.
+bool rows_share(const void *a, uint64_t n_a, int64_t stride_a, const void *b, uint64_t n_b,
+                int64_t stride_b, uint64_t cols, int dtype);
 int embedding(const katsu_embedding &d, const int32_t *ids, const void *table, void *out,
               hipStream_t st);
 size_t embedding_bwd_bytes(const katsu_embedding &d);

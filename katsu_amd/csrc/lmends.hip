@@ -342,6 +342,37 @@ bool embedding_out_ok(uint64_t rows, uint64_t cols, int64_t stride) {
     return rows < 2 || stride >= (int64_t)cols;
 }
 
+bool rows_share(const void *a, uint64_t n_a, int64_t stride_a, const void *b, uint64_t n_b,
+                int64_t stride_b, uint64_t cols, int dtype) {
+    if (n_a == 0 || n_b == 0 || cols == 0) return false;
+    struct Rows {
+        __int128 at, step, len;
+        uint64_t n;
+        __int128 end() const { return at + (__int128)(n - 1) * step + len; }
+    };
+    const int size = dtype == KATSU_F32 ? 4 : 2;
+    auto rows = [&](const void *p, uint64_t n, int64_t stride) {
+        Rows r{(__int128)(uintptr_t)p, (__int128)stride * size, (__int128)cols * size, n};
+        if (n == 1 || r.step <= r.len) r = {r.at, 0, r.end() - r.at, 1};  // no gaps
+        return r;
+    };
+    Rows x = rows(a, n_a, stride_a), y = rows(b, n_b, stride_b);
+    if (x.end() <= y.at || y.end() <= x.at) return false;
+    if (x.n > 1 && x.step == y.step) {  // parts of the same wider rows
+        if (y.at < x.at) std::swap(x, y);
+        const __int128 d = (y.at - x.at) % x.step;
+        return d < x.len || d + y.len > x.step;
+    }
+    if (x.n > y.n) std::swap(x, y);
+    for (uint64_t i = 0; i < x.n; ++i) {
+        const __int128 at = x.at + (__int128)i * x.step, before = at - y.at - y.len;
+        // y's first row that ends behind this one's beginning
+        const __int128 j = before < 0 ? 0 : y.n > 1 ? before / y.step + 1 : 1;
+        if (j < (__int128)y.n && y.at + j * y.step < at + x.len) return true;
+    }
+    return false;
+}
+
 int embedding(const katsu_embedding &d, const int32_t *ids, const void *table, void *out,
               hipStream_t st) {
     EmbedArgs a = embed_args(d, ids);

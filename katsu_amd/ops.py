@@ -553,7 +553,8 @@ def _embedding(table, out, ids, scale, beta):
 
 def embedding(ids, table, scale=1.0, out=None):
     """[T, C]: scale times the rows of table [V, C] that ids (int32 [T]) name; zeros where an id is
-    not in [0, V), as for padding.  Rows of table and out may have any stride."""
+    not in [0, V), as for padding.  Rows of table and out may have any stride; they share no
+    memory."""
     if out is None:
         out = table.new_empty((ids.numel(), table.shape[-1]))
     d = _embedding(table, out, ids, scale, 0.0)
@@ -565,8 +566,8 @@ def embedding(ids, table, scale=1.0, out=None):
 def embedding_backward(dout, ids, vocab, scale=1.0, out=None, beta=0.0, workspace=None):
     """The gradient of embedding's table [vocab, C] from dout [T, C]: each row the sum of its
     tokens' gradients, times scale; tokens with an id that is no row add nothing.  beta=1
-    accumulates into `out` and leaves rows without a token as they are.  The same call gives the
-    same bits.  `workspace`: an optional device tensor of embedding_workspace_bytes()."""
+    accumulates into `out` and leaves rows without a token as they are; out shares no memory with
+    dout.  The same call gives the same bits.  `workspace`: an optional device tensor of embedding_workspace_bytes()."""
     if out is None:
         if beta != 0.0:
             raise ValueError("beta=1 needs the gradient that it accumulates into")
