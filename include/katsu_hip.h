@@ -502,12 +502,13 @@ typedef struct katsu_distillation {
 int katsu_hip_distillation_dev(const katsu_distillation *d, const void *logits,
                                const int32_t *ids, const void *teacher, float *loss, float *stats,
                                void *stream);
-/* The gradient; dlogits may be logits, with the same stride. */
+/* The gradient; dlogits may be logits, with the same stride, or shares no
+ * memory with them. */
 int katsu_hip_distillation_bwd_dev(const katsu_distillation *d, const float *dloss,
                                    const void *logits, const int32_t *ids, const void *teacher,
                                    const float *stats, void *dlogits, void *stream);
 /* Both in one pass over the logits, where dloss is known before the loss is;
- * dlogits may be logits, with the same stride. */
+ * dlogits as above. */
 int katsu_hip_distillation_step_dev(const katsu_distillation *d, const void *logits,
                                     const int32_t *ids, const void *teacher, const float *dloss,
                                     float *loss, void *dlogits, void *stream);

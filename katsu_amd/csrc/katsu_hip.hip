@@ -3481,10 +3481,12 @@ int katsu_hip_distillation_dev(const katsu_distillation *d, const void *logits,
     return distillation(*d, logits, ids, teacher, loss, stats, (hipStream_t)stream);
 }
 
-// An output of the logits' shape: rows of its own, and where it is the logits, row by row.
+// An output of the logits' shape: rows of its own, which are the logits row by row or share no memory
+// with them.
 static bool dlogits_ok(const katsu_distillation &d, const void *logits, const void *dlogits) {
-    return embedding_out_ok(d.rows, d.vocab, d.out_stride) &&
-           (logits != dlogits || d.rows < 2 || d.stride == d.out_stride);
+    if (!embedding_out_ok(d.rows, d.vocab, d.out_stride)) return false;
+    if (logits == dlogits) return d.rows < 2 || d.stride == d.out_stride;
+    return !rows_share(logits, d.rows, d.stride, dlogits, d.rows, d.out_stride, d.vocab, d.dtype);
 }
 
 int katsu_hip_distillation_bwd_dev(const katsu_distillation *d, const float *dloss,

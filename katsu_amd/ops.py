@@ -703,7 +703,8 @@ def distillation(logits, ids, teacher, temperature=1.0):
 
 def distillation_backward(dloss, logits, ids, teacher, stats, temperature=1.0, out=None):
     """The gradient of the logits from dloss (float32 [rows], any stride) and distillation's operands
-    and stats; zeros in rows without an entry.  `out` may be the logits."""
+    and stats; zeros in rows without an entry.  `out` may be the logits; otherwise it shares no memory
+    with them."""
     out = torch.empty_like(logits) if out is None else out
     d = _distillation(logits, ids, teacher, temperature, out, dloss)
     if (stats.dtype is not torch.float32 or stats.device != logits.device
@@ -718,7 +719,7 @@ def distillation_backward(dloss, logits, ids, teacher, stats, temperature=1.0, o
 def distillation_step(logits, ids, teacher, dloss, temperature=1.0, out=None):
     """(loss, gradient of the logits) in one pass over them, where dloss (float32 [rows], any
     stride: what the sum or the mean of the losses gives each) is known beforehand.  `out`, the
-    gradient, may be the logits."""
+    gradient, may be the logits; otherwise it shares no memory with them."""
     out = torch.empty_like(logits) if out is None else out
     d = _distillation(logits, ids, teacher, temperature, out, dloss)
     loss = logits.new_empty(d.rows, dtype=torch.float32)

@@ -96,3 +96,42 @@ def test_embedding_taken(dev):
             call(i, o)
             assert torch.equal(buf, want), ((a, rows, s), (b, n, t), cols)
     assert done > 100
+
+
+def test_distillation_refuses():
+    """Without a GPU: only calls that are refused; the logits' own place is another test's."""
+    for (a, rows, s), (b, _, t), cols, share in _cases(4000, 1, True):
+        if share and a != b:
+            d = _distill(rows=rows, vocab=cols, top=1, stride=s, out_stride=t)
+            assert L.katsu_hip_distillation_bwd_dev(d, P, _at(a), P, P, P, _at(b),
+                                                    None) == _abi.E_INVALID
+            assert L.katsu_hip_distillation_step_dev(d, _at(a), P, P, P, P, _at(b),
+                                                     None) == _abi.E_INVALID
+
+
+@pytest.mark.gpu
+def test_distillation_taken(dev):
+    """Rows between each other's, and the logits' own place: the results of rows apart."""
+    g = torch.Generator().manual_seed(3)
+    base = torch.randn(ROOM, generator=g).to(dev)
+    done = 0
+    for (a, rows, s), (b, _, t), cols, share in _cases(1500, 2, True):
+        if share and ((a, s) != (b, t) or s < cols):
+            continue
+        done += 1
+        ids = (torch.arange(rows, device=dev).int() % cols)[:, None].contiguous()
+        t_, dloss = torch.zeros(rows, 1, device=dev), torch.ones(rows, device=dev)
+        for call in (lambda z, o: ops.distillation_step(z, ids, t_, dloss, out=o)[1],
+                     lambda z, o: ops.distillation_backward(
+                         dloss, z, ids, t_, ops.distillation(z, ids, t_)[1], out=o)):
+            buf, want = base.clone(), base.clone()
+            i, o = buf.as_strided((rows, cols), (s, 1), a), buf.as_strided((rows, cols), (t, 1), b)
+            apart = call(i.clone(memory_format=torch.contiguous_format),
+                         torch.empty(rows, cols, device=dev))
+            want.as_strided((rows, cols), (t, 1), b).copy_(apart)
+            call(i, o)
+            # The order of at most six terms' sum may be another one.
+            assert ((buf - want).abs() <= 32 * 2.0 ** -24).all(), ((a, rows, s), (b, t), cols)
+            o.copy_(want.as_strided((rows, cols), (t, 1), b))
+            assert torch.equal(buf, want)
+    assert done > 100
