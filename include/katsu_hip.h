@@ -459,8 +459,9 @@ int katsu_hip_qk_norm_rotary_dev(const katsu_qk_norm_rotary *d, const void *q, c
                                  void *stream);
 
 /* Its gradient, from dq and dk, the gradients of the outputs, and the forward
- * call's operands: dx_q and dx_k (strides q_out_stride and k_out_stride; they
- * may be dq and dk, or q and k, with the same strides), dw_q and dw_k where
+ * call's operands: dx_q and dx_k (strides q_out_stride and k_out_stride; dx_q
+ * may be dq or q, dx_k dk or k, with the same strides; otherwise they share no
+ * memory with an input or each other, as above), dw_q and dw_k where
  * w_q and w_k are given, summed over tokens and heads in float32 in a fixed
  * order through a workspace as above. */
 typedef struct katsu_qk_norm_rotary_grads {

@@ -3383,8 +3383,8 @@ int katsu_hip_embedding_dev(const katsu_embedding *d, const int32_t *ids, const 
         return KATSU_E_INVALID;
     if (d->tokens == 0) return KATSU_OK;
     if (!ids || !out || (d->vocab > 0 && !table)) return KATSU_E_INVALID;
-    if (rows_share(table, d->vocab, d->table_stride, out, d->tokens, d->out_stride, d->cols,
-                   d->dtype))
+    if (rows_share(table, d->vocab, d->table_stride, d->cols, out, d->tokens, d->out_stride,
+                   d->cols, d->dtype))
         return KATSU_E_INVALID;
     return embedding(*d, ids, table, out, (hipStream_t)stream);
 }
@@ -3402,8 +3402,8 @@ int katsu_hip_embedding_bwd_dev(const katsu_embedding *d, const void *dout, cons
         return KATSU_E_INVALID;
     if (d->vocab == 0 || (d->tokens == 0 && d->accumulate)) return KATSU_OK;
     if (!dtable || (d->tokens > 0 && (!dout || !ids))) return KATSU_E_INVALID;
-    if (rows_share(dout, d->tokens, d->out_stride, dtable, d->vocab, d->table_stride, d->cols,
-                   d->dtype))
+    if (rows_share(dout, d->tokens, d->out_stride, d->cols, dtable, d->vocab, d->table_stride,
+                   d->cols, d->dtype))
         return KATSU_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
     void *ws = nullptr;
@@ -3425,6 +3425,14 @@ int katsu_hip_qk_norm_rotary_dev(const katsu_qk_norm_rotary *d, const void *q, c
                                     d->heads, d->head_dim)) ||
         (d->k_heads && !rotary_out_ok(d->k_stride, d->k_out_stride, k == k_out, d->tokens,
                                       d->k_heads, d->head_dim)))
+        return KATSU_E_INVALID;
+    // Heads are read while others are written: an output is its own input or shares with none.
+    const uint64_t n = d->heads, m = d->k_heads;
+    if (heads_share(*d, q_out, n, d->q_out_stride, k_out, m, d->k_out_stride) ||
+        heads_share(*d, q_out, n, d->q_out_stride, k, m, d->k_stride) ||
+        heads_share(*d, k_out, m, d->k_out_stride, q, n, d->q_stride) ||
+        (q_out != q && heads_share(*d, q_out, n, d->q_out_stride, q, n, d->q_stride)) ||
+        (k_out != k && heads_share(*d, k_out, m, d->k_out_stride, k, m, d->k_stride)))
         return KATSU_E_INVALID;
     return qk_norm_rotary(*d, q, k, w_q, w_k, table, positions, q_out, k_out,
                           (hipStream_t)stream);
@@ -3462,6 +3470,22 @@ int katsu_hip_qk_norm_rotary_bwd_dev(const katsu_qk_norm_rotary *d,
              !rotary_out_ok(g->dk_stride, d->k_out_stride, dk == dx_k, d->tokens, d->k_heads,
                             d->head_dim)))
             return KATSU_E_INVALID;
+        // As in the forward call, with two inputs that an output may be.
+        auto share = [&](const void *out, uint64_t n, const int64_t(&s)[2], const void *in,
+                         uint64_t n_in, const int64_t(&s_in)[2], bool own) {
+            return !(own && out == in) && heads_share(*d, out, n, s, in, n_in, s_in);
+        };
+        const uint64_t n = d->heads, m = d->k_heads;
+        if (share(dx_q, n, d->q_out_stride, dx_k, m, d->k_out_stride, false) ||
+            share(dx_q, n, d->q_out_stride, q, n, d->q_stride, true) ||
+            share(dx_q, n, d->q_out_stride, dq, n, g->dq_stride, true) ||
+            share(dx_q, n, d->q_out_stride, k, m, d->k_stride, false) ||
+            share(dx_q, n, d->q_out_stride, dk, m, g->dk_stride, false) ||
+            share(dx_k, m, d->k_out_stride, k, m, d->k_stride, true) ||
+            share(dx_k, m, d->k_out_stride, dk, m, g->dk_stride, true) ||
+            share(dx_k, m, d->k_out_stride, q, n, d->q_stride, false) ||
+            share(dx_k, m, d->k_out_stride, dq, n, g->dq_stride, false))
+            return KATSU_E_INVALID;
     }
     hipStream_t st = (hipStream_t)stream;
     void *ws = nullptr;
@@ -3486,7 +3510,8 @@ int katsu_hip_distillation_dev(const katsu_distillation *d, const void *logits,
 static bool dlogits_ok(const katsu_distillation &d, const void *logits, const void *dlogits) {
     if (!embedding_out_ok(d.rows, d.vocab, d.out_stride)) return false;
     if (logits == dlogits) return d.rows < 2 || d.stride == d.out_stride;
-    return !rows_share(logits, d.rows, d.stride, dlogits, d.rows, d.out_stride, d.vocab, d.dtype);
+    return !rows_share(logits, d.rows, d.stride, d.vocab, dlogits, d.rows, d.out_stride, d.vocab,
+                       d.dtype);
 }
 
 int katsu_hip_distillation_bwd_dev(const katsu_distillation *d, const float *dloss,

@@ -58,14 +58,19 @@ bool embedding_ok(const katsu_embedding &d);
 // Whether rows of these columns can be written with this stride.
 bool embedding_out_ok(uint64_t rows, uint64_t cols, int64_t stride);
 // Whether any of n_a rows of a and n_b rows of b share memory.
-bool rows_share(const void *a, uint64_t n_a, int64_t stride_a, const void *b, uint64_t n_b,
-                int64_t stride_b, uint64_t cols, int dtype);
+bool rows_share(const void *a, uint64_t n_a, int64_t stride_a, uint64_t cols_a, const void *b,
+                uint64_t n_b, int64_t stride_b, uint64_t cols_b, int dtype);
 int embedding(const katsu_embedding &d, const int32_t *ids, const void *table, void *out,
               hipStream_t st);
 size_t embedding_bwd_bytes(const katsu_embedding &d);
 int embedding_bwd(const katsu_embedding &d, const void *dout, const int32_t *ids, void *dtable,
                   void *ws, hipStream_t st);
 
+// Whether heads of a and heads of b share memory: begin at one place, or, where heads or tokens lie
+// side by side in both, share any.
+bool heads_share(const katsu_qk_norm_rotary &d, const void *a, uint64_t heads_a,
+                 const int64_t (&stride_a)[2], const void *b, uint64_t heads_b,
+                 const int64_t (&stride_b)[2]);
 bool qk_norm_rotary_ok(const katsu_qk_norm_rotary &d);
 int qk_norm_rotary(const katsu_qk_norm_rotary &d, const void *q, const void *k, const void *w_q,
                    const void *w_k, const float *table, const int32_t *positions, void *q_out,

@@ -342,21 +342,21 @@ bool embedding_out_ok(uint64_t rows, uint64_t cols, int64_t stride) {
     return rows < 2 || stride >= (int64_t)cols;
 }
 
-bool rows_share(const void *a, uint64_t n_a, int64_t stride_a, const void *b, uint64_t n_b,
-                int64_t stride_b, uint64_t cols, int dtype) {
-    if (n_a == 0 || n_b == 0 || cols == 0) return false;
+bool rows_share(const void *a, uint64_t n_a, int64_t stride_a, uint64_t cols_a, const void *b,
+                uint64_t n_b, int64_t stride_b, uint64_t cols_b, int dtype) {
+    if (n_a == 0 || n_b == 0 || cols_a == 0 || cols_b == 0) return false;
     struct Rows {
         __int128 at, step, len;
         uint64_t n;
         __int128 end() const { return at + (__int128)(n - 1) * step + len; }
     };
     const int size = dtype == KATSU_F32 ? 4 : 2;
-    auto rows = [&](const void *p, uint64_t n, int64_t stride) {
+    auto rows = [&](const void *p, uint64_t n, int64_t stride, uint64_t cols) {
         Rows r{(__int128)(uintptr_t)p, (__int128)stride * size, (__int128)cols * size, n};
         if (n == 1 || r.step <= r.len) r = {r.at, 0, r.end() - r.at, 1};  // no gaps
         return r;
     };
-    Rows x = rows(a, n_a, stride_a), y = rows(b, n_b, stride_b);
+    Rows x = rows(a, n_a, stride_a, cols_a), y = rows(b, n_b, stride_b, cols_b);
     if (x.end() <= y.at || y.end() <= x.at) return false;
     if (x.n > 1 && x.step == y.step) {  // parts of the same wider rows
         if (y.at < x.at) std::swap(x, y);
@@ -402,6 +402,30 @@ int embedding_bwd(const katsu_embedding &d, const void *dout, const int32_t *ids
     a.add = d.accumulate;
     return d.dtype == KATSU_F32 ? embed_grad<float>(d, a, (char *)ws, st)
                                 : embed_grad<__bf16>(d, a, (char *)ws, st);
+}
+
+bool heads_share(const katsu_qk_norm_rotary &d, const void *a, uint64_t heads_a,
+                 const int64_t (&stride_a)[2], const void *b, uint64_t heads_b,
+                 const int64_t (&stride_b)[2]) {
+    if (d.tokens == 0 || heads_a == 0 || heads_b == 0) return false;
+    if (a == b) return true;
+    struct Rows {
+        uint64_t n, cols;
+        int64_t stride;
+    };
+    const int64_t D = (int64_t)d.head_dim;
+    auto rows = [&](uint64_t heads, const int64_t(&s)[2], Rows &r) {
+        if (heads == 1 || s[1] == D)  // a token's heads side by side
+            r = {d.tokens, heads * d.head_dim, s[0]};
+        else if (d.tokens == 1 || s[0] == D)  // a head's tokens
+            r = {heads, d.tokens * d.head_dim, s[1]};
+        else
+            return false;
+        return true;
+    };
+    Rows x, y;
+    return rows(heads_a, stride_a, x) && rows(heads_b, stride_b, y) &&
+           rows_share(a, x.n, x.stride, x.cols, b, y.n, y.stride, y.cols, d.dtype);
 }
 
 bool qk_norm_rotary_ok(const katsu_qk_norm_rotary &d) {

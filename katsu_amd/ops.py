@@ -626,7 +626,8 @@ def qk_norm_rotary(q, k, table=None, positions=None, w_q=None, w_k=None, eps=1e-
     """(q', k'): each head of q and k [tokens, heads, channels] (k may be None) divided by its
     channels' root mean square, times w_q or w_k ([channels], None: no weight), then turned as
     rotary does by rows of `table` (None: not turned), in one pass and rounded once.  At most 512
-    channels, adjacent; any token and head strides.  out_q may be q, and out_k k."""
+    channels, adjacent; any token and head strides.  out_q may be q, and out_k k; otherwise they
+    share no memory with an operand or each other."""
     out_q = torch.empty_like(q) if out_q is None else out_q
     if k is not None and out_k is None:
         out_k = torch.empty_like(k)
@@ -640,8 +641,9 @@ def qk_norm_rotary(q, k, table=None, positions=None, w_q=None, w_k=None, eps=1e-
 def qk_norm_rotary_backward(dq, dk, q, k, table=None, positions=None, w_q=None, w_k=None,
                             eps=1e-6, interleaved=False, out_q=None, out_k=None, workspace=None):
     """(dx_q, dx_k, dw_q, dw_k) from dq and dk, the gradients of qk_norm_rotary's outputs, and its
-    operands; None for those that were not given.  out_q and out_k receive dx_q and dx_k and may be
-    dq and dk.  `workspace`: an optional device tensor of qk_norm_rotary_workspace_bytes()."""
+    operands; None for those that were not given.  out_q and out_k receive dx_q and dx_k; out_q may
+    be dq or q, out_k dk or k; otherwise they share no memory with an operand or each other.
+    `workspace`: an optional device tensor of qk_norm_rotary_workspace_bytes()."""
     out_q = torch.empty_like(q) if out_q is None else out_q
     if k is not None and out_k is None:
         out_k = torch.empty_like(k)
