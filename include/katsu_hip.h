@@ -445,8 +445,11 @@ int katsu_hip_embedding_bwd_dev(const katsu_embedding *d, const void *dout, cons
  *   n = x / sqrt(mean(x^2) + eps) * w,  y = n turned as katsu_hip_rotary_dev does
  * with w_q and w_k of head_dim (1..512) values, or NULL for none; rotary_dim 0
  * (and table NULL) leaves the turn out.  Operands, positions and strides are as
- * in katsu_hip_rotary_dev; k may be NULL with k_heads 0.  q_out may be q, and
- * k_out k, with the same strides.  n is not rounded before the turn. */
+ * in katsu_hip_rotary_dev, the heads of outputs too; k may be NULL with k_heads
+ * 0.  q_out may be q, and k_out k, with the same strides; otherwise the outputs
+ * share no memory with an input or each other (looked at where heads or tokens
+ * lie side by side, or both tensors begin at one place).  n is not rounded
+ * before the turn.  x^2 is float32: a head with values beyond 1.8e19 becomes 0. */
 typedef struct katsu_qk_norm_rotary {
     int32_t dtype, interleaved;
     uint64_t tokens, heads, k_heads, head_dim, rotary_dim, length;
@@ -479,8 +482,8 @@ int katsu_hip_qk_norm_rotary_bwd_dev(const katsu_qk_norm_rotary *d,
 /* The loss of rows x vocab logits z against a teacher's top logits t, `top`
  * (0..1024) of them a row at the columns ids (both [rows][top], contiguous).
  * The temperature is positive and finite, and so is log2(e) / temperature in
- * float32 (4.23e-39 is too small).  Over a row's entries whose id is in
- * [0, vocab), with tau the temperature:
+ * float32 (4.23e-39 is too small).  Probabilities below 2^-126 are 0.  Over a
+ * row's entries whose id is in [0, vocab), with tau the temperature:
  *   p = softmax(t / tau),  P = softmax(z / tau) over all columns,
  *   loss = tau^2 sum_k p_k (log p_k - log P[id_k]),
  *   dlogits[v] = dloss tau (P[v] - sum of the p_k with id_k = v)

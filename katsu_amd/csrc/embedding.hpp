@@ -1,11 +1,15 @@
 // embedding.hpp -- rows of a table by token, times a scale, and the table's gradient.
 //
 //   out[t] = scale table[ids[t]]                       (zeros where ids[t] is no row)
-//   dtable[v] = (dtable[v] +) scale sum over t with ids[t] = v of dout[t], t rising
+//   dtable[v] = (dtable[v] +) scale sum over t with ids[t] = v of dout[t]
+//
+// A row's sum is float32, its order the tokens' inside a tile (below) and fixed by ids and sizes.
 //
 // HBM-bound: each row is read and written once (16384 tokens of 32000 x 2048 float32: 40 us, 212 MB
 // moved, 5.3 TB/s; the gradient in bfloat16, 200 MB: 64 us, of which adding and writing zeros 47,
-// 4.3 TB/s, the sort before it 11, the join behind it 6; a copy reaches 4.7).
+// 4.3 TB/s, the sort before it 11, the join behind it 6; a copy of as much reaches 5.1).  A wave a
+// token whatever its width: rows of 256 bfloat16 use half of its lanes (262144 tokens: 84 us, 32
+// by the bytes; their gradient 100, 28 by the bytes), rows of 32 four (72 us, 4 by the bytes).
 #pragma once
 
 #include "lmvec.hpp"
@@ -375,15 +379,17 @@ __global__ void __launch_bounds__(256) embed_there_kernel(const EmbedSort s) {
     if (k < s.vocab && k != before) atomicOr(s.there + (k >> 5), 1u << (k & 31));
 }
 
-// A wave a tile's chunk of 64 pieces, kEmbedAhead tokens' rows in flight (16: 66 us in tiles of 32 rows
-// of 4 KB; 8: 68).
+// A wave a tile's chunk of 64 pieces, kEmbedAhead tokens' rows in flight (16384 tokens, 32000 x 2048
+// bfloat16, all launches: 64.4 us with 16, 65.1 with 8, 67.7 with 32; 65536 tokens of 256 columns
+// 57, 57 and 64).
 template <typename T>
 __global__ void __launch_bounds__(256) embed_tile_kernel(const EmbedTiles t) {
     constexpr int E = Piece<T>::E, U = kEmbedAhead;
     const EmbedArgs &a = t.a;
     const int lane = threadIdx.x & 63;
     const int64_t id = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-    // One of each kind by turns, so that zeros are written while rows are awaited.
+    // One of each kind by turns (16384 tokens, 32000 x 2048 bfloat16: 63 us, all tiles first 61, all
+    // zeros first 65; 8192 tokens of 4096 columns 81, 82 and 80).
     const int64_t both = min(t.tile_blocks, t.zero_blocks);
     if (id >= t.tile_blocks + t.zero_blocks) return;
     const int64_t block = id < 2 * both ? (id & 1 ? t.tile_blocks : 0) + id / 2

@@ -5,12 +5,14 @@
 //
 // and its gradient, with g = the gradient of y turned back:
 //   dw = sum over tokens and heads of g x r,  dx = r g w - x r^3 mean(g w x)
-// where both of a head's sums are taken at once.
+// where both of a head's sums are taken at once.  Squares are float32: a head with values beyond
+// 1.8e19 becomes 0, and without eps one of values below 1e-19 is inexact or infinite.
 //
-// HBM-bound: a head stays in its lanes' registers, so each operand is read once and each
-// result written once (8192 tokens, 16 + 4 heads of 128, bfloat16: 18.5 us, 4.75 TB/s, vector
-// instructions 62% of the time; the gradient of 16384 tokens, 32 + 8 heads: 109 us, 4.6 TB/s; of
-// 6000 tokens, 16 + 4: 24 us and 4 for the sums of dw).
+// A head stays in its lanes' registers, so each operand is read once and each result written once:
+// HBM-bound where heads are many (the gradient of 16384 tokens, 32 + 8 heads of 128, bfloat16: 110
+// us, 4.6 TB/s).  8192 tokens, 16 + 4 heads: 24.4 us, 3.7 TB/s (a copy of as much takes 19.1), vector
+// instructions 62% of the time; 18.4 where the caches hold the outputs.  The gradient of 6000
+// tokens, 16 + 4: 24.4 us, vector instructions 68% of the time, and 4 for the sums of dw.
 #pragma once
 
 #include "lmvec.hpp"

@@ -74,11 +74,12 @@ EmbedPlan embed_plan(const katsu_embedding &d) {
         while (n >> b) ++b;
         return b;
     };
-    // By rows: 256 tokens 14 us, 18 by slabs; 500 tokens 19 and 18 (32000 x 256 float32).  Slabs: one a
-    // CU, more where a block's LDS does not hold its rows' counts.  Their blocks all read all
-    // ids, so with more tokens or rows the passes: 65536 tokens 54 us, 57 in passes, 131072 tokens 90
-    // and 73 (32000 x 256 bfloat16); 20000 tokens, 10^6 rows 112 and 96; where one pass is enough,
-    // 32768 tokens 36 and 36, 65536 tokens 55 and 40 (1001 rows).
+    // By rows: 256 tokens 13 us, 21 by slabs (32000 x 256 float32); 500 tokens would take 18 and 21, but
+    // with eight ids a lane instead of four 256 tokens 14.  Slabs: one a CU, more where a block's LDS
+    // does not hold its rows' counts.  Their blocks all read all ids, so with more tokens or rows the
+    // passes: 16384 tokens 28 us, 46 in passes, 65536 tokens 57 and 59, 131072 tokens 94 and 74 (32000
+    // x 256 bfloat16); 20000 tokens, 10^6 rows of 128 115 and 100; where one pass is enough, 32768
+    // tokens 38 and 38, 65536 tokens 60 and 44 (1001 rows).
     p.per = (int)std::min<int64_t>(cdiv(V, kCUs * 32) * 32, kEmbedSlab);
     const int64_t slabs = cdiv(V, p.per);
     p.passes = (int)cdiv(bits(V), kEmbedBits);
@@ -93,8 +94,9 @@ EmbedPlan embed_plan(const katsu_embedding &d) {
         p.bits = (int)cdiv(bits(V), p.passes);
     }
     const int chunks = (int)cdiv((int64_t)d.cols, 64 * (d.dtype == KATSU_F32 ? 4 : 8));
-    // Tiles of 8 tokens, more where that makes enough waves: longer tiles leave fewer parts (16384
-    // tokens, 32000 x 2048 bfloat16: 70 us in tiles of 64, 66 of 32, 77 of 16).
+    // Tiles of 8 tokens, more where that makes enough waves: longer tiles leave fewer parts (8192 tokens,
+    // 32000 x 4096 bfloat16: 83 us in tiles of 32, 86 of 64, 91 of 16; 65536 tokens of 256 columns 57,
+    // 60 and 64; 16384 of 2048 64.3, 64.5 and 64.9).
     p.tile = 8;
     while (cdiv(T, p.tile) * chunks > 2048 && p.tile < 1024) p.tile *= 2;
     p.tiles = cdiv(T, p.tile);

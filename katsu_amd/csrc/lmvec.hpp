@@ -48,7 +48,7 @@ __device__ __forceinline__ void store_piece(T *p, int64_t i, int64_t n, const fl
 // The same as it is in memory, in four registers.  From an array of values, as above, the compiler
 // makes three accesses, one of which the one at a row's end, value by value, shares, and holds a
 // register for each value of bfloat16.  Whole accesses are faster where the memory is all
-// (130000 rows of 2 KB set to zero: 66 and 38 us; 16384 rows of 8 KB looked up: 47 and 35), not in
+// (130000 rows of 2 KB set to zero: 67 and 51 us; 16384 rows of 8 KB looked up: 53 and 40), not in
 // the norms' gradient, which has no registers for what is then loaded early (114 and 136 us).
 template <typename T>
 struct RawPiece {
