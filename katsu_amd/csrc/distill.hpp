@@ -9,7 +9,8 @@
 // A row without such an entry, or with none above -inf, has loss and gradient 0, and its
 // logits are not read.  M = max z, L = sum exp((z - M)/tau), T the teacher's.  Differences of
 // logits are taken first, so that large ones lose nothing, and stay logits: over a tau below 1 the
-// type's lowest value would be infinite, and tau^2 is 0 or infinite before tau is.
+// type's lowest value would be infinite, and tau^2 is 0 or infinite before tau is.  They are summed
+// as fourths, which are as exact: the sum of the whole ones may be infinite where tau times it is not.
 //
 // An exponential is exp2 of a difference times log2(e)/tau in float32, whose rounding (1.3e-8 of it at
 // a tau of 1) grows with the distance: totals are 5.5e-8 too large for normal logits of deviation
@@ -193,14 +194,15 @@ __device__ __forceinline__ void distill_loss(const DistillArgs &a, int64_t row,
                                              const DistillRow<NT> &d, const DistillSum &s,
                                              float *part) {
     const T *z = (const T *)a.z + row * a.z_row;
-    const float rest = a.tau * (logf(s.l) - logf(d.total));
+    const float rest = 0.25f * (a.tau * (logf(s.l) - logf(d.total)));
     float v = 0.f;
 #pragma unroll
     for (int i = 0; i < DistillRow<NT>::N; ++i)
         if (d.id[i] >= 0 && d.p[i] != 0.f)
-            v += d.p[i] * (((d.t[i] - d.largest) - ((float)z[d.id[i]] - s.m)) + rest);
+            v += d.p[i] * ((0.25f * d.t[i] - 0.25f * d.largest) -
+                           (0.25f * (float)z[d.id[i]] - 0.25f * s.m) + rest);
     v = block_join<NT>(v, part, JoinSum());
-    if (threadIdx.x == 0) a.loss[row] = a.tau * v;
+    if (threadIdx.x == 0) a.loss[row] = 4.f * (a.tau * v);
 }
 
 // The teacher's columns among [c0, c1): an entry's value, of which the first of equal ids takes the

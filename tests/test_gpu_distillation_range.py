@@ -62,3 +62,23 @@ def test_infinite_and_zero_losses(dev, rows):
         loss, _, grad, loss2, grad2 = _all(dev, *one, tau)
         assert not loss.any() and not loss2.any(), tau
         assert not grad.any() and not grad2.any(), tau
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("tau", [0.125, 0.3, 0.49])
+@pytest.mark.parametrize("rows", [3, 280])
+def test_all_of_the_teacher_masked(dev, dt, tau, rows):
+    """Every column that the teacher names at the lowest value, so that a sum of the differences, weighted
+    with probabilities whose sum may be above 1, is no float32 before it is multiplied by tau; and with
+    a logit near the largest value, as one difference is none."""
+    low = torch.finfo(dt).min
+    z, ids, t, dloss = _inputs(rows, 400, 9, dt, pad=False)
+    ids[:] = torch.arange(9) * 7
+    z[:, :100] = low
+    z[1::3, 300] = -low * 0.9
+    want, dz, ltol, gtol = reference(z, ids, t, tau, dloss)
+    assert (want > 1e37).all() and (want < 3.39e38).all() and (ltol < 1e-5 * want).all()
+    loss, _, grad, loss2, grad2 = _all(dev, z, ids, t, dloss, tau)
+    for a, b in ((loss, grad), (loss2, grad2)):
+        close(a, want, ltol)
+        close(b, dz, gtol)
