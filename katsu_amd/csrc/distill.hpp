@@ -16,8 +16,8 @@
 // a tau of 1) grows with the distance: totals are 5.5e-8 too large for normal logits of deviation
 // 2.5.  Results below 2^-126 are 0.
 //
-// The loss in one pass with each thread's running maximum and sum: 4096 x 32000 bfloat16 51 us, 4.8
-// TB/s, where the vector unit is busy 83% of the time as well.  The gradient 1000 x 32001 float32
+// The loss in one pass with each thread's running maximum and sum: 4096 x 32000 bfloat16 51-53 us,
+// 4.7-4.8 TB/s, where the vector unit is busy 83% of the time as well.  The gradient 1000 x 32001 float32
 // 62 us, 4.3 TB/s; both in a pass, 8192 x 32000 bfloat16, 203 us, 5.0 TB/s: HBM (a copy of as much
 // reaches 5.1 to 5.3).
 #pragma once
