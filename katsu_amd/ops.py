@@ -567,7 +567,8 @@ def embedding_backward(dout, ids, vocab, scale=1.0, out=None, beta=0.0, workspac
     """The gradient of embedding's table [vocab, C] from dout [T, C]: each row the sum of its
     tokens' gradients, times scale; tokens with an id that is no row add nothing.  beta=1
     accumulates into `out` and leaves rows without a token as they are; out shares no memory with
-    dout.  The same call gives the same bits.  `workspace`: an optional device tensor of embedding_workspace_bytes()."""
+    dout.  The same call gives the same bits.  `workspace`: an optional device tensor of
+    embedding_workspace_bytes()."""
     if out is None:
         if beta != 0.0:
             raise ValueError("beta=1 needs the gradient that it accumulates into")
